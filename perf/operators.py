@@ -35,6 +35,7 @@ EPS = 1e-5
 # Bounds of a drawn case, those of the largest listed ones.
 MAX_NORM = 2048 * 4096
 MAX_ROUTE = 512 * 128 * 2048
+MAX_BYTES = 7.9e8  # of weights that a pass reads
 MAX_WEIGHTS = 8 * 14336 * 4096
 MAX_PAIRS = 64
 
@@ -89,16 +90,14 @@ def _draw_layer(rng, kind):
     # the norm's output serves the gate and up products, in blocks of their activations
     cols = BLOCK[gate] * _log(rng, max(1, 256 // BLOCK[gate]), 4096 // BLOCK[gate])
     ffn = BLOCK[down] * _log(rng, max(1, 256 // BLOCK[down]), 14336 // BLOCK[down])
-    while experts * cols * ffn > MAX_WEIGHTS:
-        ffn = BLOCK[down] * max(1, ffn // (2 * BLOCK[down]))
-        if ffn == BLOCK[down]:
-            break
     tokens = 1 if rng.random() < 0.4 else _log(rng, 2, 40)
     tokens = max(1, min(tokens, MAX_PAIRS // slots))
     case = {"kind": kind, "tokens": tokens, "experts": experts, "slots": slots, "cols": cols, "ffn": ffn, "gate": gate,
             "down": down}
     if kind == "ffn":
         case.update(packed=rng.random() < 0.5, residual=rng.random() < 0.5, dropped=rng.choice((0.0, 0.0, 0.3)))
+    while experts * cols * case["ffn"] > MAX_WEIGHTS or work(case)["bytes"] > MAX_BYTES:
+        case["ffn"] = BLOCK[down] * (case["ffn"] // (2 * BLOCK[down]))
     return case
 
 
