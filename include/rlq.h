@@ -310,6 +310,81 @@ int32_t rlq_block_sums(rlq_context *ctx, const rlq_weights *w, const float *x, u
 int32_t rlq_block_sums_ex(rlq_context *ctx, const rlq_weights *w, const float *x, uint64_t batch, uint32_t flags,
                           int32_t *isum, int32_t *imin, float *y, void *stream, rlq_error *err);
 
+/* ---- mixture-of-experts layers --------------------------------------------------
+ * The half of a decoder layer around rlq_mul_mat_id: the norm whose packed output
+ * the products take, the router that makes the expert ids, and the experts'
+ * products of a few tokens with SiLU and the weighted sum.  All pointers are
+ * device pointers.  Data errors are the token's own: its outputs are held back as
+ * described, those of the other tokens are written, and rlq_sync reports the
+ * first.  Outputs may take the place of inputs of the same shape (residual to
+ * total or y), but may not overlap otherwise. */
+
+/* RMSNorm of `rows` rows of `cols` values in the reference's f32 operations
+ * (crates/model-runtime/src/math.rs:203-228; the bits rlq_llama_step's norms have):
+ *   total = x + residual      (x where residual is null)
+ *   y = total * (1 / sqrt(mean(total^2) + eps)) * weight
+ *   q = y in blocks of q_dtype, RLQ_Q8_K or RLQ_Q8_0, as rlq_quantize_device
+ *       writes them: the packed right-hand side of rlq_mul_mat, rlq_mul_mat_id
+ *       and rlq_moe_ffn
+ * total, y and q may each be null, not all three; q_dtype is not looked at where q
+ * is null.  cols: whole blocks of q_dtype, at most 32768; rows at most 65535
+ * (RLQ_UNIMPLEMENTED beyond); eps positive and finite (RLQ_INVALID_CONFIG, a = 2).
+ * f32 pointers 4-byte aligned (16 and cols % 4 == 0: wide loads), q 4-byte
+ * aligned for Q8_K and 2 for Q8_0.  At rlq_sync, with b = the row:
+ * RLQ_NON_FINITE (a = RLQ_CHECK_RMS_SCALE or RLQ_CHECK_RMS_OUTPUT), or
+ * RLQ_UNREPRESENTABLE_SCALE (a = block); nothing of that row is written. */
+int32_t rlq_rms_norm(rlq_context *ctx, const float *x, const float *residual, const float *weight, uint64_t rows,
+                     uint64_t cols, float eps, float *total, float *y, uint32_t q_dtype, uint8_t *q, void *stream,
+                     rlq_error *err);
+
+/* The router: logits[t][e] = router row e . x row t, router [experts, cols] and x
+ * [tokens, cols] f32, added up in f64 and rounded once.  The rest is computed in
+ * f64 from those: scores = softmax(logits), or sigmoid(logits) with
+ * RLQ_ROUTE_SIGMOID; ids[t][..] (i32) = the `slots` experts of the largest logits, or
+ * with a bias [experts] of the largest score + bias, the lowest index of equal
+ * ones; weights[t][..] = their scores (without the bias), with
+ * RLQ_ROUTE_NORMALIZE divided by their sum (0 where that is 0), times scale,
+ * rounded once.  A bias of -infinity or NaN switches an expert off; places for which no
+ * expert is left get id -1 and weight 0, as rlq_mul_mat_id and rlq_moe_ffn take
+ * them.  bias and logits may be null.  1 <= slots <= experts (RLQ_TENSOR_SHAPE);
+ * slots at most 64, experts 1024, tokens 65535 (RLQ_UNIMPLEMENTED).  Pointers
+ * 4-byte aligned (router and x 16 and cols % 4 == 0: wide loads).  A token with a
+ * logit that is not finite gets ids of -1 and weights of 0: RLQ_NON_FINITE at
+ * rlq_sync (a = RLQ_CHECK_MATRIX_OUTPUT, b = the token). */
+#define RLQ_ROUTE_SIGMOID 1u
+#define RLQ_ROUTE_NORMALIZE 2u
+int32_t rlq_moe_route(rlq_context *ctx, const float *router, const float *x, uint64_t tokens, uint64_t cols,
+                      uint64_t experts, uint64_t slots, uint32_t flags, float scale, const float *bias, int32_t *ids,
+                      float *weights, float *logits, void *stream, rlq_error *err);
+
+/* The experts of a mixture-of-experts layer for a few tokens: for token t and
+ * its places s with expert e = ids[t][s] in [0, experts)
+ *   g = gate[e] . x[t], u = up[e] . x[t]       (the products of rlq_mul_mat_id)
+ *   h = silu(g) * u
+ *   y[t] = residual[t] + sum over s of weights[t][s] * (down[e] . h)
+ * gate, up [cols -> ffn] and down [ffn -> rows of y]: stacks of one number of
+ * experts (n3 = 1), gate and up of one type, down of any.  x: f32 rows (x_dtype 0,
+ * 16-byte aligned; quantized as rlq_mul_mat_id does) or rows of gate's activation
+ * type (Q8_K 4-byte aligned, Q8_0 2-byte), taken as given but for the Q8_K bsums, which are those
+ * of the levels.  The block integers are exact; their sums run in f64 and are
+ * rounded once where g, u, h and y become f32, so y does not depend on what shares
+ * a call.  h is quantized like any f32 column of down.  ids and weights [tokens,
+ * slots]; -1: no expert (its weight is not looked at), a token without any gets
+ * its residual.  residual may be null (0), and may be y.
+ * 32 tokens share a pass over the weights of the experts that they use; more
+ * tokens take further passes (a prompt is better served by rlq_mul_mat_id).
+ * Capturing: make the same call once before, for the scratch.
+ * Errors: RLQ_TENSOR_SHAPE (stacks that do not match, slots 0),
+ * RLQ_TENSOR_UNSUPPORTED (up's type, x_dtype), RLQ_UNIMPLEMENTED (more than 1024
+ * experts, 64 slots or 65535 tokens).  At rlq_sync, the token's row of y being left
+ * as it was: RLQ_TENSOR_BOUNDS (an id outside [-1, experts); a = its index),
+ * RLQ_NON_FINITE_INPUT / RLQ_UNREPRESENTABLE_SCALE of x (b = the token), then of h
+ * RLQ_NON_FINITE (a = RLQ_CHECK_MATRIX_INPUT) / RLQ_UNREPRESENTABLE_SCALE (a =
+ * block), b = the token. */
+int32_t rlq_moe_ffn(rlq_context *ctx, const rlq_weights *gate, const rlq_weights *up, const rlq_weights *down,
+                    uint32_t x_dtype, const void *x, uint64_t tokens, const int32_t *ids, const float *weights,
+                    uint64_t slots, const float *residual, float *y, void *stream, rlq_error *err);
+
 /* ---- dense Llama decode step ------------------------------------------------
  * LlamaModel of crates/model-runtime/src/llama.rs with quantized matrices,
  * resident on one GPU with its f32 KV cache.  Every matrix product runs the

@@ -134,6 +134,7 @@ class _Err(ctypes.Structure):
 
 # Every entry point of include/rlq.h with its ctypes signature.
 _P, _U64, _U32, _I32 = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int32
+_F32 = ctypes.c_float
 _E = ctypes.POINTER(_Err)
 SIGNATURES = {
     "rlq_status_string": ([_I32], ctypes.c_char_p),
@@ -159,6 +160,9 @@ SIGNATURES = {
     "rlq_matmul_noalloc": ([_P, _P, _P, _U64, _P, _P, _P, _E], _I32),
     "rlq_matmul_argmax": ([_P, _P, _P, _U64, _P, _P, _P, _E], _I32),
     "rlq_quantize_device": ([_P, _U32, _P, _U64, _U64, _P, _P, _E], _I32),
+    "rlq_rms_norm": ([_P, _P, _P, _P, _U64, _U64, _F32, _P, _P, _U32, _P, _P, _E], _I32),
+    "rlq_moe_route": ([_P, _P, _P, _U64, _U64, _U64, _U64, _U32, _F32, _P, _P, _P, _P, _P, _E], _I32),
+    "rlq_moe_ffn": ([_P, _P, _P, _P, _U32, _P, _U64, _P, _P, _U64, _P, _P, _P, _E], _I32),
     "rlq_sync": ([_P, _P, _E], _I32),
     "rlq_block_sums": ([_P, _P, _P, _U64, _P, _P, _P, _E], _I32),
     "rlq_block_sums_ex": ([_P, _P, _P, _U64, _U32, _P, _P, _P, _P, _E], _I32),
@@ -479,6 +483,103 @@ class Context:
         err = _Err()
         _check(_lib.rlq_mul_mat_id(self._h, w._h, int(x_dtype), xp, ncols, tokens, _dev_ptr(ids, torch.int32),
                                    slots, _dev_ptr(y, torch.float32), _stream_ptr(stream), ctypes.byref(err)), err)
+        return y
+
+    def rms_norm(self, x, weight, eps, residual=None, packed=None, normed=True, total=None, y=None, q=None, stream=None):
+        """The residual's addition and the RMS norm of x [..., cols] f32 with
+        weight [cols] (math.rs:203-228): (total, y, q) with total = x + residual
+        (None without a residual, unless a tensor for it is given), y the
+        normed rows (None if not normed) and q, where `packed` is DType.Q8_K or
+        Q8_0, y's blocks [rows, row_bytes(packed, cols)] uint8, the packed
+        right-hand side of mul_mat, mul_mat_id and moe_ffn.  Outputs may be
+        given; total and y may take the place of x or residual."""
+        cols = weight.numel()
+        if x.shape[-1] != cols or (residual is not None and residual.shape != x.shape):
+            raise ValueError("x and residual must be [..., cols] with the weight's cols")
+        rows = x.numel() // cols if cols else 0
+        if residual is not None and total is None:
+            total = torch.empty_like(x)
+        if normed and y is None:
+            y = torch.empty_like(x)
+        if packed is not None:
+            nbytes = row_bytes(packed, cols)
+            if q is None:
+                q = torch.empty((rows, nbytes), dtype=torch.uint8, device=x.device)
+        elif q is not None:
+            raise ValueError("q needs the packed type")
+        for t, n in ((total, rows * cols), (y, rows * cols), (q, rows * nbytes if packed is not None else 0)):
+            if t is not None and t.numel() != n:
+                raise ValueError("an output's size does not match x")
+        err = _Err()
+        f32 = torch.float32
+        _check(_lib.rlq_rms_norm(self._h, _dev_ptr(x, f32), None if residual is None else _dev_ptr(residual, f32),
+                                 _dev_ptr(weight, f32), rows, cols, float(eps),
+                                 None if total is None else _dev_ptr(total, f32), None if y is None else _dev_ptr(y, f32),
+                                 0 if packed is None else int(packed), None if q is None else _dev_ptr(q, torch.uint8),
+                                 _stream_ptr(stream), ctypes.byref(err)), err)
+        return total, y, q
+
+    ROUTE_SIGMOID, ROUTE_NORMALIZE = 1, 2
+
+    def moe_route(self, router, x, top_k, gating="softmax", normalize=True, scale=1.0, bias=None, logits=False, ids=None,
+                  weights=None, stream=None):
+        """The best top_k experts of every token and their weights: router
+        [experts, cols] f32, x [tokens, cols] f32 -> (ids int32 [tokens, top_k],
+        weights f32 [tokens, top_k], logits f32 [tokens, experts], None unless
+        asked for with True or a tensor).  gating: "softmax" or "sigmoid" of the
+        logits; bias [experts] is added to the scores for the choice only (-inf:
+        never chosen; places with no expert left get id -1 and weight 0)."""
+        if gating not in ("softmax", "sigmoid"):
+            raise ValueError("gating must be softmax or sigmoid")
+        experts, cols = router.shape
+        x2 = _columns(x, cols)
+        tokens, top_k = x2.shape[0], int(top_k)
+        if ids is None:
+            ids = torch.empty((tokens, top_k), dtype=torch.int32, device=x.device)
+        if weights is None:
+            weights = torch.empty((tokens, top_k), dtype=torch.float32, device=x.device)
+        if logits is True:
+            logits = torch.empty((tokens, experts), dtype=torch.float32, device=x.device)
+        elif logits is False:
+            logits = None
+        if ids.numel() != tokens * top_k or weights.numel() != tokens * top_k \
+                or (logits is not None and logits.numel() != tokens * experts) \
+                or (bias is not None and bias.numel() != experts):
+            raise ValueError("ids, weights, logits or bias of another size")
+        err = _Err()
+        f32 = torch.float32
+        flags = (self.ROUTE_SIGMOID if gating == "sigmoid" else 0) | (self.ROUTE_NORMALIZE if normalize else 0)
+        _check(_lib.rlq_moe_route(self._h, _dev_ptr(router, f32), _dev_ptr(x2, f32), tokens, cols, experts, top_k, flags,
+                                  float(scale), None if bias is None else _dev_ptr(bias, f32), _dev_ptr(ids, torch.int32),
+                                  _dev_ptr(weights, f32), None if logits is None else _dev_ptr(logits, f32),
+                                  _stream_ptr(stream), ctypes.byref(err)), err)
+        return ids, weights, logits
+
+    def moe_ffn(self, gate, up, down, x, ids, weights, x_dtype=DType.F32, residual=None, y=None, stream=None):
+        """The experts of a mixture-of-experts layer for a few tokens: stacked
+        gate, up [cols -> ffn] and down [ffn -> out] Weights of one number of
+        experts; x [tokens, cols] f32, or uint8 rows of gate's activation type
+        when x_dtype is it; ids int32 and weights f32 [tokens, slots] (id -1: no
+        expert) -> y [tokens, out] = residual + the weighted sum of
+        down(silu(gate x) * up x) over a token's experts."""
+        x_dtype = DType(x_dtype)
+        tokens, slots = ids.shape
+        f32 = torch.float32
+        known = x_dtype in (DType.F32, DType.Q8_0, DType.Q8_K)  # (the library refuses the others)
+        if known and x.numel() != tokens * (gate.cols if x_dtype == DType.F32 else row_bytes(x_dtype, gate.cols)):
+            raise ValueError("x must hold the gate's cols for every row of ids")
+        if weights.shape != ids.shape:
+            raise ValueError("weights must have the shape of ids")
+        if y is None:
+            y = torch.empty((tokens, down.rows), dtype=f32, device=x.device)
+        if y.numel() != tokens * down.rows or (residual is not None and residual.numel() != y.numel()):
+            raise ValueError("y and residual must hold the down matrix's rows for every token")
+        err = _Err()
+        _check(_lib.rlq_moe_ffn(self._h, gate._h, up._h, down._h, int(x_dtype),
+                                _dev_ptr(x, f32 if x_dtype == DType.F32 else torch.uint8), tokens,
+                                _dev_ptr(ids, torch.int32), _dev_ptr(weights, f32), slots,
+                                None if residual is None else _dev_ptr(residual, f32), _dev_ptr(y, f32),
+                                _stream_ptr(stream), ctypes.byref(err)), err)
         return y
 
     def sync(self, stream=None):

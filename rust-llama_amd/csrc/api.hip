@@ -107,7 +107,7 @@ struct rlq_context {
     // replaced; its counter set to 0 when the buffer is made, and left at 0 by
     // every launch); column_keys: one per column, of an argmax after a GEMM that
     // uses them (argmax_one_group)
-    DevBuf planes, keys, column_keys, stage_in, stage_w, stage_out, gate;
+    DevBuf planes, keys, column_keys, stage_in, stage_w, stage_out, gate, logits, moe;
     Retired* retired = nullptr;
 };
 
@@ -401,7 +401,8 @@ void rlq_context_destroy(rlq_context* ctx) {
     if (!ctx) return;
     DeviceGuard g(ctx->device);
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
-    for (DevBuf* b : {&ctx->planes, &ctx->keys, &ctx->column_keys, &ctx->stage_in, &ctx->stage_w, &ctx->stage_out, &ctx->gate})
+    for (DevBuf* b : {&ctx->planes, &ctx->keys, &ctx->column_keys, &ctx->stage_in, &ctx->stage_w, &ctx->stage_out, &ctx->gate,
+                      &ctx->logits, &ctx->moe})
         if (b->p) (void)hipFree(b->p);
     while (Retired* r = ctx->retired) {
         ctx->retired = r->next;
@@ -949,6 +950,99 @@ int32_t rlq_quantize_device(rlq_context* ctx, uint32_t dtype, const float* x, ui
         HIP_TRY(launch_finite_scan(x, n, ew, s));
         HIP_TRY(launch_encode_k(dtype, x, n, out, ew, s));
     }
+    return ok(err);
+}
+
+// ---- mixture-of-experts layers ------------------------------------------------------
+
+// RMSNorm (crates/model-runtime/src/math.rs:203-228) with the residual's addition
+// and the quantizers of the products' right-hand sides.
+int32_t rlq_rms_norm(rlq_context* ctx, const float* x, const float* residual, const float* weight, uint64_t rows,
+                     uint64_t cols, float eps, float* total, float* y, uint32_t q_dtype, uint8_t* q, void* stream,
+                     rlq_error* err) {
+    if (!ctx) return fail(err, RLQ_INVALID_ARGUMENT);
+    if (q) {
+        if (!dtype_known(q_dtype)) return fail(err, RLQ_INVALID_TYPE, q_dtype);
+        if (q_dtype != kQ8_K && q_dtype != kQ8_0) return fail(err, RLQ_UNIMPLEMENTED, q_dtype);
+        uint64_t rb;
+        const int32_t rc = row_bytes(q_dtype, cols, &rb, err);
+        if (rc) return rc;
+    }
+    if (cols == 0) return fail(err, RLQ_INVALID_MATRIX_SHAPE, 0, rows, cols);
+    if (!(eps > 0.0f) || !(eps <= 3.402823466e38f)) return fail(err, RLQ_INVALID_CONFIG, 0, 2);
+    if (cols > kNormMaxCols) return fail(err, RLQ_UNIMPLEMENTED, 0, cols, kNormMaxCols);
+    if (rows > 65535) return fail(err, RLQ_UNIMPLEMENTED, 0, rows, 65535);  // the error keys' row field
+    if (rows == 0) return ok(err);
+    if (!x || !weight || (!total && !y && !q) || (total && total == y)) return fail(err, RLQ_INVALID_ARGUMENT);
+    if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)weight | (uintptr_t)total | (uintptr_t)y) & 3)
+        return fail(err, RLQ_INVALID_ARGUMENT);
+    if ((uintptr_t)q & (q_dtype == kQ8_K ? 3 : 1)) return fail(err, RLQ_INVALID_ARGUMENT, q_dtype);
+    DeviceGuard g(ctx->device);
+    const NormArgs a{x, residual, weight, (uint32_t)rows, (uint32_t)cols, eps, total, y, q ? q_dtype : 0, q, ctx->err_words};
+    HIP_TRY(launch_rms_norm(a, pick(ctx, stream)));
+    return ok(err);
+}
+
+int32_t rlq_moe_route(rlq_context* ctx, const float* router, const float* x, uint64_t tokens, uint64_t cols,
+                      uint64_t experts, uint64_t slots, uint32_t flags, float scale, const float* bias, int32_t* ids,
+                      float* weights, float* logits, void* stream, rlq_error* err) {
+    if (!ctx) return fail(err, RLQ_INVALID_ARGUMENT);
+    if (flags & ~(RLQ_ROUTE_SIGMOID | RLQ_ROUTE_NORMALIZE)) return fail(err, RLQ_INVALID_ARGUMENT, 0, flags);
+    if (cols == 0 || experts == 0) return fail(err, RLQ_INVALID_MATRIX_SHAPE, 0, experts, cols);
+    if (slots == 0 || slots > experts) return fail(err, RLQ_TENSOR_SHAPE, 0, slots, experts);
+    if (experts > kMoeMaxExperts) return fail(err, RLQ_UNIMPLEMENTED, 0, experts, kMoeMaxExperts);
+    if (slots > kMoeMaxSlots) return fail(err, RLQ_UNIMPLEMENTED, 0, slots, kMoeMaxSlots);
+    if (tokens > 65535) return fail(err, RLQ_UNIMPLEMENTED, 0, tokens, 65535);  // the error keys' token field
+    if (cols > (1ull << 30)) return fail(err, RLQ_UNIMPLEMENTED, 0, cols, 1ull << 30);
+    if (tokens == 0) return ok(err);
+    if (!router || !x || !ids || !weights) return fail(err, RLQ_INVALID_ARGUMENT);
+    if (((uintptr_t)router | (uintptr_t)x | (uintptr_t)bias | (uintptr_t)ids | (uintptr_t)weights | (uintptr_t)logits) & 3)
+        return fail(err, RLQ_INVALID_ARGUMENT);
+    DeviceGuard g(ctx->device);
+    const hipStream_t s = pick(ctx, stream);
+    if (!logits) {
+        HIP_TRY(ensure(ctx, ctx->logits, tokens * experts * sizeof(float), s));
+        logits = (float*)ctx->logits.p;
+    }
+    const RouteArgs a{router, x, bias, (uint32_t)tokens, (uint32_t)experts, (uint32_t)cols, (uint32_t)slots,
+                      flags & RLQ_ROUTE_SIGMOID, flags & RLQ_ROUTE_NORMALIZE, scale, logits, ids, weights, ctx->err_words};
+    HIP_TRY(launch_moe_route(a, s));
+    return ok(err);
+}
+
+// The products of MUL_MAT_ID (crates/tensor/src/cpu_index.rs:169-236) for the
+// gate, up and down matrices of the same experts, and what lies between them.
+int32_t rlq_moe_ffn(rlq_context* ctx, const rlq_weights* gate, const rlq_weights* up, const rlq_weights* down,
+                    uint32_t x_dtype, const void* x, uint64_t tokens, const int32_t* ids, const float* weights,
+                    uint64_t slots, const float* residual, float* y, void* stream, rlq_error* err) {
+    if (!ctx || !gate || !up || !down) return fail(err, RLQ_INVALID_ARGUMENT);
+    if (gate->device != ctx->device || up->device != ctx->device || down->device != ctx->device)
+        return fail(err, RLQ_INVALID_ARGUMENT, gate->dtype);
+    uint32_t at;
+    const int32_t rc = activation_dtype(gate->dtype, &at, err);
+    if (rc) return rc;
+    if (gate->n3 != 1 || up->n3 != 1 || down->n3 != 1 || up->n2 != gate->n2 || down->n2 != gate->n2)
+        return fail(err, RLQ_TENSOR_SHAPE, gate->dtype, gate->n2, up->n2 != gate->n2 ? up->n2 : down->n2);
+    if (up->rows != gate->rows || up->cols != gate->cols) return fail(err, RLQ_TENSOR_SHAPE, up->dtype, up->rows, up->cols);
+    if (down->cols != gate->rows) return fail(err, RLQ_TENSOR_SHAPE, down->dtype, down->rows, down->cols);
+    if (slots == 0) return fail(err, RLQ_TENSOR_SHAPE, gate->dtype, slots, gate->n2);
+    if (up->dtype != gate->dtype) return fail(err, RLQ_TENSOR_UNSUPPORTED, up->dtype);
+    if (x_dtype != 0 && x_dtype != at) return fail(err, RLQ_TENSOR_UNSUPPORTED, x_dtype);
+    if (gate->n2 > kMoeMaxExperts) return fail(err, RLQ_UNIMPLEMENTED, gate->dtype, gate->n2, kMoeMaxExperts);
+    if (slots > kMoeMaxSlots) return fail(err, RLQ_UNIMPLEMENTED, gate->dtype, slots, kMoeMaxSlots);
+    if (tokens > 65535) return fail(err, RLQ_UNIMPLEMENTED, gate->dtype, tokens, 65535);  // the error keys' token field
+    if (tokens == 0) return ok(err);
+    if (!x || !ids || !weights || !y) return fail(err, RLQ_INVALID_ARGUMENT, gate->dtype);
+    if ((uintptr_t)x & (x_dtype == 0 ? 15 : x_dtype == kQ8_K ? 3 : 1)) return fail(err, RLQ_INVALID_ARGUMENT, gate->dtype);
+    if (((uintptr_t)ids | (uintptr_t)weights | (uintptr_t)residual | (uintptr_t)y) & 3)
+        return fail(err, RLQ_INVALID_ARGUMENT, gate->dtype);
+    MoeCall c{gate->dev, up->dev, down->dev, gate->mat_bytes, down->mat_bytes, gate->dtype, down->dtype, gate->n2,
+              gate->cols, gate->rows, down->rows, tokens, slots, x, x_dtype != 0, ids, weights, residual, y, ctx->err_words};
+    if (!moe_takes(c)) return fail(err, RLQ_UNIMPLEMENTED, gate->dtype, gate->rows, gate->cols);
+    DeviceGuard g(ctx->device);
+    const hipStream_t s = pick(ctx, stream);
+    HIP_TRY(ensure(ctx, ctx->moe, moe_bytes(c), s));
+    HIP_TRY(launch_moe_ffn(c, ctx->moe.p, s));
     return ok(err);
 }
 

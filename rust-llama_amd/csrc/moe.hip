@@ -1,0 +1,812 @@
+// moe.hip - a mixture-of-experts layer on gfx950: the router, and the experts'
+// products of a few tokens with what lies between them.
+//
+// Router (moe_route):  z = R x, scores = softmax(z) or sigmoid(z), the best
+// experts by z (or by score + bias) with their scores as weights.
+//
+// Experts (moe_ffn), for every token t and place s with expert e = ids[t][s] >= 0:
+//   g = G_e a_t,  u = U_e a_t            a_t: the token's Q8_K / Q8_0 blocks
+//   h = g / (1 + exp(-g)) * u            rounded to f32, then to blocks again
+//   y_t = residual_t + sum_s w_ts D_e h
+// The products are those of MUL_MAT_ID (crates/tensor/src/cpu_index.rs:169-236):
+// exact integers per block of 256 (or 32 for Q8_0), but added up in f64 and
+// rounded once, to g, u and y.  No order of the sums shows in those roundings
+// (but for one value in about 2^29 that lies next to a border), so the results do
+// not depend on how many tokens share a call or how K is split: h rounds to the
+// same levels in every one of them.
+#include "rlq_device.hpp"
+#include "rlq_igops.hpp"
+#include "rlq_internal.hpp"
+#include "rlq_layout.hpp"
+#include "rlq_q8k.hpp"
+
+namespace rlq {
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// ---------------------------------------------------------------------------
+// Router
+// ---------------------------------------------------------------------------
+
+// Four values of a row from element e on; past the end: 0.
+template <bool VEC>
+__device__ __forceinline__ float4 route_load(const float* p, uint32_t e, uint32_t n) {
+    if constexpr (VEC) return e < n ? *(const float4*)(p + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    return make_float4(e < n ? p[e] : 0.0f, e + 1 < n ? p[e + 1] : 0.0f, e + 2 < n ? p[e + 2] : 0.0f,
+                       e + 3 < n ? p[e + 3] : 0.0f);
+}
+
+// z of 16 tokens x 16 experts per workgroup on v_mfma_f64_16x16x4_f64, K split over
+// W waves in slices of 32 (lane l holds row l % 16, values 8 (l / 16) .. + 7 of
+// the slice), the waves' sums added in wave order.
+template <int W, bool VEC>
+__global__ __launch_bounds__(64 * W) void route_logits_kernel(RouteArgs a) {
+    __shared__ double part[W][4][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, kq = lane >> 4;
+    const uint32_t t0 = blockIdx.y * 16, e0 = blockIdx.x * 16, K = a.cols;
+    const float* x = a.x + (uint64_t)(t0 + i < a.tokens ? t0 + i : a.tokens - 1) * K;
+    const float* r = a.router + (uint64_t)(e0 + i < a.experts ? e0 + i : a.experts - 1) * K;
+    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+    for (uint32_t k = wave * 32; k < K; k += W * 32) {
+        const uint32_t e = k + 8 * kq;
+        const float4 x0 = route_load<VEC>(x, e, K), x1 = route_load<VEC>(x, e + 4, K);
+        const float4 r0 = route_load<VEC>(r, e, K), r1 = route_load<VEC>(r, e + 4, K);
+        const float xv[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+        const float rv[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)xv[j], (double)rv[j], acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v) part[wave][v][lane] = acc[v];
+    __syncthreads();
+    for (uint32_t o = threadIdx.x; o < 256; o += 64 * W) {
+        // value v of lane l: token 4 v + l / 16, expert l % 16
+        const uint32_t v = o >> 6, l = o & 63, t = t0 + 4 * v + (l >> 4), e = e0 + (l & 15);
+        double z = 0.0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) z += part[w][v][l];
+        if (t < a.tokens && e < a.experts) a.logits[(uint64_t)t * a.experts + e] = (float)z;
+    }
+}
+
+// The first of the best among the wave's lanes, each with its own candidate.
+struct RouteBest {
+    double rank;
+    uint32_t expert;
+};
+__device__ __forceinline__ RouteBest route_best(RouteBest b) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const double r = __shfl_xor(b.rank, m, 64);
+        const uint32_t e = (uint32_t)__shfl_xor((int)b.expert, m, 64);
+        if (r > b.rank || (r == b.rank && e < b.expert)) b = RouteBest{r, e};
+    }
+    return b;
+}
+
+// One wave per token; lane l holds experts l, l + 64, ... (NI of them).
+template <int NI>
+__global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs a) {
+    const uint32_t lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6), E = a.experts;
+    if (t >= a.tokens) return;
+    const float* z = a.logits + (uint64_t)t * E;
+    double score[NI], rank[NI];
+    double top = -INFINITY;
+    int bad = 0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const uint32_t e = lane + 64 * i;
+        const float v = e < E ? z[e] : 0.0f;
+        bad |= !finite(v);
+        score[i] = (double)v;
+        if (e < E) top = score[i] > top ? score[i] : top;
+    }
+    int32_t* ids = a.ids + (uint64_t)t * a.slots;
+    float* weights = a.weights + (uint64_t)t * a.slots;
+    if (__ballot(bad)) {
+        if (lane < a.slots) ids[lane] = -1, weights[lane] = 0.0f;
+        if (lane == 0) report_error(a.err_word, model_key(t, kStOOut, 0));
+        return;
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const double o = __shfl_xor(top, m, 64);
+        top = o > top ? o : top;
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const uint32_t e = lane + 64 * i;
+        rank[i] = score[i];
+        score[i] = a.sigmoid ? 1.0 / (1.0 + exp(-score[i])) : exp(score[i] - top);
+        if (e < E) sum += score[i];
+    }
+    if (!a.sigmoid) {
+        sum = wave_sum_f64(sum);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) score[i] = score[i] / sum;
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const uint32_t e = lane + 64 * i;
+        if (a.bias && e < E) rank[i] = score[i] + (double)a.bias[e];
+        if (e >= E || !(rank[i] > -INFINITY)) rank[i] = -INFINITY;  // (a bias of NaN: never chosen)
+    }
+    int32_t id = -1;  // of place `lane`
+    double weight = 0.0;
+    for (uint32_t s = 0; s < a.slots; ++s) {
+        RouteBest b{-INFINITY, ~0u};
+        double mine = 0.0;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            if (rank[i] > b.rank) b = RouteBest{rank[i], lane + 64 * i}, mine = score[i];
+        const uint32_t own = b.expert;
+        b = route_best(b);
+        if (b.expert == ~0u) break;  // no expert left for the places from s on
+        const double w = __shfl(mine, (int)(b.expert & 63), 64);
+        if (own == b.expert) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                if (lane + 64 * i == own) rank[i] = -INFINITY;
+        }
+        if (lane == s) id = (int32_t)b.expert, weight = w;
+    }
+    if (a.normalize) {
+        const double all = wave_sum_f64(weight);
+        weight = all > 0.0 ? weight / all : 0.0;
+    }
+    if (lane < a.slots) ids[lane] = id, weights[lane] = (float)(weight * (double)a.scale);
+}
+
+hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s) {
+    if (a.tokens == 0 || a.experts == 0 || a.cols == 0 || a.experts > kMoeMaxExperts || a.slots == 0 ||
+        a.slots > kMoeMaxSlots || a.slots > a.experts || a.tokens > 65535)
+        return hipErrorInvalidValue;
+    const bool vec = (((uintptr_t)a.x | (uintptr_t)a.router) & 15) == 0 && a.cols % 4 == 0;
+    const dim3 tiles((a.experts + 15) / 16, (a.tokens + 15) / 16);
+    if (vec) hipLaunchKernelGGL((route_logits_kernel<8, true>), tiles, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((route_logits_kernel<8, false>), tiles, dim3(512), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const dim3 grid((a.tokens + 3) / 4);
+    if (a.experts <= 64) hipLaunchKernelGGL((route_topk_kernel<1>), grid, dim3(256), 0, s, a);
+    else if (a.experts <= 256) hipLaunchKernelGGL((route_topk_kernel<4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((route_topk_kernel<16>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Experts: the plan and the activation images
+//
+// A pass takes up to 32 tokens.  Its plan lists the experts in use in ascending
+// order; expert j of them serves the tokens of mask[j], in columns cols[j][..]
+// ascending, whose h rows start at base[j].  A token that names an expert twice
+// is one column of it, with the sum of both weights.
+//
+// An image holds activations of T tokens in chunks of 256 values (of a Q8_0 row's
+// last chunk, a part; the rest is 0):
+//   q     [chunk][k-step 8][k half 2][token][16 int8]
+//   sums  [chunk][k half 2][token][8 f16]      (weights with mins)
+//   f     [chunk][token] f64, for Q8_0 [chunk][k-step][token]: the block's scale
+//         (of h: times the token's weight for the expert, 0 without one)
+// in the slot order of rlq_layout.hpp for Q4_K and Q5_K.  x has one image, h one
+// per expert in use, expert after expert, so that the down product runs over all
+// of them as over one long row.
+// ---------------------------------------------------------------------------
+
+// The first thing that is wrong with a token keeps its row of y as it was.
+__device__ __forceinline__ void moe_bad(const MoeArgs& a, uint32_t t, uint64_t key) {
+    report_error(a.err_word, key);
+    atomicOr(&a.bad[t], 1u);
+}
+
+__device__ __forceinline__ void moe_plan(const MoeArgs& a) {
+    __shared__ uint32_t mask[kMoeMaxExperts], wave_n[8], wave_b[8];
+    __shared__ uint16_t place[kMoeMaxExperts];
+    __shared__ int32_t ids[kMoeTokens * kMoeMaxSlots];
+    __shared__ float weights[kMoeTokens * kMoeMaxSlots];
+    const uint32_t tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = nt >> 6;
+    const uint32_t pairs = a.tokens * a.slots;
+    for (uint32_t e = tid; e < a.experts; e += nt) mask[e] = 0;
+    __syncthreads();
+    for (uint32_t p = tid; p < pairs; p += nt) {
+        int32_t id = a.ids[p];
+        const uint32_t t = p / a.slots;
+        if (id >= 0 && id < (int32_t)a.experts) {
+            atomicOr(&mask[id], 1u << t);
+        } else if (id != -1) {
+            moe_bad(a, t, bounds_key((uint64_t)a.token0 * a.slots + p));
+            id = -1;
+        }
+        ids[p] = id, weights[p] = a.weights[p];
+    }
+    __syncthreads();
+    uint32_t used = 0, rows = 0;
+    for (uint32_t e0 = 0; e0 < a.experts; e0 += nt) {
+        const uint32_t e = e0 + tid, m = e < a.experts ? mask[e] : 0, c = (uint32_t)__builtin_popcount(m);
+        // this expert's place among the used ones, and its first row
+        const unsigned long long some = __ballot(m != 0);
+        uint32_t before = c;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = (uint32_t)__shfl_up((int)before, d, 64);
+            if (lane >= (uint32_t)d) before += o;
+        }
+        if (lane == 63) wave_n[wave] = (uint32_t)__builtin_popcountll(some), wave_b[wave] = before;
+        __syncthreads();
+        uint32_t j = used + (uint32_t)__builtin_popcountll(some & ((1ull << lane) - 1)), b = rows + before - c;
+        for (uint32_t w = 0; w < waves; ++w) {
+            if (w < wave) j += wave_n[w], b += wave_b[w];
+            used += wave_n[w], rows += wave_b[w];
+        }
+        if (m) a.expert[j] = e, a.base[j] = b, a.mask[j] = m, place[e] = (uint16_t)j;
+        __syncthreads();
+    }
+    if (tid == 0) *a.n_used = used;
+    for (uint32_t p = tid; p < pairs; p += nt) {  // a token's first place with an expert speaks for all of them
+        const int32_t id = ids[p];
+        const uint32_t t = p / a.slots, end = (t + 1) * a.slots;
+        bool first = id >= 0;
+        for (uint32_t o = t * a.slots; o < p; ++o) first = first && ids[o] != id;
+        if (!first) continue;
+        double w = 0.0;
+        for (uint32_t o = p; o < end; ++o)
+            if (ids[o] == id) w += (double)weights[o];
+        const uint32_t j = place[id];
+        a.wsum[j * kMoeTokens + t] = w;
+        a.column[j * kMoeTokens + (uint32_t)__builtin_popcount(mask[id] & ((1u << t) - 1))] = (uint8_t)t;
+    }
+}
+
+// One lane's 16 values (r16 of a chunk's 16 lanes) of token t into an image.
+template <uint32_t T>
+__device__ __forceinline__ void image_put(const MoeImage& im, uint32_t tokens, uint64_t chunk, uint32_t r16, uint32_t t,
+                                          const uint32_t (&q)[4], int32_t bsum, double f) {
+    const uint4 w = ig_slots(T) ? q45_slots(q, r16 & 1) : make_uint4(q[0], q[1], q[2], q[3]);
+    *(uint4*)(im.q + ((chunk * 16 + r16) * tokens + t) * 16) = w;
+    if constexpr (ig_mins(T)) im.sums[((chunk * 2 + (r16 >> 3)) * tokens + t) * 8 + (r16 & 7)] = (_Float16)bsum;
+    if constexpr (T == kQ8_0) {
+        if (!(r16 & 1)) im.f[(chunk * 8 + (r16 >> 1)) * tokens + t] = f;
+    } else {
+        if (r16 == 0) im.f[chunk * tokens + t] = f;
+    }
+}
+
+// Quantizes one lane's 16 values for weights of type T; returns the kind of the
+// block's data error, or -1.
+template <uint32_t T>
+__device__ __forceinline__ int image_quantize(const float (&v)[16], uint32_t r16, uint32_t (&q)[4], float& d, int32_t& bsum,
+                                              uint32_t& index) {
+    if constexpr (T == kQ8_0) {
+        bsum = 0;
+        return q8_0_pair16(v, r16 & 1, q, d, index);
+    } else {
+        const Q8KRow o = q8k_row16(v, r16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = o.q[k];
+        d = o.d, bsum = o.bsum, index = o.index;
+        return o.kind;
+    }
+}
+
+// Workgroup 0: the plan.  The others: one chunk of x each, 16 lanes per token, from
+// f32 rows or from packed blocks (taken as given; the 16-value sums are those of
+// the levels).  flags[chunk][token]: a data error in the token's chunk.
+template <uint32_t T, bool PACKED>
+__global__ __launch_bounds__(512) void moe_prepare_kernel(MoeArgs a) {
+    if (blockIdx.x == 0) {
+        if (threadIdx.x < kMoeTokens) a.bad[threadIdx.x] = 0;
+        __syncthreads();
+        moe_plan(a);
+        return;
+    }
+    const uint32_t c = blockIdx.x - 1, r16 = threadIdx.x & 15, t = threadIdx.x >> 4, K = a.cols, e0 = c * 256 + r16 * 16;
+    if (t >= a.tokens) return;
+    uint32_t q[4] = {0, 0, 0, 0};
+    float d = 0.0f;
+    int32_t bsum = 0;
+    int kind = -1;
+    if constexpr (PACKED) {
+        if (e0 < K) {
+            if constexpr (T == kQ8_0) {
+                const uint16_t* b = (const uint16_t*)((const uint8_t*)a.x + ((uint64_t)t * (K / 32) + e0 / 32) * 34);
+                d = half_bits_to_float_exact(b[0]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    q[k] = (uint32_t)b[1 + 8 * (r16 & 1) + 2 * k] | (uint32_t)b[2 + 8 * (r16 & 1) + 2 * k] << 16;
+            } else {
+                const uint32_t* b = (const uint32_t*)((const uint8_t*)a.x + ((uint64_t)t * (K / 256) + c) * 292);
+                d = __uint_as_float(b[0]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) q[k] = b[1 + 4 * r16 + k];
+                for (int k = 0; k < 4; ++k) bsum = dot4(q[k], 0x01010101u, bsum);
+            }
+        }
+    } else {
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = 0.0f;
+        if (e0 < K) {
+            const float4* src = (const float4*)((const float*)a.x + (uint64_t)t * K + e0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float4 f = src[k];
+                v[4 * k] = f.x, v[4 * k + 1] = f.y, v[4 * k + 2] = f.z, v[4 * k + 3] = f.w;
+            }
+        }
+        uint32_t index;
+        kind = image_quantize<T>(v, r16, q, d, bsum, index);
+        if (kind >= 0) {
+            const uint64_t block = T == kQ8_0 ? e0 / 32 : c, first = T == kQ8_0 ? e0 / 32 * 32ull : c * 256ull;
+            if (T == kQ8_0 ? !(r16 & 1) : r16 == 0)
+                report_error(a.err_word, kind == kKindNonFinite ? error_key(a.token0 + t, kKindNonFinite, first + index)
+                                                                : error_key(a.token0 + t, kKindScale, block));
+        }
+    }
+    image_put<T>(a.xi, a.tokens, c, r16, t, q, bsum, (double)d);
+    const unsigned long long m = __ballot(kind >= 0) >> (threadIdx.x & 48) & 0xffffull;
+    if (r16 == 0) a.flags[c * a.tokens + t] = m != 0;
+}
+
+// h of expert j's tokens, one chunk, for the down matrices' type.
+template <uint32_t T>
+__global__ __launch_bounds__(512) void moe_h_kernel(MoeArgs a) {
+    const uint32_t c = blockIdx.x, j = blockIdx.y, r16 = threadIdx.x & 15, t = threadIdx.x >> 4;
+    if (j >= *a.n_used || t >= a.tokens) return;
+    const uint32_t mask = a.mask[j], e0 = c * 256 + r16 * 16;
+    const bool mine = (mask >> t) & 1u;
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = 0.0f;
+    if (mine && e0 < a.ffn) {
+        const uint32_t row = a.base[j] + (uint32_t)__builtin_popcount(mask & ((1u << t) - 1));
+        const float4* src = (const float4*)(a.h + (uint64_t)row * a.ffn + e0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float4 f = src[k];
+            v[4 * k] = f.x, v[4 * k + 1] = f.y, v[4 * k + 2] = f.z, v[4 * k + 3] = f.w;
+        }
+    }
+    uint32_t q[4], index;
+    float d;
+    int32_t bsum;
+    const int kind = image_quantize<T>(v, r16, q, d, bsum, index);
+    if (kind == kKindScale && (T == kQ8_0 ? !(r16 & 1) : r16 == 0))  // (a non-finite h was reported where it was made)
+        moe_bad(a, t, model_key(a.token0 + t, kStDownQuant, T == kQ8_0 ? e0 / 32 : c));
+    image_put<T>(a.hi, a.tokens, (uint64_t)j * gridDim.x + c, r16, t, q, bsum, mine ? a.wsum[j * kMoeTokens + t] * (double)d : 0.0);
+}
+
+// ---------------------------------------------------------------------------
+// The products
+//
+// A wave multiplies 32 weight rows with up to 32 columns, a chunk of 256 values
+// at a time: the weights and the activations come straight into registers, one
+// chunk ahead (Ig<T>::refill), and the integers A (and B, Mn) of the chunk are
+// folded into f64 sums.  Lane (ln, kh): row ln of the 32 as weights, column ln as
+// activations, and of the products row ln, columns 8 (i / 4) + 4 kh + i % 4.
+// The two 16-row halves hf = ln / 16 of the 32 rows are
+//   up    the gate and the up tile of the same 16 rows, the columns an expert's
+//         tokens: the two factors of an h lie 16 lanes apart;
+//   down  the same 16-row tile at two different chunks, whose activations are
+//         columns 0..15 and 16..31: a row's products are those of its own half.
+// ---------------------------------------------------------------------------
+template <uint32_t T>
+struct MoeWeights {
+    static constexpr uint32_t kChunk = Ig<T>::kChunk;
+    static constexpr int kFactors = 1;
+    typename Ig<T>::Raw r;
+};
+template <>
+struct MoeWeights<kQ8_0> {
+    static constexpr uint32_t kChunk = 4 * kQ80Chunk;
+    static constexpr int kFactors = 8;
+    uint4 q[8];
+    uint32_t d[4];
+};
+
+// A workgroup's LDS: its waves' f64 sums, and each wave's column scales of its
+// current chunk.
+template <uint32_t T>
+constexpr uint32_t moe_lds(uint32_t ks, uint32_t sums, uint32_t groups) {
+    return ks * (sums * 512 + groups * MoeWeights<T>::kFactors * 256);
+}
+
+// Where a lane's rows have their current chunk, which one of the image it is, and
+// whether it counts (the last pair of chunks may have one only).  pairs: Q8_0
+// block pairs of the chunk (reading stops there; the image is 0 beyond).
+struct MoeAt {
+    const uint8_t* w;
+    uint32_t chunk, pairs;
+    bool live;
+};
+
+// One wave's chunks.  at(it): where step it is.  fold(g, f, term): adds a chunk's
+// (Q8_0: a block's) products of column group g, term(i, fa, y) being y plus fa
+// times product i of the lane's row; f: the group's 32 column scales.  HALVES:
+// rows of the second half take the columns from 16 on.
+template <uint32_t T, int NG, bool HALVES, typename At, typename Fold>
+__device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, const uint32_t (&tok)[NG], uint32_t steps,
+                                         uint32_t ln, uint32_t kh, double* fd, At&& at, Fold&& fold) {
+    using M = MoeWeights<T>;
+    if (steps == 0) return;
+    const uint32_t n = ln & 15;
+    const bool upper = HALVES && ln >= 16;
+    M m;
+    i32x4 act[NG][4];
+    f16x8 bs[NG];
+    double f[NG][M::kFactors];
+    const uint64_t sq = (uint64_t)tokens * 16;  // bytes of one k half
+    auto load_act = [&](int s, uint32_t c) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+            act[g][s % 4] = *(const i32x4*)(im.q + ((uint64_t)c * 16 + s * 2 + kh) * sq + tok[g] * 16);
+    };
+    auto load_scales = [&](const MoeAt& p) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+#pragma unroll
+            for (int k = 0; k < M::kFactors; ++k) {
+                const double v = im.f[((uint64_t)p.chunk * M::kFactors + k) * tokens + tok[g]];
+                f[g][k] = p.live ? v : 0.0;
+            }
+            if constexpr (ig_mins(T)) bs[g] = *(const f16x8*)(im.sums + (((uint64_t)p.chunk * 2 + kh) * tokens + tok[g]) * 8);
+        }
+    };
+    auto pair_of = [&](const MoeAt& p, uint32_t k) { return p.w + (k < p.pairs ? k : p.pairs - 1) * kQ80Chunk; };
+    auto load_q8 = [&](const MoeAt& p, int s) {
+        if constexpr (T == kQ8_0) m.q[s] = ig_ld16(pair_of(p, s / 2) + (16 * (2 * (s & 1) + kh) + n) * 16);
+    };
+    auto load_d8 = [&](const MoeAt& p) {
+        if constexpr (T == kQ8_0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m.d[k] = *(const uint32_t*)(pair_of(p, k) + 1024 + n * 4);
+        }
+    };
+    MoeAt p = at(0);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) load_act(s, p.chunk);
+    load_scales(p);
+    if constexpr (T == kQ8_0) {
+#pragma unroll
+        for (int s = 0; s < 8; ++s) load_q8(p, s);
+        load_d8(p);
+    } else {
+        ig_load<T>(m.r, p.w, n, kh);
+    }
+    // one step; more: the next step's loads follow the last use of what they replace
+    auto step = [&](auto more_, uint32_t it) {
+        constexpr bool more = decltype(more_)::value;
+        MoeAt nx = p;
+        if (more) nx = at(it + 1);
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+            if (kh == 0) {
+#pragma unroll
+                for (int k = 0; k < M::kFactors; ++k) fd[(g * M::kFactors + k) * 32 + ln] = f[g][k];
+            }
+        if constexpr (T == kQ8_0) {
+            uint32_t dw4[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) dw4[k] = m.d[k];
+            if (more) load_d8(nx), load_scales(nx);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const i32x4 w = __builtin_bit_cast(i32x4, m.q[s]);
+                const double dw = (double)half_to_float((s & 1) ? dw4[s / 2] >> 16 : dw4[s / 2]);
+                i32x16 I[NG];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) I[g] = ig_mfma(act[g][s % 4], w, (i32x16){});
+                if (more) load_q8(nx, s);
+                if (s < 4) load_act(s + 4, p.chunk);
+                else if (more) load_act(s - 4, nx.chunk);
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+                    fold(g, fd + (g * M::kFactors + s) * 32, [&](int i, double fa, double y) {
+                        const int32_t v = upper ? I[g][i + 8 * HALVES] : I[g][i];
+                        return __builtin_fma((double)v, fa * dw, y);  // (fa * dw is exact: 22 bits, of h with its weight rounded)
+                    });
+            }
+        } else {
+            using W = Ig<T>;
+            const typename W::Pre pre = W::pre(m.r, kh);
+            const double d = (double)W::d(m.r);
+            double dmin = 0.0;
+            f16x8 mins = {};
+            if constexpr (ig_mins(T)) dmin = (double)W::dmin(m.r), mins = W::mins(m.r, kh);
+            if (more) W::head(m.r, nx.w, n);
+            i32x16 A[NG], B[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) A[g] = (i32x16){}, B[g] = (i32x16){};
+            ig_steps([&](auto s_) {
+                constexpr int S = decltype(s_)::value;
+                i32x4 wa, wb;
+                W::template ops<S>(m.r, pre, wa, wb);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    A[g] = ig_mfma(act[g][S % 4], wa, A[g]);
+                    if (W::kPlanes == 2) B[g] = ig_mfma(act[g][S % 4], wb, B[g]);
+                }
+                if (more) W::template refill<S>(m.r, nx.w, n, kh);
+                if (S < 4) load_act(S + 4, p.chunk);
+                else if (more) load_act(S - 4, nx.chunk);
+            });
+            f32x16 mn[NG];
+            if constexpr (ig_mins(T)) {
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+                    mn[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bs[g], mins, (f32x16){}, 0, 0, 0);
+            }
+            if (more) load_scales(nx);
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                fold(g, fd + g * 32, [&](int i, double fa, double y) {
+                    const int k = i + 8 * HALVES;
+                    const int32_t a = upper ? A[g][k] : A[g][i];
+                    int32_t I = a;
+                    if (W::kPlanes == 2) I = (int32_t)(((uint32_t)a << W::kShift) + (uint32_t)(upper ? B[g][k] : B[g][i]));
+                    double v = d * (double)I;  // exact: 11 and 31 bits
+                    if constexpr (ig_mins(T)) v = __builtin_fma(-dmin, (double)(upper ? mn[g][k] : mn[g][i]), v);
+                    return __builtin_fma(fa, v, y);
+                });
+        }
+        p = nx;
+    };
+    for (uint32_t it = 0; it + 1 < steps; ++it) step(std::true_type{}, it);
+    step(std::false_type{}, steps - 1);
+}
+
+// Q8_0 block pairs of chunk c of a row with npairs of them (other types: unused).
+__device__ __forceinline__ uint32_t moe_pairs(uint32_t npairs, uint32_t c) {
+    const uint32_t left = npairs - 4 * c;
+    return left < 4 ? left : 4;
+}
+
+// h of 16 rows for expert j's tokens: wave kg takes every KS-th chunk of K.  NQ:
+// groups of eight columns that the tokens of the pass can need.
+template <uint32_t T, int KS, int NQ>
+__global__ __launch_bounds__(64 * KS) void moe_up_kernel(MoeArgs a) {
+    extern __shared__ __align__(16) double lds[];
+    const uint32_t lane = threadIdx.x & 63, kg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t ln = lane & 31, kh = lane >> 5;
+    const uint32_t j = blockIdx.x / a.up_tiles, tile = blockIdx.x - j * a.up_tiles;
+    if (blockIdx.x == 0)  // the prepare launch's flags, for the down kernel
+        for (uint32_t i = threadIdx.x; i < a.x_chunks * a.tokens; i += 64 * KS)
+            if (a.flags[i]) atomicOr(&a.bad[i % a.tokens], 1u);
+    if (j >= *a.n_used) return;
+    const uint32_t live = (uint32_t)__builtin_popcount(a.mask[j]), nchunk = a.x_chunks;
+    const uint32_t tok[1] = {a.column[j * kMoeTokens + (ln < live ? ln : 0)]};
+    const uint8_t* wt = ((ln >> 4) ? a.up : a.gate) + (uint64_t)a.expert[j] * a.up_bytes + (uint64_t)tile * a.x_row_bytes;
+    double* part = lds;
+    double* fd = lds + KS * NQ * 4 * 64 + kg * (MoeWeights<T>::kFactors * 32);
+    double y[NQ * 4];
+#pragma unroll
+    for (int i = 0; i < NQ * 4; ++i) y[i] = 0.0;
+    const uint32_t steps = kg < nchunk ? (nchunk - 1 - kg) / KS + 1 : 0;
+    moe_walk<T, 1, false>(
+        a.xi, a.tokens, tok, steps, ln, kh, fd,
+        [&](uint32_t it) {
+            const uint32_t c = kg + it * KS;
+            return MoeAt{wt + (uint64_t)c * MoeWeights<T>::kChunk, c, moe_pairs(a.x_pairs, c), true};
+        },
+        [&](int, const double* f, auto&& term) {
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+                if ((uint32_t)(8 * q) < live) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[4 * q + k] = term(4 * q + k, f[8 * q + 4 * kh + k], y[4 * q + k]);
+                }
+        });
+#pragma unroll
+    for (int i = 0; i < NQ * 4; ++i) part[(kg * NQ * 4 + i) * 64 + lane] = y[i];
+    __syncthreads();
+    for (uint32_t o = threadIdx.x; o < live * 16; o += 64 * KS) {
+        const uint32_t c = o >> 4, r = o & 15, i = 4 * (c >> 3) + (c & 3), l = ((c >> 2) & 1) * 32 + r;
+        double g = 0.0, u = 0.0;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            g += part[(k * NQ * 4 + i) * 64 + l];
+            u += part[(k * NQ * 4 + i) * 64 + l + 16];
+        }
+        const double gf = (double)(float)g, uf = (double)(float)u;
+        const float h = (float)(gf / (1.0 + exp(-gf)) * uf);
+        if (!finite(h)) {
+            const uint32_t t = a.column[j * kMoeTokens + c];
+            moe_bad(a, t, model_key(a.token0 + t, kStDownIn, 0));
+        }
+        a.h[(uint64_t)(a.base[j] + c) * a.ffn + tile * 16 + r] = h;
+    }
+}
+
+// y of 16 rows for every token: wave kg takes every KS-th pair of chunks of all
+// experts' h, one for each half of its rows.  NG groups of 16 tokens, NQ of eight
+// inside each.
+template <uint32_t T, int KS, int NG, int NQ>
+__global__ __launch_bounds__(64 * KS) void moe_down_kernel(MoeArgs a) {
+    extern __shared__ __align__(16) double lds[];
+    __shared__ uint16_t expert[kMoeMaxExperts];
+    const uint32_t lane = threadIdx.x & 63, kg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t ln = lane & 31, kh = lane >> 5, hf = ln >> 4;
+    const uint32_t tile = blockIdx.x, nchunk = a.h_chunks, used = *a.n_used, total = used * nchunk;
+    for (uint32_t i = threadIdx.x; i < used; i += 64 * KS) expert[i] = (uint16_t)a.expert[i];
+    __syncthreads();
+    uint32_t tok[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) tok[g] = 16 * g + (ln & 15) < a.tokens ? 16 * g + (ln & 15) : a.tokens - 1;
+    double* part = lds;
+    constexpr int kSums = NG * NQ * 4;
+    double* fd = lds + KS * kSums * 64 + kg * (NG * MoeWeights<T>::kFactors * 32);
+    double y[kSums];
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) y[i] = 0.0;
+    const uint32_t steps = 2 * kg < total ? (total - 1 - 2 * kg) / (2 * KS) + 1 : 0;
+    moe_walk<T, NG, true>(
+        a.hi, a.tokens, tok, steps, ln, kh, fd,
+        [&](uint32_t it) {
+            const uint32_t want = 2 * (kg + it * KS) + hf, at = want < total ? want : total - 1;
+            const uint32_t j = at / nchunk, c = at - j * nchunk;
+            const uint8_t* w = a.down + (uint64_t)expert[j] * a.down_bytes + (uint64_t)tile * a.h_row_bytes;
+            return MoeAt{w + (uint64_t)c * MoeWeights<T>::kChunk, at, moe_pairs(a.h_pairs, c), want < total};
+        },
+        [&](int g, const double* f, auto&& term) {
+#pragma unroll
+            for (int i = 0; i < NQ * 4; ++i) {
+                double& s = y[g * NQ * 4 + i];
+                s = term(i, f[16 * hf + 8 * (i / 4) + 4 * kh + i % 4], s);
+            }
+        });
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) part[(kg * kSums + i) * 64 + lane] = y[i];
+    __syncthreads();
+    for (uint32_t o = threadIdx.x; o < a.tokens * 16; o += 64 * KS) {
+        const uint32_t t = o >> 4, r = o & 15, t16 = t & 15, row = tile * 16 + r;
+        if (row >= a.out_rows || a.bad[t]) continue;
+        const uint32_t i = (t >> 4) * NQ * 4 + 4 * (t16 >> 3) + (t16 & 3), l = ((t16 >> 2) & 1) * 32 + r;
+        const uint64_t to = (uint64_t)t * a.out_rows + row;
+        double v = a.residual ? (double)a.residual[to] : 0.0;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) v += part[(k * kSums + i) * 64 + l] + part[(k * kSums + i) * 64 + l + 16];
+        a.y[to] = (float)v;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Launch
+// ---------------------------------------------------------------------------
+static uint64_t moe_align(uint64_t v) { return (v + 255) & ~255ull; }
+static uint64_t moe_chunks(uint64_t cols) { return (cols + 255) / 256; }
+
+// The scratch of a pass; base null: only its size.
+static size_t moe_carve(const MoeCall& c, uint32_t tokens, uint8_t* base, MoeArgs* a) {
+    uint64_t at = 0;
+    auto take = [&](uint64_t bytes) {
+        uint8_t* p = base + at;
+        at += moe_align(bytes);
+        return p;
+    };
+    auto image = [&](uint32_t t, uint64_t chunks) {
+        MoeImage im;
+        im.q = take(chunks * tokens * 256);
+        im.sums = (_Float16*)take(ig_mins(t) ? chunks * tokens * 32 : 0);
+        im.f = (double*)take(chunks * tokens * (t == kQ8_0 ? 64 : 8));
+        return im;
+    };
+    const uint64_t pairs = (uint64_t)tokens * c.slots, used = pairs < c.experts ? pairs : c.experts;
+    MoeArgs m{};
+    m.n_used = (uint32_t*)take(4);
+    m.bad = (uint32_t*)take(kMoeTokens * 4);
+    m.expert = (uint32_t*)take(used * 4);
+    m.base = (uint32_t*)take(used * 4);
+    m.mask = (uint32_t*)take(used * 4);
+    m.column = take(used * kMoeTokens);
+    m.wsum = (double*)take(used * kMoeTokens * 8);
+    m.flags = (uint32_t*)take(moe_chunks(c.cols) * tokens * 4);
+    m.xi = image(c.up_type, moe_chunks(c.cols));
+    m.h = (float*)take(pairs * c.ffn * 4);
+    m.hi = image(c.down_type, used * moe_chunks(c.ffn));
+    if (a) *a = m;
+    return at;
+}
+
+size_t moe_bytes(const MoeCall& c) {
+    return moe_carve(c, c.tokens < kMoeTokens ? (uint32_t)c.tokens : kMoeTokens, nullptr, nullptr);
+}
+
+// Whether every launch of the call stays below 2^32 threads and its chunks below
+// 2^31.
+bool moe_takes(const MoeCall& c) {
+    const uint64_t t = c.tokens < kMoeTokens ? c.tokens : kMoeTokens;
+    const uint64_t used = t * c.slots < c.experts ? t * c.slots : c.experts;
+    return c.experts <= kMoeMaxExperts && c.slots <= kMoeMaxSlots && c.tokens <= 65535 && c.cols <= (1u << 30) &&
+           c.ffn <= (1u << 30) && used * layout_tiles(c.ffn) * 1024 <= 0xffffffffull &&
+           layout_tiles(c.out_rows) * 1024 <= 0xffffffffull && used * moe_chunks(c.ffn) * 512 <= 0xffffffffull &&
+           (moe_chunks(c.cols) + 1) * 512 <= 0xffffffffull;
+}
+
+template <uint32_t T, int KS, int NQ>
+static hipError_t moe_up_launch(const MoeArgs& a, uint32_t used, hipStream_t s) {
+    static LdsLimit lim;
+    constexpr uint32_t lds = moe_lds<T>(KS, NQ * 4, 1);
+    const hipError_t e = lim.raise((const void*)moe_up_kernel<T, KS, NQ>, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((moe_up_kernel<T, KS, NQ>), dim3(used * a.up_tiles), dim3(64 * KS), lds, s, a);
+    return hipGetLastError();
+}
+template <uint32_t T, int KS, int NG, int NQ>
+static hipError_t moe_down_launch(const MoeArgs& a, hipStream_t s) {
+    static LdsLimit lim;
+    constexpr uint32_t lds = moe_lds<T>(KS, NG * NQ * 4, NG);
+    const hipError_t e = lim.raise((const void*)moe_down_kernel<T, KS, NG, NQ>, lds + 2 * kMoeMaxExperts);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((moe_down_kernel<T, KS, NG, NQ>), dim3((a.out_rows + 15) / 16), dim3(64 * KS), lds, s, a);
+    return hipGetLastError();
+}
+
+template <uint32_t T>
+static hipError_t moe_up_any(const MoeArgs& a, bool packed, uint32_t used, hipStream_t s) {
+    const dim3 grid(1 + a.x_chunks);
+    if (packed) hipLaunchKernelGGL((moe_prepare_kernel<T, true>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((moe_prepare_kernel<T, false>), grid, dim3(512), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (a.tokens <= 8) return moe_up_launch<T, 8, 1>(a, used, s);
+    if (a.tokens <= 16) return moe_up_launch<T, 4, 2>(a, used, s);
+    return moe_up_launch<T, 4, 4>(a, used, s);
+}
+template <uint32_t T>
+static hipError_t moe_down_any(const MoeArgs& a, uint32_t used, hipStream_t s) {
+    hipLaunchKernelGGL((moe_h_kernel<T>), dim3(a.h_chunks, used), dim3((a.tokens * 16 + 63) / 64 * 64), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (a.tokens <= 8) return moe_down_launch<T, 16, 1, 1>(a, s);
+    if (a.tokens <= 16) return moe_down_launch<T, 8, 1, 2>(a, s);
+    return moe_down_launch<T, 8, 2, 2>(a, s);
+}
+
+hipError_t launch_moe_ffn(const MoeCall& c, void* scratch, hipStream_t s) {
+    if (c.tokens == 0 || c.slots == 0 || c.experts == 0 || !moe_takes(c)) return hipErrorInvalidValue;
+    uint64_t row_bytes = c.cols * 4;  // of x
+    if (c.packed) row_bytes = c.up_type == kQ8_0 ? c.cols / 32 * 34 : c.cols / 256 * 292;
+    for (uint64_t t0 = 0; t0 < c.tokens; t0 += kMoeTokens) {
+        const uint32_t n = c.tokens - t0 < kMoeTokens ? (uint32_t)(c.tokens - t0) : kMoeTokens;
+        MoeArgs a{};
+        moe_carve(c, n, (uint8_t*)scratch, &a);
+        a.tokens = n, a.token0 = (uint32_t)t0, a.slots = (uint32_t)c.slots, a.experts = (uint32_t)c.experts;
+        a.cols = (uint32_t)c.cols, a.ffn = (uint32_t)c.ffn, a.out_rows = (uint32_t)c.out_rows;
+        a.x = (const uint8_t*)c.x + t0 * row_bytes;
+        a.ids = c.ids + t0 * c.slots, a.weights = c.weights + t0 * c.slots;
+        a.residual = c.residual ? c.residual + t0 * c.out_rows : nullptr;
+        a.y = c.y + t0 * c.out_rows;
+        a.gate = c.gate, a.up = c.up, a.down = c.down, a.up_bytes = c.up_bytes, a.down_bytes = c.down_bytes;
+        a.up_tiles = (uint32_t)layout_tiles(c.ffn);
+        a.x_chunks = (uint32_t)moe_chunks(c.cols), a.h_chunks = (uint32_t)moe_chunks(c.ffn);
+        a.x_pairs = (uint32_t)((c.cols / 32 + 1) / 2), a.h_pairs = (uint32_t)((c.ffn / 32 + 1) / 2);
+        a.x_row_bytes = layout_chunks_per_tile(c.up_type, c.cols) * layout_chunk_bytes(c.up_type);
+        a.h_row_bytes = layout_chunks_per_tile(c.down_type, c.ffn) * layout_chunk_bytes(c.down_type);
+        a.err_word = c.err_word;
+        const uint64_t pairs = (uint64_t)n * c.slots;
+        const uint32_t used = (uint32_t)(pairs < c.experts ? pairs : c.experts);
+        hipError_t e = hipErrorInvalidValue;
+        switch (c.up_type) {
+            case kQ8_0: e = moe_up_any<kQ8_0>(a, c.packed, used, s); break;
+            case kQ2_K: e = moe_up_any<kQ2_K>(a, c.packed, used, s); break;
+            case kQ3_K: e = moe_up_any<kQ3_K>(a, c.packed, used, s); break;
+            case kQ4_K: e = moe_up_any<kQ4_K>(a, c.packed, used, s); break;
+            case kQ5_K: e = moe_up_any<kQ5_K>(a, c.packed, used, s); break;
+            case kQ6_K: e = moe_up_any<kQ6_K>(a, c.packed, used, s); break;
+        }
+        if (e != hipSuccess) return e;
+        switch (c.down_type) {
+            case kQ8_0: e = moe_down_any<kQ8_0>(a, used, s); break;
+            case kQ2_K: e = moe_down_any<kQ2_K>(a, used, s); break;
+            case kQ3_K: e = moe_down_any<kQ3_K>(a, used, s); break;
+            case kQ4_K: e = moe_down_any<kQ4_K>(a, used, s); break;
+            case kQ5_K: e = moe_down_any<kQ5_K>(a, used, s); break;
+            case kQ6_K: e = moe_down_any<kQ6_K>(a, used, s); break;
+            default: e = hipErrorInvalidValue;
+        }
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+}  // namespace rlq

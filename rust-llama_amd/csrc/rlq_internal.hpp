@@ -179,6 +179,76 @@ hipError_t launch_igemm_ids(uint32_t t, const uint8_t* w, uint64_t rows, uint64_
                             bool packed, const IgRoute& r, float* y, uint64_t ldy, void* scratch,
                             unsigned long long* err_word, hipStream_t s);
 
+// ---- norm.hip ----
+// Rows t = x + residual (may be null), y = RMSNorm(t) * weight, and y's blocks of
+// q_type (kQ8_K, kQ8_0, or 0: none); total, y may be null.  A data error of a row
+// (model keys with the row as the layer) leaves that row's outputs as they were.
+constexpr uint32_t kNormMaxCols = 32768;
+struct NormArgs {
+    const float *x, *residual, *weight;
+    uint32_t rows, cols;
+    float eps;
+    float *total, *y;
+    uint32_t q_type;
+    uint8_t* q;
+    unsigned long long* err_word;
+};
+hipError_t launch_rms_norm(const NormArgs& a, hipStream_t s);
+
+// ---- moe.hip ----
+constexpr uint32_t kMoeMaxExperts = 1024, kMoeMaxSlots = 64;
+constexpr uint32_t kMoeTokens = 32;  // of one pass over the experts
+// logits[t][e] = router row e . x row t, then every token's best `slots` experts
+// and their weights; bias (may be null) is added to the scores for the choice.
+struct RouteArgs {
+    const float *router, *x, *bias;
+    uint32_t tokens, experts, cols, slots, sigmoid, normalize;
+    float scale;
+    float* logits;
+    int32_t* ids;
+    float* weights;
+    unsigned long long* err_word;
+};
+hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s);
+// The experts' products of `tokens` tokens; scratch: moe_bytes.
+struct MoeCall {
+    const uint8_t *gate, *up, *down;   // tiled stacks of `experts` matrices
+    uint64_t up_bytes, down_bytes;     // of one matrix
+    uint32_t up_type, down_type;
+    uint64_t experts, cols, ffn, out_rows, tokens, slots;
+    const void* x;  // f32 rows, or (packed) rows of activation blocks
+    bool packed;
+    const int32_t* ids;
+    const float *weights, *residual;
+    float* y;
+    unsigned long long* err_word;
+};
+bool moe_takes(const MoeCall& c);
+size_t moe_bytes(const MoeCall& c);
+hipError_t launch_moe_ffn(const MoeCall& c, void* scratch, hipStream_t s);
+struct MoeImage {
+    uint8_t* q;
+    _Float16* sums;
+    double* f;
+};
+struct MoeArgs {  // of one pass
+    const uint8_t *gate, *up, *down;
+    uint64_t up_bytes, down_bytes, x_row_bytes, h_row_bytes;  // a matrix; a 16-row tile
+    uint32_t tokens, token0, slots, experts, cols, ffn, out_rows;
+    uint32_t up_tiles, x_chunks, h_chunks, x_pairs, h_pairs;
+    const void* x;
+    const int32_t* ids;
+    const float *weights, *residual;
+    float* y;
+    unsigned long long* err_word;
+    // the plan and the workspace (moe.hip)
+    uint32_t *n_used, *bad, *expert, *base, *mask, *flags;
+    uint8_t* column;
+    double* wsum;
+    MoeImage xi, hi;
+    float* h;
+};
+
 // ---- llama.hip ----
 // The dense Llama decode step (crates/model-runtime/src/llama.rs:222-392)
 // over resident weights.  Dimensions are validated by the caller.
