@@ -420,6 +420,11 @@ struct MoeAt {
     bool live;
 };
 
+// b where mask is all ones, a where it is 0.  (A plain choice between two elements of
+// a product becomes one element at a variable place, which costs a compare and a
+// move for each of the sixteen.)
+__device__ __forceinline__ uint32_t bits_or(uint32_t mask, uint32_t a, uint32_t b) { return (mask & b) | (~mask & a); }
+
 // One wave's chunks.  at(it): where step it is.  fold(g, f, term): adds a chunk's
 // (Q8_0: a block's) products of column group g, term(i, fa, y) being y plus fa
 // times product i of the lane's row; f: the group's 32 column scales.  HALVES:
@@ -430,7 +435,7 @@ __device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, co
     using M = MoeWeights<T>;
     if (steps == 0) return;
     const uint32_t n = ln & 15;
-    const bool upper = HALVES && ln >= 16;
+    const uint32_t upper = HALVES && ln >= 16 ? ~0u : 0u;
     M m;
     i32x4 act[NG][4];
     f16x8 bs[NG];
@@ -502,8 +507,8 @@ __device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, co
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
                     fold(g, fd + (g * M::kFactors + s) * 32, [&](int i, double fa, double y) {
-                        const int32_t v = upper ? I[g][i + 8 * HALVES] : I[g][i];
-                        return __builtin_fma((double)v, fa * dw, y);  // (fa * dw is exact: 22 bits, of h with its weight rounded)
+                        const int32_t v = HALVES ? (int32_t)bits_or(upper, I[g][i], I[g][i + 8 * HALVES]) : I[g][i];
+                        return __builtin_fma((double)v, fa * dw, y);
                     });
             }
         } else {
@@ -540,12 +545,18 @@ __device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, co
 #pragma unroll
             for (int g = 0; g < NG; ++g)
                 fold(g, fd + g * 32, [&](int i, double fa, double y) {
-                    const int k = i + 8 * HALVES;
-                    const int32_t a = upper ? A[g][k] : A[g][i];
-                    int32_t I = a;
-                    if (W::kPlanes == 2) I = (int32_t)(((uint32_t)a << W::kShift) + (uint32_t)(upper ? B[g][k] : B[g][i]));
-                    double v = d * (double)I;  // exact: 11 and 31 bits
-                    if constexpr (ig_mins(T)) v = __builtin_fma(-dmin, (double)(upper ? mn[g][k] : mn[g][i]), v);
+                    auto block = [&](int k) {
+                        return W::kPlanes == 2 ? ((uint32_t)A[g][k] << W::kShift) + (uint32_t)B[g][k] : (uint32_t)A[g][k];
+                    };
+                    uint32_t I = block(i);
+                    if constexpr (HALVES) I = bits_or(upper, I, block(i + 8));
+                    double v = d * (double)(int32_t)I;  // exact: 11 and 31 bits
+                    if constexpr (ig_mins(T)) {
+                        float m = mn[g][i];
+                        if constexpr (HALVES)
+                            m = __uint_as_float(bits_or(upper, __float_as_uint(m), __float_as_uint(mn[g][i + 8])));
+                        v = __builtin_fma(-dmin, (double)m, v);
+                    }
                     return __builtin_fma(fa, v, y);
                 });
         }
@@ -748,9 +759,9 @@ static hipError_t moe_up_any(const MoeArgs& a, bool packed, uint32_t used, hipSt
     else hipLaunchKernelGGL((moe_prepare_kernel<T, false>), grid, dim3(512), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.tokens <= 8) return moe_up_launch<T, 8, 1>(a, used, s);
+    if (a.tokens <= 8) return moe_up_launch<T, 4, 1>(a, used, s);
     if (a.tokens <= 16) return moe_up_launch<T, 4, 2>(a, used, s);
-    return moe_up_launch<T, 4, 4>(a, used, s);
+    return moe_up_launch<T, 2, 4>(a, used, s);
 }
 template <uint32_t T>
 static hipError_t moe_down_any(const MoeArgs& a, uint32_t used, hipStream_t s) {
@@ -758,7 +769,7 @@ static hipError_t moe_down_any(const MoeArgs& a, uint32_t used, hipStream_t s) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.tokens <= 8) return moe_down_launch<T, 16, 1, 1>(a, s);
-    if (a.tokens <= 16) return moe_down_launch<T, 8, 1, 2>(a, s);
+    if (a.tokens <= 16) return moe_down_launch<T, 16, 1, 2>(a, s);
     return moe_down_launch<T, 8, 2, 2>(a, s);
 }
 
