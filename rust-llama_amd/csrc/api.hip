@@ -107,7 +107,8 @@ struct rlq_context {
     // replaced; its counter set to 0 when the buffer is made, and left at 0 by
     // every launch); column_keys: one per column, of an argmax after a GEMM that
     // uses them (argmax_one_group)
-    DevBuf planes, keys, column_keys, stage_in, stage_w, stage_out, gate, logits, moe;
+    // arrivals: moe_route's counters, 0 between launches
+    DevBuf planes, keys, column_keys, stage_in, stage_w, stage_out, gate, logits, arrivals, moe;
     Retired* retired = nullptr;
 };
 
@@ -402,7 +403,7 @@ void rlq_context_destroy(rlq_context* ctx) {
     DeviceGuard g(ctx->device);
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
     for (DevBuf* b : {&ctx->planes, &ctx->keys, &ctx->column_keys, &ctx->stage_in, &ctx->stage_w, &ctx->stage_out, &ctx->gate,
-                      &ctx->logits, &ctx->moe})
+                      &ctx->logits, &ctx->arrivals, &ctx->moe})
         if (b->p) (void)hipFree(b->p);
     while (Retired* r = ctx->retired) {
         ctx->retired = r->next;
@@ -1004,8 +1005,12 @@ int32_t rlq_moe_route(rlq_context* ctx, const float* router, const float* x, uin
         HIP_TRY(ensure(ctx, ctx->logits, tokens * experts * sizeof(float), s));
         logits = (float*)ctx->logits.p;
     }
+    bool grown = false;
+    HIP_TRY(ensure(ctx, ctx->arrivals, (tokens * sizeof(uint32_t) + 7) / 8 * 8, s, &grown));
+    if (grown) HIP_TRY(launch_fill_u64((unsigned long long*)ctx->arrivals.p, ctx->arrivals.n / 8, 0ull, s));
     const RouteArgs a{router, x, bias, (uint32_t)tokens, (uint32_t)experts, (uint32_t)cols, (uint32_t)slots,
-                      flags & RLQ_ROUTE_SIGMOID, flags & RLQ_ROUTE_NORMALIZE, scale, logits, ids, weights, ctx->err_words};
+                      flags & RLQ_ROUTE_SIGMOID, flags & RLQ_ROUTE_NORMALIZE, scale, logits, ids, weights,
+                      (uint32_t*)ctx->arrivals.p, ctx->err_words};
     HIP_TRY(launch_moe_route(a, s));
     return ok(err);
 }

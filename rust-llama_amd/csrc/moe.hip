@@ -36,70 +36,43 @@ __device__ __forceinline__ float4 route_load(const float* p, uint32_t e, uint32_
                        e + 3 < n ? p[e + 3] : 0.0f);
 }
 
-// z of 16 tokens x 16 experts per workgroup on v_mfma_f64_16x16x4_f64, K split over
-// W waves in slices of 32 (lane l holds row l % 16, values 8 (l / 16) .. + 7 of
-// the slice), the waves' sums added in wave order.
-template <int W, bool VEC>
-__global__ __launch_bounds__(64 * W) void route_logits_kernel(RouteArgs a) {
-    __shared__ double part[W][4][64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, kq = lane >> 4;
-    const uint32_t t0 = blockIdx.y * 16, e0 = blockIdx.x * 16, K = a.cols;
-    const float* x = a.x + (uint64_t)(t0 + i < a.tokens ? t0 + i : a.tokens - 1) * K;
-    const float* r = a.router + (uint64_t)(e0 + i < a.experts ? e0 + i : a.experts - 1) * K;
-    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
-    for (uint32_t k = wave * 32; k < K; k += W * 32) {
-        const uint32_t e = k + 8 * kq;
-        const float4 x0 = route_load<VEC>(x, e, K), x1 = route_load<VEC>(x, e + 4, K);
-        const float4 r0 = route_load<VEC>(r, e, K), r1 = route_load<VEC>(r, e + 4, K);
-        const float xv[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-        const float rv[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)xv[j], (double)rv[j], acc, 0, 0, 0);
-    }
-#pragma unroll
-    for (int v = 0; v < 4; ++v) part[wave][v][lane] = acc[v];
-    __syncthreads();
-    for (uint32_t o = threadIdx.x; o < 256; o += 64 * W) {
-        // value v of lane l: token 4 v + l / 16, expert l % 16
-        const uint32_t v = o >> 6, l = o & 63, t = t0 + 4 * v + (l >> 4), e = e0 + (l & 15);
-        double z = 0.0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) z += part[w][v][l];
-        if (t < a.tokens && e < a.experts) a.logits[(uint64_t)t * a.experts + e] = (float)z;
-    }
+// The maximum over the wave, in every lane (call them with every lane active).
+__device__ __forceinline__ double wave_max_f64(double v) {
+    auto up = [](double a, double b) { return b > a ? b : a; };
+    v = up(v, dpp_d<kQuadXor1>(v));
+    v = up(v, dpp_d<kQuadXor2>(v));
+    v = up(v, dpp_d<kRowHalfMirror>(v));
+    v = up(v, dpp_d<kRowRor8>(v));
+    return up(up(readlane_d(v, 0), readlane_d(v, 16)), up(readlane_d(v, 32), readlane_d(v, 48)));
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    auto up = [](uint32_t a, uint32_t b) { return b > a ? b : a; };
+    v = up(v, (uint32_t)dpp_i<kQuadXor1>((int32_t)v));
+    v = up(v, (uint32_t)dpp_i<kQuadXor2>((int32_t)v));
+    v = up(v, (uint32_t)dpp_i<kRowHalfMirror>((int32_t)v));
+    v = up(v, (uint32_t)dpp_i<kRowRor8>((int32_t)v));
+    auto at = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+    return up(up(at(0), at(16)), up(at(32), at(48)));
 }
 
-// The first of the best among the wave's lanes, each with its own candidate.
-struct RouteBest {
-    double rank;
-    uint32_t expert;
-};
-__device__ __forceinline__ RouteBest route_best(RouteBest b) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const double r = __shfl_xor(b.rank, m, 64);
-        const uint32_t e = (uint32_t)__shfl_xor((int)b.expert, m, 64);
-        if (r > b.rank || (r == b.rank && e < b.expert)) b = RouteBest{r, e};
-    }
-    return b;
-}
-
-// One wave per token; lane l holds experts l, l + 64, ... (NI of them).
+// The best experts of token t by one wave; lane l holds experts l, l + 64, ...
+// (NI of them).  Ranks are f64 (score + bias), or with no bias the f32 logits as
+// ordered u32 keys (1 and up; equal floats have equal keys): a round of the
+// search is then about 30 instructions instead of 100.
+// z: the token's logits in LDS, or null: in a.logits, where other workgroups may
+// have put some (read at the level at which route_put's exchanges are performed).
 template <int NI>
-__global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs a) {
-    const uint32_t lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6), E = a.experts;
-    if (t >= a.tokens) return;
-    const float* z = a.logits + (uint64_t)t * E;
-    double score[NI], rank[NI];
-    double top = -INFINITY;
+__device__ __forceinline__ void route_choose(const RouteArgs& a, uint32_t t, const float* z) {
+    const uint32_t lane = threadIdx.x & 63, E = a.experts;
+    float v[NI];
     int bad = 0;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
         const uint32_t e = lane + 64 * i;
-        const float v = e < E ? z[e] : 0.0f;
-        bad |= !finite(v);
-        score[i] = (double)v;
-        if (e < E) top = score[i] > top ? score[i] : top;
+        v[i] = 0.0f;
+        if (e < E)
+            v[i] = z ? z[e] : __hip_atomic_load(a.logits + (uint64_t)t * E + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        bad |= !finite(v[i]);
     }
     int32_t* ids = a.ids + (uint64_t)t * a.slots;
     float* weights = a.weights + (uint64_t)t * a.slots;
@@ -108,48 +81,71 @@ __global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs a) {
         if (lane == 0) report_error(a.err_word, model_key(t, kStOOut, 0));
         return;
     }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const double o = __shfl_xor(top, m, 64);
-        top = o > top ? o : top;
-    }
-    double sum = 0.0;
+    uint32_t key[NI], best = 0;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-        const uint32_t e = lane + 64 * i;
-        rank[i] = score[i];
-        score[i] = a.sigmoid ? 1.0 / (1.0 + exp(-score[i])) : exp(score[i] - top);
-        if (e < E) sum += score[i];
+        const uint32_t b = __float_as_uint(v[i] == 0.0f ? 0.0f : v[i]);
+        key[i] = lane + 64 * i < E ? ((b >> 31) ? ~b : b | 0x80000000u) : 0;
+        best = key[i] > best ? key[i] : best;
     }
-    if (!a.sigmoid) {
+    best = wave_max_u32(best);
+    double score[NI];
+    if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) score[i] = 1.0 / (1.0 + exp(-(double)v[i]));
+    } else {
+        const double top = (double)__uint_as_float((best >> 31) ? best ^ 0x80000000u : ~best);
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            score[i] = exp((double)v[i] - top);
+            if (lane + 64 * i < E) sum += score[i];
+        }
         sum = wave_sum_f64(sum);
 #pragma unroll
         for (int i = 0; i < NI; ++i) score[i] = score[i] / sum;
     }
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const uint32_t e = lane + 64 * i;
-        if (a.bias && e < E) rank[i] = score[i] + (double)a.bias[e];
-        if (e >= E || !(rank[i] > -INFINITY)) rank[i] = -INFINITY;  // (a bias of NaN: never chosen)
-    }
     int32_t id = -1;  // of place `lane`
     double weight = 0.0;
-    for (uint32_t s = 0; s < a.slots; ++s) {
-        RouteBest b{-INFINITY, ~0u};
-        double mine = 0.0;
+    // the lowest of the experts that `mine` marks takes place s; taken(i): it leaves
+    auto take = [&](uint32_t s, auto&& mine, auto&& taken) {
+        bool found = false;
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-            if (rank[i] > b.rank) b = RouteBest{rank[i], lane + 64 * i}, mine = score[i];
-        const uint32_t own = b.expert;
-        b = route_best(b);
-        if (b.expert == ~0u) break;  // no expert left for the places from s on
-        const double w = __shfl(mine, (int)(b.expert & 63), 64);
-        if (own == b.expert) {
-#pragma unroll
-            for (int i = 0; i < NI; ++i)
-                if (lane + 64 * i == own) rank[i] = -INFINITY;
+        for (int i = 0; i < NI; ++i) {
+            if (found) continue;  // (uniform)
+            const unsigned long long m = __ballot(mine(i));
+            if (!m) continue;
+            found = true;
+            const int l = __builtin_ctzll(m);
+            const double w = readlane_d(score[i], l);
+            if ((int)lane == l) taken(i);
+            if (lane == s) id = l + 64 * i, weight = w;
         }
-        if (lane == s) id = (int32_t)b.expert, weight = w;
+    };
+    if (!a.bias) {
+        for (uint32_t s = 0; s < a.slots; ++s) {  // (slots <= experts)
+            take(s, [&](int i) { return key[i] == best; }, [&](int i) { key[i] = 0; });
+            best = key[0];
+#pragma unroll
+            for (int i = 1; i < NI; ++i) best = key[i] > best ? key[i] : best;
+            best = wave_max_u32(best);
+        }
+    } else {
+        double rank[NI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const uint32_t e = lane + 64 * i;
+            rank[i] = e < E ? score[i] + (double)a.bias[e] : -INFINITY;
+            if (!(rank[i] > -INFINITY)) rank[i] = -INFINITY;  // (a bias of NaN: never chosen)
+        }
+        for (uint32_t s = 0; s < a.slots; ++s) {
+            double most = rank[0];
+#pragma unroll
+            for (int i = 1; i < NI; ++i) most = rank[i] > most ? rank[i] : most;
+            most = wave_max_f64(most);
+            if (!(most > -INFINITY)) break;  // no expert left for the places from s on
+            take(s, [&](int i) { return rank[i] == most; }, [&](int i) { rank[i] = -INFINITY; });
+        }
     }
     if (a.normalize) {
         const double all = wave_sum_f64(weight);
@@ -158,21 +154,199 @@ __global__ __launch_bounds__(256) void route_topk_kernel(RouteArgs a) {
     if (lane < a.slots) ids[lane] = id, weights[lane] = (float)(weight * (double)a.scale);
 }
 
+// A workgroup's logits zs[n tokens][m experts] of tokens from t0 and experts from e0
+// on; then the last of the `parts` workgroups of these tokens to arrive chooses
+// their experts.  With one part they are in LDS already.  Otherwise they are put
+// where every workgroup can read them: an exchange is performed at the device's
+// coherent level when it returns, and its result is waited for, so the count after
+// the barrier needs no release (which would write the whole L2 back).
+template <int W, int NI>
+__device__ __forceinline__ void route_finish(const RouteArgs& a, const float* zs, uint32_t t0, uint32_t n, uint32_t e0,
+                                             uint32_t m, uint32_t group, uint32_t parts) {
+    __shared__ uint32_t last;
+    n = a.tokens - t0 < n ? a.tokens - t0 : n;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n * m; i += 64 * W) {
+        const uint32_t b = i / m, e = e0 + i - b * m;
+        float* to = a.logits + (uint64_t)(t0 + b) * a.experts + e;
+        if (parts == 1) {
+            *to = zs[i];
+        } else {
+            const uint32_t old = __hip_atomic_exchange((uint32_t*)to, __float_as_uint(zs[i]), __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("" ::"v"(old) : "memory");
+        }
+    }
+    if (parts > 1) {
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const uint32_t old = __hip_atomic_fetch_add(a.count + group, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last = old == parts - 1;
+            if (last) __hip_atomic_store(a.count + group, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!last) return;
+    }
+    for (uint32_t k = threadIdx.x >> 6; k < n; k += W) route_choose<NI>(a, t0 + k, parts == 1 ? zs + k * m : nullptr);
+}
+
+// TB tokens, whose rows lie in LDS, and a run of experts per workgroup; a wave takes
+// one expert at a time, 2048 values of its row in flight while the next are
+// loaded, K over its lanes.
+//
+// Bound: a launch, two memory latencies and the choice; where workgroups have
+// several experts a wave, the loads' latency (two experts at a time did not pay:
+// 128 experts of 2048 values, 128 tokens 16.0 us with one, 15.7 with two; 8 of
+// 4096, 512 tokens 8.4 and 12.1).  One token: 8 experts of 4096 values 4.9 us (29 as
+// two launches, the products on MFMA), 128 of 2048 6.4.
+template <int TB, int NI, bool VEC>
+__global__ __launch_bounds__(512) void route_few_kernel(RouteArgs a) {
+    extern __shared__ __align__(16) float xs[];  // [TB][K up to a multiple of 2048], logits [TB][experts of the run]
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = a.cols, E = a.experts;
+    const uint32_t t0 = blockIdx.y * TB, per = (E + gridDim.x - 1) / gridDim.x, e0 = blockIdx.x * per;
+    const uint32_t e1 = e0 + per < E ? e0 + per : E, pad = (K + 2047) / 2048 * 2048;
+    float* zs = xs + TB * pad;
+    float4 r[8];
+    auto load = [&](uint32_t e, uint32_t k0) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) r[u] = route_load<VEC>(a.router + (uint64_t)e * K, k0 + 256 * u + 4 * lane, K);
+    };
+    uint32_t e = e0 + wave;
+    if (e < e1) load(e, 0);
+#pragma unroll
+    for (int b = 0; b < TB; ++b) {
+        const float* x = a.x + (uint64_t)(t0 + b < a.tokens ? t0 + b : a.tokens - 1) * K;
+        for (uint32_t k = 4 * threadIdx.x; k < pad; k += 2048) *(float4*)(xs + b * pad + k) = route_load<VEC>(x, k, K);
+    }
+    __syncthreads();
+    for (; e < e1; e += 8) {
+        double z[TB][2] = {};
+        for (uint32_t k0 = 0; k0 < K; k0 += 2048) {
+            float4 w[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) w[u] = r[u];
+            if (k0 + 2048 < K) load(e, k0 + 2048);
+            else if (e + 8 < e1) load(e + 8, 0);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const double rd[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+                for (int b = 0; b < TB; ++b) {
+                    const float4 x = *(const float4*)(xs + b * pad + k0 + 256 * u + 4 * lane);
+                    z[b][0] = __builtin_fma((double)x.x, rd[0], z[b][0]);
+                    z[b][1] = __builtin_fma((double)x.y, rd[1], z[b][1]);
+                    z[b][0] = __builtin_fma((double)x.z, rd[2], z[b][0]);
+                    z[b][1] = __builtin_fma((double)x.w, rd[3], z[b][1]);
+                }
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < TB; ++b) {
+            const double v = wave_sum_f64(z[b][0] + z[b][1]);
+            if (lane == 0) zs[b * (e1 - e0) + e - e0] = (float)v;
+        }
+    }
+    route_finish<8, NI>(a, zs, t0, TB, e0, e1 - e0, blockIdx.y, gridDim.x);
+}
+
+// z of 16 tokens x 16 experts per workgroup on v_mfma_f64_16x16x4_f64, K split over
+// W waves in slices of 32 (lane l holds row l % 16, values 8 (l / 16) .. + 7 of
+// the slice), two slices loaded ahead, the waves' sums added in wave order.
+//
+// Bound: 512 tokens, 128 experts of 2048 values 19 us, of which the f64 products
+// are 3.4 at the rate of the matrix cores; a launch, the sums' way through LDS, the
+// exchange of the logits and the choice take 10 (measured with K = 32).
+template <int W, int NI, bool VEC>
+__global__ __launch_bounds__(64 * W) void route_many_kernel(RouteArgs a) {
+    __shared__ double part[W][4][64];
+    __shared__ float zs[256];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, kq = lane >> 4;
+    const uint32_t t0 = blockIdx.y * 16, e0 = blockIdx.x * 16, m = a.experts - e0 < 16 ? a.experts - e0 : 16, K = a.cols;
+    const float* x = a.x + (uint64_t)(t0 + i < a.tokens ? t0 + i : a.tokens - 1) * K;
+    const float* r = a.router + (uint64_t)(e0 + i < a.experts ? e0 + i : a.experts - 1) * K;
+    f64x4 acc[2] = {{0.0, 0.0, 0.0, 0.0}, {0.0, 0.0, 0.0, 0.0}};
+    float4 v[2][4];
+    auto load = [&](float4 (&d)[4], uint32_t k) {
+        const uint32_t e = k + 8 * kq;
+        d[0] = route_load<VEC>(x, e, K), d[1] = route_load<VEC>(x, e + 4, K);
+        d[2] = route_load<VEC>(r, e, K), d[3] = route_load<VEC>(r, e + 4, K);
+    };
+    load(v[0], wave * 32);
+    load(v[1], wave * 32 + W * 32);
+    for (uint32_t k = wave * 32; k < K; k += 2 * W * 32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float4(&d)[4] = v[h];
+            const float xv[8] = {d[0].x, d[0].y, d[0].z, d[0].w, d[1].x, d[1].y, d[1].z, d[1].w};
+            const float rv[8] = {d[2].x, d[2].y, d[2].z, d[2].w, d[3].x, d[3].y, d[3].z, d[3].w};
+            load(v[h], k + (2 + h) * W * 32);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)  // (a slice past the end is zeros)
+                acc[j & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)xv[j], (double)rv[j], acc[j & 1], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) part[wave][q][lane] = acc[0][q] + acc[1][q];
+    __syncthreads();
+    for (uint32_t o = threadIdx.x; o < 256; o += 64 * W) {
+        // value q of lane l: token 4 q + l / 16, expert l % 16
+        const uint32_t q = o >> 6, l = o & 63, e = l & 15;
+        double z = 0.0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) z += part[w][q][l];
+        if (e < m) zs[(4 * q + (l >> 4)) * m + e] = (float)z;
+    }
+    route_finish<W, NI>(a, zs, t0, 16, e0, m, blockIdx.y, gridDim.x);
+}
+
+// The grid of route_few_kernel: a part for every eight experts (one a wave) while
+// there are CUs for them, `per` experts each.
+static uint32_t route_per(const RouteArgs& a, uint32_t groups) {
+    const uint32_t cus = (uint32_t)device_cus(), most = cus > groups ? cus / groups : 1, eights = (a.experts + 7) / 8;
+    const uint32_t parts = eights < most ? eights : most;
+    return (a.experts + parts - 1) / parts;
+}
+
+template <int TB, int NI, bool VEC>
+static hipError_t route_few_launch(const RouteArgs& a, uint32_t groups, uint32_t per, hipStream_t s) {
+    static LdsLimit lim;
+    const uint32_t lds = TB * ((a.cols + 2047) / 2048 * 2048 + per) * 4;
+    const hipError_t e = lim.raise((const void*)route_few_kernel<TB, NI, VEC>, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((route_few_kernel<TB, NI, VEC>), dim3((a.experts + per - 1) / per, groups), dim3(512), lds, s, a);
+    return hipGetLastError();
+}
+
+// One token a workgroup while every eight experts of every token can have a CU, else
+// two (us: 64 tokens, 8 experts of 4096 values 5.7 against 6.8 with two; 128 tokens,
+// 128 of 2048 16.1 against 14.0).  Such a workgroup's time grows with its steps (a
+// wave's experts times 2048 values of K, times the rounds of workgroups), the MFMA
+// tiles' with K alone: few / tiles, 512 tokens, 32 experts of 2048 values (4 steps)
+// 11.8 / 15.4, 64 (8) 18.1 / 15.9, 128 (16) 32.0 / 19.0; 200 tokens, 60 of 896 (4) 11.6
+// / 10.3; 100 tokens, 256 of 4096 (14) 26.8 / 24.8; 30 tokens, 256 of 7168 (8) 20.0 /
+// 34.5.  Rows of more than 16384 values do not fit LDS.
+template <int NI, bool VEC>
+static hipError_t route_launch(const RouteArgs& a, hipStream_t s) {
+    const uint32_t cus = (uint32_t)device_cus();
+    const bool one = (uint64_t)a.tokens * ((a.experts + 7) / 8) <= cus;
+    const uint32_t groups = one ? a.tokens : (a.tokens + 1) / 2, per = route_per(a, groups);
+    const uint64_t rounds = ((uint64_t)groups * ((a.experts + per - 1) / per) + cus - 1) / cus;
+    const uint64_t steps = (uint64_t)((per + 7) / 8) * ((a.cols + 2047) / 2048) * rounds;
+    if (a.cols <= 16384 && (one || steps <= 2 + a.cols / 512))
+        return one ? route_few_launch<1, NI, VEC>(a, groups, per, s) : route_few_launch<2, NI, VEC>(a, groups, per, s);
+    hipLaunchKernelGGL((route_many_kernel<16, NI, VEC>), dim3((a.experts + 15) / 16, (a.tokens + 15) / 16), dim3(1024), 0, s,
+                       a);
+    return hipGetLastError();
+}
+
 hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s) {
     if (a.tokens == 0 || a.experts == 0 || a.cols == 0 || a.experts > kMoeMaxExperts || a.slots == 0 ||
         a.slots > kMoeMaxSlots || a.slots > a.experts || a.tokens > 65535)
         return hipErrorInvalidValue;
     const bool vec = (((uintptr_t)a.x | (uintptr_t)a.router) & 15) == 0 && a.cols % 4 == 0;
-    const dim3 tiles((a.experts + 15) / 16, (a.tokens + 15) / 16);
-    if (vec) hipLaunchKernelGGL((route_logits_kernel<8, true>), tiles, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((route_logits_kernel<8, false>), tiles, dim3(512), 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    const dim3 grid((a.tokens + 3) / 4);
-    if (a.experts <= 64) hipLaunchKernelGGL((route_topk_kernel<1>), grid, dim3(256), 0, s, a);
-    else if (a.experts <= 256) hipLaunchKernelGGL((route_topk_kernel<4>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((route_topk_kernel<16>), grid, dim3(256), 0, s, a);
-    return hipGetLastError();
+    if (a.experts <= 64) return vec ? route_launch<1, true>(a, s) : route_launch<1, false>(a, s);
+    if (a.experts <= 256) return vec ? route_launch<4, true>(a, s) : route_launch<4, false>(a, s);
+    return vec ? route_launch<16, true>(a, s) : route_launch<16, false>(a, s);
 }
 
 // ---------------------------------------------------------------------------

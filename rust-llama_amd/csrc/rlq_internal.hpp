@@ -207,6 +207,7 @@ struct RouteArgs {
     float* logits;
     int32_t* ids;
     float* weights;
+    uint32_t* count;  // per token: 0 between launches (workgroups that share tokens count each other)
     unsigned long long* err_word;
 };
 hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s);
