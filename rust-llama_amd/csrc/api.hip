@@ -107,7 +107,7 @@ struct rlq_context {
     // replaced; its counter set to 0 when the buffer is made, and left at 0 by
     // every launch); column_keys: one per column, of an argmax after a GEMM that
     // uses them (argmax_one_group)
-    // arrivals: moe_route's counters, 0 between launches
+    // arrivals: counters of moe_route and moe_ffn, 0 between launches
     DevBuf planes, keys, column_keys, stage_in, stage_w, stage_out, gate, logits, arrivals, moe;
     Retired* retired = nullptr;
 };
@@ -173,6 +173,14 @@ hipError_t ensure_image(rlq_context* ctx, size_t need, hipStream_t s, bool* fits
     if (e != hipErrorOutOfMemory) return e;
     (void)hipGetLastError();
     return hipSuccess;
+}
+
+// `words` arrival counters, which every launch leaves at 0.
+hipError_t ensure_arrivals(rlq_context* ctx, uint64_t words, hipStream_t s) {
+    bool grown = false;
+    const hipError_t e = ensure(ctx, ctx->arrivals, (words * sizeof(uint32_t) + 7) / 8 * 8, s, &grown);
+    if (e != hipSuccess || !grown) return e;
+    return launch_fill_u64((unsigned long long*)ctx->arrivals.p, ctx->arrivals.n / 8, 0ull, s);
 }
 
 struct DeviceGuard {
@@ -1005,9 +1013,7 @@ int32_t rlq_moe_route(rlq_context* ctx, const float* router, const float* x, uin
         HIP_TRY(ensure(ctx, ctx->logits, tokens * experts * sizeof(float), s));
         logits = (float*)ctx->logits.p;
     }
-    bool grown = false;
-    HIP_TRY(ensure(ctx, ctx->arrivals, (tokens * sizeof(uint32_t) + 7) / 8 * 8, s, &grown));
-    if (grown) HIP_TRY(launch_fill_u64((unsigned long long*)ctx->arrivals.p, ctx->arrivals.n / 8, 0ull, s));
+    HIP_TRY(ensure_arrivals(ctx, tokens, s));
     const RouteArgs a{router, x, bias, (uint32_t)tokens, (uint32_t)experts, (uint32_t)cols, (uint32_t)slots,
                       flags & RLQ_ROUTE_SIGMOID, flags & RLQ_ROUTE_NORMALIZE, scale, logits, ids, weights,
                       (uint32_t*)ctx->arrivals.p, ctx->err_words};
@@ -1042,11 +1048,14 @@ int32_t rlq_moe_ffn(rlq_context* ctx, const rlq_weights* gate, const rlq_weights
     if (((uintptr_t)ids | (uintptr_t)weights | (uintptr_t)residual | (uintptr_t)y) & 3)
         return fail(err, RLQ_INVALID_ARGUMENT, gate->dtype);
     MoeCall c{gate->dev, up->dev, down->dev, gate->mat_bytes, down->mat_bytes, gate->dtype, down->dtype, gate->n2,
-              gate->cols, gate->rows, down->rows, tokens, slots, x, x_dtype != 0, ids, weights, residual, y, ctx->err_words};
+              gate->cols, gate->rows, down->rows, tokens, slots, x, x_dtype != 0, ids, weights, residual, y, nullptr,
+              ctx->err_words};
     if (!moe_takes(c)) return fail(err, RLQ_UNIMPLEMENTED, gate->dtype, gate->rows, gate->cols);
     DeviceGuard g(ctx->device);
     const hipStream_t s = pick(ctx, stream);
     HIP_TRY(ensure(ctx, ctx->moe, moe_bytes(c), s));
+    HIP_TRY(ensure_arrivals(ctx, moe_counters(c), s));
+    c.count = (uint32_t*)ctx->arrivals.p;
     HIP_TRY(launch_moe_ffn(c, ctx->moe.p, s));
     return ok(err);
 }

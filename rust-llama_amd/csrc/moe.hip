@@ -581,8 +581,8 @@ struct MoeWeights<kQ8_0> {
 // A workgroup's LDS: its waves' f64 sums, and each wave's column scales of its
 // current chunk.
 template <uint32_t T>
-constexpr uint32_t moe_lds(uint32_t ks, uint32_t sums, uint32_t groups) {
-    return ks * (sums * 512 + groups * MoeWeights<T>::kFactors * 256);
+constexpr uint32_t moe_lds(uint32_t ks, uint32_t sums) {
+    return ks * (sums * 512 + MoeWeights<T>::kFactors * 256);
 }
 
 // Where a lane's rows have their current chunk, which one of the image it is, and
@@ -599,37 +599,32 @@ struct MoeAt {
 // move for each of the sixteen.)
 __device__ __forceinline__ uint32_t bits_or(uint32_t mask, uint32_t a, uint32_t b) { return (mask & b) | (~mask & a); }
 
-// One wave's chunks.  at(it): where step it is.  fold(g, f, term): adds a chunk's
-// (Q8_0: a block's) products of column group g, term(i, fa, y) being y plus fa
-// times product i of the lane's row; f: the group's 32 column scales.  HALVES:
-// rows of the second half take the columns from 16 on.
-template <uint32_t T, int NG, bool HALVES, typename At, typename Fold>
-__device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, const uint32_t (&tok)[NG], uint32_t steps,
-                                         uint32_t ln, uint32_t kh, double* fd, At&& at, Fold&& fold) {
+// One wave's chunks.  at(it): where step it is.  fold(f, term): adds a chunk's
+// (Q8_0: a block's) products, term(i, fa, y) being y plus fa times product i of the
+// lane's row; f: the 32 column scales.  HALVES: rows of the second half take the
+// columns from 16 on.  R: k-steps whose activations are in flight.
+template <uint32_t T, bool HALVES, int R, typename At, typename Fold>
+__device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, uint32_t tok, uint32_t steps, uint32_t ln,
+                                         uint32_t kh, double* fd, At&& at, Fold&& fold) {
     using M = MoeWeights<T>;
     if (steps == 0) return;
     const uint32_t n = ln & 15;
     const uint32_t upper = HALVES && ln >= 16 ? ~0u : 0u;
     M m;
-    i32x4 act[NG][4];
-    f16x8 bs[NG];
-    double f[NG][M::kFactors];
+    i32x4 act[R];
+    f16x8 bs;
+    double f[M::kFactors];
     const uint64_t sq = (uint64_t)tokens * 16;  // bytes of one k half
     auto load_act = [&](int s, uint32_t c) {
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-            act[g][s % 4] = *(const i32x4*)(im.q + ((uint64_t)c * 16 + s * 2 + kh) * sq + tok[g] * 16);
+        act[s % R] = *(const i32x4*)(im.q + ((uint64_t)c * 16 + s * 2 + kh) * sq + tok * 16);
     };
     auto load_scales = [&](const MoeAt& p) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-#pragma unroll
-            for (int k = 0; k < M::kFactors; ++k) {
-                const double v = im.f[((uint64_t)p.chunk * M::kFactors + k) * tokens + tok[g]];
-                f[g][k] = p.live ? v : 0.0;
-            }
-            if constexpr (ig_mins(T)) bs[g] = *(const f16x8*)(im.sums + (((uint64_t)p.chunk * 2 + kh) * tokens + tok[g]) * 8);
+        for (int k = 0; k < M::kFactors; ++k) {
+            const double v = im.f[((uint64_t)p.chunk * M::kFactors + k) * tokens + tok];
+            f[k] = p.live ? v : 0.0;
         }
+        if constexpr (ig_mins(T)) bs = *(const f16x8*)(im.sums + (((uint64_t)p.chunk * 2 + kh) * tokens + tok) * 8);
     };
     auto pair_of = [&](const MoeAt& p, uint32_t k) { return p.w + (k < p.pairs ? k : p.pairs - 1) * kQ80Chunk; };
     auto load_q8 = [&](const MoeAt& p, int s) {
@@ -643,7 +638,7 @@ __device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, co
     };
     MoeAt p = at(0);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) load_act(s, p.chunk);
+    for (int s = 0; s < R; ++s) load_act(s, p.chunk);
     load_scales(p);
     if constexpr (T == kQ8_0) {
 #pragma unroll
@@ -657,12 +652,14 @@ __device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, co
         constexpr bool more = decltype(more_)::value;
         MoeAt nx = p;
         if (more) nx = at(it + 1);
+        if (kh == 0) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
-            if (kh == 0) {
-#pragma unroll
-                for (int k = 0; k < M::kFactors; ++k) fd[(g * M::kFactors + k) * 32 + ln] = f[g][k];
-            }
+            for (int k = 0; k < M::kFactors; ++k) fd[k * 32 + ln] = f[k];
+        }
+        auto next_act = [&](int s) {
+            if (s + R < 8) load_act(s + R, p.chunk);
+            else if (more) load_act(s + R - 8, nx.chunk);
+        };
         if constexpr (T == kQ8_0) {
             uint32_t dw4[4];
 #pragma unroll
@@ -672,18 +669,13 @@ __device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, co
             for (int s = 0; s < 8; ++s) {
                 const i32x4 w = __builtin_bit_cast(i32x4, m.q[s]);
                 const double dw = (double)half_to_float((s & 1) ? dw4[s / 2] >> 16 : dw4[s / 2]);
-                i32x16 I[NG];
-#pragma unroll
-                for (int g = 0; g < NG; ++g) I[g] = ig_mfma(act[g][s % 4], w, (i32x16){});
+                const i32x16 I = ig_mfma(act[s % R], w, (i32x16){});
                 if (more) load_q8(nx, s);
-                if (s < 4) load_act(s + 4, p.chunk);
-                else if (more) load_act(s - 4, nx.chunk);
-#pragma unroll
-                for (int g = 0; g < NG; ++g)
-                    fold(g, fd + (g * M::kFactors + s) * 32, [&](int i, double fa, double y) {
-                        const int32_t v = HALVES ? (int32_t)bits_or(upper, I[g][i], I[g][i + 8 * HALVES]) : I[g][i];
-                        return __builtin_fma((double)v, fa * dw, y);
-                    });
+                next_act(s);
+                fold(fd + s * 32, [&](int i, double fa, double y) {
+                    const int32_t v = HALVES ? (int32_t)bits_or(upper, I[i], I[i + 8 * HALVES]) : I[i];
+                    return __builtin_fma((double)v, fa * dw, y);
+                });
             }
         } else {
             using W = Ig<T>;
@@ -693,46 +685,33 @@ __device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, co
             f16x8 mins = {};
             if constexpr (ig_mins(T)) dmin = (double)W::dmin(m.r), mins = W::mins(m.r, kh);
             if (more) W::head(m.r, nx.w, n);
-            i32x16 A[NG], B[NG];
-#pragma unroll
-            for (int g = 0; g < NG; ++g) A[g] = (i32x16){}, B[g] = (i32x16){};
+            i32x16 A = {}, B = {};
             ig_steps([&](auto s_) {
                 constexpr int S = decltype(s_)::value;
                 i32x4 wa, wb;
                 W::template ops<S>(m.r, pre, wa, wb);
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    A[g] = ig_mfma(act[g][S % 4], wa, A[g]);
-                    if (W::kPlanes == 2) B[g] = ig_mfma(act[g][S % 4], wb, B[g]);
-                }
+                A = ig_mfma(act[S % R], wa, A);
+                if (W::kPlanes == 2) B = ig_mfma(act[S % R], wb, B);
                 if (more) W::template refill<S>(m.r, nx.w, n, kh);
-                if (S < 4) load_act(S + 4, p.chunk);
-                else if (more) load_act(S - 4, nx.chunk);
+                next_act(S);
             });
-            f32x16 mn[NG];
-            if constexpr (ig_mins(T)) {
-#pragma unroll
-                for (int g = 0; g < NG; ++g)
-                    mn[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bs[g], mins, (f32x16){}, 0, 0, 0);
-            }
+            f32x16 mn = {};
+            if constexpr (ig_mins(T)) mn = __builtin_amdgcn_mfma_f32_32x32x16_f16(bs, mins, (f32x16){}, 0, 0, 0);
             if (more) load_scales(nx);
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-                fold(g, fd + g * 32, [&](int i, double fa, double y) {
-                    auto block = [&](int k) {
-                        return W::kPlanes == 2 ? ((uint32_t)A[g][k] << W::kShift) + (uint32_t)B[g][k] : (uint32_t)A[g][k];
-                    };
-                    uint32_t I = block(i);
-                    if constexpr (HALVES) I = bits_or(upper, I, block(i + 8));
-                    double v = d * (double)(int32_t)I;  // exact: 11 and 31 bits
-                    if constexpr (ig_mins(T)) {
-                        float m = mn[g][i];
-                        if constexpr (HALVES)
-                            m = __uint_as_float(bits_or(upper, __float_as_uint(m), __float_as_uint(mn[g][i + 8])));
-                        v = __builtin_fma(-dmin, (double)m, v);
-                    }
-                    return __builtin_fma(fa, v, y);
-                });
+            fold(fd, [&](int i, double fa, double y) {
+                auto block = [&](int k) {
+                    return W::kPlanes == 2 ? ((uint32_t)A[k] << W::kShift) + (uint32_t)B[k] : (uint32_t)A[k];
+                };
+                uint32_t I = block(i);
+                if constexpr (HALVES) I = bits_or(upper, I, block(i + 8));
+                double v = d * (double)(int32_t)I;  // exact: 11 and 31 bits
+                if constexpr (ig_mins(T)) {
+                    float m = mn[i];
+                    if constexpr (HALVES) m = __uint_as_float(bits_or(upper, __float_as_uint(m), __float_as_uint(mn[i + 8])));
+                    v = __builtin_fma(-dmin, (double)m, v);
+                }
+                return __builtin_fma(fa, v, y);
+            });
         }
         p = nx;
     };
@@ -748,8 +727,17 @@ __device__ __forceinline__ uint32_t moe_pairs(uint32_t npairs, uint32_t c) {
 
 // h of 16 rows for expert j's tokens: wave kg takes every KS-th chunk of K.  NQ:
 // groups of eight columns that the tokens of the pass can need.
+//
+// Registers decide how many chunks a CU has in flight.  To eight columns the
+// activations of a whole chunk are loaded ahead (8 experts of 14336x4096 Q4_K, one
+// token of top-2 32.9 us against 35.7 with half a chunk), but for Q8_0, whose eight
+// scales a chunk take registers (16 experts of 1952x928, 5 tokens 12.6 us with four
+// waves a SIMD, 14.1 with a whole chunk ahead).  32 columns' sums leave room for three
+// waves a SIMD (32 tokens 133 us, 156 with the compiler's choice of two; 148 with a
+// whole chunk ahead, which spills).
 template <uint32_t T, int KS, int NQ>
-__global__ __launch_bounds__(64 * KS) void moe_up_kernel(MoeArgs a) {
+__global__ __launch_bounds__(64 * KS) __attribute__((amdgpu_waves_per_eu(NQ == 4 ? 3 : (NQ == 2 || T == kQ8_0 ? 4 : 2)))) void
+moe_up_kernel(MoeArgs a) {
     extern __shared__ __align__(16) double lds[];
     const uint32_t lane = threadIdx.x & 63, kg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t ln = lane & 31, kh = lane >> 5;
@@ -759,7 +747,7 @@ __global__ __launch_bounds__(64 * KS) void moe_up_kernel(MoeArgs a) {
             if (a.flags[i]) atomicOr(&a.bad[i % a.tokens], 1u);
     if (j >= *a.n_used) return;
     const uint32_t live = (uint32_t)__builtin_popcount(a.mask[j]), nchunk = a.x_chunks;
-    const uint32_t tok[1] = {a.column[j * kMoeTokens + (ln < live ? ln : 0)]};
+    const uint32_t tok = a.column[j * kMoeTokens + (ln < live ? ln : 0)];
     const uint8_t* wt = ((ln >> 4) ? a.up : a.gate) + (uint64_t)a.expert[j] * a.up_bytes + (uint64_t)tile * a.x_row_bytes;
     double* part = lds;
     double* fd = lds + KS * NQ * 4 * 64 + kg * (MoeWeights<T>::kFactors * 32);
@@ -767,13 +755,13 @@ __global__ __launch_bounds__(64 * KS) void moe_up_kernel(MoeArgs a) {
 #pragma unroll
     for (int i = 0; i < NQ * 4; ++i) y[i] = 0.0;
     const uint32_t steps = kg < nchunk ? (nchunk - 1 - kg) / KS + 1 : 0;
-    moe_walk<T, 1, false>(
+    moe_walk<T, false, NQ == 1 && T != kQ8_0 ? 8 : 4>(
         a.xi, a.tokens, tok, steps, ln, kh, fd,
         [&](uint32_t it) {
             const uint32_t c = kg + it * KS;
             return MoeAt{wt + (uint64_t)c * MoeWeights<T>::kChunk, c, moe_pairs(a.x_pairs, c), true};
         },
-        [&](int, const double* f, auto&& term) {
+        [&](const double* f, auto&& term) {
 #pragma unroll
             for (int q = 0; q < NQ; ++q)
                 if ((uint32_t)(8 * q) < live) {
@@ -802,55 +790,100 @@ __global__ __launch_bounds__(64 * KS) void moe_up_kernel(MoeArgs a) {
     }
 }
 
-// y of 16 rows for every token: wave kg takes every KS-th pair of chunks of all
-// experts' h, one for each half of its rows.  NG groups of 16 tokens, NQ of eight
-// inside each.
-template <uint32_t T, int KS, int NG, int NQ>
-__global__ __launch_bounds__(64 * KS) void moe_down_kernel(MoeArgs a) {
+// y of a tile of rows for every token, over the h of all experts in use as one long
+// row of chunks, of which the workgroup takes its part and its waves take turns.
+//   up to 16 tokens  16 rows (HALVES): a pair of chunks at a time, one for each half
+//   more             32 rows: a chunk at a time, all 32 columns
+// Where the tiles alone leave CUs idle, `parts` workgroups share a tile: they put
+// their f64 sums where all can read them (by exchanges whose results are waited for,
+// as the router does), and the last to arrive adds them in part order.
+template <uint32_t T, int KS, int NQ>
+__global__ __launch_bounds__(64 * KS) __attribute__((amdgpu_waves_per_eu(KS == 16 ? 4 : 3))) void
+moe_down_kernel(MoeArgs a) {
+    constexpr bool HALVES = NQ < 4;
+    constexpr uint32_t kRows = HALVES ? 16 : 32, kStep = HALVES ? 2 : 1;
     extern __shared__ __align__(16) double lds[];
     __shared__ uint16_t expert[kMoeMaxExperts];
+    __shared__ uint32_t last;
     const uint32_t lane = threadIdx.x & 63, kg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t ln = lane & 31, kh = lane >> 5, hf = ln >> 4;
-    const uint32_t tile = blockIdx.x, nchunk = a.h_chunks, used = *a.n_used, total = used * nchunk;
+    const uint32_t tile = blockIdx.x / a.parts, part = blockIdx.x - tile * a.parts;
+    const uint32_t nchunk = a.h_chunks, used = *a.n_used;
+    // this part's chunks, whole steps of them but for the last part's end
+    const uint32_t all = used * nchunk, steps_all = (all + kStep - 1) / kStep;
+    const uint32_t c0 = (uint32_t)((uint64_t)steps_all * part / a.parts) * kStep;
+    const uint32_t c1 = part + 1 < a.parts ? (uint32_t)((uint64_t)steps_all * (part + 1) / a.parts) * kStep : all;
     for (uint32_t i = threadIdx.x; i < used; i += 64 * KS) expert[i] = (uint16_t)a.expert[i];
     __syncthreads();
-    uint32_t tok[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) tok[g] = 16 * g + (ln & 15) < a.tokens ? 16 * g + (ln & 15) : a.tokens - 1;
-    double* part = lds;
-    constexpr int kSums = NG * NQ * 4;
-    double* fd = lds + KS * kSums * 64 + kg * (NG * MoeWeights<T>::kFactors * 32);
+    const uint32_t col = HALVES ? ln & 15 : ln, tok = col < a.tokens ? col : a.tokens - 1;
+    uint32_t t16 = HALVES ? tile : 2 * tile + hf;
+    t16 = t16 < a.out_tiles ? t16 : a.out_tiles - 1;  // (rows past the end are never stored)
+    const uint8_t* wt = a.down + (uint64_t)t16 * a.h_row_bytes;
+    constexpr int kSums = NQ * 4;
+    double* sums = lds;
+    double* fd = lds + KS * kSums * 64 + kg * (MoeWeights<T>::kFactors * 32);
     double y[kSums];
 #pragma unroll
     for (int i = 0; i < kSums; ++i) y[i] = 0.0;
-    const uint32_t steps = 2 * kg < total ? (total - 1 - 2 * kg) / (2 * KS) + 1 : 0;
-    moe_walk<T, NG, true>(
+    const uint32_t first = c0 + kStep * kg, steps = first < c1 ? (c1 - 1 - first) / (kStep * KS) + 1 : 0;
+    moe_walk<T, HALVES, 4>(
         a.hi, a.tokens, tok, steps, ln, kh, fd,
         [&](uint32_t it) {
-            const uint32_t want = 2 * (kg + it * KS) + hf, at = want < total ? want : total - 1;
+            const uint32_t want = first + it * (kStep * KS) + (HALVES ? hf : 0), at = want < c1 ? want : c1 - 1;
             const uint32_t j = at / nchunk, c = at - j * nchunk;
-            const uint8_t* w = a.down + (uint64_t)expert[j] * a.down_bytes + (uint64_t)tile * a.h_row_bytes;
-            return MoeAt{w + (uint64_t)c * MoeWeights<T>::kChunk, at, moe_pairs(a.h_pairs, c), want < total};
+            return MoeAt{wt + (uint64_t)expert[j] * a.down_bytes + (uint64_t)c * MoeWeights<T>::kChunk, at,
+                         moe_pairs(a.h_pairs, c), want < c1};
         },
-        [&](int g, const double* f, auto&& term) {
+        [&](const double* f, auto&& term) {
 #pragma unroll
-            for (int i = 0; i < NQ * 4; ++i) {
-                double& s = y[g * NQ * 4 + i];
-                s = term(i, f[16 * hf + 8 * (i / 4) + 4 * kh + i % 4], s);
-            }
+            for (int i = 0; i < kSums; ++i)
+                y[i] = term(i, f[(HALVES ? 16 * hf : 0) + 8 * (i / 4) + 4 * kh + i % 4], y[i]);
         });
 #pragma unroll
-    for (int i = 0; i < kSums; ++i) part[(kg * kSums + i) * 64 + lane] = y[i];
+    for (int i = 0; i < kSums; ++i) sums[(kg * kSums + i) * 64 + lane] = y[i];
     __syncthreads();
-    for (uint32_t o = threadIdx.x; o < a.tokens * 16; o += 64 * KS) {
-        const uint32_t t = o >> 4, r = o & 15, t16 = t & 15, row = tile * 16 + r;
-        if (row >= a.out_rows || a.bad[t]) continue;
-        const uint32_t i = (t >> 4) * NQ * 4 + 4 * (t16 >> 3) + (t16 & 3), l = ((t16 >> 2) & 1) * 32 + r;
-        const uint64_t to = (uint64_t)t * a.out_rows + row;
-        double v = a.residual ? (double)a.residual[to] : 0.0;
+    // value o: row o % kRows of token o / kRows
+    auto total = [&](uint32_t o) {
+        const uint32_t t = o / kRows, r = o % kRows, i = 4 * (t >> 3) + (t & 3), l = ((t >> 2) & 1) * 32 + r;
+        double v = 0.0;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) v += part[(k * kSums + i) * 64 + l] + part[(k * kSums + i) * 64 + l + 16];
-        a.y[to] = (float)v;
+        for (int k = 0; k < KS; ++k) {
+            v += sums[(k * kSums + i) * 64 + l];
+            if (HALVES) v += sums[(k * kSums + i) * 64 + l + 16];
+        }
+        return v;
+    };
+    auto store = [&](uint32_t o, double v) {
+        const uint32_t t = o / kRows, row = tile * kRows + o % kRows;
+        if (row >= a.out_rows || a.bad[t]) return;
+        const uint64_t to = (uint64_t)t * a.out_rows + row;
+        a.y[to] = (float)(a.residual ? (double)a.residual[to] + v : v);
+    };
+    const uint32_t n = a.tokens * kRows;
+    if (a.parts == 1) {
+        for (uint32_t o = threadIdx.x; o < n; o += 64 * KS) store(o, total(o));
+        return;
+    }
+    unsigned long long* mine = a.sums + ((uint64_t)tile * a.parts + part) * n;
+    for (uint32_t o = threadIdx.x; o < n; o += 64 * KS) {
+        const unsigned long long old = __hip_atomic_exchange(mine + o, (unsigned long long)__double_as_longlong(total(o)),
+                                                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("" ::"v"(old) : "memory");
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t old = __hip_atomic_fetch_add(a.count + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = old == a.parts - 1;
+        if (last) __hip_atomic_store(a.count + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last) return;
+    for (uint32_t o = threadIdx.x; o < n; o += 64 * KS) {
+        double v = 0.0;
+        for (uint32_t p = 0; p < a.parts; ++p)
+            v += __longlong_as_double((long long)__hip_atomic_load(a.sums + ((uint64_t)tile * a.parts + p) * n + o,
+                                                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        store(o, v);
     }
 }
 
@@ -859,6 +892,26 @@ __global__ __launch_bounds__(64 * KS) void moe_down_kernel(MoeArgs a) {
 // ---------------------------------------------------------------------------
 static uint64_t moe_align(uint64_t v) { return (v + 255) & ~255ull; }
 static uint64_t moe_chunks(uint64_t cols) { return (cols + 255) / 256; }
+
+// Row tiles of the down product: 16 rows to 16 tokens, then 32.
+static uint64_t moe_out_tiles(const MoeCall& c, uint32_t tokens) {
+    const uint64_t t = layout_tiles(c.out_rows);
+    return tokens <= 16 ? t : (t + 1) / 2;
+}
+// Workgroups that share a tile of the down product: as many as there are CUs for, but
+// a step for every wave of each (us with 1 / 2 / 4: 4096 rows, 32 tokens, 8 experts of
+// 56 chunks 128 / 83 / 90; 928 rows, 16 experts of 8 chunks of Q8_0 14.7 / 11.2 / 10.6;
+// 2048 rows, one token, 6 experts of 6 chunks 8.7 / 9.3 / 14.7).
+static uint32_t moe_parts(const MoeCall& c, uint32_t tokens) {
+    const uint64_t tiles = moe_out_tiles(c, tokens), pairs = (uint64_t)tokens * c.slots;
+    const uint64_t chunks = (pairs < c.experts ? pairs : c.experts) * moe_chunks(c.ffn);
+    // of 16 waves that take a pair of chunks a step, or 12 that take one
+    const uint64_t steps = tokens <= 16 ? (chunks + 31) / 32 : (chunks + 11) / 12;
+    uint64_t parts = (uint64_t)device_cus() / tiles;
+    parts = parts < steps ? parts : steps;
+    return (uint32_t)(parts < 1 ? 1 : parts < 8 ? parts : 8);
+}
+uint64_t moe_counters(const MoeCall& c) { return layout_tiles(c.out_rows); }
 
 // The scratch of a pass; base null: only its size.
 static size_t moe_carve(const MoeCall& c, uint32_t tokens, uint8_t* base, MoeArgs* a) {
@@ -887,6 +940,8 @@ static size_t moe_carve(const MoeCall& c, uint32_t tokens, uint8_t* base, MoeArg
     m.flags = (uint32_t*)take(moe_chunks(c.cols) * tokens * 4);
     m.xi = image(c.up_type, moe_chunks(c.cols));
     m.h = (float*)take(pairs * c.ffn * 4);
+    m.parts = moe_parts(c, tokens);
+    m.sums = (unsigned long long*)take(m.parts > 1 ? moe_out_tiles(c, tokens) * m.parts * tokens * (tokens <= 16 ? 16 : 32) * 8 : 0);
     m.hi = image(c.down_type, used * moe_chunks(c.ffn));
     if (a) *a = m;
     return at;
@@ -903,26 +958,27 @@ bool moe_takes(const MoeCall& c) {
     const uint64_t used = t * c.slots < c.experts ? t * c.slots : c.experts;
     return c.experts <= kMoeMaxExperts && c.slots <= kMoeMaxSlots && c.tokens <= 65535 && c.cols <= (1u << 30) &&
            c.ffn <= (1u << 30) && used * layout_tiles(c.ffn) * 1024 <= 0xffffffffull &&
-           layout_tiles(c.out_rows) * 1024 <= 0xffffffffull && used * moe_chunks(c.ffn) * 512 <= 0xffffffffull &&
+           layout_tiles(c.out_rows) * 8 * 1024 <= 0xffffffffull && used * moe_chunks(c.ffn) * 512 <= 0xffffffffull &&
            (moe_chunks(c.cols) + 1) * 512 <= 0xffffffffull;
 }
 
 template <uint32_t T, int KS, int NQ>
 static hipError_t moe_up_launch(const MoeArgs& a, uint32_t used, hipStream_t s) {
     static LdsLimit lim;
-    constexpr uint32_t lds = moe_lds<T>(KS, NQ * 4, 1);
+    constexpr uint32_t lds = moe_lds<T>(KS, NQ * 4);
     const hipError_t e = lim.raise((const void*)moe_up_kernel<T, KS, NQ>, lds);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((moe_up_kernel<T, KS, NQ>), dim3(used * a.up_tiles), dim3(64 * KS), lds, s, a);
     return hipGetLastError();
 }
-template <uint32_t T, int KS, int NG, int NQ>
+template <uint32_t T, int KS, int NQ>
 static hipError_t moe_down_launch(const MoeArgs& a, hipStream_t s) {
     static LdsLimit lim;
-    constexpr uint32_t lds = moe_lds<T>(KS, NG * NQ * 4, NG);
-    const hipError_t e = lim.raise((const void*)moe_down_kernel<T, KS, NG, NQ>, lds + 2 * kMoeMaxExperts);
+    constexpr uint32_t lds = moe_lds<T>(KS, NQ * 4), tiles = NQ < 4 ? 1 : 2;
+    const hipError_t e = lim.raise((const void*)moe_down_kernel<T, KS, NQ>, lds + 2 * kMoeMaxExperts);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((moe_down_kernel<T, KS, NG, NQ>), dim3((a.out_rows + 15) / 16), dim3(64 * KS), lds, s, a);
+    hipLaunchKernelGGL((moe_down_kernel<T, KS, NQ>), dim3((a.out_tiles + tiles - 1) / tiles * a.parts), dim3(64 * KS), lds, s,
+                       a);
     return hipGetLastError();
 }
 
@@ -942,9 +998,9 @@ static hipError_t moe_down_any(const MoeArgs& a, uint32_t used, hipStream_t s) {
     hipLaunchKernelGGL((moe_h_kernel<T>), dim3(a.h_chunks, used), dim3((a.tokens * 16 + 63) / 64 * 64), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.tokens <= 8) return moe_down_launch<T, 16, 1, 1>(a, s);
-    if (a.tokens <= 16) return moe_down_launch<T, 16, 1, 2>(a, s);
-    return moe_down_launch<T, 8, 2, 2>(a, s);
+    if (a.tokens <= 8) return moe_down_launch<T, 16, 1>(a, s);
+    if (a.tokens <= 16) return moe_down_launch<T, 16, 2>(a, s);
+    return moe_down_launch<T, 12, 4>(a, s);
 }
 
 hipError_t launch_moe_ffn(const MoeCall& c, void* scratch, hipStream_t s) {
@@ -962,7 +1018,8 @@ hipError_t launch_moe_ffn(const MoeCall& c, void* scratch, hipStream_t s) {
         a.residual = c.residual ? c.residual + t0 * c.out_rows : nullptr;
         a.y = c.y + t0 * c.out_rows;
         a.gate = c.gate, a.up = c.up, a.down = c.down, a.up_bytes = c.up_bytes, a.down_bytes = c.down_bytes;
-        a.up_tiles = (uint32_t)layout_tiles(c.ffn);
+        a.up_tiles = (uint32_t)layout_tiles(c.ffn), a.out_tiles = (uint32_t)layout_tiles(c.out_rows);
+        a.count = c.count;
         a.x_chunks = (uint32_t)moe_chunks(c.cols), a.h_chunks = (uint32_t)moe_chunks(c.ffn);
         a.x_pairs = (uint32_t)((c.cols / 32 + 1) / 2), a.h_pairs = (uint32_t)((c.ffn / 32 + 1) / 2);
         a.x_row_bytes = layout_chunks_per_tile(c.up_type, c.cols) * layout_chunk_bytes(c.up_type);

@@ -222,10 +222,12 @@ struct MoeCall {
     const int32_t* ids;
     const float *weights, *residual;
     float* y;
+    uint32_t* count;  // moe_counters words, 0 between launches
     unsigned long long* err_word;
 };
 bool moe_takes(const MoeCall& c);
 size_t moe_bytes(const MoeCall& c);
+uint64_t moe_counters(const MoeCall& c);
 hipError_t launch_moe_ffn(const MoeCall& c, void* scratch, hipStream_t s);
 struct MoeImage {
     uint8_t* q;
@@ -236,7 +238,7 @@ struct MoeArgs {  // of one pass
     const uint8_t *gate, *up, *down;
     uint64_t up_bytes, down_bytes, x_row_bytes, h_row_bytes;  // a matrix; a 16-row tile
     uint32_t tokens, token0, slots, experts, cols, ffn, out_rows;
-    uint32_t up_tiles, x_chunks, h_chunks, x_pairs, h_pairs;
+    uint32_t up_tiles, out_tiles, x_chunks, h_chunks, x_pairs, h_pairs, parts;
     const void* x;
     const int32_t* ids;
     const float *weights, *residual;
@@ -248,6 +250,8 @@ struct MoeArgs {  // of one pass
     double* wsum;
     MoeImage xi, hi;
     float* h;
+    unsigned long long* sums;  // of the parts of the down product's tiles
+    uint32_t* count;           // 0 between launches: parts that have arrived, per tile
 };
 
 // ---- llama.hip ----
