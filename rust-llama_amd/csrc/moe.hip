@@ -36,7 +36,7 @@ __device__ __forceinline__ float4 route_load(const float* p, uint32_t e, uint32_
                        e + 3 < n ? p[e + 3] : 0.0f);
 }
 
-// The maximum over the wave, in every lane (call them with every lane active).
+// The maximum over the wave, in every lane (call it with every lane active).
 __device__ __forceinline__ double wave_max_f64(double v) {
     auto up = [](double a, double b) { return b > a ? b : a; };
     v = up(v, dpp_d<kQuadXor1>(v));
@@ -44,15 +44,6 @@ __device__ __forceinline__ double wave_max_f64(double v) {
     v = up(v, dpp_d<kRowHalfMirror>(v));
     v = up(v, dpp_d<kRowRor8>(v));
     return up(up(readlane_d(v, 0), readlane_d(v, 16)), up(readlane_d(v, 32), readlane_d(v, 48)));
-}
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-    auto up = [](uint32_t a, uint32_t b) { return b > a ? b : a; };
-    v = up(v, (uint32_t)dpp_i<kQuadXor1>((int32_t)v));
-    v = up(v, (uint32_t)dpp_i<kQuadXor2>((int32_t)v));
-    v = up(v, (uint32_t)dpp_i<kRowHalfMirror>((int32_t)v));
-    v = up(v, (uint32_t)dpp_i<kRowRor8>((int32_t)v));
-    auto at = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
-    return up(up(at(0), at(16)), up(at(32), at(48)));
 }
 
 // The best experts of token t by one wave; lane l holds experts l, l + 64, ...

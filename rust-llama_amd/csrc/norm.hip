@@ -15,100 +15,166 @@
 
 namespace rlq {
 
-// A store of 16 bytes at any address (Q8_0 blocks are 34 bytes long).
-struct __attribute__((packed)) Bytes16 {
-    uint32_t w[4];
+// Four bytes at any address (a Q8_0 block is 34 bytes long).
+struct __attribute__((packed)) Bytes4 {
+    uint32_t w;
 };
 
-// 16 values of a row from element e0 on; past the end: 0.
+// Four values of a row from element e on; past the end: 0.
 template <bool VEC>
-__device__ __forceinline__ void norm_load(const float* p, uint32_t e0, uint32_t n, float (&v)[16]) {
+__device__ __forceinline__ void norm_load(const float* p, uint32_t e, uint32_t n, float (&v)[4]) {
     if constexpr (VEC) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (e0 + 4 * k < n) f = *(const float4*)(p + e0 + 4 * k);
-            v[4 * k] = f.x, v[4 * k + 1] = f.y, v[4 * k + 2] = f.z, v[4 * k + 3] = f.w;
-        }
+        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (e < n) f = *(const float4*)(p + e);
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
     } else {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = e0 + k < n ? p[e0 + k] : 0.0f;
+        for (int k = 0; k < 4; ++k) v[k] = e + k < n ? p[e + k] : 0.0f;
     }
 }
 template <bool VEC>
-__device__ __forceinline__ void norm_store(float* p, uint32_t e0, uint32_t n, const float (&v)[16]) {
+__device__ __forceinline__ void norm_store(float* p, uint32_t e, uint32_t n, const float (&v)[4]) {
     if constexpr (VEC) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (e0 + 4 * k < n) *(float4*)(p + e0 + 4 * k) = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+        if (e < n) *(float4*)(p + e) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-            if (e0 + k < n) p[e0 + k] = v[k];
+        for (int k = 0; k < 4; ++k)
+            if (e + k < n) p[e + k] = v[k];
     }
 }
 
-// L lanes per row (several rows share a workgroup of 256 below 256 lanes), U
-// units of 16 values per lane: unit u of the row is lane u % L's number u / L.
-// A row is read once and stays in registers until every check of it has passed;
-// then it is written, so a row with a data error keeps its old outputs.
+constexpr int kRowShl4 = 0x104;  // lane i <- i + 4 within each 16 lanes
+
+// Four levels of a lane, the block's scale, and whether the scale is no finite
+// number (activation.rs:20-28, encode.rs:80-90).
+struct NormQ {
+    uint32_t q;
+    float d;
+    int32_t bsum;  // Q8_K, in the first lane of each four: the sum of its 16 levels
+    bool bad;
+};
+
+// U Q8_K blocks by a wave, four values of each a lane (the arithmetic of
+// rlq_q8k.hpp's q8k_row16; see there for the rounding), of which the first `count`
+// exist.  The first value of largest magnitude is that of the first lane that holds
+// it, the lanes being in order; the divisions of all blocks run in one go, in a lane
+// for each.  The values are finite, or the row is refused anyway.
+template <int U>
+__device__ __forceinline__ void norm_q8k(const float (&v)[U][4], uint32_t count, NormQ (&o)[U]) {
+    const uint32_t lane = threadIdx.x & 63;
+    float top = 0.0f;  // lane k: block k's
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+        float m = v[k][0];
+#pragma unroll
+        for (int j = 1; j < 4; ++j) m = fabsf(v[k][j]) > fabsf(m) ? v[k][j] : m;
+        const uint32_t mag = __float_as_uint(m) & 0x7fffffffu;
+        const uint32_t most = wave_max_u32(mag);
+        const int first = __builtin_ctzll(__ballot(mag == most));
+        const float f = readlane_f(m, first);
+        top = lane == (uint32_t)k ? f : top;
+    }
+    const bool some = top != 0.0f;
+    const float inverse = some ? -127.0f / top : 0.0f, d = some ? 1.0f / inverse : 0.0f;
+    const unsigned long long bad = __ballot(lane < count && (!finite(inverse) || !finite(d)));
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+        const float inv = readlane_f(inverse, k);
+        uint32_t b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(inv * v[k][j] + 12582912.0f);
+        o[k].q = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u) | __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+        o[k].d = readlane_f(d, k);
+        int32_t s = dot4(o[k].q, 0x01010101u, 0);
+        s += dpp_i<kQuadXor1>(s);
+        o[k].bsum = s + dpp_i<kQuadXor2>(s);
+        o[k].bad = (bad >> k) & 1;
+    }
+}
+
+// One Q8_0 block by eight lanes, four values each (q8_0_pair16 in another layout).
+__device__ __forceinline__ NormQ norm_q8_0(const float (&v)[4]) {
+    float am = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    am = fmaxf(am, dpp_f<kQuadXor1>(am));
+    am = fmaxf(am, dpp_f<kQuadXor2>(am));
+    am = fmaxf(am, dpp_f<kRowHalfMirror>(am));
+    NormQ o{0, am / 127.0f, 0, false};
+    o.bad = !finite(o.d) || (o.d != 0.0f && !finite(1.0f / o.d)) || (float_to_half_bits(o.d) & 0x7c00u) == 0x7c00u;
+    const float inv = o.d != 0.0f ? 1.0f / o.d : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float r = __builtin_roundf(v[k] * inv);  // half away from zero, saturating
+        r = r > 127.0f ? 127.0f : (r < -128.0f ? -128.0f : r);
+        o.q |= ((uint32_t)(int32_t)r & 0xffu) << (8 * k);
+    }
+    return o;
+}
+
+// L lanes per row (four rows share a workgroup of 256 at 64), U times four values per
+// lane: lane r holds values 4 (r + k L) .. + 3, so that every load and store of a wave
+// is one run of 1 KB.  A row is read once and stays in registers until every check
+// of it has passed; then it is written, so a row with a data error keeps its old
+// outputs.
 //
 // The f64 sum runs in a parallel order.  Two orders of the same n nonnegative
 // terms differ by at most 2 (n - 1) 2^-53 of their sum, so where both ends of
 // that interval give one f32 mean, the reference's mean is that f32 too;
 // otherwise (about one row of 4096 values in 65000) the sum is repeated in the
 // reference's order.
+//
+// Bound: memory: 2048 rows of 4096 values into f32 and Q8_K 14.1 us back to back, 5.4 TB/s (20.8
+// with sixteen neighbouring values a lane, whose loads and stores touch four times the
+// lines); with a residual and its sum 23 us, 6.2 TB/s.  One row: a launch, the loads, two
+// barriers and the stores, 4.5 us.
 template <int L, int U, bool VEC>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(NormArgs a) {
-    constexpr int kWaves = L / 64;  // of a row, where it has whole waves
-    __shared__ double red[L > 64 ? 4 * kWaves : 1];
-    const uint32_t r = threadIdx.x % L, n = a.cols, units = (n + 15) / 16;
+    constexpr int kWaves = L / 64;  // of a row
+    __shared__ double red[kWaves];
+    const uint32_t r = threadIdx.x % L, n = a.cols;
     const uint32_t row = blockIdx.x * (L < 256 ? 256 / L : 1) + threadIdx.x / L;
     const bool live = row < a.rows;  // (uniform in a row's lanes)
     const uint64_t at = (uint64_t)(live ? row : 0) * n;
     const float* x = a.x + at;
     const float* res = a.residual ? a.residual + at : nullptr;
+    const uint32_t have = live ? n : 0;
 
-    float t[U][16], y[U][16];
+    float t[U][4], y[U][4];
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-        const uint32_t e0 = (r + k * L) * 16;
-        norm_load<VEC>(x, e0, live ? n : 0, t[k]);
-        norm_load<VEC>(a.weight, e0, n, y[k]);
-    }
+    for (int k = 0; k < U; ++k) norm_load<VEC>(x, 4 * (r + k * L), have, t[k]);
     if (res) {
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-            float v[16];
-            norm_load<VEC>(res, (r + k * L) * 16, live ? n : 0, v);
+        for (int k = 0; k < U; ++k) norm_load<VEC>(res, 4 * (r + k * L), have, y[k]);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) t[k][j] = t[k][j] + v[j];
-        }
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[k][j] = t[k][j] + y[k][j];
     }
+#pragma unroll
+    for (int k = 0; k < U; ++k) norm_load<VEC>(a.weight, 4 * (r + k * L), n, y[k]);
     double ss = 0.0;
 #pragma unroll
     for (int k = 0; k < U; ++k)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) ss += (double)(t[k][j] * t[k][j]);
-    ss = row16_sum_f64(ss);
-    if constexpr (L == 64) ss = rows_sum_f64(ss);
+        for (int j = 0; j < 4; ++j) ss += (double)(t[k][j] * t[k][j]);
+    ss = wave_sum_f64(ss);
     if constexpr (L > 64) {
-        if ((threadIdx.x & 15) == 0) red[threadIdx.x >> 4] = ss;
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
         __syncthreads();
         ss = 0.0;
 #pragma unroll
-        for (int w = 0; w < 4 * kWaves; ++w) ss += red[w];
+        for (int w = 0; w < kWaves; ++w) ss += red[w];
     }
     const double dn = (double)n, eps = dn * 2.3e-16 * ss;  // 2^-52 n sum, with a margin
     float mean = (float)(ss / dn);
     if ((float)((ss - eps) / dn) != (float)((ss + eps) / dn)) {  // (uniform in a row's lanes)
         double seq = 0.0;
-        if constexpr (L <= 64) {
+        if constexpr (L == 64) {
 #pragma unroll
             for (int k = 0; k < U; ++k)
-                for (uint32_t o = 0; o < L && o + k * L < units; ++o)
+                for (uint32_t o = 0; o < 64 && 4 * (o + k * 64) < n; ++o)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) seq += (double)__shfl(t[k][j] * t[k][j], (int)o, L);
+                    for (int j = 0; j < 4; ++j)  // (past the end: + 0)
+                        seq += (double)readlane_f(t[k][j] * t[k][j], (int)o);
         } else {
             __syncthreads();  // every thread has read red[]
             if (threadIdx.x < 64) {
@@ -133,14 +199,11 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(NormArgs a)
         bad = 1;
         if (r == 0) report_error(a.err_word, model_key(row, kStFfnNormScale, 0));
     }
-    uint32_t q[U][4];
-    float d[U];
-    int32_t bsum[U];
     bool off = false;  // math.rs:227
 #pragma unroll
     for (int k = 0; k < U; ++k)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < 4; ++j) {
             y[k][j] = t[k][j] * scale * y[k][j];
             off |= !finite(y[k][j]);
         }
@@ -148,51 +211,47 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(NormArgs a)
         bad = 1;
         report_error(a.err_word, model_key(row, kStFfnNormOut, 0));
     }
+    NormQ q[U];
     if (a.q_type) {  // (then n is a multiple of the block, so a block's lanes stay together)
+        if (a.q_type == kQ8_K) {
+            const uint32_t blocks = have / 256, w = r / 64;  // of the row; the wave's first one
+            norm_q8k<U>(y, blocks > w ? (blocks - w + kWaves - 1) / kWaves : 0, q);
+        }
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-            const uint32_t u = r + k * L;
-            if (!live || u >= units) continue;
-            int kind;
-            if (a.q_type == kQ8_K) {
-                const Q8KRow o = q8k_row16(y[k], u & 15);
-#pragma unroll
-                for (int w = 0; w < 4; ++w) q[k][w] = o.q[w];
-                d[k] = o.d, bsum[k] = o.bsum, kind = o.kind;
-            } else {
-                uint32_t index;
-                kind = q8_0_pair16(y[k], u & 1, q[k], d[k], index);
-            }
-            if (kind >= 0) {  // a non-finite value has been reported above, and sorts first
+            const uint32_t e = 4 * (r + k * L);
+            if (e >= have) continue;
+            if (a.q_type == kQ8_0) q[k] = norm_q8_0(y[k]);
+            if (q[k].bad) {  // (a value that is not finite has been reported above, and sorts first)
                 bad = 1;
-                if (kind == kKindScale)
-                    report_error(a.err_word, model_key(row, kStGuQuant, u / (a.q_type == kQ8_K ? 16 : 2)));
+                report_error(a.err_word, model_key(row, kStGuQuant, e / (a.q_type == kQ8_K ? 256 : 32)));
             }
         }
     }
-    if constexpr (L > 64) {
-        bad = __syncthreads_or(bad);
-    } else {
-        const unsigned long long m = __ballot(bad);
-        bad = L == 64 ? m != 0 : ((m >> (threadIdx.x & 48)) & 0xffffull) != 0;
-    }
+    if constexpr (L > 64) bad = __syncthreads_or(bad);
+    else bad = __ballot(bad) != 0;
     if (bad || !live) return;
+    uint8_t* blocks = a.q + ((uint64_t)row * (n / 256) + r / 64) * 292;
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-        const uint32_t u = r + k * L, e0 = u * 16;
-        if (u >= units) continue;
-        if (a.total) norm_store<VEC>(a.total + at, e0, n, t[k]);
-        if (a.y) norm_store<VEC>(a.y + at, e0, n, y[k]);
+        const uint32_t e = 4 * (r + k * L);
+        if (e >= n) continue;
+        if (a.total) norm_store<VEC>(a.total + at, e, n, t[k]);
+        if (a.y) norm_store<VEC>(a.y + at, e, n, y[k]);
         if (a.q_type == kQ8_K) {
-            uint8_t* o = a.q + ((uint64_t)row * (n / 256) + u / 16) * 292;
-            if ((u & 15) == 0) *(float*)o = d[k];
-            *(Bytes16*)(o + 4 + 16 * (u & 15)) = Bytes16{{q[k][0], q[k][1], q[k][2], q[k][3]}};
-            *(int16_t*)(o + 260 + 2 * (u & 15)) = (int16_t)bsum[k];
+            uint8_t* o = blocks + k * (kWaves * 292);
+            const uint32_t l = r % 64;
+            *(uint32_t*)(o + 4 + 4 * l) = q[k].q;
+            // the scale (lane 4) and the sums, two a lane (every eighth)
+            const uint32_t next = (uint32_t)dpp_i<kRowShl4>(q[k].bsum);
+            const uint32_t pair = ((uint32_t)q[k].bsum & 0xffffu) | next << 16;
+            if (l % 8 == 0 || l == 4)
+                *(uint32_t*)(o + (l == 4 ? 0 : 260 + l / 2)) = l == 4 ? __float_as_uint(q[k].d) : pair;
         } else if (a.q_type == kQ8_0) {
-            uint8_t* o = a.q + ((uint64_t)row * (n / 32) + u / 2) * 34;
-            // d is the f32 of a half: converting it back is exact
-            if ((u & 1) == 0) *(uint16_t*)o = (uint16_t)float_to_half_bits(d[k]);
-            *(Bytes16*)(o + 2 + 16 * (u & 1)) = Bytes16{{q[k][0], q[k][1], q[k][2], q[k][3]}};
+            uint8_t* o = a.q + (at + e) / 32 * 34;
+            const uint32_t l = e / 4 % 8;
+            ((Bytes4*)(o + 2 + 4 * l))->w = q[k].q;
+            if (l == 0) *(uint16_t*)o = (uint16_t)float_to_half_bits(q[k].d);
         }
     }
 }
@@ -210,13 +269,14 @@ hipError_t launch_rms_norm(const NormArgs& a, hipStream_t s) {
     if (a.rows == 0 || a.cols == 0 || a.cols > kNormMaxCols) return hipErrorInvalidValue;
     uintptr_t low = (uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.weight | (uintptr_t)a.total | (uintptr_t)a.y;
     const bool vec = (low & 15) == 0 && a.cols % 4 == 0;
-    const uint32_t units = (a.cols + 15) / 16;
-    if (units <= 16) return norm_launch<16, 1>(a, vec, s);
-    if (units <= 64) return norm_launch<64, 1>(a, vec, s);
-    if (units <= 256) return norm_launch<256, 1>(a, vec, s);
-    if (units <= 512) return norm_launch<256, 2>(a, vec, s);
-    if (units <= 1024) return norm_launch<1024, 1>(a, vec, s);
-    return norm_launch<1024, 2>(a, vec, s);
+    const uint32_t fours = (a.cols + 3) / 4;
+    if (fours <= 64) return norm_launch<64, 1>(a, vec, s);
+    if (fours <= 256) return norm_launch<64, 4>(a, vec, s);
+    if (fours <= 512) return norm_launch<256, 2>(a, vec, s);
+    if (fours <= 1024) return norm_launch<256, 4>(a, vec, s);
+    if (fours <= 2048) return norm_launch<256, 8>(a, vec, s);
+    if (fours <= 4096) return norm_launch<1024, 4>(a, vec, s);
+    return norm_launch<1024, 8>(a, vec, s);
 }
 
 }  // namespace rlq

@@ -171,6 +171,16 @@ __device__ __forceinline__ float wave_max_dpp(float v) {
     v = fmaxf(v, dpp_f<kRowRor8>(v));
     return fmaxf(fmaxf(readlane_f(v, 0), readlane_f(v, 16)), fmaxf(readlane_f(v, 32), readlane_f(v, 48)));
 }
+// The same of whole numbers (call it with every lane active).
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    auto up = [](uint32_t a, uint32_t b) { return b > a ? b : a; };
+    v = up(v, (uint32_t)dpp_i<kQuadXor1>((int32_t)v));
+    v = up(v, (uint32_t)dpp_i<kQuadXor2>((int32_t)v));
+    v = up(v, (uint32_t)dpp_i<kRowHalfMirror>((int32_t)v));
+    v = up(v, (uint32_t)dpp_i<kRowRor8>((int32_t)v));
+    auto at = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+    return up(up(at(0), at(16)), up(at(32), at(48)));
+}
 __device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {
     for (int m = 1; m < 64; m <<= 1) {
         const uint32_t o = (uint32_t)__shfl_xor((int)v, m, 64);
