@@ -346,7 +346,8 @@ hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s) {
 // A pass takes up to 32 tokens.  Its plan lists the experts in use in ascending
 // order; expert j of them serves the tokens of mask[j], in columns cols[j][..]
 // ascending, whose h rows start at base[j].  A token that names an expert twice
-// is one column of it, with the sum of both weights.
+// is one column of it, with the sum of both weights.  A single token has no
+// plan: its places that name an expert are read from ids where they are needed.
 //
 // An image holds activations of T tokens in chunks of 256 values (of a Q8_0 row's
 // last chunk, a part; the rest is 0):
@@ -354,25 +355,53 @@ hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s) {
 //   sums  [chunk][k half 2][token][8 f16]      (weights with mins)
 //   f     [chunk][token] f64, for Q8_0 [chunk][k-step][token]: the block's scale
 //         (of h: times the token's weight for the expert, 0 without one)
-// in the slot order of rlq_layout.hpp for Q4_K and Q5_K.  x has one image, h one
-// per expert in use, expert after expert, so that the down product runs over all
-// of them as over one long row.
+// in the slot order of rlq_layout.hpp for Q4_K and Q5_K.  x has one image (in LDS for a
+// single token), h one per expert in use, expert after expert, so that the down
+// product runs over all of them as over one long row.
+//
+// A block with a data error has kMoeBad as its scale.  That NaN reaches every sum of
+// its token, and who finds a sum to be a NaN looks whether the mark is among the
+// scales (one with a NaN weight is no error): such a token's h is NaN, and its y is
+// not written.  No other value has these bits: they are no f32's, and the result of no
+// operation.
 // ---------------------------------------------------------------------------
+constexpr unsigned long long kMoeBad = 0x7ff8000000000001ull;
+__device__ __forceinline__ double moe_bad_scale() { return __longlong_as_double((long long)kMoeBad); }
+__device__ __forceinline__ bool moe_is_bad(double f) { return (unsigned long long)__double_as_longlong(f) == kMoeBad; }
 
-// The first thing that is wrong with a token keeps its row of y as it was.
-__device__ __forceinline__ void moe_bad(const MoeArgs& a, uint32_t t, uint64_t key) {
-    report_error(a.err_word, key);
-    atomicOr(&a.bad[t], 1u);
+// Whether the mark is among token t's scales of chunks c0 .. c1 - 1 (k a chunk).
+__device__ __forceinline__ bool moe_marked(const double* f, uint32_t tokens, uint32_t t, uint32_t c0, uint32_t c1, uint32_t k) {
+    for (uint64_t i = (uint64_t)c0 * k; i < (uint64_t)c1 * k; ++i)
+        if (moe_is_bad(f[i * tokens + t])) return true;
+    return false;
+}
+
+// The places of a single token that name an expert (bit s), and whether one is out
+// of range; every wave for itself.
+struct MoePlaces {
+    unsigned long long some;
+    int32_t id;  // of place `lane`
+    int wrong;   // the first place out of range, or -1
+};
+__device__ __forceinline__ MoePlaces moe_places(const MoeArgs& a) {
+    const uint32_t lane = threadIdx.x & 63;
+    MoePlaces p;
+    p.id = lane < a.slots ? a.ids[lane] : -1;
+    p.some = __ballot(p.id >= 0 && p.id < (int32_t)a.experts);
+    const unsigned long long off = __ballot(p.id < -1 || p.id >= (int32_t)a.experts);
+    p.wrong = off ? __builtin_ctzll(off) : -1;
+    return p;
 }
 
 __device__ __forceinline__ void moe_plan(const MoeArgs& a) {
-    __shared__ uint32_t mask[kMoeMaxExperts], wave_n[8], wave_b[8];
+    __shared__ uint32_t mask[kMoeMaxExperts], wave_n[8], wave_b[8], bad;
     __shared__ uint16_t place[kMoeMaxExperts];
     __shared__ int32_t ids[kMoeTokens * kMoeMaxSlots];
     __shared__ float weights[kMoeTokens * kMoeMaxSlots];
     const uint32_t tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = nt >> 6;
     const uint32_t pairs = a.tokens * a.slots;
     for (uint32_t e = tid; e < a.experts; e += nt) mask[e] = 0;
+    if (tid == 0) bad = 0;
     __syncthreads();
     for (uint32_t p = tid; p < pairs; p += nt) {
         int32_t id = a.ids[p];
@@ -380,7 +409,8 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& a) {
         if (id >= 0 && id < (int32_t)a.experts) {
             atomicOr(&mask[id], 1u << t);
         } else if (id != -1) {
-            moe_bad(a, t, bounds_key((uint64_t)a.token0 * a.slots + p));
+            report_error(a.err_word, bounds_key((uint64_t)a.token0 * a.slots + p));
+            atomicOr(&bad, 1u << t);
             id = -1;
         }
         ids[p] = id, weights[p] = a.weights[p];
@@ -407,7 +437,7 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& a) {
         if (m) a.expert[j] = e, a.base[j] = b, a.mask[j] = m, place[e] = (uint16_t)j;
         __syncthreads();
     }
-    if (tid == 0) *a.n_used = used;
+    if (tid == 0) *a.n_used = used, *a.bad = bad;
     for (uint32_t p = tid; p < pairs; p += nt) {  // a token's first place with an expert speaks for all of them
         const int32_t id = ids[p];
         const uint32_t t = p / a.slots, end = (t + 1) * a.slots;
@@ -423,7 +453,17 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& a) {
     }
 }
 
-// One lane's 16 values (r16 of a chunk's 16 lanes) of token t into an image.
+__device__ __forceinline__ void moe_load16(const float* p, float (&v)[16]) {
+    const float4* src = (const float4*)p;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float4 w = src[k];
+        v[4 * k] = w.x, v[4 * k + 1] = w.y, v[4 * k + 2] = w.z, v[4 * k + 3] = w.w;
+    }
+}
+
+// One lane's 16 values (r16 of a chunk's 16 lanes) of token t into an image for
+// weights of type T.
 template <uint32_t T>
 __device__ __forceinline__ void image_put(const MoeImage& im, uint32_t tokens, uint64_t chunk, uint32_t r16, uint32_t t,
                                           const uint32_t (&q)[4], int32_t bsum, double f) {
@@ -454,23 +494,17 @@ __device__ __forceinline__ int image_quantize(const float (&v)[16], uint32_t r16
     }
 }
 
-// Workgroup 0: the plan.  The others: one chunk of x each, 16 lanes per token, from
-// f32 rows or from packed blocks (taken as given; the 16-value sums are those of
-// the levels).  flags[chunk][token]: a data error in the token's chunk.
+// One lane's 16 values of chunk c of token t of x, from f32 rows or from packed
+// blocks (taken as given; the 16-value sums are those of the levels).  report: this
+// workgroup tells of a data error.
 template <uint32_t T, bool PACKED>
-__global__ __launch_bounds__(512) void moe_prepare_kernel(MoeArgs a) {
-    if (blockIdx.x == 0) {
-        if (threadIdx.x < kMoeTokens) a.bad[threadIdx.x] = 0;
-        __syncthreads();
-        moe_plan(a);
-        return;
-    }
-    const uint32_t c = blockIdx.x - 1, r16 = threadIdx.x & 15, t = threadIdx.x >> 4, K = a.cols, e0 = c * 256 + r16 * 16;
-    if (t >= a.tokens) return;
-    uint32_t q[4] = {0, 0, 0, 0};
+__device__ __forceinline__ bool moe_x(const MoeArgs& a, uint32_t c, uint32_t r16, uint32_t t, bool report, uint32_t (&q)[4],
+                                      int32_t& bsum, double& f) {
+    const uint32_t K = a.cols, e0 = c * 256 + r16 * 16;
     float d = 0.0f;
-    int32_t bsum = 0;
     int kind = -1;
+    bsum = 0;
+    q[0] = q[1] = q[2] = q[3] = 0;
     if constexpr (PACKED) {
         if (e0 < K) {
             if constexpr (T == kQ8_0) {
@@ -484,6 +518,7 @@ __global__ __launch_bounds__(512) void moe_prepare_kernel(MoeArgs a) {
                 d = __uint_as_float(b[0]);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) q[k] = b[1 + 4 * r16 + k];
+#pragma unroll
                 for (int k = 0; k < 4; ++k) bsum = dot4(q[k], 0x01010101u, bsum);
             }
         }
@@ -491,29 +526,40 @@ __global__ __launch_bounds__(512) void moe_prepare_kernel(MoeArgs a) {
         float v[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) v[k] = 0.0f;
-        if (e0 < K) {
-            const float4* src = (const float4*)((const float*)a.x + (uint64_t)t * K + e0);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float4 f = src[k];
-                v[4 * k] = f.x, v[4 * k + 1] = f.y, v[4 * k + 2] = f.z, v[4 * k + 3] = f.w;
-            }
-        }
+        if (e0 < K) moe_load16((const float*)a.x + (uint64_t)t * K + e0, v);
         uint32_t index;
         kind = image_quantize<T>(v, r16, q, d, bsum, index);
-        if (kind >= 0) {
+        if (kind >= 0 && report && (T == kQ8_0 ? !(r16 & 1) : r16 == 0)) {
             const uint64_t block = T == kQ8_0 ? e0 / 32 : c, first = T == kQ8_0 ? e0 / 32 * 32ull : c * 256ull;
-            if (T == kQ8_0 ? !(r16 & 1) : r16 == 0)
-                report_error(a.err_word, kind == kKindNonFinite ? error_key(a.token0 + t, kKindNonFinite, first + index)
-                                                                : error_key(a.token0 + t, kKindScale, block));
+            report_error(a.err_word, kind == kKindNonFinite ? error_key(a.token0 + t, kKindNonFinite, first + index)
+                                                            : error_key(a.token0 + t, kKindScale, block));
         }
     }
-    image_put<T>(a.xi, a.tokens, c, r16, t, q, bsum, (double)d);
-    const unsigned long long m = __ballot(kind >= 0) >> (threadIdx.x & 48) & 0xffffull;
-    if (r16 == 0) a.flags[c * a.tokens + t] = m != 0;
+    f = kind >= 0 ? moe_bad_scale() : (double)d;
+    return kind >= 0;
 }
 
-// h of expert j's tokens, one chunk, for the down matrices' type.
+// Workgroup 0: the plan.  The others: one chunk of x each, 16 lanes per token.
+template <uint32_t T, bool PACKED>
+__global__ __launch_bounds__(512) void moe_prepare_kernel(MoeArgs a) {
+    if (blockIdx.x == 0) {
+        moe_plan(a);
+        return;
+    }
+    const uint32_t c = blockIdx.x - 1, r16 = threadIdx.x & 15, t = threadIdx.x >> 4;
+    if (t >= a.tokens) return;
+    uint32_t q[4];
+    int32_t bsum;
+    double f;
+    moe_x<T, PACKED>(a, c, r16, t, true, q, bsum, f);
+    image_put<T>(a.xi, a.tokens, c, r16, t, q, bsum, f);
+}
+
+// h of expert j's tokens, one chunk, into the image for down matrices of type T.  (A
+// launch of its own: the workgroup of moe_up_kernel that writes the last rows of a
+// chunk could do it, but the exchanges and counts by which it knows cost all of them
+// more than the launch: 32 tokens, 8 experts of 14336x4096 162 us against 133 + 5.5; 5
+// tokens, 16 Q8_0 experts of 1952x928 18.8 against 12.6 + 4.)
 template <uint32_t T>
 __global__ __launch_bounds__(512) void moe_h_kernel(MoeArgs a) {
     const uint32_t c = blockIdx.x, j = blockIdx.y, r16 = threadIdx.x & 15, t = threadIdx.x >> 4;
@@ -523,22 +569,15 @@ __global__ __launch_bounds__(512) void moe_h_kernel(MoeArgs a) {
     float v[16];
 #pragma unroll
     for (int k = 0; k < 16; ++k) v[k] = 0.0f;
-    if (mine && e0 < a.ffn) {
-        const uint32_t row = a.base[j] + (uint32_t)__builtin_popcount(mask & ((1u << t) - 1));
-        const float4* src = (const float4*)(a.h + (uint64_t)row * a.ffn + e0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float4 f = src[k];
-            v[4 * k] = f.x, v[4 * k + 1] = f.y, v[4 * k + 2] = f.z, v[4 * k + 3] = f.w;
-        }
-    }
+    if (mine && e0 < a.ffn) moe_load16(a.h + (uint64_t)(a.base[j] + (uint32_t)__builtin_popcount(mask & ((1u << t) - 1))) * a.ffn + e0, v);
     uint32_t q[4], index;
     float d;
     int32_t bsum;
     const int kind = image_quantize<T>(v, r16, q, d, bsum, index);
-    if (kind == kKindScale && (T == kQ8_0 ? !(r16 & 1) : r16 == 0))  // (a non-finite h was reported where it was made)
-        moe_bad(a, t, model_key(a.token0 + t, kStDownQuant, T == kQ8_0 ? e0 / 32 : c));
-    image_put<T>(a.hi, a.tokens, (uint64_t)j * gridDim.x + c, r16, t, q, bsum, mine ? a.wsum[j * kMoeTokens + t] * (double)d : 0.0);
+    if (kind == kKindScale && (T == kQ8_0 ? !(r16 & 1) : r16 == 0))  // (a non-finite h has been reported)
+        report_error(a.err_word, model_key(a.token0 + t, kStDownQuant, T == kQ8_0 ? e0 / 32 : c));
+    const double f = !mine ? 0.0 : kind >= 0 ? moe_bad_scale() : a.wsum[j * kMoeTokens + t] * (double)d;
+    image_put<T>(a.hi, a.tokens, (uint64_t)j * gridDim.x + c, r16, t, q, bsum, f);
 }
 
 // ---------------------------------------------------------------------------
@@ -569,12 +608,51 @@ struct MoeWeights<kQ8_0> {
     uint32_t d[4];
 };
 
-// A workgroup's LDS: its waves' f64 sums, and each wave's column scales of its
-// current chunk.
+// A workgroup's LDS: its waves' f64 sums, each wave's column scales of its current
+// chunk, and (up, one token) the image of x.
 template <uint32_t T>
 constexpr uint32_t moe_lds(uint32_t ks, uint32_t sums) {
     return ks * (sums * 512 + MoeWeights<T>::kFactors * 256);
 }
+template <uint32_t T>
+constexpr uint32_t moe_lds_chunk() {
+    return 256 + 32 + 8 * MoeWeights<T>::kFactors;
+}
+extern __shared__ __align__(16) uint8_t moe_smem[];
+
+// Activations of one token in LDS, and of a pass in an image.
+template <uint32_t T>
+struct MoeLds {
+    uint32_t q, sums, f;  // offsets in moe_smem
+    __device__ MoeLds(uint32_t at, uint32_t chunks) : q(at), sums(at + chunks * 256), f(at + chunks * 288) {}
+    __device__ i32x4 act(uint32_t c, int s, uint32_t kh) const { return *(const i32x4*)(moe_smem + q + (c * 16 + s * 2 + kh) * 16); }
+    __device__ double scale(uint32_t c, int k) const {
+        return *(const double*)(moe_smem + f + (c * MoeWeights<T>::kFactors + k) * 8);
+    }
+    __device__ f16x8 sums8(uint32_t c, uint32_t kh) const { return *(const f16x8*)(moe_smem + sums + (c * 2 + kh) * 16); }
+    __device__ void put(uint32_t c, uint32_t r16, const uint32_t (&v)[4], int32_t bsum, double sc) const {
+        const uint4 w = ig_slots(T) ? q45_slots(v, r16 & 1) : make_uint4(v[0], v[1], v[2], v[3]);
+        *(uint4*)(moe_smem + q + (c * 16 + r16) * 16) = w;
+        if (ig_mins(T)) *(_Float16*)(moe_smem + sums + c * 32 + r16 * 2) = (_Float16)bsum;
+        if (T == kQ8_0) {
+            if (!(r16 & 1)) *(double*)(moe_smem + f + (c * 8 + (r16 >> 1)) * 8) = sc;
+        } else {
+            if (r16 == 0) *(double*)(moe_smem + f + c * 8) = sc;
+        }
+    }
+};
+template <uint32_t T>
+struct MoeGlobal {
+    const MoeImage& im;
+    uint32_t tokens, tok;  // tok: the lane's column
+    __device__ i32x4 act(uint32_t c, int s, uint32_t kh) const {
+        return *(const i32x4*)(im.q + (((uint64_t)c * 16 + s * 2 + kh) * tokens + tok) * 16);
+    }
+    __device__ double scale(uint32_t c, int k) const { return im.f[((uint64_t)c * MoeWeights<T>::kFactors + k) * tokens + tok]; }
+    __device__ f16x8 sums8(uint32_t c, uint32_t kh) const {
+        return *(const f16x8*)(im.sums + (((uint64_t)c * 2 + kh) * tokens + tok) * 8);
+    }
+};
 
 // Where a lane's rows have their current chunk, which one of the image it is, and
 // whether it counts (the last pair of chunks may have one only).  pairs: Q8_0
@@ -590,32 +668,33 @@ struct MoeAt {
 // move for each of the sixteen.)
 __device__ __forceinline__ uint32_t bits_or(uint32_t mask, uint32_t a, uint32_t b) { return (mask & b) | (~mask & a); }
 
-// One wave's chunks.  at(it): where step it is.  fold(f, term): adds a chunk's
+// One wave's chunks of src.  at(it): where step it is.  stage(): called once, by every
+// wave, while the first weights are on their way.  fold(f, term): adds a chunk's
 // (Q8_0: a block's) products, term(i, fa, y) being y plus fa times product i of the
 // lane's row; f: the 32 column scales.  HALVES: rows of the second half take the
 // columns from 16 on.  R: k-steps whose activations are in flight.
-template <uint32_t T, bool HALVES, int R, typename At, typename Fold>
-__device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, uint32_t tok, uint32_t steps, uint32_t ln,
-                                         uint32_t kh, double* fd, At&& at, Fold&& fold) {
+template <uint32_t T, bool HALVES, int R, typename Src, typename At, typename Stage, typename Fold>
+__device__ __forceinline__ void moe_walk(const Src& src, uint32_t steps, uint32_t ln, uint32_t kh, double* fd, At&& at,
+                                         Stage&& stage, Fold&& fold) {
     using M = MoeWeights<T>;
-    if (steps == 0) return;
+    if (steps == 0) {
+        stage();
+        return;
+    }
     const uint32_t n = ln & 15;
     const uint32_t upper = HALVES && ln >= 16 ? ~0u : 0u;
     M m;
     i32x4 act[R];
     f16x8 bs;
     double f[M::kFactors];
-    const uint64_t sq = (uint64_t)tokens * 16;  // bytes of one k half
-    auto load_act = [&](int s, uint32_t c) {
-        act[s % R] = *(const i32x4*)(im.q + ((uint64_t)c * 16 + s * 2 + kh) * sq + tok * 16);
-    };
+    auto load_act = [&](int s, uint32_t c) { act[s % R] = src.act(c, s, kh); };
     auto load_scales = [&](const MoeAt& p) {
 #pragma unroll
         for (int k = 0; k < M::kFactors; ++k) {
-            const double v = im.f[((uint64_t)p.chunk * M::kFactors + k) * tokens + tok];
+            const double v = src.scale(p.chunk, k);
             f[k] = p.live ? v : 0.0;
         }
-        if constexpr (ig_mins(T)) bs = *(const f16x8*)(im.sums + (((uint64_t)p.chunk * 2 + kh) * tokens + tok) * 8);
+        if constexpr (ig_mins(T)) bs = src.sums8(p.chunk, kh);
     };
     auto pair_of = [&](const MoeAt& p, uint32_t k) { return p.w + (k < p.pairs ? k : p.pairs - 1) * kQ80Chunk; };
     auto load_q8 = [&](const MoeAt& p, int s) {
@@ -628,9 +707,13 @@ __device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, ui
         }
     };
     MoeAt p = at(0);
+    auto first_acts = [&] {
 #pragma unroll
-    for (int s = 0; s < R; ++s) load_act(s, p.chunk);
-    load_scales(p);
+        for (int s = 0; s < R; ++s) load_act(s, p.chunk);
+        load_scales(p);
+    };
+    constexpr bool kStaged = std::is_same<Src, MoeLds<T>>::value;
+    if (!kStaged) first_acts();
     if constexpr (T == kQ8_0) {
 #pragma unroll
         for (int s = 0; s < 8; ++s) load_q8(p, s);
@@ -638,6 +721,8 @@ __device__ __forceinline__ void moe_walk(const MoeImage& im, uint32_t tokens, ui
     } else {
         ig_load<T>(m.r, p.w, n, kh);
     }
+    stage();
+    if (kStaged) first_acts();
     // one step; more: the next step's loads follow the last use of what they replace
     auto step = [&](auto more_, uint32_t it) {
         constexpr bool more = decltype(more_)::value;
@@ -726,40 +811,73 @@ __device__ __forceinline__ uint32_t moe_pairs(uint32_t npairs, uint32_t c) {
 // waves a SIMD, 14.1 with a whole chunk ahead).  32 columns' sums leave room for three
 // waves a SIMD (32 tokens 133 us, 156 with the compiler's choice of two; 148 with a
 // whole chunk ahead, which spills).
-template <uint32_t T, int KS, int NQ>
+//
+// kMoeOne, kMoeOnePacked: a single token, without a plan: every workgroup reads the
+// ids and makes the image of x in LDS while its first weights are on their way.
+enum MoeFrom { kMoePlan, kMoeOne, kMoeOnePacked };
+template <uint32_t T, int KS, int NQ, MoeFrom FROM>
 __global__ __launch_bounds__(64 * KS) __attribute__((amdgpu_waves_per_eu(NQ == 4 ? 3 : (NQ == 2 || T == kQ8_0 ? 4 : 2)))) void
 moe_up_kernel(MoeArgs a) {
-    extern __shared__ __align__(16) double lds[];
+    constexpr bool ONE = FROM != kMoePlan;
+    constexpr uint32_t kF = MoeWeights<T>::kFactors;
+    __shared__ uint32_t bad;
     const uint32_t lane = threadIdx.x & 63, kg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t ln = lane & 31, kh = lane >> 5;
     const uint32_t j = blockIdx.x / a.up_tiles, tile = blockIdx.x - j * a.up_tiles;
-    if (blockIdx.x == 0)  // the prepare launch's flags, for the down kernel
-        for (uint32_t i = threadIdx.x; i < a.x_chunks * a.tokens; i += 64 * KS)
-            if (a.flags[i]) atomicOr(&a.bad[i % a.tokens], 1u);
-    if (j >= *a.n_used) return;
-    const uint32_t live = (uint32_t)__builtin_popcount(a.mask[j]), nchunk = a.x_chunks;
-    const uint32_t tok = a.column[j * kMoeTokens + (ln < live ? ln : 0)];
-    const uint8_t* wt = ((ln >> 4) ? a.up : a.gate) + (uint64_t)a.expert[j] * a.up_bytes + (uint64_t)tile * a.x_row_bytes;
-    double* part = lds;
-    double* fd = lds + KS * NQ * 4 * 64 + kg * (MoeWeights<T>::kFactors * 32);
+    uint32_t mask = 1, base = j, expert;
+    if constexpr (ONE) {
+        const MoePlaces p = moe_places(a);
+        if (p.wrong >= 0) {
+            if (blockIdx.x == 0 && threadIdx.x == 0) report_error(a.err_word, bounds_key((uint64_t)a.token0 * a.slots + p.wrong));
+            return;
+        }
+        if (j >= (uint32_t)__builtin_popcountll(p.some)) return;
+        unsigned long long left = p.some;
+        for (uint32_t k = 0; k < j; ++k) left &= left - 1;
+        expert = (uint32_t)__builtin_amdgcn_readlane(p.id, __builtin_ctzll(left));
+    } else {
+        if (j >= *a.n_used) return;
+        mask = a.mask[j], base = a.base[j], expert = a.expert[j];
+    }
+    const uint32_t live = (uint32_t)__builtin_popcount(mask), nchunk = a.x_chunks;
+    const uint8_t* wt = ((ln >> 4) ? a.up : a.gate) + (uint64_t)expert * a.up_bytes + (uint64_t)tile * a.x_row_bytes;
+    double* part = (double*)moe_smem;
+    double* fd = part + KS * NQ * 4 * 64 + kg * (kF * 32);
     double y[NQ * 4];
 #pragma unroll
     for (int i = 0; i < NQ * 4; ++i) y[i] = 0.0;
     const uint32_t steps = kg < nchunk ? (nchunk - 1 - kg) / KS + 1 : 0;
-    moe_walk<T, false, NQ == 1 && T != kQ8_0 ? 8 : 4>(
-        a.xi, a.tokens, tok, steps, ln, kh, fd,
-        [&](uint32_t it) {
-            const uint32_t c = kg + it * KS;
-            return MoeAt{wt + (uint64_t)c * MoeWeights<T>::kChunk, c, moe_pairs(a.x_pairs, c), true};
-        },
-        [&](const double* f, auto&& term) {
+    const MoeLds<T> xs(moe_lds<T>(KS, NQ * 4), nchunk);
+    auto at = [&](uint32_t it) {
+        const uint32_t c = kg + it * KS;
+        return MoeAt{wt + (uint64_t)c * MoeWeights<T>::kChunk, c, moe_pairs(a.x_pairs, c), true};
+    };
+    auto fold = [&](const double* f, auto&& term) {
 #pragma unroll
-            for (int q = 0; q < NQ; ++q)
-                if ((uint32_t)(8 * q) < live) {
+        for (int q = 0; q < NQ; ++q)
+            if ((uint32_t)(8 * q) < live) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) y[4 * q + k] = term(4 * q + k, f[8 * q + 4 * kh + k], y[4 * q + k]);
-                }
-        });
+                for (int k = 0; k < 4; ++k) y[4 * q + k] = term(4 * q + k, f[8 * q + 4 * kh + k], y[4 * q + k]);
+            }
+    };
+    if constexpr (ONE) {
+        auto stage = [&] {
+            if (threadIdx.x == 0) bad = 0;
+            __syncthreads();
+            for (uint32_t c = threadIdx.x >> 4; c < nchunk; c += 4 * KS) {
+                uint32_t q[4];
+                int32_t bsum;
+                double f;
+                if (moe_x<T, FROM == kMoeOnePacked>(a, c, lane & 15, 0, blockIdx.x == 0, q, bsum, f)) bad = 1;
+                xs.put(c, lane & 15, q, bsum, f);
+            }
+            __syncthreads();
+        };
+        moe_walk<T, false, 4>(xs, steps, ln, kh, fd, at, stage, fold);
+    } else {
+        const MoeGlobal<T> x{a.xi, a.tokens, a.column[j * kMoeTokens + (ln < live ? ln : 0)]};
+        moe_walk<T, false, NQ == 1 && T != kQ8_0 ? 8 : 4>(x, steps, ln, kh, fd, at, [] {}, fold);
+    }
 #pragma unroll
     for (int i = 0; i < NQ * 4; ++i) part[(kg * NQ * 4 + i) * 64 + lane] = y[i];
     __syncthreads();
@@ -772,12 +890,13 @@ moe_up_kernel(MoeArgs a) {
             u += part[(k * NQ * 4 + i) * 64 + l + 16];
         }
         const double gf = (double)(float)g, uf = (double)(float)u;
-        const float h = (float)(gf / (1.0 + exp(-gf)) * uf);
+        float h = (float)(gf / (1.0 + exp(-gf)) * uf);
         if (!finite(h)) {
-            const uint32_t t = a.column[j * kMoeTokens + c];
-            moe_bad(a, t, model_key(a.token0 + t, kStDownIn, 0));
+            const uint32_t t = ONE ? 0 : a.column[j * kMoeTokens + c];
+            if (ONE ? bad != 0 : moe_marked(a.xi.f, a.tokens, t, 0, nchunk, kF)) h = __builtin_nanf("");
+            else report_error(a.err_word, model_key(a.token0 + t, kStDownIn, 0));
         }
-        a.h[(uint64_t)(a.base[j] + c) * a.ffn + tile * 16 + r] = h;
+        a.h[(uint64_t)(base + c) * a.ffn + tile * 16 + r] = h;
     }
 }
 
@@ -788,48 +907,86 @@ moe_up_kernel(MoeArgs a) {
 // Where the tiles alone leave CUs idle, `parts` workgroups share a tile: they put
 // their f64 sums where all can read them (by exchanges whose results are waited for,
 // as the router does), and the last to arrive adds them in part order.
-template <uint32_t T, int KS, int NQ>
+//
+// ONE: a single token.  Every workgroup reads the ids, and makes the image of its part
+// of h in LDS while its first weights are on their way.
+template <uint32_t T, int KS, int NQ, bool ONE>
 __global__ __launch_bounds__(64 * KS) __attribute__((amdgpu_waves_per_eu(KS == 16 ? 4 : 3))) void
 moe_down_kernel(MoeArgs a) {
     constexpr bool HALVES = NQ < 4;
     constexpr uint32_t kRows = HALVES ? 16 : 32, kStep = HALVES ? 2 : 1;
-    extern __shared__ __align__(16) double lds[];
     __shared__ uint16_t expert[kMoeMaxExperts];
-    __shared__ uint32_t last;
+    __shared__ float weight[ONE ? kMoeMaxSlots : 1];
+    __shared__ uint32_t last, marked;
     const uint32_t lane = threadIdx.x & 63, kg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t ln = lane & 31, kh = lane >> 5, hf = ln >> 4;
     const uint32_t tile = blockIdx.x / a.parts, part = blockIdx.x - tile * a.parts;
-    const uint32_t nchunk = a.h_chunks, used = *a.n_used;
+    const uint32_t nchunk = a.h_chunks;
+    uint32_t used, bad = 0;  // bad: tokens whose ids are out of range
+    if constexpr (ONE) {
+        const MoePlaces p = moe_places(a);
+        bad = p.wrong >= 0;
+        used = bad ? 0 : (uint32_t)__builtin_popcountll(p.some);
+        if (kg == 0 && ((p.some >> lane) & 1)) {
+            const uint32_t j = (uint32_t)__builtin_popcountll(p.some & ((1ull << lane) - 1));
+            expert[j] = (uint16_t)p.id, weight[j] = a.weights[lane];
+        }
+        if (threadIdx.x == 0) marked = 0;
+    } else {
+        used = *a.n_used, bad = *a.bad;
+        for (uint32_t i = threadIdx.x; i < used; i += 64 * KS) expert[i] = (uint16_t)a.expert[i];
+    }
+    __syncthreads();
     // this part's chunks, whole steps of them but for the last part's end
     const uint32_t all = used * nchunk, steps_all = (all + kStep - 1) / kStep;
     const uint32_t c0 = (uint32_t)((uint64_t)steps_all * part / a.parts) * kStep;
     const uint32_t c1 = part + 1 < a.parts ? (uint32_t)((uint64_t)steps_all * (part + 1) / a.parts) * kStep : all;
-    for (uint32_t i = threadIdx.x; i < used; i += 64 * KS) expert[i] = (uint16_t)a.expert[i];
-    __syncthreads();
     const uint32_t col = HALVES ? ln & 15 : ln, tok = col < a.tokens ? col : a.tokens - 1;
     uint32_t t16 = HALVES ? tile : 2 * tile + hf;
     t16 = t16 < a.out_tiles ? t16 : a.out_tiles - 1;  // (rows past the end are never stored)
     const uint8_t* wt = a.down + (uint64_t)t16 * a.h_row_bytes;
     constexpr int kSums = NQ * 4;
-    double* sums = lds;
-    double* fd = lds + KS * kSums * 64 + kg * (MoeWeights<T>::kFactors * 32);
+    constexpr uint32_t kF = MoeWeights<T>::kFactors;
+    double* sums = (double*)moe_smem;
+    double* fd = sums + KS * kSums * 64 + kg * (kF * 32);
     double y[kSums];
 #pragma unroll
     for (int i = 0; i < kSums; ++i) y[i] = 0.0;
     const uint32_t first = c0 + kStep * kg, steps = first < c1 ? (c1 - 1 - first) / (kStep * KS) + 1 : 0;
-    moe_walk<T, HALVES, 4>(
-        a.hi, a.tokens, tok, steps, ln, kh, fd,
-        [&](uint32_t it) {
-            const uint32_t want = first + it * (kStep * KS) + (HALVES ? hf : 0), at = want < c1 ? want : c1 - 1;
-            const uint32_t j = at / nchunk, c = at - j * nchunk;
-            return MoeAt{wt + (uint64_t)expert[j] * a.down_bytes + (uint64_t)c * MoeWeights<T>::kChunk, at,
-                         moe_pairs(a.h_pairs, c), want < c1};
-        },
-        [&](const double* f, auto&& term) {
+    auto at = [&](uint32_t it) {
+        const uint32_t want = first + it * (kStep * KS) + (HALVES ? hf : 0), i = want < c1 ? want : c1 - 1;
+        const uint32_t j = i / nchunk, c = i - j * nchunk;
+        return MoeAt{wt + (uint64_t)expert[j] * a.down_bytes + (uint64_t)c * MoeWeights<T>::kChunk, ONE ? i - c0 : i,
+                     moe_pairs(a.h_pairs, c), want < c1};
+    };
+    auto fold = [&](const double* f, auto&& term) {
 #pragma unroll
-            for (int i = 0; i < kSums; ++i)
-                y[i] = term(i, f[(HALVES ? 16 * hf : 0) + 8 * (i / 4) + 4 * kh + i % 4], y[i]);
-        });
+        for (int i = 0; i < kSums; ++i) y[i] = term(i, f[(HALVES ? 16 * hf : 0) + 8 * (i / 4) + 4 * kh + i % 4], y[i]);
+    };
+    if constexpr (ONE) {
+        const MoeLds<T> hs(moe_lds<T>(KS, kSums), c1 - c0);
+        auto stage = [&] {
+            const uint32_t r16 = lane & 15;
+            for (uint32_t i = c0 + (threadIdx.x >> 4); i < c1; i += 4 * KS) {
+                const uint32_t j = i / nchunk, c = i - j * nchunk, e0 = c * 256 + r16 * 16;
+                float v[16], d;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = 0.0f;
+                if (e0 < a.ffn) moe_load16(a.h + (uint64_t)j * a.ffn + e0, v);
+                uint32_t q[4], index;
+                int32_t bsum;
+                const int kind = image_quantize<T>(v, r16, q, d, bsum, index);
+                if (kind >= 0) marked = 1;
+                if (kind == kKindScale && tile == 0 && (T == kQ8_0 ? !(r16 & 1) : r16 == 0))
+                    report_error(a.err_word, model_key(a.token0, kStDownQuant, T == kQ8_0 ? e0 / 32 : c));
+                hs.put(i - c0, r16, q, bsum, (double)weight[j] * (double)d);
+            }
+            __syncthreads();
+        };
+        moe_walk<T, HALVES, 4>(hs, steps, ln, kh, fd, at, stage, fold);
+    } else {
+        moe_walk<T, HALVES, 4>(MoeGlobal<T>{a.hi, a.tokens, tok}, steps, ln, kh, fd, at, [] {}, fold);
+    }
 #pragma unroll
     for (int i = 0; i < kSums; ++i) sums[(kg * kSums + i) * 64 + lane] = y[i];
     __syncthreads();
@@ -842,11 +999,12 @@ moe_down_kernel(MoeArgs a) {
             v += sums[(k * kSums + i) * 64 + l];
             if (HALVES) v += sums[(k * kSums + i) * 64 + l + 16];
         }
-        return v;
+        const bool off = ONE ? marked != 0 : v != v && moe_marked(a.hi.f, a.tokens, t, c0, c1, kF);
+        return off ? moe_bad_scale() : v;
     };
     auto store = [&](uint32_t o, double v) {
         const uint32_t t = o / kRows, row = tile * kRows + o % kRows;
-        if (row >= a.out_rows || a.bad[t]) return;
+        if (row >= a.out_rows || ((bad >> t) & 1) || moe_is_bad(v)) return;
         const uint64_t to = (uint64_t)t * a.out_rows + row;
         a.y[to] = (float)(a.residual ? (double)a.residual[to] + v : v);
     };
@@ -871,10 +1029,14 @@ moe_down_kernel(MoeArgs a) {
     if (!last) return;
     for (uint32_t o = threadIdx.x; o < n; o += 64 * KS) {
         double v = 0.0;
-        for (uint32_t p = 0; p < a.parts; ++p)
-            v += __longlong_as_double((long long)__hip_atomic_load(a.sums + ((uint64_t)tile * a.parts + p) * n + o,
-                                                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-        store(o, v);
+        bool off = false;
+        for (uint32_t p = 0; p < a.parts; ++p) {
+            const double one = __longlong_as_double((long long)__hip_atomic_load(
+                a.sums + ((uint64_t)tile * a.parts + p) * n + o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+            off |= moe_is_bad(one);
+            v += one;
+        }
+        store(o, off ? moe_bad_scale() : v);
     }
 }
 
@@ -902,8 +1064,6 @@ static uint32_t moe_parts(const MoeCall& c, uint32_t tokens) {
     parts = parts < steps ? parts : steps;
     return (uint32_t)(parts < 1 ? 1 : parts < 8 ? parts : 8);
 }
-uint64_t moe_counters(const MoeCall& c) { return layout_tiles(c.out_rows); }
-
 // The scratch of a pass; base null: only its size.
 static size_t moe_carve(const MoeCall& c, uint32_t tokens, uint8_t* base, MoeArgs* a) {
     uint64_t at = 0;
@@ -919,16 +1079,16 @@ static size_t moe_carve(const MoeCall& c, uint32_t tokens, uint8_t* base, MoeArg
         im.f = (double*)take(chunks * tokens * (t == kQ8_0 ? 64 : 8));
         return im;
     };
-    const uint64_t pairs = (uint64_t)tokens * c.slots, used = pairs < c.experts ? pairs : c.experts;
+    const uint64_t pairs = (uint64_t)tokens * c.slots;
+    const uint64_t used = pairs < c.experts || tokens == 1 ? pairs : c.experts;  // (one token: its places, each on its own)
     MoeArgs m{};
     m.n_used = (uint32_t*)take(4);
-    m.bad = (uint32_t*)take(kMoeTokens * 4);
+    m.bad = (uint32_t*)take(4);
     m.expert = (uint32_t*)take(used * 4);
     m.base = (uint32_t*)take(used * 4);
     m.mask = (uint32_t*)take(used * 4);
     m.column = take(used * kMoeTokens);
     m.wsum = (double*)take(used * kMoeTokens * 8);
-    m.flags = (uint32_t*)take(moe_chunks(c.cols) * tokens * 4);
     m.xi = image(c.up_type, moe_chunks(c.cols));
     m.h = (float*)take(pairs * c.ffn * 4);
     m.parts = moe_parts(c, tokens);
@@ -938,60 +1098,78 @@ static size_t moe_carve(const MoeCall& c, uint32_t tokens, uint8_t* base, MoeArg
     return at;
 }
 
+// What the largest of a call's passes needs (the last one may have fewer tokens).
 size_t moe_bytes(const MoeCall& c) {
-    return moe_carve(c, c.tokens < kMoeTokens ? (uint32_t)c.tokens : kMoeTokens, nullptr, nullptr);
+    const size_t most = moe_carve(c, c.tokens < kMoeTokens ? (uint32_t)c.tokens : kMoeTokens, nullptr, nullptr);
+    const uint32_t rest = (uint32_t)(c.tokens % kMoeTokens);
+    const size_t last = rest ? moe_carve(c, rest, nullptr, nullptr) : 0;
+    return most > last ? most : last;
 }
+
+// Arrival counters: one per tile of the down product.
+uint64_t moe_counters(const MoeCall& c) { return layout_tiles(c.out_rows); }
 
 // Whether every launch of the call stays below 2^32 threads and its chunks below
 // 2^31.
 bool moe_takes(const MoeCall& c) {
     const uint64_t t = c.tokens < kMoeTokens ? c.tokens : kMoeTokens;
-    const uint64_t used = t * c.slots < c.experts ? t * c.slots : c.experts;
+    const uint64_t used = t * c.slots < c.experts || t == 1 ? t * c.slots : c.experts;
     return c.experts <= kMoeMaxExperts && c.slots <= kMoeMaxSlots && c.tokens <= 65535 && c.cols <= (1u << 30) &&
            c.ffn <= (1u << 30) && used * layout_tiles(c.ffn) * 1024 <= 0xffffffffull &&
            layout_tiles(c.out_rows) * 8 * 1024 <= 0xffffffffull && used * moe_chunks(c.ffn) * 512 <= 0xffffffffull &&
            (moe_chunks(c.cols) + 1) * 512 <= 0xffffffffull;
 }
 
-template <uint32_t T, int KS, int NQ>
+// Chunks of h that a workgroup of the down product has at most, of a single token.
+static uint32_t moe_one_chunks(const MoeArgs& a) {
+    const uint32_t all = a.slots * a.h_chunks;
+    return (all + a.parts - 1) / a.parts + 2;  // (a part is whole pairs)
+}
+// A single token whose x and h fit LDS takes two launches, others four.
+static bool moe_one(const MoeArgs& a) { return a.tokens == 1 && a.x_chunks <= 128 && moe_one_chunks(a) <= 320; }
+
+template <uint32_t T, int KS, int NQ, MoeFrom FROM>
 static hipError_t moe_up_launch(const MoeArgs& a, uint32_t used, hipStream_t s) {
     static LdsLimit lim;
-    constexpr uint32_t lds = moe_lds<T>(KS, NQ * 4);
-    const hipError_t e = lim.raise((const void*)moe_up_kernel<T, KS, NQ>, lds);
+    const uint32_t lds = moe_lds<T>(KS, NQ * 4) + (FROM == kMoePlan ? 0 : a.x_chunks * moe_lds_chunk<T>());
+    const hipError_t e = lim.raise((const void*)moe_up_kernel<T, KS, NQ, FROM>, lds + 64);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((moe_up_kernel<T, KS, NQ>), dim3(used * a.up_tiles), dim3(64 * KS), lds, s, a);
+    hipLaunchKernelGGL((moe_up_kernel<T, KS, NQ, FROM>), dim3(used * a.up_tiles), dim3(64 * KS), lds, s, a);
     return hipGetLastError();
 }
-template <uint32_t T, int KS, int NQ>
+template <uint32_t T, int KS, int NQ, bool ONE>
 static hipError_t moe_down_launch(const MoeArgs& a, hipStream_t s) {
     static LdsLimit lim;
-    constexpr uint32_t lds = moe_lds<T>(KS, NQ * 4), tiles = NQ < 4 ? 1 : 2;
-    const hipError_t e = lim.raise((const void*)moe_down_kernel<T, KS, NQ>, lds + 2 * kMoeMaxExperts);
+    constexpr uint32_t tiles = NQ < 4 ? 1 : 2;
+    const uint32_t lds = moe_lds<T>(KS, NQ * 4) + (ONE ? moe_one_chunks(a) * moe_lds_chunk<T>() : 0);
+    const hipError_t e = lim.raise((const void*)moe_down_kernel<T, KS, NQ, ONE>, lds + 2 * kMoeMaxExperts + 512);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((moe_down_kernel<T, KS, NQ>), dim3((a.out_tiles + tiles - 1) / tiles * a.parts), dim3(64 * KS), lds, s,
-                       a);
+    hipLaunchKernelGGL((moe_down_kernel<T, KS, NQ, ONE>), dim3((a.out_tiles + tiles - 1) / tiles * a.parts), dim3(64 * KS),
+                       lds, s, a);
     return hipGetLastError();
 }
 
 template <uint32_t T>
 static hipError_t moe_up_any(const MoeArgs& a, bool packed, uint32_t used, hipStream_t s) {
+    if (moe_one(a)) return packed ? moe_up_launch<T, 4, 1, kMoeOnePacked>(a, a.slots, s) : moe_up_launch<T, 4, 1, kMoeOne>(a, a.slots, s);
     const dim3 grid(1 + a.x_chunks);
     if (packed) hipLaunchKernelGGL((moe_prepare_kernel<T, true>), grid, dim3(512), 0, s, a);
     else hipLaunchKernelGGL((moe_prepare_kernel<T, false>), grid, dim3(512), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.tokens <= 8) return moe_up_launch<T, 4, 1>(a, used, s);
-    if (a.tokens <= 16) return moe_up_launch<T, 4, 2>(a, used, s);
-    return moe_up_launch<T, 2, 4>(a, used, s);
+    if (a.tokens <= 8) return moe_up_launch<T, 4, 1, kMoePlan>(a, used, s);
+    if (a.tokens <= 16) return moe_up_launch<T, 4, 2, kMoePlan>(a, used, s);
+    return moe_up_launch<T, 2, 4, kMoePlan>(a, used, s);
 }
 template <uint32_t T>
 static hipError_t moe_down_any(const MoeArgs& a, uint32_t used, hipStream_t s) {
+    if (moe_one(a)) return moe_down_launch<T, 16, 1, true>(a, s);
     hipLaunchKernelGGL((moe_h_kernel<T>), dim3(a.h_chunks, used), dim3((a.tokens * 16 + 63) / 64 * 64), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.tokens <= 8) return moe_down_launch<T, 16, 1>(a, s);
-    if (a.tokens <= 16) return moe_down_launch<T, 16, 2>(a, s);
-    return moe_down_launch<T, 12, 4>(a, s);
+    if (a.tokens <= 8) return moe_down_launch<T, 16, 1, false>(a, s);
+    if (a.tokens <= 16) return moe_down_launch<T, 16, 2, false>(a, s);
+    return moe_down_launch<T, 12, 4, false>(a, s);
 }
 
 hipError_t launch_moe_ffn(const MoeCall& c, void* scratch, hipStream_t s) {

@@ -245,13 +245,13 @@ struct MoeArgs {  // of one pass
     float* y;
     unsigned long long* err_word;
     // the plan and the workspace (moe.hip)
-    uint32_t *n_used, *bad, *expert, *base, *mask, *flags;
+    uint32_t *n_used, *bad, *expert, *base, *mask;
     uint8_t* column;
     double* wsum;
     MoeImage xi, hi;
     float* h;
     unsigned long long* sums;  // of the parts of the down product's tiles
-    uint32_t* count;           // 0 between launches: parts that have arrived, per tile
+    uint32_t* count;           // 0 between launches: parts that have arrived, per tile of y
 };
 
 // ---- llama.hip ----
