@@ -350,7 +350,8 @@ int32_t rlq_rms_norm(rlq_context *ctx, const float *x, const float *residual, co
  * slots at most 64, experts 1024, tokens 65535 (RLQ_UNIMPLEMENTED).  Pointers
  * 4-byte aligned (router and x 16 and cols % 4 == 0: wide loads).  A token with a
  * logit that is not finite gets ids of -1 and weights of 0: RLQ_NON_FINITE at
- * rlq_sync (a = RLQ_CHECK_MATRIX_OUTPUT, b = the token). */
+ * rlq_sync (a = RLQ_CHECK_MATRIX_OUTPUT, b = the token).
+ * Capturing: make the same call once before, for the scratch. */
 #define RLQ_ROUTE_SIGMOID 1u
 #define RLQ_ROUTE_NORMALIZE 2u
 int32_t rlq_moe_route(rlq_context *ctx, const float *router, const float *x, uint64_t tokens, uint64_t cols,
@@ -370,7 +371,7 @@ int32_t rlq_moe_route(rlq_context *ctx, const float *router, const float *x, uin
  * rounded once where g, u, h and y become f32, so y does not depend on what shares
  * a call.  h is quantized like any f32 column of down.  ids and weights [tokens,
  * slots]; -1: no expert (its weight is not looked at), a token without any gets
- * its residual.  residual may be null (0), and may be y.
+ * its residual, its x not being looked at.  residual may be null (0), and may be y.
  * 32 tokens share a pass over the weights of the experts that they use; more
  * tokens take further passes (a prompt is better served by rlq_mul_mat_id).
  * Capturing: make the same call once before, for the scratch.

@@ -180,7 +180,9 @@ hipError_t ensure_arrivals(rlq_context* ctx, uint64_t words, hipStream_t s) {
     bool grown = false;
     const hipError_t e = ensure(ctx, ctx->arrivals, (words * sizeof(uint32_t) + 7) / 8 * 8, s, &grown);
     if (e != hipSuccess || !grown) return e;
-    return launch_fill_u64((unsigned long long*)ctx->arrivals.p, ctx->arrivals.n / 8, 0ull, s);
+    const hipError_t f = launch_fill_u64((unsigned long long*)ctx->arrivals.p, ctx->arrivals.n / 8, 0ull, s);
+    if (f != hipSuccess) ctx->arrivals.n = 0;  // (not to be used)
+    return f;
 }
 
 struct DeviceGuard {

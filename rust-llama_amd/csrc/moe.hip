@@ -548,10 +548,16 @@ __global__ __launch_bounds__(512) void moe_prepare_kernel(MoeArgs a) {
     }
     const uint32_t c = blockIdx.x - 1, r16 = threadIdx.x & 15, t = threadIdx.x >> 4;
     if (t >= a.tokens) return;
+    bool some = false;  // x of a token without experts is not looked at
+    for (uint32_t s = r16; s < a.slots; s += 16) {
+        const int32_t id = a.ids[t * a.slots + s];
+        some |= id >= 0 && id < (int32_t)a.experts;
+    }
+    some = (__ballot(some) >> (threadIdx.x & 48)) & 0xffffu;
     uint32_t q[4];
     int32_t bsum;
     double f;
-    moe_x<T, PACKED>(a, c, r16, t, true, q, bsum, f);
+    moe_x<T, PACKED>(a, c, r16, t, some, q, bsum, f);
     image_put<T>(a.xi, a.tokens, c, r16, t, q, bsum, f);
 }
 
@@ -915,7 +921,7 @@ __global__ __launch_bounds__(64 * KS) __attribute__((amdgpu_waves_per_eu(KS == 1
 moe_down_kernel(MoeArgs a) {
     constexpr bool HALVES = NQ < 4;
     constexpr uint32_t kRows = HALVES ? 16 : 32, kStep = HALVES ? 2 : 1;
-    __shared__ uint16_t expert[kMoeMaxExperts];
+    __shared__ uint16_t expert[ONE ? kMoeMaxSlots : kMoeMaxExperts];
     __shared__ float weight[ONE ? kMoeMaxSlots : 1];
     __shared__ uint32_t last, marked;
     const uint32_t lane = threadIdx.x & 63, kg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1113,7 +1119,8 @@ uint64_t moe_counters(const MoeCall& c) { return layout_tiles(c.out_rows); }
 // 2^31.
 bool moe_takes(const MoeCall& c) {
     const uint64_t t = c.tokens < kMoeTokens ? c.tokens : kMoeTokens;
-    const uint64_t used = t * c.slots < c.experts || t == 1 ? t * c.slots : c.experts;
+    uint64_t used = t * c.slots < c.experts ? t * c.slots : c.experts;
+    used = used > c.slots ? used : c.slots;  // (a last token on its own)
     return c.experts <= kMoeMaxExperts && c.slots <= kMoeMaxSlots && c.tokens <= 65535 && c.cols <= (1u << 30) &&
            c.ffn <= (1u << 30) && used * layout_tiles(c.ffn) * 1024 <= 0xffffffffull &&
            layout_tiles(c.out_rows) * 8 * 1024 <= 0xffffffffull && used * moe_chunks(c.ffn) * 512 <= 0xffffffffull &&
@@ -1126,7 +1133,8 @@ static uint32_t moe_one_chunks(const MoeArgs& a) {
     return (all + a.parts - 1) / a.parts + 2;  // (a part is whole pairs)
 }
 // A single token whose x and h fit LDS takes two launches, others four.
-static bool moe_one(const MoeArgs& a) { return a.tokens == 1 && a.x_chunks <= 128 && moe_one_chunks(a) <= 320; }
+// (Q8_0's images are the largest: 256 chunks of h beside the waves' sums are 152 KB.)
+static bool moe_one(const MoeArgs& a) { return a.tokens == 1 && a.x_chunks <= 128 && moe_one_chunks(a) <= 256; }
 
 template <uint32_t T, int KS, int NQ, MoeFrom FROM>
 static hipError_t moe_up_launch(const MoeArgs& a, uint32_t used, hipStream_t s) {

@@ -558,3 +558,116 @@ def test_layer_of_the_three(ctx, tokens):
     assert np.linalg.norm(g - want) <= 1e-5 * np.linalg.norm(want)
     ctx.sync()
     L.close()
+
+
+@pytest.mark.parametrize("slots,cols,ffn,out,gate,down", [
+    (63, 256, 1024, 2080, DT.Q8_0, DT.Q8_0), (64, 256, 1024, 2080, DT.Q8_0, DT.Q8_0),
+    (63, 256, 1024, 2080, DT.Q4_K, DT.Q5_K), (64, 256, 1024, 2080, DT.Q4_K, DT.Q2_K),
+    (3, 32768, 64, 16, DT.Q8_0, DT.Q8_0), (3, 32800, 64, 16, DT.Q8_0, DT.Q8_0),
+    (2, 32768, 256, 40, DT.Q4_K, DT.Q6_K), (2, 33024, 256, 40, DT.Q5_K, DT.Q3_K)])
+def test_ffn_of_one_token_at_its_limits(ctx, slots, cols, ffn, out, gate, down):
+    """More places than experts, and as many values of x and of h as fit the LDS, and more."""
+    say("ffn one", slots, cols, ffn, out, gate.name, down.name)
+    L = Layer(ctx, 2, cols, ffn, out, gate, down, 170)
+    ids, weights = places(171, 1, 2, slots)
+    x = L.x(172, 1)
+    y = L.call(gpu(x), ids, weights)
+    ctx.sync()
+    L.check(y, quantized(act(gate), x), ids, weights)
+    L.close()
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 33])
+def test_ffn_does_not_look_at_x_without_experts(ctx, tokens):
+    say("ffn unseen x", tokens)
+    L = Layer(ctx, 3, 512, 256, 48, DT.Q4_K, DT.Q4_K, 175)
+    ids, weights = places(176, tokens, 3, 2)
+    x, res = L.x(177, tokens), normal(178, tokens, 48)
+    for t in {0, tokens - 1}:
+        ids[t] = -1
+        x[t, 5], x[t, 400] = np.nan, np.inf
+    y = L.call(gpu(x), ids, weights, residual=gpu(res))
+    ctx.sync()
+    L.check(y, quantized(DT.Q8_K, np.where((ids < 0).all(1, keepdims=True), np.float32(0), x)), ids, weights, res)
+    L.close()
+
+
+@pytest.mark.parametrize("down", [DT.Q4_K, DT.Q8_0], ids=lambda t: t.name)
+@pytest.mark.parametrize("tokens", [8, 16, 32])
+def test_ffn_of_several_bad_tokens(ctx, tokens, down):
+    """Every way of a token to fail in one call, where workgroups share the tiles of y."""
+    say("ffn several bad", tokens, down.name)
+    L = Layer(ctx, 4, 512, 4096, 48, DT.Q4_K, down, 180)
+    ids, weights = places(181, tokens, 4, 2)
+    x, res = L.x(182, tokens), normal(183, tokens, 48)
+    x[1, 300] = np.nan
+    x[2] *= np.float32(1e25)   # h is infinite
+    x[3] *= np.float32(1e-19)  # h's scale is (nearly) not a number
+    weights[4, 0] = np.nan     # no error
+    ids[5, 1] = 9
+    y = torch.full((tokens, 48), 7.0, device="cuda")
+    L.call(gpu(x), ids, weights, residual=gpu(res), y=y)
+    with pytest.raises(rlq.QuantError) as e:
+        ctx.sync()
+    assert (e.value.name, e.value.a) == ("Bounds", 11)
+    assert bool((y[[1, 2, 3, 5]] == 7.0).all()) and bool(torch.isnan(y[4]).all())
+    good = [t for t in range(tokens) if t not in (1, 2, 3, 4, 5)]
+    x[1:6], ids[1:6] = 0, -1
+    L.check(y, quantized(DT.Q8_K, x), ids, weights, res, rows=good)
+    ctx.sync()
+    L.close()
+
+
+@pytest.mark.parametrize("tokens,experts,cols,k", [(1, 8, 1024, 2), (3, 128, 512, 8), (40, 128, 2048, 8), (300, 60, 896, 6),
+                                                   (20, 30, 17000, 3)])
+def test_route_replayed(ctx, tokens, experts, cols, k):
+    """The counts by which workgroups know each other are as they were after every
+    call: replays among eager calls of other sizes."""
+    say("route replayed", tokens, experts, cols, k)
+    c = rlq.Context(0)
+    router, x = gpu(normal(190, experts, cols) / np.float32(np.sqrt(cols))), torch.zeros((tokens, cols), device="cuda")
+    c.moe_route(router, x, k)
+    c.sync()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ids, weights, _ = c.moe_route(router, x, k)
+    for n in range(4):
+        rows = normal(191 + n, tokens, cols)
+        x.copy_(gpu(rows))
+        graph.replay()
+        wi, ww = plain_route(router.cpu().numpy(), rows, k)[1:]
+        assert np.array_equal(ids.cpu().numpy(), wi)
+        assert np.all(np.abs(weights.cpu().numpy() - ww) <= (2.0 ** -24 + 2.0 ** -45) * np.abs(ww) + 2.0 ** -150)
+        eager = c.moe_route(router, x, k)
+        assert torch.equal(eager[0], ids) and torch.equal(eager[1], weights)
+        check_route(c, normal(195, 64, 64), normal(196 + n, 50 * n + 1, 64), 2)
+    c.sync()
+    c.close()
+
+
+@pytest.mark.parametrize("tokens", [1, 7, 33])
+def test_ffn_replayed(ctx, tokens):
+    say("ffn replayed", tokens)
+    c = rlq.Context(0)
+    L = Layer(c, 6, 512, 2048, 256, DT.Q5_K, DT.Q6_K, 200)
+    x, ids, weights = torch.zeros((tokens, 512), device="cuda"), *map(gpu, places(201, tokens, 6, 2))
+    c.moe_ffn(*L.w, x, ids, weights)
+    c.sync()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = c.moe_ffn(*L.w, x, ids, weights)
+    for n in range(4):
+        i, w = places(202 + n, tokens, 6, 2, 0.2)
+        ids.copy_(gpu(i)), weights.copy_(gpu(w)), x.copy_(gpu(L.x(206 + n, tokens)))
+        graph.replay()
+        eager = c.moe_ffn(*L.w, x, ids, weights)
+        c.sync()
+        assert torch.equal(y, eager)
+        L.check(y, quantized(DT.Q8_K, x.cpu().numpy()), i, w)
+        other = 1 + 12 * n  # of another number of parts
+        i, w = places(210, other, 6, 2)
+        c.moe_ffn(*L.w, gpu(L.x(211, other)), gpu(i), gpu(w))
+    c.sync()
+    L.close(), c.close()
