@@ -349,15 +349,18 @@ hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s) {
 // is one column of it, with the sum of both weights.  A single token has no
 // plan: its places that name an expert are read from ids where they are needed.
 //
-// An image holds activations of T tokens in chunks of 256 values (of a Q8_0 row's
-// last chunk, a part; the rest is 0):
-//   q     [chunk][k-step 8][k half 2][token][16 int8]
-//   sums  [chunk][k half 2][token][8 f16]      (weights with mins)
-//   f     [chunk][token] f64, for Q8_0 [chunk][k-step][token]: the block's scale
-//         (of h: times the token's weight for the expert, 0 without one)
-// in the slot order of rlq_layout.hpp for Q4_K and Q5_K.  x has one image (in LDS for a
-// single token), h one per expert in use, expert after expert, so that the down
-// product runs over all of them as over one long row.
+// The images hold activations in chunks of 256 values (of a Q8_0 row's last chunk, a
+// part; the rest is 0), in the slot order of rlq_layout.hpp for Q4_K and Q5_K: 256
+// levels, their 16 f16 sums (weights with mins) and a f64 scale (Q8_0: 8), of h times
+// the token's weight for the expert.
+//   x  [chunk][token], a chunk's levels in two lines of its own: an expert takes some
+//      of the tokens (32 tokens, 8 experts of 14336x4096 121 us against 135 with the
+//      tokens' 16-byte pieces side by side)
+//   h  expert after expert, so that the down product runs over all of them as over
+//      one long row; of each [chunk], and of that the pieces of its own tokens side by
+//      side: q [k-step 8][k half 2][column][16 int8], sums [k half 2][column][8 f16],
+//      f [column] or [k-step][column]
+// A single token's images lie in LDS.
 //
 // A block with a data error has kMoeBad as its scale.  That NaN reaches every sum of
 // its token, and who finds a sum to be a NaN looks whether the mark is among the
@@ -369,12 +372,7 @@ constexpr unsigned long long kMoeBad = 0x7ff8000000000001ull;
 __device__ __forceinline__ double moe_bad_scale() { return __longlong_as_double((long long)kMoeBad); }
 __device__ __forceinline__ bool moe_is_bad(double f) { return (unsigned long long)__double_as_longlong(f) == kMoeBad; }
 
-// Whether the mark is among token t's scales of chunks c0 .. c1 - 1 (k a chunk).
-__device__ __forceinline__ bool moe_marked(const double* f, uint32_t tokens, uint32_t t, uint32_t c0, uint32_t c1, uint32_t k) {
-    for (uint64_t i = (uint64_t)c0 * k; i < (uint64_t)c1 * k; ++i)
-        if (moe_is_bad(f[i * tokens + t])) return true;
-    return false;
-}
+__device__ __forceinline__ bool moe_is_out(double f) { return (unsigned long long)__double_as_longlong(f) == 1ull << 63; }
 
 // The places of a single token that name an expert (bit s), and whether one is out
 // of range; every wave for itself.
@@ -462,18 +460,18 @@ __device__ __forceinline__ void moe_load16(const float* p, float (&v)[16]) {
     }
 }
 
-// One lane's 16 values (r16 of a chunk's 16 lanes) of token t into an image for
-// weights of type T.
+// One lane's 16 values (r16 of a chunk's 16 lanes) into an image for weights of type T:
+// column c of n that lie side by side, the first at place `at` of the image.
 template <uint32_t T>
-__device__ __forceinline__ void image_put(const MoeImage& im, uint32_t tokens, uint64_t chunk, uint32_t r16, uint32_t t,
+__device__ __forceinline__ void image_put(const MoeImage& im, uint64_t at, uint32_t c, uint32_t n, uint32_t r16,
                                           const uint32_t (&q)[4], int32_t bsum, double f) {
     const uint4 w = ig_slots(T) ? q45_slots(q, r16 & 1) : make_uint4(q[0], q[1], q[2], q[3]);
-    *(uint4*)(im.q + ((chunk * 16 + r16) * tokens + t) * 16) = w;
-    if constexpr (ig_mins(T)) im.sums[((chunk * 2 + (r16 >> 3)) * tokens + t) * 8 + (r16 & 7)] = (_Float16)bsum;
+    *(uint4*)(im.q + at * 256 + (r16 * n + c) * 16) = w;
+    if constexpr (ig_mins(T)) im.sums[at * 16 + ((r16 >> 3) * n + c) * 8 + (r16 & 7)] = (_Float16)bsum;
     if constexpr (T == kQ8_0) {
-        if (!(r16 & 1)) im.f[(chunk * 8 + (r16 >> 1)) * tokens + t] = f;
+        if (!(r16 & 1)) im.f[at * 8 + (r16 >> 1) * n + c] = f;
     } else {
-        if (r16 == 0) im.f[chunk * tokens + t] = f;
+        if (r16 == 0) im.f[at + c] = f;
     }
 }
 
@@ -558,7 +556,7 @@ __global__ __launch_bounds__(512) void moe_prepare_kernel(MoeArgs a) {
     int32_t bsum;
     double f;
     moe_x<T, PACKED>(a, c, r16, t, some, q, bsum, f);
-    image_put<T>(a.xi, a.tokens, c, r16, t, q, bsum, f);
+    image_put<T>(a.xi, (uint64_t)c * a.tokens + t, 0, 1, r16, q, bsum, f);
 }
 
 // h of expert j's tokens, one chunk, into the image for down matrices of type T.  (A
@@ -570,20 +568,21 @@ template <uint32_t T>
 __global__ __launch_bounds__(512) void moe_h_kernel(MoeArgs a) {
     const uint32_t c = blockIdx.x, j = blockIdx.y, r16 = threadIdx.x & 15, t = threadIdx.x >> 4;
     if (j >= *a.n_used || t >= a.tokens) return;
-    const uint32_t mask = a.mask[j], e0 = c * 256 + r16 * 16;
-    const bool mine = (mask >> t) & 1u;
+    const uint32_t mask = a.mask[j], n = (uint32_t)__builtin_popcount(mask), e0 = c * 256 + r16 * 16;
+    if (!((mask >> t) & 1u)) return;
+    const uint32_t col = (uint32_t)__builtin_popcount(mask & ((1u << t) - 1)), row = a.base[j] + col;
     float v[16];
 #pragma unroll
     for (int k = 0; k < 16; ++k) v[k] = 0.0f;
-    if (mine && e0 < a.ffn) moe_load16(a.h + (uint64_t)(a.base[j] + (uint32_t)__builtin_popcount(mask & ((1u << t) - 1))) * a.ffn + e0, v);
+    if (e0 < a.ffn) moe_load16(a.h + (uint64_t)row * a.ffn + e0, v);
     uint32_t q[4], index;
     float d;
     int32_t bsum;
     const int kind = image_quantize<T>(v, r16, q, d, bsum, index);
     if (kind == kKindScale && (T == kQ8_0 ? !(r16 & 1) : r16 == 0))  // (a non-finite h has been reported)
         report_error(a.err_word, model_key(a.token0 + t, kStDownQuant, T == kQ8_0 ? e0 / 32 : c));
-    const double f = !mine ? 0.0 : kind >= 0 ? moe_bad_scale() : a.wsum[j * kMoeTokens + t] * (double)d;
-    image_put<T>(a.hi, a.tokens, (uint64_t)j * gridDim.x + c, r16, t, q, bsum, f);
+    const double f = kind >= 0 ? moe_bad_scale() : a.wsum[j * kMoeTokens + t] * (double)d;
+    image_put<T>(a.hi, (uint64_t)a.base[j] * gridDim.x + c * n, col, n, r16, q, bsum, f);
 }
 
 // ---------------------------------------------------------------------------
@@ -626,16 +625,31 @@ constexpr uint32_t moe_lds_chunk() {
 }
 extern __shared__ __align__(16) uint8_t moe_smem[];
 
-// Activations of one token in LDS, and of a pass in an image.
+// Where a lane's rows have their current chunk, which place of the image it is, and
+// whether it counts for the lane's column.  pairs: Q8_0 block pairs of the chunk (reading
+// stops there; the image is 0 beyond).  Of h, mask: the tokens whose columns are there;
+// col: the lane's one.
+struct MoeAt {
+    const uint8_t* w;
+    uint32_t chunk, pairs;
+    bool live;
+    uint32_t mask, col;
+    __device__ uint32_t columns() const { return (uint32_t)__builtin_popcount(mask); }
+};
+
+// Activations: of one token in LDS, of x and of h in global memory (images are below 4 GiB).
 template <uint32_t T>
 struct MoeLds {
+    static constexpr bool kStaged = true;
     uint32_t q, sums, f;  // offsets in moe_smem
     __device__ MoeLds(uint32_t at, uint32_t chunks) : q(at), sums(at + chunks * 256), f(at + chunks * 288) {}
-    __device__ i32x4 act(uint32_t c, int s, uint32_t kh) const { return *(const i32x4*)(moe_smem + q + (c * 16 + s * 2 + kh) * 16); }
-    __device__ double scale(uint32_t c, int k) const {
-        return *(const double*)(moe_smem + f + (c * MoeWeights<T>::kFactors + k) * 8);
+    __device__ i32x4 act(const MoeAt& p, int s, uint32_t kh) const {
+        return *(const i32x4*)(moe_smem + q + (p.chunk * 16 + s * 2 + kh) * 16);
     }
-    __device__ f16x8 sums8(uint32_t c, uint32_t kh) const { return *(const f16x8*)(moe_smem + sums + (c * 2 + kh) * 16); }
+    __device__ double scale(const MoeAt& p, int k) const {
+        return *(const double*)(moe_smem + f + (p.chunk * MoeWeights<T>::kFactors + k) * 8);
+    }
+    __device__ f16x8 sums8(const MoeAt& p, uint32_t kh) const { return *(const f16x8*)(moe_smem + sums + (p.chunk * 2 + kh) * 16); }
     __device__ void put(uint32_t c, uint32_t r16, const uint32_t (&v)[4], int32_t bsum, double sc) const {
         const uint4 w = ig_slots(T) ? q45_slots(v, r16 & 1) : make_uint4(v[0], v[1], v[2], v[3]);
         *(uint4*)(moe_smem + q + (c * 16 + r16) * 16) = w;
@@ -648,25 +662,30 @@ struct MoeLds {
     }
 };
 template <uint32_t T>
-struct MoeGlobal {
+struct MoeX {
+    static constexpr bool kStaged = false;
     const MoeImage& im;
     uint32_t tokens, tok;  // tok: the lane's column
-    __device__ i32x4 act(uint32_t c, int s, uint32_t kh) const {
-        return *(const i32x4*)(im.q + (((uint64_t)c * 16 + s * 2 + kh) * tokens + tok) * 16);
+    __device__ uint32_t place(const MoeAt& p) const { return p.chunk * tokens + tok; }
+    __device__ i32x4 act(const MoeAt& p, int s, uint32_t kh) const {
+        return *(const i32x4*)(im.q + (uint64_t)(place(p) * 256 + kh * 16) + s * 32);
     }
-    __device__ double scale(uint32_t c, int k) const { return im.f[((uint64_t)c * MoeWeights<T>::kFactors + k) * tokens + tok]; }
-    __device__ f16x8 sums8(uint32_t c, uint32_t kh) const {
-        return *(const f16x8*)(im.sums + (((uint64_t)c * 2 + kh) * tokens + tok) * 8);
-    }
+    __device__ double scale(const MoeAt& p, int k) const { return im.f[(uint64_t)(place(p) * MoeWeights<T>::kFactors) + k]; }
+    __device__ f16x8 sums8(const MoeAt& p, uint32_t kh) const { return *(const f16x8*)(im.sums + (place(p) * 16 + kh * 8)); }
 };
-
-// Where a lane's rows have their current chunk, which one of the image it is, and
-// whether it counts (the last pair of chunks may have one only).  pairs: Q8_0
-// block pairs of the chunk (reading stops there; the image is 0 beyond).
-struct MoeAt {
-    const uint8_t* w;
-    uint32_t chunk, pairs;
-    bool live;
+template <uint32_t T>
+struct MoeH {
+    static constexpr bool kStaged = false;
+    const MoeImage& im;
+    __device__ i32x4 act(const MoeAt& p, int s, uint32_t kh) const {
+        return *(const i32x4*)(im.q + (p.chunk * 16 + (s * 2 + kh) * p.columns() + p.col) * 16);
+    }
+    __device__ double scale(const MoeAt& p, int k) const {
+        return im.f[p.chunk * MoeWeights<T>::kFactors + k * p.columns() + p.col];
+    }
+    __device__ f16x8 sums8(const MoeAt& p, uint32_t kh) const {
+        return *(const f16x8*)(im.sums + (p.chunk * 2 + kh * p.columns() + p.col) * 8);
+    }
 };
 
 // b where mask is all ones, a where it is 0.  (A plain choice between two elements of
@@ -677,9 +696,11 @@ __device__ __forceinline__ uint32_t bits_or(uint32_t mask, uint32_t a, uint32_t 
 // One wave's chunks of src.  at(it): where step it is.  stage(): called once, by every
 // wave, while the first weights are on their way.  fold(f, term): adds a chunk's
 // (Q8_0: a block's) products, term(i, fa, y) being y plus fa times product i of the
-// lane's row; f: the 32 column scales.  HALVES: rows of the second half take the
+// lane's row; f: the 32 column scales, 0 where the chunk is not the column's.  GUARD:
+// there the products are left out, as weights may have scales that are not finite
+// (the scale is then -0, which none is otherwise).  HALVES: rows of the second half take the
 // columns from 16 on.  R: k-steps whose activations are in flight.
-template <uint32_t T, bool HALVES, int R, typename Src, typename At, typename Stage, typename Fold>
+template <uint32_t T, bool HALVES, int R, bool GUARD, typename Src, typename At, typename Stage, typename Fold>
 __device__ __forceinline__ void moe_walk(const Src& src, uint32_t steps, uint32_t ln, uint32_t kh, double* fd, At&& at,
                                          Stage&& stage, Fold&& fold) {
     using M = MoeWeights<T>;
@@ -693,14 +714,14 @@ __device__ __forceinline__ void moe_walk(const Src& src, uint32_t steps, uint32_
     i32x4 act[R];
     f16x8 bs;
     double f[M::kFactors];
-    auto load_act = [&](int s, uint32_t c) { act[s % R] = src.act(c, s, kh); };
+    auto load_act = [&](int s, const MoeAt& p) { act[s % R] = src.act(p, s, kh); };
     auto load_scales = [&](const MoeAt& p) {
 #pragma unroll
         for (int k = 0; k < M::kFactors; ++k) {
-            const double v = src.scale(p.chunk, k);
-            f[k] = p.live ? v : 0.0;
+            const double v = src.scale(p, k);
+            f[k] = GUARD ? (p.live ? v + 0.0 : -0.0) : (p.live ? v : 0.0);
         }
-        if constexpr (ig_mins(T)) bs = src.sums8(p.chunk, kh);
+        if constexpr (ig_mins(T)) bs = src.sums8(p, kh);
     };
     auto pair_of = [&](const MoeAt& p, uint32_t k) { return p.w + (k < p.pairs ? k : p.pairs - 1) * kQ80Chunk; };
     auto load_q8 = [&](const MoeAt& p, int s) {
@@ -715,11 +736,10 @@ __device__ __forceinline__ void moe_walk(const Src& src, uint32_t steps, uint32_
     MoeAt p = at(0);
     auto first_acts = [&] {
 #pragma unroll
-        for (int s = 0; s < R; ++s) load_act(s, p.chunk);
+        for (int s = 0; s < R; ++s) load_act(s, p);
         load_scales(p);
     };
-    constexpr bool kStaged = std::is_same<Src, MoeLds<T>>::value;
-    if (!kStaged) first_acts();
+    if (!Src::kStaged) first_acts();
     if constexpr (T == kQ8_0) {
 #pragma unroll
         for (int s = 0; s < 8; ++s) load_q8(p, s);
@@ -728,7 +748,7 @@ __device__ __forceinline__ void moe_walk(const Src& src, uint32_t steps, uint32_
         ig_load<T>(m.r, p.w, n, kh);
     }
     stage();
-    if (kStaged) first_acts();
+    if (Src::kStaged) first_acts();
     // one step; more: the next step's loads follow the last use of what they replace
     auto step = [&](auto more_, uint32_t it) {
         constexpr bool more = decltype(more_)::value;
@@ -739,8 +759,8 @@ __device__ __forceinline__ void moe_walk(const Src& src, uint32_t steps, uint32_
             for (int k = 0; k < M::kFactors; ++k) fd[k * 32 + ln] = f[k];
         }
         auto next_act = [&](int s) {
-            if (s + R < 8) load_act(s + R, p.chunk);
-            else if (more) load_act(s + R - 8, nx.chunk);
+            if (s + R < 8) load_act(s + R, p);
+            else if (more) load_act(s + R - 8, nx);
         };
         if constexpr (T == kQ8_0) {
             uint32_t dw4[4];
@@ -755,6 +775,7 @@ __device__ __forceinline__ void moe_walk(const Src& src, uint32_t steps, uint32_
                 if (more) load_q8(nx, s);
                 next_act(s);
                 fold(fd + s * 32, [&](int i, double fa, double y) {
+                    if (GUARD && moe_is_out(fa)) return y;
                     const int32_t v = HALVES ? (int32_t)bits_or(upper, I[i], I[i + 8 * HALVES]) : I[i];
                     return __builtin_fma((double)v, fa * dw, y);
                 });
@@ -781,6 +802,7 @@ __device__ __forceinline__ void moe_walk(const Src& src, uint32_t steps, uint32_
             if constexpr (ig_mins(T)) mn = __builtin_amdgcn_mfma_f32_32x32x16_f16(bs, mins, (f32x16){}, 0, 0, 0);
             if (more) load_scales(nx);
             fold(fd, [&](int i, double fa, double y) {
+                if (GUARD && moe_is_out(fa)) return y;
                 auto block = [&](int k) {
                     return W::kPlanes == 2 ? ((uint32_t)A[k] << W::kShift) + (uint32_t)B[k] : (uint32_t)A[k];
                 };
@@ -822,7 +844,7 @@ __device__ __forceinline__ uint32_t moe_pairs(uint32_t npairs, uint32_t c) {
 // ids and makes the image of x in LDS while its first weights are on their way.
 enum MoeFrom { kMoePlan, kMoeOne, kMoeOnePacked };
 template <uint32_t T, int KS, int NQ, MoeFrom FROM>
-__global__ __launch_bounds__(64 * KS) __attribute__((amdgpu_waves_per_eu(NQ == 4 ? 3 : (NQ == 2 || T == kQ8_0 ? 4 : 2)))) void
+__global__ __launch_bounds__(64 * KS) __attribute__((amdgpu_waves_per_eu(NQ >= 2 ? 3 : (T == kQ8_0 ? 4 : 2)))) void
 moe_up_kernel(MoeArgs a) {
     constexpr bool ONE = FROM != kMoePlan;
     constexpr uint32_t kF = MoeWeights<T>::kFactors;
@@ -856,7 +878,7 @@ moe_up_kernel(MoeArgs a) {
     const MoeLds<T> xs(moe_lds<T>(KS, NQ * 4), nchunk);
     auto at = [&](uint32_t it) {
         const uint32_t c = kg + it * KS;
-        return MoeAt{wt + (uint64_t)c * MoeWeights<T>::kChunk, c, moe_pairs(a.x_pairs, c), true};
+        return MoeAt{wt + (uint64_t)c * MoeWeights<T>::kChunk, c, moe_pairs(a.x_pairs, c), true, 0, 0};
     };
     auto fold = [&](const double* f, auto&& term) {
 #pragma unroll
@@ -879,10 +901,10 @@ moe_up_kernel(MoeArgs a) {
             }
             __syncthreads();
         };
-        moe_walk<T, false, 4>(xs, steps, ln, kh, fd, at, stage, fold);
+        moe_walk<T, false, 4, false>(xs, steps, ln, kh, fd, at, stage, fold);
     } else {
-        const MoeGlobal<T> x{a.xi, a.tokens, a.column[j * kMoeTokens + (ln < live ? ln : 0)]};
-        moe_walk<T, false, NQ == 1 && T != kQ8_0 ? 8 : 4>(x, steps, ln, kh, fd, at, [] {}, fold);
+        const MoeX<T> x{a.xi, a.tokens, a.column[j * kMoeTokens + (ln < live ? ln : 0)]};
+        moe_walk<T, false, NQ == 1 && T != kQ8_0 ? 8 : 4, false>(x, steps, ln, kh, fd, at, [] {}, fold);
     }
 #pragma unroll
     for (int i = 0; i < NQ * 4; ++i) part[(kg * NQ * 4 + i) * 64 + lane] = y[i];
@@ -899,7 +921,11 @@ moe_up_kernel(MoeArgs a) {
         float h = (float)(gf / (1.0 + exp(-gf)) * uf);
         if (!finite(h)) {
             const uint32_t t = ONE ? 0 : a.column[j * kMoeTokens + c];
-            if (ONE ? bad != 0 : moe_marked(a.xi.f, a.tokens, t, 0, nchunk, kF)) h = __builtin_nanf("");
+            bool marked = ONE && bad != 0;
+            if constexpr (!ONE) {
+                for (uint64_t k = 0; k < nchunk * kF; ++k) marked |= moe_is_bad(a.xi.f[(k / kF * a.tokens + t) * kF + k % kF]);
+            }
+            if (marked) h = __builtin_nanf("");
             else report_error(a.err_word, model_key(a.token0 + t, kStDownIn, 0));
         }
         a.h[(uint64_t)(base + c) * a.ffn + tile * 16 + r] = h;
@@ -921,7 +947,7 @@ __global__ __launch_bounds__(64 * KS) __attribute__((amdgpu_waves_per_eu(KS == 1
 moe_down_kernel(MoeArgs a) {
     constexpr bool HALVES = NQ < 4;
     constexpr uint32_t kRows = HALVES ? 16 : 32, kStep = HALVES ? 2 : 1;
-    __shared__ uint16_t expert[ONE ? kMoeMaxSlots : kMoeMaxExperts];
+    __shared__ uint2 plan[ONE ? kMoeMaxSlots : kMoeMaxExperts];  // expert | base << 16, mask
     __shared__ float weight[ONE ? kMoeMaxSlots : 1];
     __shared__ uint32_t last, marked;
     const uint32_t lane = threadIdx.x & 63, kg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -935,19 +961,19 @@ moe_down_kernel(MoeArgs a) {
         used = bad ? 0 : (uint32_t)__builtin_popcountll(p.some);
         if (kg == 0 && ((p.some >> lane) & 1)) {
             const uint32_t j = (uint32_t)__builtin_popcountll(p.some & ((1ull << lane) - 1));
-            expert[j] = (uint16_t)p.id, weight[j] = a.weights[lane];
+            plan[j] = make_uint2((uint32_t)p.id, 1), weight[j] = a.weights[lane];
         }
         if (threadIdx.x == 0) marked = 0;
     } else {
         used = *a.n_used, bad = *a.bad;
-        for (uint32_t i = threadIdx.x; i < used; i += 64 * KS) expert[i] = (uint16_t)a.expert[i];
+        for (uint32_t i = threadIdx.x; i < used; i += 64 * KS) plan[i] = make_uint2(a.expert[i] | a.base[i] << 16, a.mask[i]);
     }
     __syncthreads();
     // this part's chunks, whole steps of them but for the last part's end
     const uint32_t all = used * nchunk, steps_all = (all + kStep - 1) / kStep;
     const uint32_t c0 = (uint32_t)((uint64_t)steps_all * part / a.parts) * kStep;
     const uint32_t c1 = part + 1 < a.parts ? (uint32_t)((uint64_t)steps_all * (part + 1) / a.parts) * kStep : all;
-    const uint32_t col = HALVES ? ln & 15 : ln, tok = col < a.tokens ? col : a.tokens - 1;
+    const uint32_t tok = HALVES ? ln & 15 : ln;  // the lane's column
     uint32_t t16 = HALVES ? tile : 2 * tile + hf;
     t16 = t16 < a.out_tiles ? t16 : a.out_tiles - 1;  // (rows past the end are never stored)
     const uint8_t* wt = a.down + (uint64_t)t16 * a.h_row_bytes;
@@ -962,12 +988,28 @@ moe_down_kernel(MoeArgs a) {
     auto at = [&](uint32_t it) {
         const uint32_t want = first + it * (kStep * KS) + (HALVES ? hf : 0), i = want < c1 ? want : c1 - 1;
         const uint32_t j = i / nchunk, c = i - j * nchunk;
-        return MoeAt{wt + (uint64_t)expert[j] * a.down_bytes + (uint64_t)c * MoeWeights<T>::kChunk, ONE ? i - c0 : i,
-                     moe_pairs(a.h_pairs, c), want < c1};
+        const uint2 p = plan[j];
+        const uint8_t* w = wt + (uint64_t)(p.x & 0xffffu) * a.down_bytes + (uint64_t)c * MoeWeights<T>::kChunk;
+        const uint32_t pairs = moe_pairs(a.h_pairs, c);
+        if constexpr (ONE) return MoeAt{w, i - c0, pairs, want < c1, 1, 0};
+        const bool mine = (p.y >> tok) & 1u;  // others take the first column's levels, with no scale
+        const uint32_t n = (uint32_t)__builtin_popcount(p.y), before = (uint32_t)__builtin_popcount(p.y & ((1u << tok) - 1));
+        return MoeAt{w, (p.x >> 16) * nchunk + c * n, pairs, mine && want < c1, p.y, mine ? before : 0};
     };
     auto fold = [&](const double* f, auto&& term) {
 #pragma unroll
         for (int i = 0; i < kSums; ++i) y[i] = term(i, f[(HALVES ? 16 * hf : 0) + 8 * (i / 4) + 4 * kh + i % 4], y[i]);
+    };
+    // A sum that is not finite: once more, with the products that are not the column's
+    // left out.
+    auto again = [&] {
+        double all = 0.0;
+#pragma unroll
+        for (int i = 0; i < kSums; ++i) all += y[i] - y[i];
+        if (!__ballot(all != 0.0)) return false;
+#pragma unroll
+        for (int i = 0; i < kSums; ++i) y[i] = 0.0;
+        return true;
     };
     if constexpr (ONE) {
         const MoeLds<T> hs(moe_lds<T>(KS, kSums), c1 - c0);
@@ -989,9 +1031,11 @@ moe_down_kernel(MoeArgs a) {
             }
             __syncthreads();
         };
-        moe_walk<T, HALVES, 4>(hs, steps, ln, kh, fd, at, stage, fold);
+        moe_walk<T, HALVES, 2, false>(hs, steps, ln, kh, fd, at, stage, fold);
+        if (again()) moe_walk<T, HALVES, 2, true>(hs, steps, ln, kh, fd, at, [] {}, fold);
     } else {
-        moe_walk<T, HALVES, 4>(MoeGlobal<T>{a.hi, a.tokens, tok}, steps, ln, kh, fd, at, [] {}, fold);
+        moe_walk<T, HALVES, 4, false>(MoeH<T>{a.hi}, steps, ln, kh, fd, at, [] {}, fold);
+        if (again()) moe_walk<T, HALVES, 4, true>(MoeH<T>{a.hi}, steps, ln, kh, fd, at, [] {}, fold);
     }
 #pragma unroll
     for (int i = 0; i < kSums; ++i) sums[(kg * kSums + i) * 64 + lane] = y[i];
@@ -1005,7 +1049,16 @@ moe_down_kernel(MoeArgs a) {
             v += sums[(k * kSums + i) * 64 + l];
             if (HALVES) v += sums[(k * kSums + i) * 64 + l + 16];
         }
-        const bool off = ONE ? marked != 0 : v != v && moe_marked(a.hi.f, a.tokens, t, c0, c1, kF);
+        bool off = ONE && marked != 0;
+        if (!ONE && v != v) {
+            for (uint32_t c = c0; c < c1 && !off; ++c) {
+                const uint2 p = plan[c / nchunk];
+                if (!((p.y >> t) & 1u)) continue;
+                const uint32_t n = (uint32_t)__builtin_popcount(p.y), at = ((p.x >> 16) * nchunk + c % nchunk * n) * kF;
+                for (uint32_t k = 0; k < kF; ++k)
+                    off |= moe_is_bad(a.hi.f[at + k * n + (uint32_t)__builtin_popcount(p.y & ((1u << t) - 1))]);
+            }
+        }
         return off ? moe_bad_scale() : v;
     };
     auto store = [&](uint32_t o, double v) {
@@ -1064,8 +1117,8 @@ static uint64_t moe_out_tiles(const MoeCall& c, uint32_t tokens) {
 static uint32_t moe_parts(const MoeCall& c, uint32_t tokens) {
     const uint64_t tiles = moe_out_tiles(c, tokens), pairs = (uint64_t)tokens * c.slots;
     const uint64_t chunks = (pairs < c.experts ? pairs : c.experts) * moe_chunks(c.ffn);
-    // of 16 waves that take a pair of chunks a step, or 12 that take one
-    const uint64_t steps = tokens <= 16 ? (chunks + 31) / 32 : (chunks + 11) / 12;
+    // 16 or 12 waves that take a pair of chunks a step, or 12 that take one
+    const uint64_t step = tokens <= 8 ? 32 : tokens <= 16 ? 24 : 12, steps = (chunks + step - 1) / step;
     uint64_t parts = (uint64_t)device_cus() / tiles;
     parts = parts < steps ? parts : steps;
     return (uint32_t)(parts < 1 ? 1 : parts < 8 ? parts : 8);
@@ -1078,11 +1131,11 @@ static size_t moe_carve(const MoeCall& c, uint32_t tokens, uint8_t* base, MoeArg
         at += moe_align(bytes);
         return p;
     };
-    auto image = [&](uint32_t t, uint64_t chunks) {
+    auto image = [&](uint32_t t, uint64_t places) {
         MoeImage im;
-        im.q = take(chunks * tokens * 256);
-        im.sums = (_Float16*)take(ig_mins(t) ? chunks * tokens * 32 : 0);
-        im.f = (double*)take(chunks * tokens * (t == kQ8_0 ? 64 : 8));
+        im.q = take(places * 256);
+        im.sums = (_Float16*)take(ig_mins(t) ? places * 32 : 0);
+        im.f = (double*)take(places * (t == kQ8_0 ? 64 : 8));
         return im;
     };
     const uint64_t pairs = (uint64_t)tokens * c.slots;
@@ -1095,11 +1148,11 @@ static size_t moe_carve(const MoeCall& c, uint32_t tokens, uint8_t* base, MoeArg
     m.mask = (uint32_t*)take(used * 4);
     m.column = take(used * kMoeTokens);
     m.wsum = (double*)take(used * kMoeTokens * 8);
-    m.xi = image(c.up_type, moe_chunks(c.cols));
+    m.xi = image(c.up_type, moe_chunks(c.cols) * tokens);
     m.h = (float*)take(pairs * c.ffn * 4);
     m.parts = moe_parts(c, tokens);
     m.sums = (unsigned long long*)take(m.parts > 1 ? moe_out_tiles(c, tokens) * m.parts * tokens * (tokens <= 16 ? 16 : 32) * 8 : 0);
-    m.hi = image(c.down_type, used * moe_chunks(c.ffn));
+    m.hi = image(c.down_type, pairs * moe_chunks(c.ffn));
     if (a) *a = m;
     return at;
 }
@@ -1115,8 +1168,8 @@ size_t moe_bytes(const MoeCall& c) {
 // Arrival counters: one per tile of the down product.
 uint64_t moe_counters(const MoeCall& c) { return layout_tiles(c.out_rows); }
 
-// Whether every launch of the call stays below 2^32 threads and its chunks below
-// 2^31.
+// Whether every launch of the call stays below 2^32 threads and its images of x and
+// h below 4 GiB.
 bool moe_takes(const MoeCall& c) {
     const uint64_t t = c.tokens < kMoeTokens ? c.tokens : kMoeTokens;
     uint64_t used = t * c.slots < c.experts ? t * c.slots : c.experts;
@@ -1124,7 +1177,8 @@ bool moe_takes(const MoeCall& c) {
     return c.experts <= kMoeMaxExperts && c.slots <= kMoeMaxSlots && c.tokens <= 65535 && c.cols <= (1u << 30) &&
            c.ffn <= (1u << 30) && used * layout_tiles(c.ffn) * 1024 <= 0xffffffffull &&
            layout_tiles(c.out_rows) * 8 * 1024 <= 0xffffffffull && used * moe_chunks(c.ffn) * 512 <= 0xffffffffull &&
-           (moe_chunks(c.cols) + 1) * 512 <= 0xffffffffull;
+           (moe_chunks(c.cols) + 1) * 512 <= 0xffffffffull && t * moe_chunks(c.cols) * 256 <= 0xffffffffull &&
+           t * c.slots * moe_chunks(c.ffn) * 256 <= 0xffffffffull;
 }
 
 // Chunks of h that a workgroup of the down product has at most, of a single token.
@@ -1150,7 +1204,7 @@ static hipError_t moe_down_launch(const MoeArgs& a, hipStream_t s) {
     static LdsLimit lim;
     constexpr uint32_t tiles = NQ < 4 ? 1 : 2;
     const uint32_t lds = moe_lds<T>(KS, NQ * 4) + (ONE ? moe_one_chunks(a) * moe_lds_chunk<T>() : 0);
-    const hipError_t e = lim.raise((const void*)moe_down_kernel<T, KS, NQ, ONE>, lds + 2 * kMoeMaxExperts + 512);
+    const hipError_t e = lim.raise((const void*)moe_down_kernel<T, KS, NQ, ONE>, lds + (ONE ? kMoeMaxSlots : kMoeMaxExperts) * 8 + 512);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((moe_down_kernel<T, KS, NQ, ONE>), dim3((a.out_tiles + tiles - 1) / tiles * a.parts), dim3(64 * KS),
                        lds, s, a);
@@ -1176,7 +1230,7 @@ static hipError_t moe_down_any(const MoeArgs& a, uint32_t used, hipStream_t s) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.tokens <= 8) return moe_down_launch<T, 16, 1, false>(a, s);
-    if (a.tokens <= 16) return moe_down_launch<T, 16, 2, false>(a, s);
+    if (a.tokens <= 16) return moe_down_launch<T, 12, 2, false>(a, s);
     return moe_down_launch<T, 12, 4, false>(a, s);
 }
 

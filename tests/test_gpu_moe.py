@@ -671,3 +671,49 @@ def test_ffn_replayed(ctx, tokens):
         c.moe_ffn(*L.w, gpu(L.x(211, other)), gpu(i), gpu(w))
     c.sync()
     L.close(), c.close()
+
+
+HALF = {DT.Q8_0: 0, DT.Q2_K: 80, DT.Q3_K: 108, DT.Q4_K: 0, DT.Q5_K: 2, DT.Q6_K: 208}  # a scale (Q5_K: the minimums') in a block
+
+
+@pytest.mark.parametrize("t", TYPES, ids=lambda t: t.name)
+@pytest.mark.parametrize("tokens", [1, 2, 7, 14, 30])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_ffn_of_an_expert_with_a_bad_scale(ctx, t, tokens, bad):
+    """One scale of one row of an expert: the tokens that use it see it in that row of y
+    (of gate: they have no h), the others have the bits of a sound expert."""
+    say("ffn bad scale", t.name, tokens, bad)
+    E, K, F, R, size, rb = 4, 512, 2048, 40, O.TYPE_SIZE[int(t)], 32 if t == DT.Q8_0 else 256
+    gate, up, down = (_weights(t, E * r, c, 220 + k) for k, (r, c) in enumerate(((F, K), (F, K), (R, F))))
+
+    def weights(data, rows, cols, hurt):
+        b = np.frombuffer(bytes(data), np.uint8).copy().reshape(E, rows, cols // rb, size)
+        if hurt:
+            b[2, 7, -1, HALF[t]:HALF[t] + 2] = np.array([bad], np.float16).view(np.uint8)
+        return rlq.Weights(ctx, t, b.reshape(-1), rows, cols, E)
+
+    clean = [weights(gate, F, K, False), weights(up, F, K, False), weights(down, R, F, False)]
+    hurt = [weights(gate, F, K, True), weights(down, R, F, True)]
+    ids, w = places(221, tokens, E, 2)
+    ids[0] = [1, 2]
+    mean = float(np.sqrt(np.mean(values(t, gate, E * F, K) ** 2) * K))
+    x, ids_d, w_d = gpu(normal(222, tokens, K) / np.float32(mean)), gpu(ids), gpu(w)
+    uses = torch.from_numpy((ids == 2).any(1)).cuda()
+    want = ctx.moe_ffn(*clean, x, ids_d, w_d)
+    ctx.sync()
+    y = ctx.moe_ffn(clean[0], clean[1], hurt[1], x, ids_d, w_d)
+    ctx.sync()
+    assert torch.equal(y[~uses], want[~uses]) and not bool(torch.isfinite(y[uses][:, 7]).any())
+    keep = [r for r in range(R) if r != 7]
+    assert torch.equal(y[:, keep], want[:, keep])
+    one = ctx.moe_ffn(clean[0], clean[1], hurt[1], x[:1].contiguous(), ids_d[:1].contiguous(), w_d[:1].contiguous())
+    assert torch.equal(one.nan_to_num(nan=123.0), y[:1].nan_to_num(nan=123.0))
+    ctx.sync()
+    y = torch.full((tokens, R), 7.0, device="cuda")
+    ctx.moe_ffn(hurt[0], clean[1], clean[2], x, ids_d, w_d, y=y)
+    with pytest.raises(rlq.QuantError) as e:
+        ctx.sync()
+    assert (e.value.name, e.value.a, e.value.b) == ("NonFinite", 3, 0)
+    assert torch.equal(y[~uses], want[~uses]) and bool((y[uses] == 7.0).all())
+    for m in clean + hurt:
+        m.close()
