@@ -344,7 +344,7 @@ hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s) {
 // Experts: the plan and the activation images
 //
 // A pass takes up to 32 tokens.  Its plan lists the experts in use in ascending
-// order; expert j of them serves the tokens of mask[j], in columns cols[j][..]
+// order; expert j of them serves the tokens of mask[j], in columns column[j][..]
 // ascending, whose h rows start at base[j].  A token that names an expert twice
 // is one column of it, with the sum of both weights.  A single token has no
 // plan: its places that name an expert are read from ids where they are needed.
@@ -371,7 +371,8 @@ hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s) {
 constexpr unsigned long long kMoeBad = 0x7ff8000000000001ull;
 __device__ __forceinline__ double moe_bad_scale() { return __longlong_as_double((long long)kMoeBad); }
 __device__ __forceinline__ bool moe_is_bad(double f) { return (unsigned long long)__double_as_longlong(f) == kMoeBad; }
-
+// The scale of a column that a chunk does not concern, where products with it are left
+// out: no scale is -0.
 __device__ __forceinline__ bool moe_is_out(double f) { return (unsigned long long)__double_as_longlong(f) == 1ull << 63; }
 
 // The places of a single token that name an expert (bit s), and whether one is out
@@ -563,7 +564,8 @@ __global__ __launch_bounds__(512) void moe_prepare_kernel(MoeArgs a) {
 // launch of its own: the workgroup of moe_up_kernel that writes the last rows of a
 // chunk could do it, but the exchanges and counts by which it knows cost all of them
 // more than the launch: 32 tokens, 8 experts of 14336x4096 162 us against 133 + 5.5; 5
-// tokens, 16 Q8_0 experts of 1952x928 18.8 against 12.6 + 4.)
+// tokens, 16 Q8_0 experts of 1952x928 18.8 against 12.6 + 4.  In the LDS of the down
+// product's workgroups, as a single token's: 17.0 against 10.9 + 4.4.)
 template <uint32_t T>
 __global__ __launch_bounds__(512) void moe_h_kernel(MoeArgs a) {
     const uint32_t c = blockIdx.x, j = blockIdx.y, r16 = threadIdx.x & 15, t = threadIdx.x >> 4;
@@ -832,19 +834,21 @@ __device__ __forceinline__ uint32_t moe_pairs(uint32_t npairs, uint32_t c) {
 // h of 16 rows for expert j's tokens: wave kg takes every KS-th chunk of K.  NQ:
 // groups of eight columns that the tokens of the pass can need.
 //
-// Registers decide how many chunks a CU has in flight.  To eight columns the
-// activations of a whole chunk are loaded ahead (8 experts of 14336x4096 Q4_K, one
-// token of top-2 32.9 us against 35.7 with half a chunk), but for Q8_0, whose eight
-// scales a chunk take registers (16 experts of 1952x928, 5 tokens 12.6 us with four
-// waves a SIMD, 14.1 with a whole chunk ahead).  32 columns' sums leave room for three
-// waves a SIMD (32 tokens 133 us, 156 with the compiler's choice of two; 148 with a
-// whole chunk ahead, which spills).
+// Registers decide how many chunks a CU has in flight: four waves a SIMD to eight
+// columns, three beyond, whose sums would spill (8 experts of 14336x4096 Q4_K, 16
+// tokens 113 us against 123 with four).  Half a chunk's activations are loaded ahead; a
+// whole one gains nothing.
+//
+// Bound: memory, 8 tokens 5.3 TB/s of weights; from 16 tokens on the matrix cores and
+// the vector units next to it (113 us, 32 tokens 129).  Small experts are over
+// before the memory is busy: 4 tokens, 64 of 1536x2048 Q5_K 27 us, 3.6 TB/s.
 //
 // kMoeOne, kMoeOnePacked: a single token, without a plan: every workgroup reads the
-// ids and makes the image of x in LDS while its first weights are on their way.
+// ids and makes the image of x in LDS while its first weights are on their way (8 experts
+// of 14336x4096 28 to 36 us; with a launch for the image 33 + 5).
 enum MoeFrom { kMoePlan, kMoeOne, kMoeOnePacked };
 template <uint32_t T, int KS, int NQ, MoeFrom FROM>
-__global__ __launch_bounds__(64 * KS) __attribute__((amdgpu_waves_per_eu(NQ >= 2 ? 3 : (T == kQ8_0 ? 4 : 2)))) void
+__global__ __launch_bounds__(64 * KS) __attribute__((amdgpu_waves_per_eu(NQ >= 2 ? 3 : 4))) void
 moe_up_kernel(MoeArgs a) {
     constexpr bool ONE = FROM != kMoePlan;
     constexpr uint32_t kF = MoeWeights<T>::kFactors;
@@ -904,7 +908,7 @@ moe_up_kernel(MoeArgs a) {
         moe_walk<T, false, 4, false>(xs, steps, ln, kh, fd, at, stage, fold);
     } else {
         const MoeX<T> x{a.xi, a.tokens, a.column[j * kMoeTokens + (ln < live ? ln : 0)]};
-        moe_walk<T, false, NQ == 1 && T != kQ8_0 ? 8 : 4, false>(x, steps, ln, kh, fd, at, [] {}, fold);
+        moe_walk<T, false, 4, false>(x, steps, ln, kh, fd, at, [] {}, fold);
     }
 #pragma unroll
     for (int i = 0; i < NQ * 4; ++i) part[(kg * NQ * 4 + i) * 64 + lane] = y[i];
@@ -936,6 +940,10 @@ moe_up_kernel(MoeArgs a) {
 // row of chunks, of which the workgroup takes its part and its waves take turns.
 //   up to 16 tokens  16 rows (HALVES): a pair of chunks at a time, one for each half
 //   more             32 rows: a chunk at a time, all 32 columns
+// Bound: memory; one token of top-2, 56 chunks each, 4096 rows of Q6_K 28 us (3.4 TB/s),
+// Q4_K 19; 8 tokens, 8 experts 55 us (4.8), 16 60, 32 72.  Six experts of 6 chunks take
+// 10.5: a launch, two latencies and the joining.
+//
 // Where the tiles alone leave CUs idle, `parts` workgroups share a tile: they put
 // their f64 sums where all can read them (by exchanges whose results are waited for,
 // as the router does), and the last to arrive adds them in part order.
@@ -1111,9 +1119,10 @@ static uint64_t moe_out_tiles(const MoeCall& c, uint32_t tokens) {
     return tokens <= 16 ? t : (t + 1) / 2;
 }
 // Workgroups that share a tile of the down product: as many as there are CUs for, but
-// a step for every wave of each (us with 1 / 2 / 4: 4096 rows, 32 tokens, 8 experts of
-// 56 chunks 128 / 83 / 90; 928 rows, 16 experts of 8 chunks of Q8_0 14.7 / 11.2 / 10.6;
-// 2048 rows, one token, 6 experts of 6 chunks 8.7 / 9.3 / 14.7).
+// a step for every wave of each (us with 1 / 2 / 4, the rule's number first: 2: 4096 rows, 32
+// tokens, 8 experts of 56 chunks 106 / 73 / 84; 4: 928 rows, 5 tokens, 16 experts of 8
+// chunks of Q8_0 14.1 / 11.4 / 10.8; 2: 2048 rows, 16 tokens, 64 experts of 6 chunks 54 / 34
+// / 40; 1: 4096 rows, 8 tokens, 8 experts of 56 chunks 55 / 60 / 73).
 static uint32_t moe_parts(const MoeCall& c, uint32_t tokens) {
     const uint64_t tiles = moe_out_tiles(c, tokens), pairs = (uint64_t)tokens * c.slots;
     const uint64_t chunks = (pairs < c.experts ? pairs : c.experts) * moe_chunks(c.ffn);
@@ -1187,7 +1196,8 @@ static uint32_t moe_one_chunks(const MoeArgs& a) {
     return (all + a.parts - 1) / a.parts + 2;  // (a part is whole pairs)
 }
 // A single token whose x and h fit LDS takes two launches, others four.
-// (Q8_0's images are the largest: 256 chunks of h beside the waves' sums are 152 KB.)
+// (Q8_0's images are the largest: 256 chunks of h beside the waves' sums are 152 KB.  One
+// token, 64 experts of 1536x2048 Q5_K, top-6: 21 us a call with two launches, 27 with four.)
 static bool moe_one(const MoeArgs& a) { return a.tokens == 1 && a.x_chunks <= 128 && moe_one_chunks(a) <= 256; }
 
 template <uint32_t T, int KS, int NQ, MoeFrom FROM>
