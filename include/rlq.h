@@ -377,7 +377,7 @@ int32_t rlq_moe_route(rlq_context *ctx, const float *router, const float *x, uin
  * Capturing: make the same call once before, for the scratch.
  * Errors: RLQ_TENSOR_SHAPE (stacks that do not match, slots 0),
  * RLQ_TENSOR_UNSUPPORTED (up's type, x_dtype), RLQ_UNIMPLEMENTED (more than 1024
- * experts, 64 slots or 65535 tokens).  At rlq_sync, the token's row of y being left
+ * experts, 64 slots or 65535 tokens, or 2^32 values of x or h in a pass).  At rlq_sync, the token's row of y being left
  * as it was: RLQ_TENSOR_BOUNDS (an id outside [-1, experts); a = its index),
  * RLQ_NON_FINITE_INPUT / RLQ_UNREPRESENTABLE_SCALE of x (b = the token), then of h
  * RLQ_NON_FINITE (a = RLQ_CHECK_MATRIX_INPUT) / RLQ_UNREPRESENTABLE_SCALE (a =

@@ -496,20 +496,26 @@ class Context:
         cols = weight.numel()
         if x.shape[-1] != cols or (residual is not None and residual.shape != x.shape):
             raise ValueError("x and residual must be [..., cols] with the weight's cols")
-        rows = x.numel() // cols if cols else 0
-        if residual is not None and total is None:
+        n = x.numel()
+        rows = n // cols if cols else 0
+        if total is not None:
+            if total.numel() != n:
+                raise ValueError("total's size is not x's")
+        elif residual is not None:
             total = torch.empty_like(x)
-        if normed and y is None:
+        if y is not None:
+            if y.numel() != n:
+                raise ValueError("y's size is not x's")
+        elif normed:
             y = torch.empty_like(x)
         if packed is not None:
             nbytes = row_bytes(packed, cols)
             if q is None:
-                q = torch.empty((rows, nbytes), dtype=torch.uint8, device=x.device)
+                q = x.new_empty((rows, nbytes), dtype=torch.uint8)
+            elif q.numel() != rows * nbytes:
+                raise ValueError("q must hold x's rows in blocks")
         elif q is not None:
             raise ValueError("q needs the packed type")
-        for t, n in ((total, rows * cols), (y, rows * cols), (q, rows * nbytes if packed is not None else 0)):
-            if t is not None and t.numel() != n:
-                raise ValueError("an output's size does not match x")
         err = _Err()
         f32 = torch.float32
         _check(_lib.rlq_rms_norm(self._h, _dev_ptr(x, f32), None if residual is None else _dev_ptr(residual, f32),
@@ -535,11 +541,11 @@ class Context:
         x2 = _columns(x, cols)
         tokens, top_k = x2.shape[0], int(top_k)
         if ids is None:
-            ids = torch.empty((tokens, top_k), dtype=torch.int32, device=x.device)
+            ids = x.new_empty((tokens, top_k), dtype=torch.int32)
         if weights is None:
-            weights = torch.empty((tokens, top_k), dtype=torch.float32, device=x.device)
+            weights = x.new_empty((tokens, top_k))
         if logits is True:
-            logits = torch.empty((tokens, experts), dtype=torch.float32, device=x.device)
+            logits = x.new_empty((tokens, experts))
         elif logits is False:
             logits = None
         if ids.numel() != tokens * top_k or weights.numel() != tokens * top_k \
@@ -571,7 +577,7 @@ class Context:
         if weights.shape != ids.shape:
             raise ValueError("weights must have the shape of ids")
         if y is None:
-            y = torch.empty((tokens, down.rows), dtype=f32, device=x.device)
+            y = weights.new_empty((tokens, down.rows))
         if y.numel() != tokens * down.rows or (residual is not None and residual.numel() != y.numel()):
             raise ValueError("y and residual must hold the down matrix's rows for every token")
         err = _Err()

@@ -344,8 +344,8 @@ hipError_t launch_moe_route(const RouteArgs& a, hipStream_t s) {
 // Experts: the plan and the activation images
 //
 // A pass takes up to 32 tokens.  Its plan lists the experts in use in ascending
-// order; expert j of them serves the tokens of mask[j], in columns column[j][..]
-// ascending, whose h rows start at base[j].  A token that names an expert twice
+// order as (expert, base, mask): the expert serves the tokens of mask, ascending, whose h
+// rows start at base.  Entries past the last one have no tokens.  A token that names an expert twice
 // is one column of it, with the sum of both weights.  A single token has no
 // plan: its places that name an expert are read from ids where they are needed.
 //
@@ -433,9 +433,10 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& a) {
             if (w < wave) j += wave_n[w], b += wave_b[w];
             used += wave_n[w], rows += wave_b[w];
         }
-        if (m) a.expert[j] = e, a.base[j] = b, a.mask[j] = m, place[e] = (uint16_t)j;
+        if (m) a.plan[j] = make_uint4(e, b, m, 0), place[e] = (uint16_t)j;
         __syncthreads();
     }
+    for (uint32_t j = used + tid; j < a.most; j += nt) a.plan[j] = make_uint4(0, 0, 0, 0);
     if (tid == 0) *a.n_used = used, *a.bad = bad;
     for (uint32_t p = tid; p < pairs; p += nt) {  // a token's first place with an expert speaks for all of them
         const int32_t id = ids[p];
@@ -446,9 +447,7 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& a) {
         double w = 0.0;
         for (uint32_t o = p; o < end; ++o)
             if (ids[o] == id) w += (double)weights[o];
-        const uint32_t j = place[id];
-        a.wsum[j * kMoeTokens + t] = w;
-        a.column[j * kMoeTokens + (uint32_t)__builtin_popcount(mask[id] & ((1u << t) - 1))] = (uint8_t)t;
+        a.wsum[place[id] * kMoeTokens + t] = w;
     }
 }
 
@@ -569,14 +568,14 @@ __global__ __launch_bounds__(512) void moe_prepare_kernel(MoeArgs a) {
 template <uint32_t T>
 __global__ __launch_bounds__(512) void moe_h_kernel(MoeArgs a) {
     const uint32_t c = blockIdx.x, j = blockIdx.y, r16 = threadIdx.x & 15, t = threadIdx.x >> 4;
-    if (j >= *a.n_used || t >= a.tokens) return;
-    const uint32_t mask = a.mask[j], n = (uint32_t)__builtin_popcount(mask), e0 = c * 256 + r16 * 16;
-    if (!((mask >> t) & 1u)) return;
-    const uint32_t col = (uint32_t)__builtin_popcount(mask & ((1u << t) - 1)), row = a.base[j] + col;
+    const uint4 p = a.plan[j];
+    if (!((p.z >> t) & 1u)) return;
+    const uint32_t n = (uint32_t)__builtin_popcount(p.z), col = (uint32_t)__builtin_popcount(p.z & ((1u << t) - 1));
+    const uint32_t e0 = c * 256 + r16 * 16;
     float v[16];
 #pragma unroll
     for (int k = 0; k < 16; ++k) v[k] = 0.0f;
-    if (e0 < a.ffn) moe_load16(a.h + (uint64_t)row * a.ffn + e0, v);
+    if (e0 < a.ffn) moe_load16(a.h + (uint64_t)(p.y + col) * a.ffn + e0, v);
     uint32_t q[4], index;
     float d;
     int32_t bsum;
@@ -584,7 +583,7 @@ __global__ __launch_bounds__(512) void moe_h_kernel(MoeArgs a) {
     if (kind == kKindScale && (T == kQ8_0 ? !(r16 & 1) : r16 == 0))  // (a non-finite h has been reported)
         report_error(a.err_word, model_key(a.token0 + t, kStDownQuant, T == kQ8_0 ? e0 / 32 : c));
     const double f = kind >= 0 ? moe_bad_scale() : a.wsum[j * kMoeTokens + t] * (double)d;
-    image_put<T>(a.hi, (uint64_t)a.base[j] * gridDim.x + c * n, col, n, r16, q, bsum, f);
+    image_put<T>(a.hi, (uint64_t)p.y * gridDim.x + c * n, col, n, r16, q, bsum, f);
 }
 
 // ---------------------------------------------------------------------------
@@ -868,8 +867,12 @@ moe_up_kernel(MoeArgs a) {
         for (uint32_t k = 0; k < j; ++k) left &= left - 1;
         expert = (uint32_t)__builtin_amdgcn_readlane(p.id, __builtin_ctzll(left));
     } else {
-        if (j >= *a.n_used) return;
-        mask = a.mask[j], base = a.base[j], expert = a.expert[j];
+        const uint4 p = a.plan[j];
+        if (!p.z) return;
+        expert = p.x, base = p.y, mask = p.z;
+        // (knowing that there is a column, the compiler drops the first branch of the folds, lets
+        // the folds of Q8_0's blocks run into each other, and spills)
+        asm volatile("" : "+s"(mask));
     }
     const uint32_t live = (uint32_t)__builtin_popcount(mask), nchunk = a.x_chunks;
     const uint8_t* wt = ((ln >> 4) ? a.up : a.gate) + (uint64_t)expert * a.up_bytes + (uint64_t)tile * a.x_row_bytes;
@@ -907,7 +910,11 @@ moe_up_kernel(MoeArgs a) {
         };
         moe_walk<T, false, 4, false>(xs, steps, ln, kh, fd, at, stage, fold);
     } else {
-        const MoeX<T> x{a.xi, a.tokens, a.column[j * kMoeTokens + (ln < live ? ln : 0)]};
+        // lane k: the token of column k (of a column past the last one the first one's)
+        const bool mine = lane < kMoeTokens && (mask >> lane) & 1u;
+        const int to = mine ? __builtin_popcount(mask & ((1u << lane) - 1)) : 63;
+        const uint32_t tok = (uint32_t)__builtin_amdgcn_ds_permute(4 * to, (int)lane);
+        const MoeX<T> x{a.xi, a.tokens, (uint32_t)__shfl((int)tok, ln < live ? (int)ln : 0, 64) & (kMoeTokens - 1)};
         moe_walk<T, false, 4, false>(x, steps, ln, kh, fd, at, [] {}, fold);
     }
 #pragma unroll
@@ -924,7 +931,9 @@ moe_up_kernel(MoeArgs a) {
         const double gf = (double)(float)g, uf = (double)(float)u;
         float h = (float)(gf / (1.0 + exp(-gf)) * uf);
         if (!finite(h)) {
-            const uint32_t t = ONE ? 0 : a.column[j * kMoeTokens + c];
+            uint32_t left = mask;  // (a single token's: 1)
+            for (uint32_t k = 0; k < c; ++k) left &= left - 1;
+            const uint32_t t = (uint32_t)__builtin_ctz(left);
             bool marked = ONE && bad != 0;
             if constexpr (!ONE) {
                 for (uint64_t k = 0; k < nchunk * kF; ++k) marked |= moe_is_bad(a.xi.f[(k / kF * a.tokens + t) * kF + k % kF]);
@@ -974,7 +983,10 @@ moe_down_kernel(MoeArgs a) {
         if (threadIdx.x == 0) marked = 0;
     } else {
         used = *a.n_used, bad = *a.bad;
-        for (uint32_t i = threadIdx.x; i < used; i += 64 * KS) plan[i] = make_uint2(a.expert[i] | a.base[i] << 16, a.mask[i]);
+        for (uint32_t i = threadIdx.x; i < a.most; i += 64 * KS) {  // (past `used` no one looks)
+            const uint4 p = a.plan[i];
+            plan[i] = make_uint2(p.x | p.y << 16, p.z);
+        }
     }
     __syncthreads();
     // this part's chunks, whole steps of them but for the last part's end
@@ -1152,10 +1164,8 @@ static size_t moe_carve(const MoeCall& c, uint32_t tokens, uint8_t* base, MoeArg
     MoeArgs m{};
     m.n_used = (uint32_t*)take(4);
     m.bad = (uint32_t*)take(4);
-    m.expert = (uint32_t*)take(used * 4);
-    m.base = (uint32_t*)take(used * 4);
-    m.mask = (uint32_t*)take(used * 4);
-    m.column = take(used * kMoeTokens);
+    m.plan = (uint4*)take(used * 16);
+    m.most = (uint32_t)used;
     m.wsum = (double*)take(used * kMoeTokens * 8);
     m.xi = image(c.up_type, moe_chunks(c.cols) * tokens);
     m.h = (float*)take(pairs * c.ffn * 4);

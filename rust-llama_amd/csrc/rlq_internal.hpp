@@ -245,8 +245,9 @@ struct MoeArgs {  // of one pass
     float* y;
     unsigned long long* err_word;
     // the plan and the workspace (moe.hip)
-    uint32_t *n_used, *bad, *expert, *base, *mask;
-    uint8_t* column;
+    uint32_t *n_used, *bad;
+    uint4* plan;
+    uint32_t most;  // entries of it
     double* wsum;
     MoeImage xi, hi;
     float* h;
