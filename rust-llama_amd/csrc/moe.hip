@@ -844,7 +844,7 @@ __device__ __forceinline__ uint32_t moe_pairs(uint32_t npairs, uint32_t c) {
 //
 // kMoeOne, kMoeOnePacked: a single token, without a plan: every workgroup reads the
 // ids and makes the image of x in LDS while its first weights are on their way (8 experts
-// of 14336x4096 28 to 36 us; with a launch for the image 33 + 5).
+// of 14336x4096, top-2, 28 to 36 us; with a launch for the image 5 more).
 enum MoeFrom { kMoePlan, kMoeOne, kMoeOnePacked };
 template <uint32_t T, int KS, int NQ, MoeFrom FROM>
 __global__ __launch_bounds__(64 * KS) __attribute__((amdgpu_waves_per_eu(NQ >= 2 ? 3 : 4))) void
@@ -1233,7 +1233,14 @@ static hipError_t moe_down_launch(const MoeArgs& a, hipStream_t s) {
 
 template <uint32_t T>
 static hipError_t moe_up_any(const MoeArgs& a, bool packed, uint32_t used, hipStream_t s) {
-    if (moe_one(a)) return packed ? moe_up_launch<T, 4, 1, kMoeOnePacked>(a, a.slots, s) : moe_up_launch<T, 4, 1, kMoeOne>(a, a.slots, s);
+    if (moe_one(a)) {
+        // K over two waves where the tiles can keep the CUs busy by themselves, else over four (us with
+        // 2 / 4, one token of top-2: 896 tiles an expert of 16 chunks 36.0 / 38.3, 512 of 32 34.4 /
+        // 41.1; top-8, 96 tiles of 16 17.3 / 14.7; top-6, 96 of 8 13.8 / 12.7)
+        const bool two = (uint64_t)a.slots * a.up_tiles >= 4ull * device_cus();
+        if (packed) return two ? moe_up_launch<T, 2, 1, kMoeOnePacked>(a, a.slots, s) : moe_up_launch<T, 4, 1, kMoeOnePacked>(a, a.slots, s);
+        return two ? moe_up_launch<T, 2, 1, kMoeOne>(a, a.slots, s) : moe_up_launch<T, 4, 1, kMoeOne>(a, a.slots, s);
+    }
     const dim3 grid(1 + a.x_chunks);
     if (packed) hipLaunchKernelGGL((moe_prepare_kernel<T, true>), grid, dim3(512), 0, s, a);
     else hipLaunchKernelGGL((moe_prepare_kernel<T, false>), grid, dim3(512), 0, s, a);

@@ -717,3 +717,22 @@ def test_ffn_of_an_expert_with_a_bad_scale(ctx, t, tokens, bad):
     assert torch.equal(y[~uses], want[~uses]) and bool((y[uses] == 7.0).all())
     for m in clean + hurt:
         m.close()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=lambda t: t.name)
+@pytest.mark.parametrize("packed", [False, True])
+def test_ffn_of_one_token_with_many_tiles(ctx, t, packed):
+    """Enough rows of h for K to be split less, and as many of K's chunks as waves, fewer and more."""
+    say("ffn many tiles", t.name, packed)
+    for cols in (256, 768):
+        L = Layer(ctx, 2, cols, 2304, 48, t, DT.Q8_0, 230)
+        ids, weights = places(231, 1, 2, 16)
+        x = L.x(232, 1)
+        if packed:
+            q = ctx.quantize(act(t), gpu(x)).view(1, -1)
+            y, a = L.call(q, ids, weights, x_dtype=act(t)), unpacked(act(t), q.cpu().numpy(), cols)
+        else:
+            y, a = L.call(gpu(x), ids, weights), quantized(act(t), x)
+        ctx.sync()
+        L.check(y, a, ids, weights)
+        L.close()
