@@ -950,7 +950,7 @@ moe_up_kernel(MoeArgs a) {
 //   up to 16 tokens  16 rows (HALVES): a pair of chunks at a time, one for each half
 //   more             32 rows: a chunk at a time, all 32 columns
 // Bound: memory; one token of top-2, 56 chunks each, 4096 rows of Q6_K 28 us (3.4 TB/s),
-// Q4_K 19; 8 tokens, 8 experts 55 us (4.8), 16 60, 32 72.  Six experts of 6 chunks take
+// Q4_K 19 to 22; 8 tokens, 8 experts 55 us (4.8), 16 60, 32 72.  Six experts of 6 chunks take
 // 10.5: a launch, two latencies and the joining.
 //
 // Where the tiles alone leave CUs idle, `parts` workgroups share a tile: they put
