@@ -840,7 +840,7 @@ __device__ __forceinline__ uint32_t moe_pairs(uint32_t npairs, uint32_t c) {
 // whole one gains nothing.
 //
 // Bound: memory, 8 tokens 5.3 TB/s of weights; from 16 tokens on the matrix cores and
-// the vector units next to it (113 us, 32 tokens 129).  Small experts are over
+// the vector units next to it (111 us, 32 tokens 128).  Small experts are over
 // before the memory is busy: 4 tokens, 64 of 1536x2048 Q5_K 27 us, 3.6 TB/s.
 //
 // kMoeOne, kMoeOnePacked: a single token, without a plan: every workgroup reads the
@@ -1248,7 +1248,11 @@ static hipError_t moe_up_any(const MoeArgs& a, bool packed, uint32_t used, hipSt
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.tokens <= 8) return moe_up_launch<T, 4, 1, kMoePlan>(a, used, s);
-    if (a.tokens <= 16) return moe_up_launch<T, 4, 2, kMoePlan>(a, used, s);
+    // (us with 2 / 4 waves: 16 tokens, 8 experts of 896 tiles 111 / 114 to 121, 64 of 96, top-6 53.3 / 55.9; 11
+    // tokens, 32 of 64 19.4 / 18.5; Q8_0, 16 tokens, 16 of 122 16.2 / 15.7)
+    if (a.tokens <= 16)
+        return (uint64_t)used * a.up_tiles >= 16ull * device_cus() ? moe_up_launch<T, 2, 2, kMoePlan>(a, used, s)
+                                                                   : moe_up_launch<T, 4, 2, kMoePlan>(a, used, s);
     return moe_up_launch<T, 2, 4, kMoePlan>(a, used, s);
 }
 template <uint32_t T>

@@ -736,3 +736,15 @@ def test_ffn_of_one_token_with_many_tiles(ctx, t, packed):
         ctx.sync()
         L.check(y, a, ids, weights)
         L.close()
+
+
+@pytest.mark.parametrize("t", [DT.Q8_0, DT.Q4_K], ids=lambda t: t.name)
+def test_ffn_of_some_tokens_with_many_tiles(ctx, t):
+    say("ffn many tiles, some tokens", t.name)
+    L = Layer(ctx, 20, 512, 3584, 24, t, DT.Q6_K, 235)
+    ids, weights = places(236, 13, 20, 4)
+    x = L.x(237, 13)
+    y = L.call(gpu(x), ids, weights)
+    ctx.sync()
+    L.check(y, quantized(act(t), x), ids, weights)
+    L.close()
