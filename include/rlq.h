@@ -372,6 +372,7 @@ int32_t rlq_moe_route(rlq_context *ctx, const float *router, const float *x, uin
  * a call.  h is quantized like any f32 column of down.  ids and weights [tokens,
  * slots]; -1: no expert (its weight is not looked at), a token without any gets
  * its residual, its x not being looked at.  residual may be null (0), and may be y.
+ * An expert's weights that are not finite concern the tokens that use it alone.
  * 32 tokens share a pass over the weights of the experts that they use; more
  * tokens take further passes (a prompt is better served by rlq_mul_mat_id).
  * Capturing: make the same call once before, for the scratch.
