@@ -393,20 +393,21 @@ __device__ __forceinline__ MoePlaces moe_places(const MoeArgs& a) {
 }
 
 __device__ __forceinline__ void moe_plan(const MoeArgs& a) {
-    __shared__ uint32_t mask[kMoeMaxExperts], wave_n[8], wave_b[8], bad;
+    __shared__ uint32_t mask[kMoeMaxExperts], wave_n[8], wave_b[8], bad, some;
     __shared__ uint16_t place[kMoeMaxExperts];
     __shared__ int32_t ids[kMoeTokens * kMoeMaxSlots];
     __shared__ float weights[kMoeTokens * kMoeMaxSlots];
     const uint32_t tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = nt >> 6;
     const uint32_t pairs = a.tokens * a.slots;
     for (uint32_t e = tid; e < a.experts; e += nt) mask[e] = 0;
-    if (tid == 0) bad = 0;
+    if (tid == 0) bad = 0, some = 0;
     __syncthreads();
     for (uint32_t p = tid; p < pairs; p += nt) {
         int32_t id = a.ids[p];
         const uint32_t t = p / a.slots;
         if (id >= 0 && id < (int32_t)a.experts) {
             atomicOr(&mask[id], 1u << t);
+            atomicOr(&some, 1u << t);
         } else if (id != -1) {
             report_error(a.err_word, bounds_key((uint64_t)a.token0 * a.slots + p));
             atomicOr(&bad, 1u << t);
@@ -437,7 +438,7 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& a) {
         __syncthreads();
     }
     for (uint32_t j = used + tid; j < a.most; j += nt) a.plan[j] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) *a.n_used = used, *a.bad = bad;
+    if (tid == 0) *a.n_used = used, *a.bad = bad, *a.some = some;
     for (uint32_t p = tid; p < pairs; p += nt) {  // a token's first place with an expert speaks for all of them
         const int32_t id = ids[p];
         const uint32_t t = p / a.slots, end = (t + 1) * a.slots;
@@ -972,18 +973,19 @@ moe_down_kernel(MoeArgs a) {
     const uint32_t ln = lane & 31, kh = lane >> 5, hf = ln >> 4;
     const uint32_t tile = blockIdx.x / a.parts, part = blockIdx.x - tile * a.parts;
     const uint32_t nchunk = a.h_chunks;
-    uint32_t used, bad = 0;  // bad: tokens whose ids are out of range
+    uint32_t used, bad = 0, some;  // bad: tokens whose ids are out of range; some: those with an expert
     if constexpr (ONE) {
         const MoePlaces p = moe_places(a);
         bad = p.wrong >= 0;
         used = bad ? 0 : (uint32_t)__builtin_popcountll(p.some);
+        some = used != 0;
         if (kg == 0 && ((p.some >> lane) & 1)) {
             const uint32_t j = (uint32_t)__builtin_popcountll(p.some & ((1ull << lane) - 1));
             plan[j] = make_uint2((uint32_t)p.id, 1), weight[j] = a.weights[lane];
         }
         if (threadIdx.x == 0) marked = 0;
     } else {
-        used = *a.n_used, bad = *a.bad;
+        used = *a.n_used, bad = *a.bad, some = *a.some;
         for (uint32_t i = threadIdx.x; i < a.most; i += 64 * KS) {  // (past `used` no one looks)
             const uint4 p = a.plan[i];
             plan[i] = make_uint2(p.x | p.y << 16, p.z);
@@ -1086,7 +1088,8 @@ moe_down_kernel(MoeArgs a) {
         const uint32_t t = o / kRows, row = tile * kRows + o % kRows;
         if (row >= a.out_rows || ((bad >> t) & 1) || moe_is_bad(v)) return;
         const uint64_t to = (uint64_t)t * a.out_rows + row;
-        a.y[to] = (float)(a.residual ? (double)a.residual[to] + v : v);
+        // (without an expert the residual as it is: a sum with +0 would take -0's sign)
+        a.y[to] = !a.residual ? (float)v : (some >> t) & 1 ? (float)((double)a.residual[to] + v) : a.residual[to];
     };
     const uint32_t n = a.tokens * kRows;
     if (a.parts == 1) {
@@ -1165,6 +1168,7 @@ static size_t moe_carve(const MoeCall& c, uint32_t tokens, uint8_t* base, MoeArg
     MoeArgs m{};
     m.n_used = (uint32_t*)take(4);
     m.bad = (uint32_t*)take(4);
+    m.some = (uint32_t*)take(4);
     m.plan = (uint4*)take(used * 16);
     m.most = (uint32_t)used;
     m.wsum = (double*)take(used * kMoeTokens * 8);

@@ -748,3 +748,29 @@ def test_ffn_of_some_tokens_with_many_tiles(ctx, t):
     ctx.sync()
     L.check(y, quantized(act(t), x), ids, weights)
     L.close()
+
+
+@pytest.mark.parametrize("tokens", [1, 4, 12, 25, 33])
+def test_ffn_of_no_expert_keeps_the_residuals_bits(ctx, tokens):
+    """A token without any expert gets its residual: -0 as -0."""
+    say("ffn residual bits", tokens)
+    L = Layer(ctx, 4, 256, 256, 40, DT.Q4_K, DT.Q6_K, 240)
+    ids, weights = places(241, tokens, 4, 2)
+    res = normal(242, tokens, 40)
+    res[:, ::3] = -0.0
+    for t in {0, tokens // 2, tokens - 1}:
+        ids[t] = -1
+    none = (ids < 0).all(1)
+    x = L.x(243, tokens)
+    y = L.call(gpu(x), ids, weights, residual=gpu(res))
+    ctx.sync()
+    assert np.array_equal(y.cpu().numpy().view(np.uint32)[none], res.view(np.uint32)[none])
+    L.check(y, quantized(DT.Q8_K, x), ids, weights, res)
+    y = gpu(res)
+    L.call(gpu(x), np.full_like(ids, -1), weights, residual=y, y=y)
+    ctx.sync()
+    assert np.array_equal(y.cpu().numpy().view(np.uint32), res.view(np.uint32))
+    y = L.call(gpu(x), np.full_like(ids, -1), weights)  # no residual: 0
+    ctx.sync()
+    assert not y.cpu().numpy().view(np.uint32).any()
+    L.close()
