@@ -343,10 +343,10 @@ int32_t rlq_rms_norm(rlq_context *ctx, const float *x, const float *residual, co
  * RLQ_ROUTE_SIGMOID; ids[t][..] (i32) = the `slots` experts of the largest logits, or
  * with a bias [experts] of the largest score + bias, the lowest index of equal
  * ones; weights[t][..] = their scores (without the bias), with
- * RLQ_ROUTE_NORMALIZE divided by their sum (0 where that is 0), times scale,
- * rounded once.  A bias of -infinity or NaN switches an expert off; places for which no
- * expert is left get id -1 and weight 0, as rlq_mul_mat_id and rlq_moe_ffn take
- * them.  bias and logits may be null.  1 <= slots <= experts (RLQ_TENSOR_SHAPE);
+ * RLQ_ROUTE_NORMALIZE divided by their sum, times scale, rounded once (0 where the
+ * sum is 0, whatever scale is).  A bias of -infinity or NaN switches an expert off; places
+ * for which no expert is left get id -1 and weight 0, as rlq_mul_mat_id and rlq_moe_ffn
+ * take them.  bias and logits may be null.  1 <= slots <= experts (RLQ_TENSOR_SHAPE);
  * slots at most 64, experts 1024, tokens 65535 (RLQ_UNIMPLEMENTED).  Pointers
  * 4-byte aligned (router and x 16 and cols % 4 == 0: wide loads).  A token with a
  * logit that is not finite gets ids of -1 and weights of 0: RLQ_NON_FINITE at

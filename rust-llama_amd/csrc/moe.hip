@@ -138,11 +138,13 @@ __device__ __forceinline__ void route_choose(const RouteArgs& a, uint32_t t, con
             take(s, [&](int i) { return rank[i] == most; }, [&](int i) { rank[i] = -INFINITY; });
         }
     }
+    bool none = id < 0;  // 0 times a scale that is not finite would be NaN
     if (a.normalize) {
         const double all = wave_sum_f64(weight);
-        weight = all > 0.0 ? weight / all : 0.0;
+        none |= !(all > 0.0);
+        weight = weight / all;
     }
-    if (lane < a.slots) ids[lane] = id, weights[lane] = (float)(weight * (double)a.scale);
+    if (lane < a.slots) ids[lane] = id, weights[lane] = none ? 0.0f : (float)(weight * (double)a.scale);
 }
 
 // A workgroup's logits zs[n tokens][m experts] of tokens from t0 and experts from e0

@@ -774,3 +774,26 @@ def test_ffn_of_no_expert_keeps_the_residuals_bits(ctx, tokens):
     ctx.sync()
     assert not y.cpu().numpy().view(np.uint32).any()
     L.close()
+
+
+@pytest.mark.parametrize("scale", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("gating", ["softmax", "sigmoid"])
+def test_route_scale_that_is_not_finite(ctx, gating, scale):
+    """Places without an expert, and those of a normalized sum of 0, have weights of
+    0 whatever the scale; the others are the scale's."""
+    say("route scale", gating, scale)
+    router, x = normal(250, 9, 64), normal(251, 5, 64)
+    bias = np.full(9, -np.inf, np.float32)
+    bias[[2, 5]] = 0.0
+    for normalize in (True, False):
+        ids, w, _ = ctx.moe_route(gpu(router), gpu(x), 4, gating=gating, normalize=normalize, scale=scale, bias=gpu(bias))
+        ctx.sync()
+        ids, w = ids.cpu().numpy(), w.cpu().numpy()
+        assert (ids[:, :2] >= 0).all() and (ids[:, 2:] == -1).all()
+        assert not w[:, 2:].view(np.uint32).any()
+        assert np.isnan(w[:, :2]).all() if np.isnan(scale) else (w[:, :2] == scale).all()
+    router, x = np.zeros((6, 4), np.float32), np.ones((2, 4), np.float32)
+    router[:, 0] = -800.0  # sigmoids of 0
+    _, w, _ = ctx.moe_route(gpu(router), gpu(x), 3, gating="sigmoid", scale=scale)
+    ctx.sync()
+    assert not w.cpu().numpy().view(np.uint32).any()
