@@ -23,6 +23,7 @@ llama.rs): embedding(token) and step(hidden, position) -> (embedding, logits)
 over quantized matrices and a resident f32 KV cache.
 """
 import atexit
+import contextlib
 import ctypes
 import enum
 import os
@@ -340,14 +341,41 @@ def _stream_ptr(stream):
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-def _columns(x, cols):
+def _on(stream, device=None):
+    """Where a call that is given a stream makes its tensors: on that stream, whose
+    order they then have.  What torch's current stream has freed may be in use there
+    until its queue is done, and what is copied there may not be whole when the call
+    runs."""
+    if stream is None:
+        return contextlib.nullcontext()
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(stream if isinstance(stream, int) else stream.cuda_stream, device=device)
+    return torch.cuda.stream(stream)
+
+
+def _empty(t, shape, dtype, stream):
+    """An output beside t of a call on the stream."""
+    if stream is None and isinstance(t, torch.Tensor):
+        return t.new_empty(shape, dtype=dtype)  # (0.3 us less than torch.empty on t's device)
+    with _on(stream if getattr(t, "is_cuda", False) else None, t.device):
+        return torch.empty(shape, dtype=dtype, device=t.device)
+
+
+def _reshape(t, shape, stream):
+    """t.reshape(shape); the copy that some strides need is made on the stream."""
+    with _on(stream if getattr(t, "is_cuda", False) else None, t.device):
+        return t.reshape(shape)
+
+
+def _columns(x, cols, stream=None):
     """x as [batch, cols]; as it is when it has that shape (a reshape costs 1 us)."""
-    return x if x.ndim == 2 and x.shape[1] == cols else x.reshape(-1, cols)
+    return x if x.ndim == 2 and x.shape[1] == cols else _reshape(x, (-1, cols), stream)
 
 
 class Context:
     """rlq_context: device scratch, the context's own stream and the device
-    error word.  Kernels run on torch's current stream unless one is given."""
+    error word.  Kernels run on torch's current stream unless one is given (a
+    torch stream or its handle); what a call makes then belongs to that stream."""
 
     def __init__(self, device=-1):
         if device >= 0 and torch is not None:
@@ -366,9 +394,9 @@ class Context:
 
     def matmul(self, w, x, y=None, stream=None):
         """MUL_MAT / Matrix::multiply: x [batch, cols] f32 -> y [batch, rows] f32."""
-        x2 = _columns(x, w.cols)
+        x2 = _columns(x, w.cols, stream)
         if y is None:
-            y = torch.empty((x2.shape[0], w.rows), dtype=torch.float32, device=x.device)
+            y = _empty(x, (x2.shape[0], w.rows), torch.float32, stream)
         err = _Err()
         _check(_lib.rlq_matmul(self._h, w._h, _dev_ptr(x2, torch.float32), x2.shape[0],
                                _dev_ptr(y, torch.float32), _stream_ptr(stream), ctypes.byref(err)), err)
@@ -379,7 +407,7 @@ class Context:
         y [rows], with the reference's finite checks of the input and the
         output (NonFinite errors at sync)."""
         if y is None:
-            y = torch.empty(w.rows, dtype=torch.float32, device=x.device)
+            y = _empty(x, w.rows, torch.float32, stream)
         err = _Err()
         _check(_lib.rlq_multiply(self._h, w._h, _dev_ptr(x, torch.float32), _dev_ptr(y, torch.float32),
                                  _stream_ptr(stream), ctypes.byref(err)), err)
@@ -387,12 +415,12 @@ class Context:
 
     def matmul_argmax(self, w, x, y=None, argmax=None, stream=None):
         """matmul followed by the greedy sampler's index per column."""
-        x2 = _columns(x, w.cols)
+        x2 = _columns(x, w.cols, stream)
         batch = x2.shape[0]
         if y is None:
-            y = torch.empty((batch, w.rows), dtype=torch.float32, device=x.device)
+            y = _empty(x, (batch, w.rows), torch.float32, stream)
         if argmax is None:
-            argmax = torch.empty(batch, dtype=torch.int32, device=x.device)
+            argmax = _empty(x, batch, torch.int32, stream)
         err = _Err()
         _check(_lib.rlq_matmul_argmax(self._h, w._h, _dev_ptr(x2, torch.float32), batch,
                                       _dev_ptr(y, torch.float32), _dev_ptr(argmax, torch.int32),
@@ -406,7 +434,7 @@ class Context:
         arguments launches the same call again with only the C call's own
         cost (for serving loops; it raises like matmul).  The tensors stay
         referenced by the function."""
-        x2 = _columns(x, w.cols)
+        x2 = _columns(x, w.cols, stream)
         batch = x2.shape[0]
         if y.numel() != batch * w.rows:
             raise ValueError("y must hold batch * rows f32 values")
@@ -436,7 +464,7 @@ class Context:
         """rlq_matmul_noalloc: matmul (argmax None) or matmul_argmax into the
         caller's y [batch, rows] (and argmax [batch] int32), with the
         library's static device scratch instead of any allocation."""
-        x2 = _columns(x, w.cols)
+        x2 = _columns(x, w.cols, stream)
         err = _Err()
         _check(_lib.rlq_matmul_noalloc(self._h, w._h, _dev_ptr(x2, torch.float32), x2.shape[0],
                                        _dev_ptr(y, torch.float32),
@@ -446,9 +474,9 @@ class Context:
 
     def quantize(self, dtype, x, stream=None):
         """GPU quantize_into for Q8_0 / Q8_K: x [batch, cols] -> GGUF bytes."""
-        x2 = x.reshape(x.shape[0] if x.dim() > 1 else 1, -1)
+        x2 = _reshape(x, (x.shape[0] if x.dim() > 1 else 1, -1), stream)
         cols = x2.shape[1]
-        out = torch.empty(x2.shape[0] * row_bytes(dtype, cols), dtype=torch.uint8, device=x.device)
+        out = _empty(x, x2.shape[0] * row_bytes(dtype, cols), torch.uint8, stream)
         err = _Err()
         _check(_lib.rlq_quantize_device(self._h, int(dtype), _dev_ptr(x2, torch.float32), cols, x2.shape[0],
                                         _dev_ptr(out, torch.uint8), _stream_ptr(stream), ctypes.byref(err)), err)
@@ -463,7 +491,7 @@ class Context:
             raise ValueError("x must be [n3, n2, ncols, cols] (f32) or [n3, n2, ncols, row bytes] (uint8)")
         n3, n2, ncols = x.shape[:3]
         if y is None:
-            y = torch.empty((n3, n2, ncols, w.rows), dtype=torch.float32, device=x.device)
+            y = _empty(x, (n3, n2, ncols, w.rows), torch.float32, stream)
         xp = _dev_ptr(x, x.dtype)  # the library checks x_dtype against the weights
         err = _Err()
         _check(_lib.rlq_mul_mat(self._h, w._h, int(x_dtype), xp, ncols, n2, n3, _dev_ptr(y, torch.float32),
@@ -478,7 +506,7 @@ class Context:
         tokens, ncols = x.shape[:2]
         slots = ids.shape[1]
         if y is None:
-            y = torch.empty((tokens, slots, w.rows), dtype=torch.float32, device=x.device)
+            y = _empty(x, (tokens, slots, w.rows), torch.float32, stream)
         xp = _dev_ptr(x, x.dtype)
         err = _Err()
         _check(_lib.rlq_mul_mat_id(self._h, w._h, int(x_dtype), xp, ncols, tokens, _dev_ptr(ids, torch.int32),
@@ -502,16 +530,16 @@ class Context:
             if total.numel() != n:
                 raise ValueError("total's size is not x's")
         elif residual is not None:
-            total = torch.empty_like(x)
+            total = _empty(x, x.shape, x.dtype, stream)
         if y is not None:
             if y.numel() != n:
                 raise ValueError("y's size is not x's")
         elif normed:
-            y = torch.empty_like(x)
+            y = _empty(x, x.shape, x.dtype, stream)
         if packed is not None:
             nbytes = row_bytes(packed, cols)
             if q is None:
-                q = x.new_empty((rows, nbytes), dtype=torch.uint8)
+                q = _empty(x, (rows, nbytes), torch.uint8, stream)
             elif q.numel() != rows * nbytes:
                 raise ValueError("q must hold x's rows in blocks")
         elif q is not None:
@@ -538,14 +566,14 @@ class Context:
         if gating not in ("softmax", "sigmoid"):
             raise ValueError("gating must be softmax or sigmoid")
         experts, cols = router.shape
-        x2 = _columns(x, cols)
+        x2 = _columns(x, cols, stream)
         tokens, top_k = x2.shape[0], int(top_k)
         if ids is None:
-            ids = x.new_empty((tokens, top_k), dtype=torch.int32)
+            ids = _empty(x, (tokens, top_k), torch.int32, stream)
         if weights is None:
-            weights = x.new_empty((tokens, top_k))
+            weights = _empty(x, (tokens, top_k), x.dtype, stream)
         if logits is True:
-            logits = x.new_empty((tokens, experts))
+            logits = _empty(x, (tokens, experts), x.dtype, stream)
         elif logits is False:
             logits = None
         if ids.numel() != tokens * top_k or weights.numel() != tokens * top_k \
@@ -577,7 +605,7 @@ class Context:
         if weights.shape != ids.shape:
             raise ValueError("weights must have the shape of ids")
         if y is None:
-            y = weights.new_empty((tokens, down.rows))
+            y = _empty(weights, (tokens, down.rows), weights.dtype, stream)
         if y.numel() != tokens * down.rows or (residual is not None and residual.numel() != y.numel()):
             raise ValueError("y and residual must hold the down matrix's rows for every token")
         err = _Err()
@@ -598,10 +626,10 @@ class Context:
         ([batch, cols] or [cols], batch <= 8), from the decode kernel of that
         batch size (matmul runs it too, or for some shapes of two and more
         columns the int8 GEMM); more columns of Q4_K: from its f16 GEMM."""
-        x2 = _columns(x, w.cols)
+        x2 = _columns(x, w.cols, stream)
         nb = w.cols // (32 if w.dtype == DType.Q8_0 else 256)
-        isum = torch.empty((w.rows, nb), dtype=torch.int32, device=x.device)
-        imin = torch.empty((w.rows, nb), dtype=torch.int32, device=x.device)
+        isum = _empty(x, (w.rows, nb), torch.int32, stream)
+        imin = _empty(x, (w.rows, nb), torch.int32, stream)
         err = _Err()
         _check(_lib.rlq_block_sums(self._h, w._h, _dev_ptr(x2, torch.float32), x2.shape[0],
                                    _dev_ptr(isum, torch.int32), _dev_ptr(imin, torch.int32),
@@ -615,12 +643,12 @@ class Context:
         flags=SUMS_SILU_PAIR the decode step's gate/up kernel runs over w (Q4_K
         / Q5_K rows whose 16-row tiles alternate gate and up) and y holds
         silu(gate) * up, rows / 2 values; otherwise y is [batch, rows]."""
-        x2 = _columns(x, w.cols)
+        x2 = _columns(x, w.cols, stream)
         nb = w.cols // (32 if w.dtype == DType.Q8_0 else 256)
-        isum = torch.empty((w.rows, nb), dtype=torch.int32, device=x.device)
-        imin = torch.empty((w.rows, nb), dtype=torch.int32, device=x.device)
+        isum = _empty(x, (w.rows, nb), torch.int32, stream)
+        imin = _empty(x, (w.rows, nb), torch.int32, stream)
         n = w.rows // 2 if flags & self.SUMS_SILU_PAIR else x2.shape[0] * w.rows
-        y = torch.empty(n, dtype=torch.float32, device=x.device)
+        y = _empty(x, n, torch.float32, stream)
         err = _Err()
         _check(_lib.rlq_block_sums_ex(self._h, w._h, _dev_ptr(x2, torch.float32), x2.shape[0], int(flags),
                                       _dev_ptr(isum, torch.int32), _dev_ptr(imin, torch.int32),
@@ -757,7 +785,8 @@ class LlamaModel:
     def embedding(self, token, out=None, stream=None):
         """LlamaModel::embedding (llama.rs:213-221) -> f32 [width] on the GPU."""
         if out is None:
-            out = torch.empty(self.config.width, dtype=torch.float32, device="cuda")
+            with _on(stream):
+                out = torch.empty(self.config.width, dtype=torch.float32, device="cuda")
         err = _Err()
         _check(_lib.rlq_llama_embedding(self._h, int(token), _dev_ptr(out, torch.float32), _stream_ptr(stream),
                                         ctypes.byref(err)), err)
@@ -768,9 +797,9 @@ class LlamaModel:
         is updated in place to the last layer's output; returns
         (embedding, logits, argmax), each None unless asked for."""
         c = self.config
-        emb = torch.empty(c.width, dtype=torch.float32, device=hidden.device) if embedding else None
-        lg = torch.empty(c.vocabulary, dtype=torch.float32, device=hidden.device) if logits else None
-        am = torch.empty(1, dtype=torch.int32, device=hidden.device) if argmax else None
+        emb = _empty(hidden, c.width, torch.float32, stream) if embedding else None
+        lg = _empty(hidden, c.vocabulary, torch.float32, stream) if logits else None
+        am = _empty(hidden, 1, torch.int32, stream) if argmax else None
         err = _Err()
         _check(_lib.rlq_llama_step(self._h, _dev_ptr(hidden, torch.float32), int(position),
                                    _dev_ptr(emb, torch.float32) if emb is not None else None,
@@ -806,10 +835,9 @@ class LlamaModel:
         norm's input) of the latest step, as fresh GPU tensors:
         (qkv, attention, ffn, ffn_input)."""
         c = self.config
-        qkv = torch.empty(c.width + 2 * c.kv_width, dtype=torch.float32, device="cuda")
-        att = torch.empty(c.width, dtype=torch.float32, device="cuda")
-        mid = torch.empty(c.width, dtype=torch.float32, device="cuda")
-        gu = torch.empty(c.feed_forward, dtype=torch.float32, device="cuda")
+        with _on(stream):
+            qkv, att, mid, gu = (torch.empty(n, dtype=torch.float32, device="cuda")
+                                 for n in (c.width + 2 * c.kv_width, c.width, c.width, c.feed_forward))
         err = _Err()
         _check(_lib.rlq_llama_intermediates(self._h, _dev_ptr(qkv, torch.float32), _dev_ptr(att, torch.float32),
                                             _dev_ptr(mid, torch.float32), _dev_ptr(gu, torch.float32),
