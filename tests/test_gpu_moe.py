@@ -797,3 +797,46 @@ def test_route_scale_that_is_not_finite(ctx, gating, scale):
     _, w, _ = ctx.moe_route(gpu(router), gpu(x), 3, gating="sigmoid", scale=scale)
     ctx.sync()
     assert not w.cpu().numpy().view(np.uint32).any()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=lambda t: t.name)
+def test_ffn_with_many_tiles_in_any_company(ctx, t):
+    """Experts of enough rows for K to be split less, from one token (two waves) to eight
+    (four), sixteen and more (two): 64 bits for all tokens, and the same bits in all of
+    these calls.  (Other orders of the f64 sums of n terms t round apart for at most
+    (n - 1) 2^-28 sum|t| / |sum| of the values.  Here y has 16 values a token, of 70 terms
+    and a ratio near 8: about one call of 33 tokens in 1000 at the most.  Of g and u, n is
+    2, and the one in 256 that is its block's largest moves y.)"""
+    say("ffn many tiles, company", t.name)
+    L = Layer(ctx, 19, 512, 3584, 16, t, DT.Q6_K, 270)
+    ids, weights = places(271, 33, 19, 5, 0.05)
+    x, res = L.x(272, 33), normal(273, 33, 16)
+    y = L.call(gpu(x), ids, weights, residual=gpu(res))
+    ctx.sync()
+    L.check(y, quantized(act(t), x), ids, weights, res)
+    for cut in (slice(0, 1), slice(7, 8), slice(1, 9), slice(3, 19), slice(20, 30), slice(14, 33)):
+        part = L.call(gpu(x[cut]), ids[cut], weights[cut], residual=gpu(res[cut]))
+        assert torch.equal(part, y[cut]), cut
+    ctx.sync()
+    L.close()
+
+
+@pytest.mark.parametrize("tokens,experts,cols,k", [(3, 11, 64, 2), (2, 100, 4096, 5), (5, 300, 36, 9), (300, 128, 2048, 8),
+                                                   (20, 30, 17000, 3), (33, 300, 16500, 4)])
+@pytest.mark.parametrize("which", ["x", "router", "both"])
+def test_route_of_unaligned_tensors(ctx, tokens, experts, cols, k, which):
+    """Both kernels' loads of x and of the router without 16-byte alignment."""
+    say("route unaligned", tokens, experts, cols, k, which)
+    router, x = normal(280, experts, cols) * np.float32(1.5 / np.sqrt(cols)), normal(281, tokens, cols)
+
+    def off(a):
+        return torch.cat([torch.zeros(1, device="cuda"), gpu(a).view(-1)])[1:].view(a.shape)
+
+    r, z = (off(router) if which != "x" else gpu(router)), (off(x) if which != "router" else gpu(x))
+    ids, w, logits = ctx.moe_route(r, z, k, logits=True)
+    aligned = ctx.moe_route(gpu(router), gpu(x), k, logits=True)
+    ctx.sync()
+    assert torch.equal(ids, aligned[0]) and torch.equal(w, aligned[1]) and torch.equal(logits, aligned[2])
+    _, wi, ww = plain_route(router, x, k)
+    assert np.array_equal(ids.cpu().numpy(), wi)
+    assert np.all(np.abs(w.cpu().numpy() - ww) <= (2.0 ** -24 + 2.0 ** -45) * np.abs(ww) + 2.0 ** -150)
