@@ -395,21 +395,20 @@ __device__ __forceinline__ MoePlaces moe_places(const MoeArgs& a) {
 }
 
 __device__ __forceinline__ void moe_plan(const MoeArgs& a) {
-    __shared__ uint32_t mask[kMoeMaxExperts], wave_n[8], wave_b[8], bad, some;
+    __shared__ uint32_t mask[kMoeMaxExperts], wave_n[8], wave_b[8], bad, served;
     __shared__ uint16_t place[kMoeMaxExperts];
     __shared__ int32_t ids[kMoeTokens * kMoeMaxSlots];
     __shared__ float weights[kMoeTokens * kMoeMaxSlots];
     const uint32_t tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = nt >> 6;
     const uint32_t pairs = a.tokens * a.slots;
     for (uint32_t e = tid; e < a.experts; e += nt) mask[e] = 0;
-    if (tid == 0) bad = 0, some = 0;
+    if (tid == 0) bad = 0, served = 0;
     __syncthreads();
     for (uint32_t p = tid; p < pairs; p += nt) {
         int32_t id = a.ids[p];
         const uint32_t t = p / a.slots;
         if (id >= 0 && id < (int32_t)a.experts) {
             atomicOr(&mask[id], 1u << t);
-            atomicOr(&some, 1u << t);
         } else if (id != -1) {
             report_error(a.err_word, bounds_key((uint64_t)a.token0 * a.slots + p));
             atomicOr(&bad, 1u << t);
@@ -436,11 +435,11 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& a) {
             if (w < wave) j += wave_n[w], b += wave_b[w];
             used += wave_n[w], rows += wave_b[w];
         }
-        if (m) a.plan[j] = make_uint4(e, b, m, 0), place[e] = (uint16_t)j;
+        if (m) a.plan[j] = make_uint4(e, b, m, 0), place[e] = (uint16_t)j, atomicOr(&served, m);
         __syncthreads();
     }
     for (uint32_t j = used + tid; j < a.most; j += nt) a.plan[j] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) *a.n_used = used, *a.bad = bad, *a.some = some;
+    if (tid == 0) *a.head = make_uint4(used, bad, served, 0);
     for (uint32_t p = tid; p < pairs; p += nt) {  // a token's first place with an expert speaks for all of them
         const int32_t id = ids[p];
         const uint32_t t = p / a.slots, end = (t + 1) * a.slots;
@@ -987,7 +986,8 @@ moe_down_kernel(MoeArgs a) {
         }
         if (threadIdx.x == 0) marked = 0;
     } else {
-        used = *a.n_used, bad = *a.bad, some = *a.some;
+        const uint4 h = *a.head;
+        used = h.x, bad = h.y, some = h.z;
         for (uint32_t i = threadIdx.x; i < a.most; i += 64 * KS) {  // (past `used` no one looks)
             const uint4 p = a.plan[i];
             plan[i] = make_uint2(p.x | p.y << 16, p.z);
@@ -1168,9 +1168,7 @@ static size_t moe_carve(const MoeCall& c, uint32_t tokens, uint8_t* base, MoeArg
     const uint64_t pairs = (uint64_t)tokens * c.slots;
     const uint64_t used = pairs < c.experts || tokens == 1 ? pairs : c.experts;  // (one token: its places, each on its own)
     MoeArgs m{};
-    m.n_used = (uint32_t*)take(4);
-    m.bad = (uint32_t*)take(4);
-    m.some = (uint32_t*)take(4);
+    m.head = (uint4*)take(16);
     m.plan = (uint4*)take(used * 16);
     m.most = (uint32_t)used;
     m.wsum = (double*)take(used * kMoeTokens * 8);

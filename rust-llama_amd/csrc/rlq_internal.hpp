@@ -245,7 +245,7 @@ struct MoeArgs {  // of one pass
     float* y;
     unsigned long long* err_word;
     // the plan and the workspace (moe.hip)
-    uint32_t *n_used, *bad, *some;
+    uint4* head;  // experts in use; tokens (bits) with an id out of range, and with an expert
     uint4* plan;
     uint32_t most;  // entries of it
     double* wsum;
