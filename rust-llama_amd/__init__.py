@@ -23,7 +23,6 @@ llama.rs): embedding(token) and step(hidden, position) -> (embedding, logits)
 over quantized matrices and a resident f32 KV cache.
 """
 import atexit
-import contextlib
 import ctypes
 import enum
 import os
@@ -341,35 +340,27 @@ def _stream_ptr(stream):
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-def _on(stream, device=None):
-    """Where a call that is given a stream makes its tensors: on that stream, whose
-    order they then have.  What torch's current stream has freed may be in use there
-    until its queue is done, and what is copied there may not be whole when the call
-    runs."""
-    if stream is None:
-        return contextlib.nullcontext()
+def _makes(x, outputs):
+    """Whether a call that is given a stream makes tensors: outputs, or the copy of a
+    strided x.  They must be that stream's (memory that torch's current stream has freed
+    may be in use there until its queue is done, and what is copied there may not be
+    whole when the call runs): such a call is made again with the stream as the current one."""
+    return isinstance(x, torch.Tensor) and (outputs or not x.is_contiguous())
+
+
+def _on(stream, x=None):
+    """The stream (a torch stream or its handle) as torch's current one."""
     if not isinstance(stream, torch.cuda.Stream):
-        stream = torch.cuda.ExternalStream(stream if isinstance(stream, int) else stream.cuda_stream, device=device)
+        device = None if x is None or not x.is_cuda else x.device
+        handle = stream if isinstance(stream, int) else stream.cuda_stream
+        # (0 is HIP's null stream; torch would make a stream of its own for it)
+        stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
     return torch.cuda.stream(stream)
 
 
-def _empty(t, shape, dtype, stream):
-    """An output beside t of a call on the stream."""
-    if stream is None and isinstance(t, torch.Tensor):
-        return t.new_empty(shape, dtype=dtype)  # (0.3 us less than torch.empty on t's device)
-    with _on(stream if getattr(t, "is_cuda", False) else None, t.device):
-        return torch.empty(shape, dtype=dtype, device=t.device)
-
-
-def _reshape(t, shape, stream):
-    """t.reshape(shape); the copy that some strides need is made on the stream."""
-    with _on(stream if getattr(t, "is_cuda", False) else None, t.device):
-        return t.reshape(shape)
-
-
-def _columns(x, cols, stream=None):
+def _columns(x, cols):
     """x as [batch, cols]; as it is when it has that shape (a reshape costs 1 us)."""
-    return x if x.ndim == 2 and x.shape[1] == cols else _reshape(x, (-1, cols), stream)
+    return x if x.ndim == 2 and x.shape[1] == cols else x.reshape(-1, cols)
 
 
 class Context:
@@ -394,9 +385,12 @@ class Context:
 
     def matmul(self, w, x, y=None, stream=None):
         """MUL_MAT / Matrix::multiply: x [batch, cols] f32 -> y [batch, rows] f32."""
-        x2 = _columns(x, w.cols, stream)
+        if stream is not None and _makes(x, y is None):
+            with _on(stream, x):
+                return self.matmul(w, x, y)
+        x2 = _columns(x, w.cols)
         if y is None:
-            y = _empty(x, (x2.shape[0], w.rows), torch.float32, stream)
+            y = torch.empty((x2.shape[0], w.rows), dtype=torch.float32, device=x.device)
         err = _Err()
         _check(_lib.rlq_matmul(self._h, w._h, _dev_ptr(x2, torch.float32), x2.shape[0],
                                _dev_ptr(y, torch.float32), _stream_ptr(stream), ctypes.byref(err)), err)
@@ -406,8 +400,11 @@ class Context:
         """Matrix::multiply (math.rs:144-169): one input vector x [cols] ->
         y [rows], with the reference's finite checks of the input and the
         output (NonFinite errors at sync)."""
+        if stream is not None and _makes(x, y is None):
+            with _on(stream, x):
+                return self.multiply(w, x, y)
         if y is None:
-            y = _empty(x, w.rows, torch.float32, stream)
+            y = torch.empty(w.rows, dtype=torch.float32, device=x.device)
         err = _Err()
         _check(_lib.rlq_multiply(self._h, w._h, _dev_ptr(x, torch.float32), _dev_ptr(y, torch.float32),
                                  _stream_ptr(stream), ctypes.byref(err)), err)
@@ -415,12 +412,15 @@ class Context:
 
     def matmul_argmax(self, w, x, y=None, argmax=None, stream=None):
         """matmul followed by the greedy sampler's index per column."""
-        x2 = _columns(x, w.cols, stream)
+        if stream is not None and _makes(x, y is None or argmax is None):
+            with _on(stream, x):
+                return self.matmul_argmax(w, x, y, argmax)
+        x2 = _columns(x, w.cols)
         batch = x2.shape[0]
         if y is None:
-            y = _empty(x, (batch, w.rows), torch.float32, stream)
+            y = torch.empty((batch, w.rows), dtype=torch.float32, device=x.device)
         if argmax is None:
-            argmax = _empty(x, batch, torch.int32, stream)
+            argmax = torch.empty(batch, dtype=torch.int32, device=x.device)
         err = _Err()
         _check(_lib.rlq_matmul_argmax(self._h, w._h, _dev_ptr(x2, torch.float32), batch,
                                       _dev_ptr(y, torch.float32), _dev_ptr(argmax, torch.int32),
@@ -434,7 +434,10 @@ class Context:
         arguments launches the same call again with only the C call's own
         cost (for serving loops; it raises like matmul).  The tensors stay
         referenced by the function."""
-        x2 = _columns(x, w.cols, stream)
+        if stream is not None and _makes(x, False):
+            with _on(stream, x):
+                return self.bind_matmul(w, x, y, argmax)
+        x2 = _columns(x, w.cols)
         batch = x2.shape[0]
         if y.numel() != batch * w.rows:
             raise ValueError("y must hold batch * rows f32 values")
@@ -464,7 +467,10 @@ class Context:
         """rlq_matmul_noalloc: matmul (argmax None) or matmul_argmax into the
         caller's y [batch, rows] (and argmax [batch] int32), with the
         library's static device scratch instead of any allocation."""
-        x2 = _columns(x, w.cols, stream)
+        if stream is not None and _makes(x, False):
+            with _on(stream, x):
+                return self.matmul_noalloc(w, x, y, argmax)
+        x2 = _columns(x, w.cols)
         err = _Err()
         _check(_lib.rlq_matmul_noalloc(self._h, w._h, _dev_ptr(x2, torch.float32), x2.shape[0],
                                        _dev_ptr(y, torch.float32),
@@ -474,9 +480,12 @@ class Context:
 
     def quantize(self, dtype, x, stream=None):
         """GPU quantize_into for Q8_0 / Q8_K: x [batch, cols] -> GGUF bytes."""
-        x2 = _reshape(x, (x.shape[0] if x.dim() > 1 else 1, -1), stream)
+        if stream is not None and _makes(x, True):
+            with _on(stream, x):
+                return self.quantize(dtype, x)
+        x2 = x.reshape(x.shape[0] if x.dim() > 1 else 1, -1)
         cols = x2.shape[1]
-        out = _empty(x, x2.shape[0] * row_bytes(dtype, cols), torch.uint8, stream)
+        out = torch.empty(x2.shape[0] * row_bytes(dtype, cols), dtype=torch.uint8, device=x.device)
         err = _Err()
         _check(_lib.rlq_quantize_device(self._h, int(dtype), _dev_ptr(x2, torch.float32), cols, x2.shape[0],
                                         _dev_ptr(out, torch.uint8), _stream_ptr(stream), ctypes.byref(err)), err)
@@ -486,12 +495,15 @@ class Context:
         """GGML MUL_MAT with broadcast (cpu_extra.rs:756-873): w stacked
         [w.n3][w.n2] matrices; x [n3, n2, ncols, cols] f32, or uint8 rows of the
         activation type when x_dtype is it -> y [n3, n2, ncols, rows] f32."""
+        if stream is not None and _makes(x, y is None):
+            with _on(stream, x):
+                return self.mul_mat(w, x, x_dtype, y)
         x_dtype = DType(x_dtype)
         if x.dim() != 4:
             raise ValueError("x must be [n3, n2, ncols, cols] (f32) or [n3, n2, ncols, row bytes] (uint8)")
         n3, n2, ncols = x.shape[:3]
         if y is None:
-            y = _empty(x, (n3, n2, ncols, w.rows), torch.float32, stream)
+            y = torch.empty((n3, n2, ncols, w.rows), dtype=torch.float32, device=x.device)
         xp = _dev_ptr(x, x.dtype)  # the library checks x_dtype against the weights
         err = _Err()
         _check(_lib.rlq_mul_mat(self._h, w._h, int(x_dtype), xp, ncols, n2, n3, _dev_ptr(y, torch.float32),
@@ -502,11 +514,14 @@ class Context:
         """GGML MUL_MAT_ID (cpu_index.rs:169-236): experts w [w.n2 matrices],
         x [tokens, ncols, cols] f32 (or activation bytes), ids [tokens, slots]
         int32 on the GPU -> y [tokens, slots, rows] f32 (0 where ids is -1)."""
+        if stream is not None and _makes(x, y is None):
+            with _on(stream, x):
+                return self.mul_mat_id(w, x, ids, x_dtype, y)
         x_dtype = DType(x_dtype)
         tokens, ncols = x.shape[:2]
         slots = ids.shape[1]
         if y is None:
-            y = _empty(x, (tokens, slots, w.rows), torch.float32, stream)
+            y = torch.empty((tokens, slots, w.rows), dtype=torch.float32, device=x.device)
         xp = _dev_ptr(x, x.dtype)
         err = _Err()
         _check(_lib.rlq_mul_mat_id(self._h, w._h, int(x_dtype), xp, ncols, tokens, _dev_ptr(ids, torch.int32),
@@ -521,6 +536,10 @@ class Context:
         Q8_0, y's blocks [rows, row_bytes(packed, cols)] uint8, the packed
         right-hand side of mul_mat, mul_mat_id and moe_ffn.  Outputs may be
         given; total and y may take the place of x or residual."""
+        if stream is not None and _makes(x, (normed and y is None) or (packed is not None and q is None) or
+                                         (residual is not None and total is None)):
+            with _on(stream, x):
+                return self.rms_norm(x, weight, eps, residual, packed, normed, total, y, q)
         cols = weight.numel()
         if x.shape[-1] != cols or (residual is not None and residual.shape != x.shape):
             raise ValueError("x and residual must be [..., cols] with the weight's cols")
@@ -530,16 +549,16 @@ class Context:
             if total.numel() != n:
                 raise ValueError("total's size is not x's")
         elif residual is not None:
-            total = _empty(x, x.shape, x.dtype, stream)
+            total = torch.empty_like(x)
         if y is not None:
             if y.numel() != n:
                 raise ValueError("y's size is not x's")
         elif normed:
-            y = _empty(x, x.shape, x.dtype, stream)
+            y = torch.empty_like(x)
         if packed is not None:
             nbytes = row_bytes(packed, cols)
             if q is None:
-                q = _empty(x, (rows, nbytes), torch.uint8, stream)
+                q = x.new_empty((rows, nbytes), dtype=torch.uint8)
             elif q.numel() != rows * nbytes:
                 raise ValueError("q must hold x's rows in blocks")
         elif q is not None:
@@ -563,17 +582,20 @@ class Context:
         asked for with True or a tensor).  gating: "softmax" or "sigmoid" of the
         logits; bias [experts] is added to the scores for the choice only (-inf:
         never chosen; places with no expert left get id -1 and weight 0)."""
+        if stream is not None and _makes(x, ids is None or weights is None or logits is True):
+            with _on(stream, x):
+                return self.moe_route(router, x, top_k, gating, normalize, scale, bias, logits, ids, weights)
         if gating not in ("softmax", "sigmoid"):
             raise ValueError("gating must be softmax or sigmoid")
         experts, cols = router.shape
-        x2 = _columns(x, cols, stream)
+        x2 = _columns(x, cols)
         tokens, top_k = x2.shape[0], int(top_k)
         if ids is None:
-            ids = _empty(x, (tokens, top_k), torch.int32, stream)
+            ids = x.new_empty((tokens, top_k), dtype=torch.int32)
         if weights is None:
-            weights = _empty(x, (tokens, top_k), x.dtype, stream)
+            weights = x.new_empty((tokens, top_k))
         if logits is True:
-            logits = _empty(x, (tokens, experts), x.dtype, stream)
+            logits = x.new_empty((tokens, experts))
         elif logits is False:
             logits = None
         if ids.numel() != tokens * top_k or weights.numel() != tokens * top_k \
@@ -596,6 +618,9 @@ class Context:
         when x_dtype is it; ids int32 and weights f32 [tokens, slots] (id -1: no
         expert) -> y [tokens, out] = residual + the weighted sum of
         down(silu(gate x) * up x) over a token's experts."""
+        if stream is not None and _makes(x, y is None):
+            with _on(stream, x):
+                return self.moe_ffn(gate, up, down, x, ids, weights, x_dtype, residual, y)
         x_dtype = DType(x_dtype)
         tokens, slots = ids.shape
         f32 = torch.float32
@@ -605,7 +630,7 @@ class Context:
         if weights.shape != ids.shape:
             raise ValueError("weights must have the shape of ids")
         if y is None:
-            y = _empty(weights, (tokens, down.rows), weights.dtype, stream)
+            y = weights.new_empty((tokens, down.rows))
         if y.numel() != tokens * down.rows or (residual is not None and residual.numel() != y.numel()):
             raise ValueError("y and residual must hold the down matrix's rows for every token")
         err = _Err()
@@ -626,10 +651,13 @@ class Context:
         ([batch, cols] or [cols], batch <= 8), from the decode kernel of that
         batch size (matmul runs it too, or for some shapes of two and more
         columns the int8 GEMM); more columns of Q4_K: from its f16 GEMM."""
-        x2 = _columns(x, w.cols, stream)
+        if stream is not None and _makes(x, True):
+            with _on(stream, x):
+                return self.block_sums(w, x)
+        x2 = _columns(x, w.cols)
         nb = w.cols // (32 if w.dtype == DType.Q8_0 else 256)
-        isum = _empty(x, (w.rows, nb), torch.int32, stream)
-        imin = _empty(x, (w.rows, nb), torch.int32, stream)
+        isum = torch.empty((w.rows, nb), dtype=torch.int32, device=x.device)
+        imin = torch.empty((w.rows, nb), dtype=torch.int32, device=x.device)
         err = _Err()
         _check(_lib.rlq_block_sums(self._h, w._h, _dev_ptr(x2, torch.float32), x2.shape[0],
                                    _dev_ptr(isum, torch.int32), _dev_ptr(imin, torch.int32),
@@ -643,12 +671,15 @@ class Context:
         flags=SUMS_SILU_PAIR the decode step's gate/up kernel runs over w (Q4_K
         / Q5_K rows whose 16-row tiles alternate gate and up) and y holds
         silu(gate) * up, rows / 2 values; otherwise y is [batch, rows]."""
-        x2 = _columns(x, w.cols, stream)
+        if stream is not None and _makes(x, True):
+            with _on(stream, x):
+                return self.block_sums_ex(w, x, flags)
+        x2 = _columns(x, w.cols)
         nb = w.cols // (32 if w.dtype == DType.Q8_0 else 256)
-        isum = _empty(x, (w.rows, nb), torch.int32, stream)
-        imin = _empty(x, (w.rows, nb), torch.int32, stream)
+        isum = torch.empty((w.rows, nb), dtype=torch.int32, device=x.device)
+        imin = torch.empty((w.rows, nb), dtype=torch.int32, device=x.device)
         n = w.rows // 2 if flags & self.SUMS_SILU_PAIR else x2.shape[0] * w.rows
-        y = _empty(x, n, torch.float32, stream)
+        y = torch.empty(n, dtype=torch.float32, device=x.device)
         err = _Err()
         _check(_lib.rlq_block_sums_ex(self._h, w._h, _dev_ptr(x2, torch.float32), x2.shape[0], int(flags),
                                       _dev_ptr(isum, torch.int32), _dev_ptr(imin, torch.int32),
@@ -784,9 +815,11 @@ class LlamaModel:
 
     def embedding(self, token, out=None, stream=None):
         """LlamaModel::embedding (llama.rs:213-221) -> f32 [width] on the GPU."""
-        if out is None:
+        if stream is not None and out is None:
             with _on(stream):
-                out = torch.empty(self.config.width, dtype=torch.float32, device="cuda")
+                return self.embedding(token, out)
+        if out is None:
+            out = torch.empty(self.config.width, dtype=torch.float32, device="cuda")
         err = _Err()
         _check(_lib.rlq_llama_embedding(self._h, int(token), _dev_ptr(out, torch.float32), _stream_ptr(stream),
                                         ctypes.byref(err)), err)
@@ -796,10 +829,13 @@ class LlamaModel:
         """LlamaModel::step (llama.rs:222-248): hidden (f32 [width] on the GPU)
         is updated in place to the last layer's output; returns
         (embedding, logits, argmax), each None unless asked for."""
+        if stream is not None and _makes(hidden, embedding or logits or argmax):
+            with _on(stream, hidden):
+                return self.step(hidden, position, embedding, logits, argmax)
         c = self.config
-        emb = _empty(hidden, c.width, torch.float32, stream) if embedding else None
-        lg = _empty(hidden, c.vocabulary, torch.float32, stream) if logits else None
-        am = _empty(hidden, 1, torch.int32, stream) if argmax else None
+        emb = torch.empty(c.width, dtype=torch.float32, device=hidden.device) if embedding else None
+        lg = torch.empty(c.vocabulary, dtype=torch.float32, device=hidden.device) if logits else None
+        am = torch.empty(1, dtype=torch.int32, device=hidden.device) if argmax else None
         err = _Err()
         _check(_lib.rlq_llama_step(self._h, _dev_ptr(hidden, torch.float32), int(position),
                                    _dev_ptr(emb, torch.float32) if emb is not None else None,
@@ -834,10 +870,14 @@ class LlamaModel:
         silu(gate) * up and the residual stream after attention (the FFN
         norm's input) of the latest step, as fresh GPU tensors:
         (qkv, attention, ffn, ffn_input)."""
+        if stream is not None:
+            with _on(stream):
+                return self.intermediates()
         c = self.config
-        with _on(stream):
-            qkv, att, mid, gu = (torch.empty(n, dtype=torch.float32, device="cuda")
-                                 for n in (c.width + 2 * c.kv_width, c.width, c.width, c.feed_forward))
+        qkv = torch.empty(c.width + 2 * c.kv_width, dtype=torch.float32, device="cuda")
+        att = torch.empty(c.width, dtype=torch.float32, device="cuda")
+        mid = torch.empty(c.width, dtype=torch.float32, device="cuda")
+        gu = torch.empty(c.feed_forward, dtype=torch.float32, device="cuda")
         err = _Err()
         _check(_lib.rlq_llama_intermediates(self._h, _dev_ptr(qkv, torch.float32), _dev_ptr(att, torch.float32),
                                             _dev_ptr(mid, torch.float32), _dev_ptr(gu, torch.float32),
