@@ -368,13 +368,18 @@ int32_t rlq_moe_route(rlq_context *ctx, const float *router, const float *x, uin
  * 16-byte aligned; quantized as rlq_mul_mat_id does) or rows of gate's activation
  * type (Q8_K 4-byte aligned, Q8_0 2-byte), taken as given but for the Q8_K bsums, which are those
  * of the levels.  The block integers are exact; their sums run in f64 and are
- * rounded once where g, u, h and y become f32, so y does not depend on what shares
- * a call.  h is quantized like any f32 column of down.  ids and weights [tokens,
+ * rounded once where g, u, h and y become f32.  h is quantized like any f32 column of
+ * down.  What shares a call with a token changes the order of those f64 sums alone: a
+ * sum of n terms t can then round to the other of two f32 neighbours, for at most
+ * n 2^-28 sum|t| / |sum| of the values (and such an h to the other of two levels, where it
+ * lies between them); otherwise y has the same bits in any company.  ids and weights [tokens,
  * slots]; -1: no expert (its weight is not looked at), a token without any gets
  * its residual, its x not being looked at.  residual may be null (0), and may be y.
  * An expert's weights that are not finite concern the tokens that use it alone.
  * 32 tokens share a pass over the weights of the experts that they use; more
- * tokens take further passes (a prompt is better served by rlq_mul_mat_id).
+ * tokens take further passes.  From 33 to 96 tokens on, by the experts' sizes, three calls
+ * of rlq_mul_mat_id with f32 columns (not packed ones: those of types with minimums keep
+ * its decode kernels) are faster, SiLU, product and weighted sum included.
  * Capturing: make the same call once before, for the scratch.
  * Errors: RLQ_TENSOR_SHAPE (stacks that do not match, slots 0),
  * RLQ_TENSOR_UNSUPPORTED (up's type, x_dtype), RLQ_UNIMPLEMENTED (more than 1024

@@ -10,10 +10,13 @@
 //   y_t = residual_t + sum_s w_ts D_e h
 // The products are those of MUL_MAT_ID (crates/tensor/src/cpu_index.rs:169-236):
 // exact integers per block of 256 (or 32 for Q8_0), but added up in f64 and
-// rounded once, to g, u and y.  No order of the sums shows in those roundings
-// (but for one value in about 2^29 that lies next to a border), so the results do
-// not depend on how many tokens share a call or how K is split: h rounds to the
-// same levels in every one of them.
+// rounded once, to g, u and y.  The order of a sum's terms depends on how many
+// tokens share a call (K splits, parts of a tile, and the weights of an expert that a
+// token names twice).  Two orders of n terms t differ by at most 2 n 2^-53 sum|t|, so
+// they round to different f32 only where a border lies in between: at most
+// n 2^-28 sum|t| / |sum| of the values, e.g. one g in some millions of 4096 values
+// (n = 16).  Only such a value, and an h of it that lies between two levels, can tell a
+// token's company.
 #include "rlq_device.hpp"
 #include "rlq_igops.hpp"
 #include "rlq_internal.hpp"
@@ -618,7 +621,7 @@ struct MoeWeights<kQ8_0> {
 };
 
 // A workgroup's LDS: its waves' f64 sums, each wave's column scales of its current
-// chunk, and (up, one token) the image of x.
+// chunk, and (one token) the image of x (up) or of its part of h (down).
 template <uint32_t T>
 constexpr uint32_t moe_lds(uint32_t ks, uint32_t sums) {
     return ks * (sums * 512 + MoeWeights<T>::kFactors * 256);

@@ -804,7 +804,7 @@ def test_ffn_with_many_tiles_in_any_company(ctx, t):
     """Experts of enough rows for K to be split less, from one token (two waves) to eight
     (four), sixteen and more (two): 64 bits for all tokens, and the same bits in all of
     these calls.  (Other orders of the f64 sums of n terms t round apart for at most
-    (n - 1) 2^-28 sum|t| / |sum| of the values.  Here y has 16 values a token, of 70 terms
+    n 2^-28 sum|t| / |sum| of the values.  Here y has 16 values a token, of 70 terms
     and a ratio near 8: about one call of 33 tokens in 1000 at the most.  Of g and u, n is
     2, and the one in 256 that is its block's largest moves y.)"""
     say("ffn many tiles, company", t.name)

@@ -1,7 +1,7 @@
 """rlq_rms_norm against the oracle: the residual's addition in numpy's f32, the
 norm by the reference's sequential arithmetic and its blocks by the reference's
-quantizers, all bit for bit.  Shapes cross the kernel's variants (16, 64, 256 and
-1024 lanes a row, one and two units a lane, rows without 16-byte alignment)."""
+quantizers, all bit for bit.  Shapes cross the kernel's variants (64, 256 and 1024
+lanes a row, one to eight units of four values a lane, rows without 16-byte alignment)."""
 import numpy as np
 import pytest
 
