@@ -379,7 +379,8 @@ int32_t rlq_moe_route(rlq_context *ctx, const float *router, const float *x, uin
  * 32 tokens share a pass over the weights of the experts that they use; more
  * tokens take further passes.  From 33 to 96 tokens on, by the experts' sizes, three calls
  * of rlq_mul_mat_id with f32 columns (not packed ones: those of types with minimums keep
- * its decode kernels) are faster, SiLU, product and weighted sum included.
+ * its decode kernels) are faster, SiLU, product and weighted sum included; with very many
+ * experts (256 of 2048x7168) from 3 to 16 tokens, too, by up to 6 %.
  * Capturing: make the same call once before, for the scratch.
  * Errors: RLQ_TENSOR_SHAPE (stacks that do not match, slots 0),
  * RLQ_TENSOR_UNSUPPORTED (up's type, x_dtype), RLQ_UNIMPLEMENTED (more than 1024
