@@ -266,7 +266,7 @@ def _plain_pages(s):
     tables.copy_(torch.where(fresh, taken, torch.where(gone.view(fresh.shape), -1, tables)))
     left = top - fresh.sum()
     place = torch.arange(free.numel(), device=free.device)
-    free.copy_(torch.where((place >= n) & (place < left), stack[:-1], free))
+    free.copy_(torch.where((place >= n) & (place < top), stack[:-1], free))
     # the new tokens, a request after the other
     ends = more.cumsum(0)
     starts = torch.cat([ends.new_zeros(1), ends])
@@ -480,7 +480,8 @@ def _exact_pages(s):
         held = -(-int(before[r]) // page)
         stack += [p for p in tables[r, :held] if p >= 0]
         tables[r, :held] = -1
-    kept, after, starts, slots, positions, requests = list(stack), [], [0], [], [], []
+    free[n:len(stack)] = stack[n:]
+    after, starts, slots, positions, requests = [], [0], [], [], []
     for r in range(len(before)):
         have, end = int(before[r]), 0 if new[r] < 0 else int(before[r] + new[r])
         for j in range(-(-have // page), -(-end // page)):
@@ -491,8 +492,6 @@ def _exact_pages(s):
         requests.append(np.full(len(at), r))
         after.append(end)
         starts.append(starts[-1] + len(at))
-    if len(stack) > n:
-        free[n:len(stack)] = kept[n:len(stack)]
     rest = np.full(s["tokens"] - starts[-1], -1)
     to = lambda v, t: torch.from_numpy(np.concatenate(v) if isinstance(v, tuple) else np.asarray(v)).to(t).cuda()  # noqa: E731
     return {"tables": to(tables, I32), "free": to(free, I32), "count": to([len(stack)], I32), "lengths": to(after, I32),
