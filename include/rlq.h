@@ -47,6 +47,7 @@ extern "C" {
  * id of that enum is accepted where a dtype is taken; ids outside the path
  * return RLQ_UNIMPLEMENTED after the reference's own checks. */
 enum rlq_dtype {
+    RLQ_F32 = 0, RLQ_F16 = 1, RLQ_BF16 = 30, /* of a KV cache */
     RLQ_Q8_0 = 8, RLQ_Q2_K = 10, RLQ_Q3_K = 11, RLQ_Q4_K = 12, RLQ_Q5_K = 13, RLQ_Q6_K = 14, RLQ_Q8_K = 15
 };
 
@@ -74,7 +75,8 @@ typedef enum rlq_status {
     RLQ_INVALID_ARGUMENT = 20,          /* null pointer or handle */
     RLQ_INVALID_CONFIG = 21,            /* a = check (see rlq_llama_create) */
     RLQ_INVALID_TOKEN = 22,             /* a = token, b = vocabulary */
-    RLQ_INVALID_STATE = 23,             /* a = KV rows held, b = max_context (cache full) */
+    RLQ_INVALID_STATE = 23,             /* a = KV rows held, b = max_context (cache full); rlq_kv_pages:
+                                           a = request, b = the reason */
     /* TensorError variants of the GGML ops (crates/tensor/src/lib.rs:35-50) */
     RLQ_TENSOR_SHAPE = 24,              /* Shape: incompatible MUL_MAT / MUL_MAT_ID dimensions */
     RLQ_TENSOR_BOUNDS = 25,             /* Bounds: an expert id outside [-1, experts); a = its index */
@@ -392,6 +394,119 @@ int32_t rlq_moe_route(rlq_context *ctx, const float *router, const float *x, uin
 int32_t rlq_moe_ffn(rlq_context *ctx, const rlq_weights *gate, const rlq_weights *up, const rlq_weights *down,
                     uint32_t x_dtype, const void *x, uint64_t tokens, const int32_t *ids, const float *weights,
                     uint64_t slots, const float *residual, float *y, void *stream, rlq_error *err);
+
+/* ---- paged KV cache --------------------------------------------------------------
+ * Several requests in one cache.  A layer's keys and values lie in pages of `page`
+ * tokens; a request's row of a block table names its pages in order.  One step of a
+ * batch is rlq_kv_pages (once), then for every layer rlq_kv_store and
+ * rlq_kv_attention; rlq_beam_select and rlq_beam_reorder serve beams.  All pointers
+ * are device pointers unless said otherwise.  What concerns one row (token, group)
+ * alone holds back the outputs of that row; the others' are written, and rlq_sync
+ * reports the first. */
+
+/* One layer.  Page p, KV head h at k + p * k_stride + h * plane bytes (v likewise),
+ * where a plane is `page` tokens of dim values each (RLQ_F32, RLQ_F16, RLQ_BF16), or for
+ * RLQ_Q8_0 page * dim levels (int8) and then page * dim / 32 f16 scales: value =
+ * level * scale of its block of 32.  page: 16, 32, 64, 128 or 256; dim: a
+ * multiple of 32 up to 256; strides in bytes, multiples of 16 and at least kv_heads
+ * planes; k and v 16-byte aligned. */
+typedef struct rlq_kv_cache {
+    void *k, *v;
+    uint32_t dtype, kv_heads, page, dim;
+    uint64_t pages, k_stride, v_stride;
+} rlq_kv_cache;
+
+/* Pages, block tables and the rows of a batch from the requests' lengths.  Request
+ * r holds before[r] tokens and gets more[r] (0: waits); more[r] < 0: it has ended.
+ * The free list is free[0 .. *count), taken from its end:
+ *   - ended requests' pages, owned[r][0 .. ceil(before / page)) without the negative
+ *     entries, go to its end, in the order of requests and columns, and these
+ *     entries become -1;
+ *   - then request after request, columns ceil(before / page) to ceil((before + more) /
+ *     page) of its row of the tables get pages off the end;
+ *   after[r] = before + more (0: ended), *count_after = what is left on the list,
+ *   starts[r] = the request's first row, starts[requests] = rows in use;
+ *   row t of request r: slots[t] = tables[r][p / page] * page + p % page with
+ *   positions[t] = p = before + t - starts[r], out_requests[t] = r; rows behind the last: -1.
+ * tables and owned are [requests, width] i32; owned null: tables.  (A table whose rows
+ * share pages, as after rlq_beam_reorder, has its own pages in `owned`.)  `pages` is the size
+ * of the free list's memory, and page numbers on it are below that.  after may be before,
+ * count_after may be count; nothing else may overlap.  At most 4096 requests and
+ * 2^31 - 1 tokens (rows of the batch, with those behind the last one).  At rlq_sync, with nothing written:
+ * RLQ_TENSOR_BOUNDS (a = the index in owned of an ended request's page not below `pages`); RLQ_INVALID_STATE (a = request,
+ * b: 0 a count that is negative or, with the ended requests' pages, above `pages`; 1 no page
+ * left; 2 more than `width` columns; 3 more than `tokens` rows; 4 before negative, or
+ * before + more past 2^31 - 1).  Capturing: make the same call once before. */
+int32_t rlq_kv_pages(rlq_context *ctx, const int32_t *before, const int32_t *more, uint64_t requests, uint64_t page,
+                     int32_t *tables, int32_t *owned, uint64_t width, int32_t *free, const int32_t *count,
+                     uint64_t pages, uint64_t tokens, int32_t *after, int32_t *count_after, int32_t *starts,
+                     int64_t *slots, int32_t *positions, int32_t *out_requests, void *stream, rlq_error *err);
+
+/* Keys and values of `tokens` tokens into their slots (page * page size + place), and
+ * the queries beside them: k, v [tokens, kv_heads, dim] and q [tokens, heads, dim] f32, tokens
+ * k_stride (v_stride, q_stride, out_stride) floats apart, such as parts of one product's
+ * rows.  The first 2 * half values of each head of q and k are rotated by
+ * positions[t] * freqs[i], i < half: neighbours (2i, 2i + 1) with RLQ_ROPE_PAIRS, as
+ * rlq_llama_step does (crates/model-runtime/src/math.rs:322-334), else values i and i +
+ * half; angles, sines and products in f64, rounded once to f32.  (rlq_llama_step's own
+ * angles are the reference's, multiplied up in f32.)  half 0: no rotation (positions and freqs are
+ * not looked at).  q and q_out may be null (heads 0), and q_out may be q.  The cache's values are those f32, rounded to
+ * nearest (Q8_0: as rlq_quantize_device).  Slots are distinct; of a slot named twice each
+ * value is one of the tokens'.  Slot -1: a row behind the batch's last one, left alone.
+ * At rlq_sync, with nothing of the token written: RLQ_TENSOR_BOUNDS (a = the token:
+ * a slot outside the cache), RLQ_NON_FINITE_INPUT (a value that is not finite, or beyond
+ * F16's or BF16's range; a = its index in [q | k | v], b = the token), RLQ_UNREPRESENTABLE_SCALE (Q8_0; a =
+ * its block in [k | v], b = the token).  At most 8388606 tokens. */
+#define RLQ_ROPE_PAIRS 1u
+int32_t rlq_kv_store(rlq_context *ctx, const rlq_kv_cache *cache, const float *q, uint64_t q_stride, uint64_t heads,
+                     const float *k, uint64_t k_stride, const float *v, uint64_t v_stride, uint64_t tokens,
+                     const int64_t *slots, const int32_t *positions, const float *freqs, uint64_t half, uint32_t flags,
+                     float *q_out, uint64_t out_stride, void *stream, rlq_error *err);
+
+/* Attention of `rows` tokens over the pages: for row t, query head h and KV head
+ * h / (heads / kv_heads)
+ *   out[t][h] = sum over tokens j of softmax_j(scale * q[t][h] . k_j) v_j,
+ * j from 0, or positions[t] + 1 - window where window is not 0, to positions[t]; token j of
+ * request r = requests[t] (null: r = t) is place j % page of page tables[r][j / page].
+ * positions -1: no token, out = 0.  requests -1: a row behind the batch's last one, left as it
+ * was.  Several rows may be of one request (a prompt's tokens; drafted ones).
+ * q, out [rows, heads, dim] f32, rows q_stride (out_stride) floats apart; tables [table_rows, width] i32.
+ * scale 0: 1 / sqrt(dim).  heads a multiple of kv_heads.  Scores, weights and sums are f32 (16-bit and
+ * 8-bit values taken as they are); what lies behind positions[t] or before the window is not
+ * looked at.  At most 65535 rows.  At rlq_sync: RLQ_TENSOR_BOUNDS (a = the row: a request or
+ * position outside the table, or a page outside the cache; its out is left as it was),
+ * RLQ_NON_FINITE (a = RLQ_CHECK_ATTENTION_OUTPUT, b = the row; a query head with such a
+ * value is left as it was).  Capturing: make the same call once before. */
+int32_t rlq_kv_attention(rlq_context *ctx, const rlq_kv_cache *cache, const float *q, uint64_t q_stride, uint64_t rows,
+                         uint64_t heads, const int32_t *tables, uint64_t table_rows, uint64_t width,
+                         const int32_t *positions, const int32_t *requests, float scale, uint64_t window, float *out,
+                         uint64_t out_stride, void *stream, rlq_error *err);
+
+/* Beam search's choice: logits [groups, beams, vocabulary] f32, rows `stride` floats apart, and the
+ * beams' scores [groups, beams] (-infinity: a beam without a place, its logits are not looked
+ * at).  Candidates are ranked by score + logit - log(sum of exp(logits of the beam)), in f64 (the
+ * exponentials f32); out_scores, parents (beam) and tokens [groups, best] are the best in
+ * order, the lowest (beam, token) of equal ones, scores rounded once.  Logits of -infinity are
+ * never chosen; places with no candidate left get -infinity, -1 and -1.  beams and best at most 64.
+ * RLQ_NON_FINITE at rlq_sync (a = RLQ_CHECK_MATRIX_OUTPUT, b = the group): a score or a logit of a
+ * live beam is NaN or +infinity; the group's places are as without candidates.  At
+ * most 65535 groups.  Capturing: make the same call once before. */
+int32_t rlq_beam_select(rlq_context *ctx, const float *logits, uint64_t stride, const float *scores, uint64_t groups,
+                        uint64_t beams, uint64_t vocabulary, uint64_t best, float *out_scores, int32_t *parents,
+                        int32_t *tokens, void *stream, rlq_error *err);
+
+/* The states after that choice: beam b of a group goes on from beam parents[b] (-1: from
+ * itself) of lengths[b] tokens, which is one number within a group.  Columns of whole pages of
+ * tables [groups * beams, width] become the parent's (the pages are then shared); the page that
+ * is partly filled is the beam's own, and the tokens in it are copied from the parent's into it, in
+ * every one of the n_layers caches (a host array; of one shape and strides).  Beams may change places.
+ * Pages that a table no longer names are still owned (rlq_kv_pages: `owned`).
+ * At most 32 beams.  At rlq_sync, with the group left as it was: RLQ_TENSOR_BOUNDS (a =
+ * group * beams + beam: a parent outside the group, a length that is negative, past the
+ * table or not the group's, or a part-filled page outside the cache). */
+int32_t rlq_beam_reorder(rlq_context *ctx, const int32_t *parents, const int32_t *lengths, uint64_t groups,
+                         uint64_t beams, int32_t *tables, uint64_t width, const rlq_kv_cache *caches,
+                         uint64_t n_layers, void *stream, rlq_error *err);
 
 /* ---- dense Llama decode step ------------------------------------------------
  * LlamaModel of crates/model-runtime/src/llama.rs with quantized matrices,

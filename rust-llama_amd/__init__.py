@@ -163,6 +163,11 @@ SIGNATURES = {
     "rlq_rms_norm": ([_P, _P, _P, _P, _U64, _U64, _F32, _P, _P, _U32, _P, _P, _E], _I32),
     "rlq_moe_route": ([_P, _P, _P, _U64, _U64, _U64, _U64, _U32, _F32, _P, _P, _P, _P, _P, _E], _I32),
     "rlq_moe_ffn": ([_P, _P, _P, _P, _U32, _P, _U64, _P, _P, _U64, _P, _P, _P, _E], _I32),
+    "rlq_kv_pages": ([_P, _P, _P, _U64, _U64, _P, _P, _U64, _P, _P, _U64, _U64, _P, _P, _P, _P, _P, _P, _P, _E], _I32),
+    "rlq_kv_store": ([_P, _P, _P, _U64, _U64, _P, _U64, _P, _U64, _U64, _P, _P, _P, _U64, _U32, _P, _U64, _P, _E], _I32),
+    "rlq_kv_attention": ([_P, _P, _P, _U64, _U64, _U64, _P, _U64, _U64, _P, _P, _F32, _U64, _P, _U64, _P, _E], _I32),
+    "rlq_beam_select": ([_P, _P, _U64, _P, _U64, _U64, _U64, _U64, _P, _P, _P, _P, _E], _I32),
+    "rlq_beam_reorder": ([_P, _P, _P, _U64, _U64, _P, _U64, _P, _U64, _P, _E], _I32),
     "rlq_sync": ([_P, _P, _E], _I32),
     "rlq_block_sums": ([_P, _P, _P, _U64, _P, _P, _P, _E], _I32),
     "rlq_block_sums_ex": ([_P, _P, _P, _U64, _U32, _P, _P, _P, _P, _E], _I32),
@@ -374,6 +379,7 @@ class Context:
         h, err = ctypes.c_void_p(), _Err()
         _check(_lib.rlq_context_create(int(device), ctypes.byref(h), ctypes.byref(err)), err)
         self._h = h
+        self._device = device if device >= 0 or torch is None else torch.cuda.current_device()
 
     def close(self):
         if getattr(self, "_h", None):
@@ -641,6 +647,184 @@ class Context:
                                 _stream_ptr(stream), ctypes.byref(err)), err)
         return y
 
+    # ---- paged KV cache
+
+    def _own(self, *tensors):
+        """Pointers of contiguous tensors on this context's device (None for None), each
+        given as (tensor, dtype)."""
+        out = []
+        for t, dtype in tensors:
+            if t is None:
+                out.append(None)
+                continue
+            out.append(_dev_ptr(t, dtype))
+            if t.device.index != self._device:
+                raise ValueError("a tensor is on another device than the context")
+        return out
+
+    def _rows(self, t, tail):
+        """(pointer, floats from row to row) of an f32 tensor [rows, *tail] whose rows are
+        contiguous but may lie apart, such as a part of a product's rows."""
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32:
+            raise TypeError("expected a torch.float32 tensor on the GPU")
+        if t.device.index != self._device:
+            raise ValueError("a tensor is on another device than the context")
+        if t.shape[1:] != tail:
+            raise ValueError(f"expected rows of {tuple(tail)}")
+        step, size = t.stride(), 1
+        for d in range(t.ndim - 1, 0, -1):
+            if step[d] != size and t.shape[d] != 1:
+                raise TypeError("expected contiguous rows")
+            size *= t.shape[d]
+        if t.shape[0] > 1 and step[0] < size:
+            raise TypeError("expected rows that do not overlap")
+        return t.data_ptr(), max(step[0], size)
+
+    def _stream(self, stream):
+        """The given stream, or torch's current one of this context's device, as a handle."""
+        if stream is None:
+            return _raw_stream(self._device) if _raw_stream else torch.cuda.current_stream(self._device).cuda_stream
+        return stream if isinstance(stream, int) else stream.cuda_stream
+
+    def kv_pages(self, lengths, new, tables, free, count, page, tokens, owned=None, out=None, stream=None):
+        """Pages, block tables and a batch's rows from the requests' lengths
+        (rlq_kv_pages): request r holds lengths[r] tokens and gets new[r] (0: it waits;
+        negative: it has ended, its pages go back).  tables int32 [requests, width] and
+        free int32 [pages], of which count int32 [1] are on the list, are updated in place;
+        so is `owned` [requests, width], the pages that are each request's own, where beams
+        share pages (else the tables are).  -> (lengths int32 [requests], count int32 [1],
+        starts int32 [requests + 1], slots int64, positions int32, requests int32 [tokens]), -1
+        in rows behind the last; out: those six tensors, given (lengths and count may be the inputs)."""
+        if stream is not None and _makes(lengths, out is None):
+            with _on(stream, lengths):
+                return self.kv_pages(lengths, new, tables, free, count, page, tokens, owned, out)
+        i32 = torch.int32
+        n, tokens = lengths.numel(), int(tokens)
+        if out is None:
+            out = (torch.empty_like(lengths), torch.empty_like(count), lengths.new_empty(n + 1),
+                   lengths.new_empty(tokens, dtype=torch.int64), lengths.new_empty(tokens), lengths.new_empty(tokens))
+        after, left, starts, slots, positions, requests = out
+        if tables.ndim != 2 or tables.shape[0] != n or new.numel() != n or count.numel() != 1 \
+                or (owned is not None and owned.shape != tables.shape):
+            raise ValueError("lengths, new, tables and owned must hold one row for each request, count one number")
+        if after.numel() != n or left.numel() != 1 or starts.numel() != n + 1 \
+                or any(t.numel() != tokens for t in (slots, positions, requests)):
+            raise ValueError("an output of another size")
+        p = self._own((lengths, i32), (new, i32), (tables, i32), (owned, i32), (free, i32), (count, i32), (after, i32),
+                      (left, i32), (starts, i32), (slots, torch.int64), (positions, i32), (requests, i32))
+        err = _Err()
+        _check(_lib.rlq_kv_pages(self._h, p[0], p[1], n, int(page), p[2], p[3], tables.shape[1], p[4], p[5], free.numel(),
+                                 tokens, *p[6:], self._stream(stream), ctypes.byref(err)), err)
+        return out
+
+    ROPE_PAIRS = 1
+
+    def kv_store(self, cache, k, v, slots, q=None, positions=None, freqs=None, pairs=True, out=None, stream=None):
+        """Keys and values f32 [tokens, kv_heads, dim] into their slots int64 [tokens] of a
+        KvCache (rlq_kv_store; -1: a row behind the last, left alone), and the queries
+        q [tokens, heads, dim] beside them.  freqs [n] f32 rotates the first 2 n values of
+        each head of q and k by positions[t] * freqs[i], neighbours as pairs or (not pairs)
+        values n apart; without it nothing is rotated.  -> the rotated q (None without q), in
+        `out` if given, which may be q.  Tokens of q, k, v and out may lie apart."""
+        if stream is not None and isinstance(k, torch.Tensor) and q is not None and out is None:
+            with _on(stream, k):
+                return self.kv_store(cache, k, v, slots, q, positions, freqs, pairs)
+        tokens, half = k.shape[0], 0 if freqs is None else freqs.numel()
+        if slots.numel() != tokens or (half and (positions is None or positions.numel() != tokens)):
+            raise ValueError("slots and positions must hold a number for each token")
+        tail = (cache.kv_heads, cache.dim)
+        (kp, ks), (vp, vs) = self._rows(k, tail), self._rows(v, tail)
+        heads, qp, qs, op, os_ = 0, None, 0, None, 0
+        if q is not None:
+            heads = q.shape[1]
+            if out is None:
+                out = q.new_empty(q.shape)
+            (qp, qs), (op, os_) = self._rows(q, (heads, cache.dim)), self._rows(out, (heads, cache.dim))
+            if q.shape[0] != tokens or out.shape[0] != tokens:
+                raise ValueError("q and out must hold the tokens of k")
+        elif out is not None:
+            raise ValueError("out needs q")
+        if v.shape[0] != tokens:
+            raise ValueError("v must hold the tokens of k")
+        sp, pp, fp = self._own((slots, torch.int64), (positions if half else None, torch.int32),
+                               (freqs if half else None, torch.float32))
+        cache._on_device(self)
+        err = _Err()
+        _check(_lib.rlq_kv_store(self._h, cache._ref, qp, qs, heads, kp, ks, vp, vs, tokens, sp, pp, fp, half,
+                                 self.ROPE_PAIRS if pairs else 0, op, os_, self._stream(stream), ctypes.byref(err)), err)
+        return out
+
+    def kv_attention(self, cache, q, tables, positions, requests=None, scale=None, window=0, out=None, stream=None):
+        """softmax(scale q K^T) V over a KvCache's pages for q [rows, heads, dim] f32
+        (rlq_kv_attention): row t sees the tokens up to positions[t] (int32; -1: none, the
+        result is 0) of request requests[t] (int32, none given: row t is request t; -1: a row
+        behind the last, left as it was), whose pages are tables[request] (int32 [requests, width]);
+        the last `window` of them if that is not 0.  scale: 1 / sqrt(dim) if none.  -> out
+        [rows, heads, dim].  Rows of q and out may lie apart."""
+        if stream is not None and isinstance(q, torch.Tensor) and out is None:
+            with _on(stream, q):
+                return self.kv_attention(cache, q, tables, positions, requests, scale, window)
+        if q.ndim != 3 or tables.ndim != 2:
+            raise ValueError("q must be [rows, heads, dim] and tables [requests, width]")
+        rows, heads = q.shape[:2]
+        if positions.numel() != rows or (requests is not None and requests.numel() != rows):
+            raise ValueError("positions and requests must hold a number for each row")
+        if out is None:
+            out = q.new_empty(q.shape)
+        tail = (heads, cache.dim)
+        (qp, qs), (op, os_) = self._rows(q, tail), self._rows(out, tail)
+        if out.shape[0] != rows:
+            raise ValueError("out must hold the rows of q")
+        tp, pp, rp = self._own((tables, torch.int32), (positions, torch.int32), (requests, torch.int32))
+        cache._on_device(self)
+        err = _Err()
+        _check(_lib.rlq_kv_attention(self._h, cache._ref, qp, qs, rows, heads, tp, tables.shape[0], tables.shape[1], pp, rp,
+                                     0.0 if scale is None else float(scale), int(window), op, os_, self._stream(stream),
+                                     ctypes.byref(err)), err)
+        return out
+
+    def beam_select(self, logits, scores, best, out=None, stream=None):
+        """The `best` continuations of each group of beams (rlq_beam_select): logits
+        [groups, beams, vocabulary] f32 (rows may lie apart) and scores [groups, beams]
+        (-inf: a beam without a place) -> (scores f32, parents int32, tokens int32
+        [groups, best]), in order of score + log-softmax; -inf, -1, -1 where no candidate is left."""
+        if stream is not None and isinstance(logits, torch.Tensor) and out is None:
+            with _on(stream, logits):
+                return self.beam_select(logits, scores, best)
+        if logits.ndim != 3 or scores.shape != logits.shape[:2]:
+            raise ValueError("logits must be [groups, beams, vocabulary] and scores [groups, beams]")
+        (groups, beams, vocabulary), best = logits.shape, int(best)
+        if beams > 1 and groups > 1 and logits.stride(0) != beams * logits.stride(1):
+            raise TypeError("expected beams one distance apart throughout")
+        flat = logits[:, 0] if beams == 1 else logits[0] if groups == 1 else logits.flatten(0, 1)
+        lp, ls = self._rows(flat, (vocabulary,))
+        if out is None:
+            out = (logits.new_empty((groups, best)), scores.new_empty((groups, best), dtype=torch.int32),
+                   scores.new_empty((groups, best), dtype=torch.int32))
+        if any(t.numel() != groups * best for t in out):
+            raise ValueError("an output of another size")
+        sp, op, pp, tp = self._own((scores, torch.float32), (out[0], torch.float32), (out[1], torch.int32), (out[2], torch.int32))
+        err = _Err()
+        _check(_lib.rlq_beam_select(self._h, lp, ls, sp, groups, beams, vocabulary, best, op, pp, tp, self._stream(stream),
+                                    ctypes.byref(err)), err)
+        return out
+
+    def beam_reorder(self, parents, lengths, tables, caches, stream=None):
+        """The beams' states after a choice (rlq_beam_reorder): parents int32 [groups, beams]
+        (-1: itself), lengths int32 [groups, beams], one number within a group; tables int32
+        [groups * beams, width] and the part-filled pages in every KvCache of `caches` are updated
+        in place."""
+        if parents.ndim != 2 or lengths.numel() != parents.numel() or tables.ndim != 2 or tables.shape[0] != parents.numel():
+            raise ValueError("parents [groups, beams], lengths and tables must hold one row for each beam")
+        pp, lp, tp = self._own((parents, torch.int32), (lengths, torch.int32), (tables, torch.int32))
+        layers = (_KvCacheT * len(caches))()
+        for i, c in enumerate(caches):
+            c._on_device(self)
+            layers[i] = c._t
+        err = _Err()
+        _check(_lib.rlq_beam_reorder(self._h, pp, lp, parents.shape[0], parents.shape[1], tp, tables.shape[1], layers,
+                                     len(caches), self._stream(stream), ctypes.byref(err)), err)
+
     def sync(self, stream=None):
         """Wait for the stream; raise the first data error recorded on the GPU."""
         err = _Err()
@@ -685,6 +869,52 @@ class Context:
                                       _dev_ptr(isum, torch.int32), _dev_ptr(imin, torch.int32),
                                       _dev_ptr(y, torch.float32), _stream_ptr(stream), ctypes.byref(err)), err)
         return isum, imin, y
+
+
+class _KvCacheT(ctypes.Structure):
+    _fields_ = [("k", _P), ("v", _P), ("dtype", _U32), ("kv_heads", _U32), ("page", _U32), ("dim", _U32), ("pages", _U64),
+                ("k_stride", _U64), ("v_stride", _U64)]
+
+
+class KvCache:
+    """One layer of a paged KV cache (rlq_kv_cache) in tensors k and v on the GPU: of
+    dtype F32, F16 or BF16 [pages, kv_heads, page, dim], or of Q8_0 uint8
+    [pages, kv_heads, page * (dim + dim / 16)]: a head's levels in a page, token after token,
+    then their f16 scales.  Pages may lie apart (a part of a larger tensor)."""
+
+    TYPES = {} if torch is None else {DType.F32: torch.float32, DType.F16: torch.float16, DType.BF16: torch.bfloat16,
+                                      DType.Q8_0: torch.uint8}
+
+    def __init__(self, k, v, dtype, page, dim):
+        dtype, page, dim = DType(dtype), int(page), int(dim)
+        tail = (page * (dim + dim // 16),) if dtype == DType.Q8_0 else (page, dim)
+        for t in (k, v):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != self.TYPES.get(dtype, t.dtype):
+                raise TypeError("expected tensors of the cache's type on the GPU")
+            if t.shape[2:] != tail or t.shape != k.shape or t.device != k.device:
+                raise ValueError(f"expected two tensors [pages, kv_heads, {', '.join(map(str, tail))}]")
+            if t[:1].numel() and not t[0].is_contiguous():
+                raise TypeError("expected contiguous pages")
+        self.k, self.v, self.dtype, self.page, self.dim = k, v, dtype, page, dim
+        self.pages, self.kv_heads = k.shape[:2]
+        size, least = k.element_size(), k[:1].numel()
+        strides = [t.stride(0) * size if self.pages > 1 else least * size for t in (k, v)]
+        self._t = _KvCacheT(k.data_ptr(), v.data_ptr(), int(dtype), self.kv_heads, page, dim, self.pages, *strides)
+        self._ref = ctypes.byref(self._t)
+
+    @classmethod
+    def make(cls, dtype, pages, kv_heads, page, dim, device="cuda"):
+        """An empty layer."""
+        dtype = DType(dtype)
+        tail = (page * (dim + dim // 16),) if dtype == DType.Q8_0 else (page, dim)
+        if dtype not in cls.TYPES:
+            raise QuantError(19, int(dtype), 0, 0, "a cache of this type")
+        k, v = (torch.zeros((pages, kv_heads, *tail), dtype=cls.TYPES[dtype], device=device) for _ in range(2))
+        return cls(k, v, dtype, page, dim)
+
+    def _on_device(self, ctx):
+        if self.k.device.index != ctx._device:
+            raise ValueError("the cache is on another device than the context")
 
 
 class Weights:

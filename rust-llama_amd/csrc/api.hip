@@ -9,6 +9,7 @@
 #include <math.h>
 #include <string.h>
 
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <stdexcept>
@@ -108,7 +109,8 @@ struct rlq_context {
     // every launch); column_keys: one per column, of an argmax after a GEMM that
     // uses them (argmax_one_group)
     // arrivals: counters of moe_route and moe_ffn, 0 between launches
-    DevBuf planes, keys, column_keys, stage_in, stage_w, stage_out, gate, logits, arrivals, moe;
+    // kv: parts of rlq_kv_attention and candidates of rlq_beam_select
+    DevBuf planes, keys, column_keys, stage_in, stage_w, stage_out, gate, logits, arrivals, moe, kv;
     Retired* retired = nullptr;
 };
 
@@ -224,6 +226,7 @@ int32_t key_to_error(unsigned long long key, uint32_t dtype, rlq_error* err) {
     const uint64_t field = key >> 41, kind = (key >> 40) & 1, index = key & ((1ull << 40) - 1);
     if (field == kModelField) {  // model-runtime checks: layer, stage, index
         const uint64_t layer = (key >> 25) & 0xffff, stage = (key >> 20) & 31, idx = key & 0xfffff;
+        if (stage == kStPages) return fail(err, RLQ_INVALID_STATE, dtype, layer, idx);
         const uint32_t check = stage_check((uint32_t)stage);
         if (check == 0) return fail(err, RLQ_UNREPRESENTABLE_SCALE, dtype, idx, layer);
         return fail(err, RLQ_NON_FINITE, dtype, check, layer);
@@ -413,7 +416,7 @@ void rlq_context_destroy(rlq_context* ctx) {
     DeviceGuard g(ctx->device);
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
     for (DevBuf* b : {&ctx->planes, &ctx->keys, &ctx->column_keys, &ctx->stage_in, &ctx->stage_w, &ctx->stage_out, &ctx->gate,
-                      &ctx->logits, &ctx->arrivals, &ctx->moe})
+                      &ctx->logits, &ctx->arrivals, &ctx->moe, &ctx->kv})
         if (b->p) (void)hipFree(b->p);
     while (Retired* r = ctx->retired) {
         ctx->retired = r->next;
@@ -1059,6 +1062,206 @@ int32_t rlq_moe_ffn(rlq_context* ctx, const rlq_weights* gate, const rlq_weights
     HIP_TRY(ensure_arrivals(ctx, moe_counters(c), s));
     c.count = (uint32_t*)ctx->arrivals.p;
     HIP_TRY(launch_moe_ffn(c, ctx->moe.p, s));
+    return ok(err);
+}
+
+// ---- paged KV cache -----------------------------------------------------------------
+
+namespace {
+
+constexpr uint64_t kKvMostRows = 65535;  // the error keys' row field
+constexpr uint64_t kKvMostTokens = kModelField - 1;  // and their column field
+
+uint64_t kv_value_bytes(uint32_t t, uint64_t dim) { return t == kF32 ? 4 * dim : t == kQ8_0 ? dim : 2 * dim; }
+uint64_t kv_scale_bytes(uint32_t t, uint64_t dim) { return t == kQ8_0 ? dim / 16 : 0; }
+
+int32_t kv_page(uint64_t page, uint32_t* log_page, rlq_error* err) {
+    for (uint32_t l = 4; l <= 8; ++l)
+        if (page == 1ull << l) return *log_page = l, ok(err);
+    return fail(err, RLQ_UNIMPLEMENTED, 0, page, 256);
+}
+
+// A cache of the caller's; null pointers in it are an error.
+int32_t kv_layer(const rlq_kv_cache* c, KvLayer* out, rlq_error* err) {
+    if (!c) return fail(err, RLQ_INVALID_ARGUMENT);
+    if (!dtype_known(c->dtype)) return fail(err, RLQ_INVALID_TYPE, c->dtype);
+    if (c->dtype != kF32 && c->dtype != kF16 && c->dtype != kBF16 && c->dtype != kQ8_0)
+        return fail(err, RLQ_UNIMPLEMENTED, c->dtype);
+    uint32_t log_page;
+    const int32_t rc = kv_page(c->page, &log_page, err);
+    if (rc) return rc;
+    if (c->dim == 0 || c->dim % 32) return fail(err, RLQ_NON_MULTIPLE, c->dtype, c->dim, 32);
+    if (c->dim > 256) return fail(err, RLQ_UNIMPLEMENTED, c->dtype, c->dim, 256);
+    if (c->kv_heads == 0 || c->pages == 0) return fail(err, RLQ_INVALID_MATRIX_SHAPE, c->dtype, c->pages, c->kv_heads);
+    if (c->kv_heads > 65535) return fail(err, RLQ_UNIMPLEMENTED, c->dtype, c->kv_heads, 65535);
+    if (c->pages > 0x7fffffff) return fail(err, RLQ_UNIMPLEMENTED, c->dtype, c->pages, 0x7fffffff);
+    const uint64_t least = (kv_value_bytes(c->dtype, c->dim) + kv_scale_bytes(c->dtype, c->dim)) * c->page * c->kv_heads;
+    for (uint64_t stride : {c->k_stride, c->v_stride}) {
+        if (stride < least) return fail(err, RLQ_INVALID_LENGTH, c->dtype, least, stride);
+        if (stride % 16) return fail(err, RLQ_NON_MULTIPLE, c->dtype, stride, 16);
+        if (stride > (~0ull >> 1) / c->pages) return fail(err, RLQ_SIZE_OVERFLOW, c->dtype);
+    }
+    if (!c->k || !c->v || c->k == c->v || (((uintptr_t)c->k | (uintptr_t)c->v) & 15))
+        return fail(err, RLQ_INVALID_ARGUMENT, c->dtype);
+    *out = KvLayer{(uint8_t*)c->k, (uint8_t*)c->v, c->k_stride, c->v_stride, c->pages, c->dtype, c->kv_heads, log_page, c->dim};
+    return ok(err);
+}
+
+bool aligned(std::initializer_list<const void*> ps, uintptr_t n) {
+    uintptr_t low = 0;
+    for (const void* p : ps) low |= (uintptr_t)p;
+    return (low & (n - 1)) == 0;
+}
+
+}  // namespace
+
+int32_t rlq_kv_pages(rlq_context* ctx, const int32_t* before, const int32_t* more, uint64_t requests, uint64_t page,
+                     int32_t* tables, int32_t* owned, uint64_t width, int32_t* free, const int32_t* count,
+                     uint64_t pages, uint64_t tokens, int32_t* after, int32_t* count_after, int32_t* starts,
+                     int64_t* slots, int32_t* positions, int32_t* out_requests, void* stream, rlq_error* err) {
+    if (!ctx) return fail(err, RLQ_INVALID_ARGUMENT);
+    uint32_t log_page;
+    const int32_t rc = kv_page(page, &log_page, err);
+    if (rc) return rc;
+    if (requests == 0) return fail(err, RLQ_INVALID_MATRIX_SHAPE, 0, requests, width);
+    if (requests > kKvMaxRequests) return fail(err, RLQ_UNIMPLEMENTED, 0, requests, kKvMaxRequests);
+    for (uint64_t n : {width, pages, tokens})
+        if (n > 0x7fffffff) return fail(err, RLQ_UNIMPLEMENTED, 0, n, 0x7fffffff);
+    if (!before || !more || !count || !after || !count_after || !starts || (width && !tables) || (pages && !free) ||
+        (tokens && (!slots || !positions || !out_requests)))
+        return fail(err, RLQ_INVALID_ARGUMENT);
+    if (!aligned({before, more, tables, owned, free, count, after, count_after, starts, positions, out_requests}, 4) ||
+        !aligned({slots}, 8))
+        return fail(err, RLQ_INVALID_ARGUMENT);
+    DeviceGuard g(ctx->device);
+    const hipStream_t s = pick(ctx, stream);
+    HIP_TRY(ensure(ctx, ctx->gate, sizeof(uint32_t), s));
+    const PagesArgs a{before, more, (uint32_t)requests, (uint32_t)width, (uint32_t)pages, log_page, (uint32_t)tokens, tables,
+                      owned ? owned : tables, free, count, after, count_after, starts, slots, positions, out_requests,
+                      (uint32_t*)ctx->gate.p, ctx->err_words};
+    HIP_TRY(launch_kv_pages(a, s));
+    return ok(err);
+}
+
+int32_t rlq_kv_store(rlq_context* ctx, const rlq_kv_cache* cache, const float* q, uint64_t q_stride, uint64_t heads,
+                     const float* k, uint64_t k_stride, const float* v, uint64_t v_stride, uint64_t tokens,
+                     const int64_t* slots, const int32_t* positions, const float* freqs, uint64_t half, uint32_t flags,
+                     float* q_out, uint64_t out_stride, void* stream, rlq_error* err) {
+    if (!ctx) return fail(err, RLQ_INVALID_ARGUMENT);
+    if (flags & ~RLQ_ROPE_PAIRS) return fail(err, RLQ_INVALID_ARGUMENT, 0, flags);
+    KvLayer c;
+    const int32_t rc = kv_layer(cache, &c, err);
+    if (rc) return rc;
+    if (half > c.dim / 2) return fail(err, RLQ_TENSOR_SHAPE, c.type, half, c.dim / 2);
+    if (heads > 65535) return fail(err, RLQ_UNIMPLEMENTED, c.type, heads, 65535);
+    const uint64_t qd = heads * c.dim, kd = (uint64_t)c.kv_heads * c.dim;
+    if (tokens > 1) {
+        if (k_stride < kd) return fail(err, RLQ_INVALID_LENGTH, c.type, kd, k_stride);
+        if (v_stride < kd) return fail(err, RLQ_INVALID_LENGTH, c.type, kd, v_stride);
+        if (heads && q_stride < qd) return fail(err, RLQ_INVALID_LENGTH, c.type, qd, q_stride);
+        if (heads && out_stride < qd) return fail(err, RLQ_INVALID_LENGTH, c.type, qd, out_stride);
+    }
+    if (tokens > kKvMostTokens) return fail(err, RLQ_UNIMPLEMENTED, c.type, tokens, kKvMostTokens);
+    if (tokens == 0) return ok(err);
+    if (!k || !v || !slots || (heads && (!q || !q_out)) || (half && (!positions || !freqs)) ||
+        (q == q_out && q_stride != out_stride && tokens > 1 && heads))
+        return fail(err, RLQ_INVALID_ARGUMENT, c.type);
+    if (!aligned({q, k, v, positions, freqs, q_out}, 4) || !aligned({slots}, 8)) return fail(err, RLQ_INVALID_ARGUMENT, c.type);
+    DeviceGuard g(ctx->device);
+    const StoreArgs a{c, q, k, v, q_stride, k_stride, v_stride, out_stride, tokens, (uint32_t)heads, slots, positions, freqs,
+                      (uint32_t)half, flags & RLQ_ROPE_PAIRS, q_out, ctx->err_words};
+    HIP_TRY(launch_kv_store(a, pick(ctx, stream)));
+    return ok(err);
+}
+
+int32_t rlq_kv_attention(rlq_context* ctx, const rlq_kv_cache* cache, const float* q, uint64_t q_stride, uint64_t rows,
+                         uint64_t heads, const int32_t* tables, uint64_t table_rows, uint64_t width,
+                         const int32_t* positions, const int32_t* requests, float scale, uint64_t window, float* out,
+                         uint64_t out_stride, void* stream, rlq_error* err) {
+    if (!ctx) return fail(err, RLQ_INVALID_ARGUMENT);
+    KvLayer c;
+    const int32_t rc = kv_layer(cache, &c, err);
+    if (rc) return rc;
+    if (heads == 0 || heads % c.kv_heads) return fail(err, RLQ_TENSOR_SHAPE, c.type, heads, c.kv_heads);
+    if (!(scale >= -3.402823466e38f) || !(scale <= 3.402823466e38f)) return fail(err, RLQ_INVALID_CONFIG, c.type, 6);
+    if (heads > 65535) return fail(err, RLQ_UNIMPLEMENTED, c.type, heads, 65535);
+    if (rows > kKvMostRows) return fail(err, RLQ_UNIMPLEMENTED, c.type, rows, kKvMostRows);
+    for (uint64_t n : {table_rows, width, window})
+        if (n > 0x7fffffff) return fail(err, RLQ_UNIMPLEMENTED, c.type, n, 0x7fffffff);
+    const uint64_t qd = heads * c.dim;
+    if (rows > 1 && q_stride < qd) return fail(err, RLQ_INVALID_LENGTH, c.type, qd, q_stride);
+    if (rows > 1 && out_stride < qd) return fail(err, RLQ_INVALID_LENGTH, c.type, qd, out_stride);
+    if (!requests && table_rows < rows) return fail(err, RLQ_TENSOR_SHAPE, c.type, table_rows, rows);
+    if (rows == 0) return ok(err);
+    if (!q || !out || !positions || (table_rows && width && !tables)) return fail(err, RLQ_INVALID_ARGUMENT, c.type);
+    if (!aligned({q, tables, positions, requests, out}, 4)) return fail(err, RLQ_INVALID_ARGUMENT, c.type);
+    DeviceGuard g(ctx->device);
+    const AttnArgs a{c, q, q_stride, out_stride, (uint32_t)rows, (uint32_t)heads, (uint32_t)table_rows, (uint32_t)width,
+                     (uint32_t)window, tables, positions, requests, scale == 0.0f ? 1.0f / sqrtf((float)c.dim) : scale, out,
+                     ctx->err_words};
+    HIP_TRY(launch_kv_attention(a, pick(ctx, stream)));
+    return ok(err);
+}
+
+int32_t rlq_beam_select(rlq_context* ctx, const float* logits, uint64_t stride, const float* scores, uint64_t groups,
+                        uint64_t beams, uint64_t vocabulary, uint64_t best, float* out_scores, int32_t* parents,
+                        int32_t* tokens, void* stream, rlq_error* err) {
+    if (!ctx) return fail(err, RLQ_INVALID_ARGUMENT);
+    if (beams == 0 || vocabulary == 0) return fail(err, RLQ_INVALID_MATRIX_SHAPE, 0, beams, vocabulary);
+    if (beams > kSelectMaxBeams) return fail(err, RLQ_UNIMPLEMENTED, 0, beams, kSelectMaxBeams);
+    if (vocabulary > 0x7fffffff) return fail(err, RLQ_UNIMPLEMENTED, 0, vocabulary, 0x7fffffff);
+    if (best == 0 || best > beams * vocabulary) return fail(err, RLQ_TENSOR_SHAPE, 0, best, beams * vocabulary);
+    if (best > kSelectMaxBest) return fail(err, RLQ_UNIMPLEMENTED, 0, best, kSelectMaxBest);
+    if (groups > kKvMostRows) return fail(err, RLQ_UNIMPLEMENTED, 0, groups, kKvMostRows);
+    if (groups * beams > 1 && stride < vocabulary) return fail(err, RLQ_INVALID_LENGTH, 0, vocabulary, stride);
+    if (groups == 0) return ok(err);
+    if (!logits || !scores || !out_scores || !parents || !tokens || parents == tokens) return fail(err, RLQ_INVALID_ARGUMENT);
+    if (!aligned({logits, scores, out_scores, parents, tokens}, 4)) return fail(err, RLQ_INVALID_ARGUMENT);
+    DeviceGuard g(ctx->device);
+    const hipStream_t s = pick(ctx, stream);
+    HIP_TRY(ensure(ctx, ctx->kv, beam_select_bytes(groups * beams, best), s));
+    const SelectArgs a{logits, stride, scores, (uint32_t)groups, (uint32_t)beams, (uint32_t)vocabulary, (uint32_t)best,
+                       out_scores, parents, tokens, ctx->err_words, nullptr, nullptr};
+    HIP_TRY(launch_beam_select(a, ctx->kv.p, s));
+    return ok(err);
+}
+
+int32_t rlq_beam_reorder(rlq_context* ctx, const int32_t* parents, const int32_t* lengths, uint64_t groups,
+                         uint64_t beams, int32_t* tables, uint64_t width, const rlq_kv_cache* caches,
+                         uint64_t n_layers, void* stream, rlq_error* err) {
+    if (!ctx || !caches || n_layers == 0) return fail(err, RLQ_INVALID_ARGUMENT);
+    KvLayer c;
+    for (uint64_t i = 0; i < n_layers; ++i) {
+        KvLayer l;
+        const int32_t rc = kv_layer(caches + i, &l, err);
+        if (rc) return rc;
+        if (i == 0) c = l;
+        if (l.type != c.type) return fail(err, RLQ_TENSOR_UNSUPPORTED, l.type);
+        if (l.kv_heads != c.kv_heads || l.log_page != c.log_page || l.dim != c.dim || l.pages != c.pages ||
+            l.k_stride != c.k_stride || l.v_stride != c.v_stride)
+            return fail(err, RLQ_TENSOR_SHAPE, l.type, i, n_layers);
+    }
+    if (beams == 0) return fail(err, RLQ_INVALID_MATRIX_SHAPE, c.type, groups, beams);
+    if (beams > kReorderMaxBeams) return fail(err, RLQ_UNIMPLEMENTED, c.type, beams, kReorderMaxBeams);
+    if (groups > kKvMostRows) return fail(err, RLQ_UNIMPLEMENTED, c.type, groups, kKvMostRows);
+    if (width > 0x7fffffff) return fail(err, RLQ_UNIMPLEMENTED, c.type, width, 0x7fffffff);
+    if (groups == 0) return ok(err);
+    if (!parents || !lengths || (width && !tables)) return fail(err, RLQ_INVALID_ARGUMENT, c.type);
+    if (!aligned({parents, lengths, tables}, 4)) return fail(err, RLQ_INVALID_ARGUMENT, c.type);
+    DeviceGuard g(ctx->device);
+    ReorderArgs a{parents, lengths, tables, (uint32_t)groups, (uint32_t)beams, (uint32_t)width, c.log_page, c.kv_heads,
+                  (uint32_t)kv_value_bytes(c.type, c.dim), (uint32_t)kv_scale_bytes(c.type, c.dim), c.pages, c.k_stride,
+                  c.v_stride, 0, 0, ctx->err_words, {}};
+    for (uint64_t i = 0; i < n_layers; i += kReorderLayers) {
+        const uint64_t n = n_layers - i < kReorderLayers ? n_layers - i : kReorderLayers;
+        for (uint64_t k = 0; k < n; ++k) {
+            a.tensors[2 * k] = (uint8_t*)caches[i + k].k;
+            a.tensors[2 * k + 1] = (uint8_t*)caches[i + k].v;
+        }
+        a.n_tensors = (uint32_t)(2 * n);
+        a.last = i + n == n_layers;
+        HIP_TRY(launch_beam_reorder(a, pick(ctx, stream)));
+    }
     return ok(err);
 }
 

@@ -45,15 +45,6 @@ __device__ __forceinline__ void norm_store(float* p, uint32_t e, uint32_t n, con
 
 constexpr int kRowShl4 = 0x104;  // lane i <- i + 4 within each 16 lanes
 
-// Four levels of a lane, the block's scale, and whether the scale is no finite
-// number (activation.rs:20-28, encode.rs:80-90).
-struct NormQ {
-    uint32_t q;
-    float d;
-    int32_t bsum;  // Q8_K, in the first lane of each four: the sum of its 16 levels
-    bool bad;
-};
-
 // U Q8_K blocks by a wave, four values of each a lane (the arithmetic of
 // rlq_q8k.hpp's q8k_row16; see there for the rounding), of which the first `count`
 // exist.  The first value of largest magnitude is that of the first lane that holds
@@ -90,24 +81,6 @@ __device__ __forceinline__ void norm_q8k(const float (&v)[U][4], uint32_t count,
         o[k].bsum = s + dpp_i<kQuadXor2>(s);
         o[k].bad = (bad >> k) & 1;
     }
-}
-
-// One Q8_0 block by eight lanes, four values each (q8_0_pair16 in another layout).
-__device__ __forceinline__ NormQ norm_q8_0(const float (&v)[4]) {
-    float am = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-    am = fmaxf(am, dpp_f<kQuadXor1>(am));
-    am = fmaxf(am, dpp_f<kQuadXor2>(am));
-    am = fmaxf(am, dpp_f<kRowHalfMirror>(am));
-    NormQ o{0, am / 127.0f, 0, false};
-    o.bad = !finite(o.d) || (o.d != 0.0f && !finite(1.0f / o.d)) || (float_to_half_bits(o.d) & 0x7c00u) == 0x7c00u;
-    const float inv = o.d != 0.0f ? 1.0f / o.d : 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        float r = __builtin_roundf(v[k] * inv);  // half away from zero, saturating
-        r = r > 127.0f ? 127.0f : (r < -128.0f ? -128.0f : r);
-        o.q |= ((uint32_t)(int32_t)r & 0xffu) << (8 * k);
-    }
-    return o;
 }
 
 // L lanes per row (four rows share a workgroup of 256 at 64), U times four values per

@@ -294,6 +294,7 @@ enum ModelStage : uint32_t {
     kStDownQuant = 15,
     kStDownOut = 16,
     kStLayerOut = 17,       // llama.rs:378 "Llama layer output"
+    kStPages = 18,          // no check of the step: a request without pages (layer: the request)
 };
 __device__ __forceinline__ uint64_t model_key(uint32_t layer, uint32_t stage, uint64_t index) {
     return (kModelField << 41) | ((uint64_t)(layer & 0xffffu) << 25) | ((uint64_t)(stage & 31u) << 20) |

@@ -12,7 +12,9 @@
 
 namespace rlq {
 
-enum DTypeId : uint32_t { kQ8_0 = 8, kQ2_K = 10, kQ3_K = 11, kQ4_K = 12, kQ5_K = 13, kQ6_K = 14, kQ8_K = 15 };
+enum DTypeId : uint32_t {
+    kF32 = 0, kF16 = 1, kQ8_0 = 8, kQ2_K = 10, kQ3_K = 11, kQ4_K = 12, kQ5_K = 13, kQ6_K = 14, kQ8_K = 15, kBF16 = 30
+};
 
 // Activations of `batch` columns in structure-of-arrays form on the device:
 //   q    int8  [batch][cols]
@@ -254,6 +256,80 @@ struct MoeArgs {  // of one pass
     unsigned long long* sums;  // of the parts of the down product's tiles
     uint32_t* count;           // 0 between launches: parts that have arrived, per tile of y
 };
+
+// ---- kv.hip ----
+// Pages for the requests' new tokens (rlq.h, rlq_kv_pages).
+constexpr uint32_t kKvMaxRequests = 4096;
+struct PagesArgs {
+    const int32_t *before, *more;
+    uint32_t requests, width, pages, log_page, tokens;
+    int32_t *tables, *owned, *free;  // owned may be tables
+    const int32_t* count;
+    int32_t *after, *count_after, *starts;
+    int64_t* slots;
+    int32_t *positions, *out_requests;
+    uint32_t* refused;  // scratch: whether the plan was refused
+    unsigned long long* err_word;
+};
+hipError_t launch_kv_pages(const PagesArgs& a, hipStream_t s);
+// One layer of a paged cache; strides in bytes from page to page.
+struct KvLayer {
+    uint8_t *k, *v;
+    uint64_t k_stride, v_stride, pages;
+    uint32_t type, kv_heads, log_page, dim;
+};
+struct StoreArgs {
+    KvLayer c;
+    const float *q, *k, *v;
+    uint64_t q_stride, k_stride, v_stride, out_stride, tokens;
+    uint32_t heads;  // of q; 0 without q
+    const int64_t* slots;
+    const int32_t* positions;
+    const float* freqs;
+    uint32_t half, pairs;
+    float* q_out;
+    unsigned long long* err_word;
+};
+hipError_t launch_kv_store(const StoreArgs& a, hipStream_t s);
+struct AttnArgs {
+    KvLayer c;
+    const float* q;
+    uint64_t q_stride, out_stride;
+    uint32_t rows, heads, table_rows, width, window;  // window 0: none
+    const int32_t *tables, *positions, *requests;     // requests may be null
+    float scale;
+    float* out;
+    unsigned long long* err_word;
+};
+hipError_t launch_kv_attention(const AttnArgs& a, hipStream_t s);
+// The beams' tables and part-filled pages after a choice; tensors: k, v, k, v, ...
+constexpr uint32_t kReorderMaxBeams = 32, kReorderLayers = 64;
+struct ReorderArgs {
+    const int32_t *parents, *lengths;
+    int32_t* tables;
+    uint32_t groups, beams, width, log_page, kv_heads, row_bytes, scale_bytes;
+    uint64_t pages, k_stride, v_stride;
+    uint32_t n_tensors, last;  // last: the launch that takes the tables over
+    unsigned long long* err_word;
+    uint8_t* tensors[2 * kReorderLayers];
+};
+hipError_t launch_beam_reorder(const ReorderArgs& a, hipStream_t s);
+
+// ---- beam.hip ----
+constexpr uint32_t kSelectMaxBeams = 64, kSelectMaxBest = 64;
+struct SelectArgs {
+    const float* logits;
+    uint64_t stride;
+    const float* scores;
+    uint32_t groups, beams, vocabulary, best;
+    float* out_scores;
+    int32_t *parents, *tokens;
+    unsigned long long* err_word;
+    double* rank;  // scratch
+    int32_t* token;
+};
+size_t beam_select_bytes(uint64_t rows, uint64_t best);
+hipError_t launch_beam_select(SelectArgs a, void* scratch, hipStream_t s);
 
 // ---- llama.hip ----
 // The dense Llama decode step (crates/model-runtime/src/llama.rs:222-392)

@@ -174,4 +174,31 @@ __device__ __forceinline__ uint4 q45_slots(const uint32_t (&q)[4], uint32_t odd)
                       __builtin_amdgcn_perm(hi1, lo1, 0x05040100u), __builtin_amdgcn_perm(hi1, lo1, 0x07060302u));
 }
 
+// Four levels of a lane, the block's scale, and whether the scale is no finite
+// number (activation.rs:20-28, encode.rs:80-90).
+struct NormQ {
+    uint32_t q;
+    float d;
+    int32_t bsum;  // Q8_K, in the first lane of each four: the sum of its 16 levels
+    bool bad;
+};
+
+// One Q8_0 block by eight lanes, four values each (q8_0_pair16 in another layout).
+__device__ __forceinline__ NormQ norm_q8_0(const float (&v)[4]) {
+    float am = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    am = fmaxf(am, dpp_f<kQuadXor1>(am));
+    am = fmaxf(am, dpp_f<kQuadXor2>(am));
+    am = fmaxf(am, dpp_f<kRowHalfMirror>(am));
+    NormQ o{0, am / 127.0f, 0, false};
+    o.bad = !finite(o.d) || (o.d != 0.0f && !finite(1.0f / o.d)) || (float_to_half_bits(o.d) & 0x7c00u) == 0x7c00u;
+    const float inv = o.d != 0.0f ? 1.0f / o.d : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float r = __builtin_roundf(v[k] * inv);  // half away from zero, saturating
+        r = r > 127.0f ? 127.0f : (r < -128.0f ? -128.0f : r);
+        o.q |= ((uint32_t)(int32_t)r & 0xffu) << (8 * k);
+    }
+    return o;
+}
+
 }  // namespace rlq
