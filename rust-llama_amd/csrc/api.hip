@@ -1196,10 +1196,15 @@ int32_t rlq_kv_attention(rlq_context* ctx, const rlq_kv_cache* cache, const floa
     if (!q || !out || !positions || (table_rows && width && !tables)) return fail(err, RLQ_INVALID_ARGUMENT, c.type);
     if (!aligned({q, tables, positions, requests, out}, 4)) return fail(err, RLQ_INVALID_ARGUMENT, c.type);
     DeviceGuard g(ctx->device);
-    const AttnArgs a{c, q, q_stride, out_stride, (uint32_t)rows, (uint32_t)heads, (uint32_t)table_rows, (uint32_t)width,
-                     (uint32_t)window, tables, positions, requests, scale == 0.0f ? 1.0f / sqrtf((float)c.dim) : scale, out,
-                     ctx->err_words};
-    HIP_TRY(launch_kv_attention(a, pick(ctx, stream)));
+    const hipStream_t s = pick(ctx, stream);
+    AttnArgs a{c, q, q_stride, out_stride, (uint32_t)rows, (uint32_t)heads, (uint32_t)table_rows, (uint32_t)width,
+               (uint32_t)window, tables, positions, requests, scale == 0.0f ? 1.0f / sqrtf((float)c.dim) : scale, out,
+               ctx->err_words, nullptr, nullptr, 0, 0};
+    HIP_TRY(ensure(ctx, ctx->kv, kv_attention_bytes(a), s));
+    HIP_TRY(ensure_arrivals(ctx, kv_attention_counters(a), s));
+    a.scratch = (float*)ctx->kv.p;
+    a.count = (uint32_t*)ctx->arrivals.p;
+    HIP_TRY(launch_kv_attention(a, s));
     return ok(err);
 }
 

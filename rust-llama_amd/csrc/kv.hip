@@ -339,115 +339,622 @@ hipError_t launch_kv_store(const StoreArgs& a, hipStream_t s) {
 // Attention
 // ---------------------------------------------------------------------------
 
-// Four values of a token from element e on.
-template <uint32_t T>
-__device__ __forceinline__ float4 kv_load4(const uint8_t* plane, uint32_t row, uint32_t e, uint32_t dim, uint32_t log_page) {
-    const uint8_t* p = plane + row * kv_row<T>(dim);
-    if constexpr (T == kF32) {
-        return *(const float4*)(p + 4 * e);
-    } else if constexpr (T == kQ8_0) {
-        const uint32_t q = *(const uint32_t*)(p + e);
-        const float d = half_to_float(*(const uint16_t*)(plane + ((uint64_t)dim << log_page) + 2 * (row * (dim / 32) + e / 32)));
-        return make_float4((float)(int8_t)q * d, (float)(int8_t)(q >> 8) * d, (float)(int8_t)(q >> 16) * d,
-                           (float)(int8_t)(q >> 24) * d);
-    } else {
-        const uint2 b = *(const uint2*)(p + 2 * e);
-        if constexpr (T == kF16)
-            return make_float4(half_to_float(b.x), half_to_float(b.x >> 16), half_to_float(b.y), half_to_float(b.y >> 16));
-        return make_float4(__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u), __uint_as_float(b.y << 16),
-                           __uint_as_float(b.y & 0xffff0000u));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// N words at an address that is a multiple of A bytes.
+template <class W, int N, int A>
+struct __attribute__((packed, aligned(A))) Words {
+    W w[N];
+};
+template <class W, int N, int A>
+__device__ __forceinline__ void words(const void* p, W (&out)[N]) {
+    const Words<W, N, A> t = *(const Words<W, N, A>*)p;
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = t.w[i];
+}
+constexpr int pow2_of(int n) { return n & -n; }
+
+__device__ __forceinline__ f32x4 mma_f16(const uint32_t (&a)[4], const uint32_t (&b)[4], f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma_bf16(const uint32_t (&a)[4], const uint32_t (&b)[4], f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// An f32 number as 16-bit terms whose sum it is to its last bits: two f16 (22 bits; the number is
+// brought near f16's upper end first, where nothing is lost below) or three bf16 (24 bits).
+// The terms of eight numbers, as operands.
+__device__ __forceinline__ void split_f16(const float (&x)[8], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const auto h = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
+        hi[i] = __builtin_bit_cast(uint32_t, h);
+        lo[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[2 * i] - (float)h[0], x[2 * i + 1] - (float)h[1]));
+    }
+}
+__device__ __forceinline__ void split_bf16(const float (&x)[8], uint32_t (&hi)[4], uint32_t (&mid)[4], uint32_t (&lo)[4]) {
+    uint32_t t[3][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        t[0][i] = __float_as_uint(x[i]);
+        const float r = x[i] - __uint_as_float(t[0][i] & 0xffff0000u);
+        t[1][i] = __float_as_uint(r);
+        t[2][i] = __float_as_uint(r - __uint_as_float(t[1][i] & 0xffff0000u));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // the upper halves of two
+        hi[i] = __builtin_amdgcn_perm(t[0][2 * i + 1], t[0][2 * i], 0x07060302u);
+        mid[i] = __builtin_amdgcn_perm(t[1][2 * i + 1], t[1][2 * i], 0x07060302u);
+        lo[i] = __builtin_amdgcn_perm(t[2][2 * i + 1], t[2][2 * i], 0x07060302u);
     }
 }
 
-// One query head of a row per workgroup: 256 tokens at a time, a thread a token for
-// the scores and a thread a value for the output, with a running maximum and sum.
-template <uint32_t T>
+// The maximum and the sum over the lanes 16 apart; every lane gets it.
+__device__ __forceinline__ float column_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float column_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+// A wave's part of the attention of up to 16 query heads (columns) over the tokens of one
+// KV head, 32 tokens at a time (two halves of 16).
+//
+//   S = K Q    v_mfma_f32_16x16x32 (f32: 16x16x4): rows are tokens, columns query heads.
+//              Lane (i, g) = (lane % 16, lane / 16) loads 16 bytes of token i.
+//   O = V^T P  rows are values, columns query heads.  Lane (i, g) gets from S the scores of
+//              tokens 4g .. 4g + 3 of each half for head i, which are its operand of P as they are;
+//              it loads dim / 16 values of these eight tokens, values i * dim / 16 and on, and pairs
+//              of tokens are put together in registers (one v_perm a pair).
+//
+// Neither goes through LDS.  The scores' operands and P are f32 numbers in 16-bit terms (split_*),
+// so the products are those of f32 with the stored values; the matrix cores have room for that:
+// 16-bit keys and values need 2 (f16) or 3 (bf16) times 256 cycles per 32 tokens of 128 values, of
+// about 1900 that HBM takes for them (one SIMD's share).  Q8_0: scores with f16 levels, block by block, times
+// the block's scale; values as f32 (level times scale, exact) on 16x16x4.
+template <uint32_t T, int NB>  // NB: blocks of 32 values
+struct AttnWave {
+    static constexpr int kDim = 32 * NB, kOwn = 2 * NB;  // values of a token that a lane holds for O
+    static constexpr bool k16 = T == kF16 || T == kBF16;
+    static constexpr float kTop = T == kF16 ? 14.0f : 0.0f;  // weights are 2^kTop times exp(s - max)
+
+    // q (columns past the last head 0): f32, or in terms
+    uint32_t q0[T == kF32 ? 1 : NB][4], q1[T == kF32 ? 1 : NB][4], q2[T == kBF16 ? NB : 1][4];
+    float qf[T == kF32 ? kOwn : 1][4];
+    int qe;          // scores: times 2^qe
+    float m, l;      // of column i: maximum, this lane's sum of weights
+    f32x4 acc[kOwn]; // of column i: values (4g + r) * kOwn + e in [e][r]
+    // a tile on its way
+    uint32_t kw[2][T == kF32 ? kOwn : NB][T == kQ8_0 ? 2 : 4];
+    uint32_t vw[8][T == kF32 ? kOwn : NB];  // (Q8_0: kOwn levels, two to a word)
+    uint32_t ks[2][T == kQ8_0 ? 2 * NB : 1], vs[8];
+
+    __device__ __forceinline__ void start(const float* q, bool some, float scale) {
+        const uint32_t g = (threadIdx.x & 63) >> 4;
+        const float f = scale * 1.44269504088896340736f;  // exp(x) = 2^(x log2 e)
+        m = -INFINITY, l = 0.0f, qe = 0;
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) acc[e] = f32x4{0, 0, 0, 0};
+        if constexpr (T == kF32) {
+#pragma unroll
+            for (int c = 0; c < kOwn; ++c) {
+                float x[4] = {};
+                if (some) words<float, 4, 4>(q + 16 * c + 4 * g, x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) qf[c][j] = x[j] * f;
+            }
+        } else {
+            float x[NB][8], top = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NB; ++c) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[c][j] = 0.0f;
+                if (some) words<float, 8, 4>(q + 32 * c + 8 * g, x[c]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[c][j] *= f, top = fmaxf(top, fabsf(x[c][j]));
+            }
+            if constexpr (T != kBF16) {  // the largest to 2^13 .. 2^14
+                top = column_max(top);
+                const int e = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+                qe = e - 14;
+#pragma unroll
+                for (int c = 0; c < NB; ++c)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[c][j] = __builtin_amdgcn_ldexpf(x[c][j], -qe);
+            }
+#pragma unroll
+            for (int c = 0; c < NB; ++c) {
+                if constexpr (T == kBF16) split_bf16(x[c], q0[c], q1[c], q2[c]);
+                else split_f16(x[c], q0[c], q1[c]);
+            }
+        }
+    }
+
+    // Keys of the 16 tokens from place `row` of a plane on; half h.
+    __device__ __forceinline__ void load_k(int h, const uint8_t* plane, uint32_t row, uint32_t log_page) {
+        const uint32_t i = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+        const uint8_t* p = plane + (row + i) * (uint32_t)kv_row<T>(kDim);
+        if constexpr (T == kQ8_0) {
+#pragma unroll
+            for (int c = 0; c < NB; ++c) words<uint32_t, 2, 8>(p + 32 * c + 8 * g, kw[h][c]);
+            words<uint32_t, 2 * NB, pow2_of(8 * NB) < 16 ? pow2_of(8 * NB) : 16>(
+                plane + ((uint32_t)kDim << log_page) + (row + 4 * g) * (2 * NB), ks[h]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < (T == kF32 ? kOwn : NB); ++c) words<uint32_t, 4, 16>(p + 64 * c + 16 * g, kw[h][c]);
+        }
+    }
+    __device__ __forceinline__ void load_v(int h, const uint8_t* plane, uint32_t row, uint32_t log_page) {
+        const uint32_t i = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t at = row + 4 * g + j;
+            const uint8_t* p = plane + at * (uint32_t)kv_row<T>(kDim);
+            if constexpr (T == kQ8_0) {
+                uint16_t t[NB];
+                words<uint16_t, NB, pow2_of(2 * NB)>(p + i * kOwn, t);
+#pragma unroll
+                for (int k = 0; k < NB; ++k) vw[4 * h + j][k] = t[k];
+                // the scale of the lane's first value, and that of its last
+                const uint8_t* s = plane + ((uint32_t)kDim << log_page) + at * (2 * NB);
+                const uint32_t b = i * kOwn / 32, c = (i * kOwn + kOwn - 1) / 32;
+                vs[4 * h + j] = *(const uint16_t*)(s + 2 * b);
+                if constexpr (32 % kOwn != 0) vs[4 * h + j] |= (uint32_t)*(const uint16_t*)(s + 2 * c) << 16;
+            } else {
+                constexpr int n = T == kF32 ? kOwn : NB;
+                words<uint32_t, n, pow2_of(4 * n) < 16 ? pow2_of(4 * n) : 16>(p + i * (4 * n), vw[4 * h + j]);
+            }
+        }
+    }
+
+    // Scores of the loaded keys: tokens 4g + r of the halves for column i, to base 2.
+    __device__ __forceinline__ void scores(float (&s)[8]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            f32x4 d = {0, 0, 0, 0};
+            if constexpr (T == kF32) {
+#pragma unroll
+                for (int c = 0; c < kOwn; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[h][c][j]), qf[c][j], d, 0, 0, 0);
+            } else if constexpr (T == kQ8_0) {
+#pragma unroll
+                for (int c = 0; c < NB; ++c) {
+                    uint32_t a[4];  // levels as f16: 1024 + (level + 128), less 1152
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t w = kw[h][c][k / 2] ^ 0x80808080u;
+                        const uint32_t u = __builtin_amdgcn_perm(0x64646464u, w, k % 2 ? 0x04030402u : 0x04010400u);
+                        a[k] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, u) - (_Float16)1152.0f);
+                    }
+                    const f32x4 z = mma_f16(a, q1[c], mma_f16(a, q0[c], f32x4{0, 0, 0, 0}));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {  // the scale of token 4g + r, block c
+                        const uint32_t w = ks[h][(r * NB + c) / 2];
+                        d[r] = __builtin_fmaf(half_to_float((r * NB + c) % 2 ? w >> 16 : w), z[r], d[r]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < NB; ++c) {
+                    if constexpr (T == kF16) d = mma_f16(kw[h][c], q1[c], mma_f16(kw[h][c], q0[c], d));
+                    else d = mma_bf16(kw[h][c], q2[c], mma_bf16(kw[h][c], q1[c], mma_bf16(kw[h][c], q0[c], d)));
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[4 * h + r] = T == kF16 || T == kQ8_0 ? __builtin_amdgcn_ldexpf(d[r], qe) : d[r];
+        }
+    }
+
+    // Weights of the scores; `all`: every token counts, else those of `seen` (bit per token).
+    __device__ __forceinline__ void weights(float (&s)[8], bool all, uint32_t seen) {
+        if (!all) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) s[t] = (seen >> t) & 1 ? s[t] : -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int t = 1; t < 8; ++t) top = fmaxf(top, s[t]);
+        if (__ballot(top > m)) {  // (rare after the first tiles)
+            const float next = fmaxf(m, column_max(top));
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+            m = next, l *= f;
+#pragma unroll
+            for (int e = 0; e < kOwn; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[e][r] *= f;
+        }
+        const float base = m - kTop;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) s[t] = __builtin_amdgcn_exp2f(s[t] - base);
+        if (!all) {  // (a column that has no token yet: -inf less -inf)
+#pragma unroll
+            for (int t = 0; t < 8; ++t) s[t] = (seen >> t) & 1 ? s[t] : 0.0f;
+        }
+        l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+    }
+
+    // Values of tokens that no column sees may be anything: they become 0.
+    __device__ __forceinline__ void drop(uint32_t seen) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            if ((seen >> t) & 1) continue;
+#pragma unroll
+            for (int k = 0; k < (T == kF32 ? kOwn : NB); ++k) vw[t][k] = 0;
+            vs[t] = 0;
+        }
+    }
+
+    __device__ __forceinline__ void products(const float (&p)[8]) {
+        if constexpr (k16) {
+            uint32_t p0[4], p1[4], p2[4];
+            if constexpr (T == kF16) split_f16(p, p0, p1);
+            else split_bf16(p, p0, p1, p2);
+#pragma unroll
+            for (int e = 0; e < kOwn; ++e) {
+                uint32_t a[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    a[k] = __builtin_amdgcn_perm(vw[2 * k + 1][e / 2], vw[2 * k][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+                if constexpr (T == kF16) acc[e] = mma_f16(a, p1, mma_f16(a, p0, acc[e]));
+                else acc[e] = mma_bf16(a, p2, mma_bf16(a, p1, mma_bf16(a, p0, acc[e])));
+            }
+        } else {
+            const uint32_t i = threadIdx.x & 15;
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const float s0 = half_to_float(vs[t]), s1 = half_to_float(vs[t] >> 16);
+#pragma unroll
+                for (int e = 0; e < kOwn; ++e) {
+                    float v;
+                    if constexpr (T == kF32) {
+                        v = __uint_as_float(vw[t][e]);
+                    } else {
+                        const float q = (float)(int8_t)(vw[t][e / 2] >> (8 * (e % 2)));
+                        v = q * (32 % kOwn == 0 || (i * kOwn + e) / 32 == i * kOwn / 32 ? s0 : s1);
+                    }
+                    acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[t], acc[e], 0, 0, 0);
+                }
+            }
+        }
+    }
+};
+
+// The tokens of a part of a row: 256, for long rows a power of two more, so that the parts are at
+// most `most`.  It follows from the row's own length alone, and parts begin at multiples of it: a
+// row's result has the same bits in any company.
+__device__ __forceinline__ uint32_t attn_part(uint32_t tokens, uint32_t most) {
+    uint32_t n = kAttnPart;
+    while ((uint64_t)n * most < tokens) n *= 2;
+    return n;
+}
+
+__device__ __forceinline__ void attn_put(float* to, float x, float y) {
+    const unsigned long long v = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
+    const unsigned long long old =
+        __hip_atomic_exchange((unsigned long long*)to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("" ::"v"(old) : "memory");
+}
+__device__ __forceinline__ float2 attn_get(const float* from) {
+    const unsigned long long v =
+        __hip_atomic_load((const unsigned long long*)from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// A workgroup takes units: a part of a row for up to 16 query heads of one KV head; its four
+// waves take every fourth 32 tokens of it and join in LDS.  The parts of a row are joined, in
+// order, by the last of them to arrive (published as the router's logits are: an exchange is
+// performed at the device's coherent level when it returns).
+template <uint32_t T, int NB>
 __global__ __launch_bounds__(256) void kv_attention_kernel(AttnArgs a) {
-    __shared__ __align__(16) float q[256], p[256];
-    __shared__ int32_t ids[256];
-    __shared__ float red[8];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, dim = a.c.dim, row = blockIdx.x, head = blockIdx.y;
-    const uint32_t kvh = head / (a.heads / a.c.kv_heads), mask = (1u << a.c.log_page) - 1;
-    const int32_t request = a.requests ? a.requests[row] : (int32_t)row;
-    if (request == -1) return;  // a row behind the batch's last
-    const int32_t last = a.positions[row];
-    if (request < 0 || (uint32_t)request >= a.table_rows || last < -1 || last >= (int64_t)a.width << a.c.log_page) {
-        if (tid == 0) report_error(a.err_word, bounds_key(row));
-        return;
-    }
-    const int32_t first = a.window && (uint32_t)last + 1 > a.window ? last + 1 - (int32_t)a.window : 0;
-    const int32_t* table = a.tables + (uint64_t)request * a.width;
-    if (tid < dim) q[tid] = a.q[row * a.q_stride + (uint64_t)head * dim + tid];
-    float m = -INFINITY, sum = 0.0f, acc = 0.0f;
-    bool lost = false;
-    const uint64_t plane = kvh * kv_plane<T>(dim, a.c.log_page);
-    for (int64_t base = first; base <= last; base += 256) {
-        const int64_t tok = base + tid;
-        __syncthreads();  // (p and ids are free, q is there)
-        float s = -INFINITY;
-        if (tok <= last) {
-            int32_t id = table[tok >> a.c.log_page];
-            if (id < 0 || (uint64_t)id >= a.c.pages) lost = true, id = 0;
-            ids[tid] = id;
-            const uint8_t* kp = a.c.k + (uint64_t)id * a.c.k_stride + plane;
-            float d = 0.0f;
-            for (uint32_t e = 0; e < dim; e += 4) {
-                const float4 k = kv_load4<T>(kp, (uint32_t)tok & mask, e, dim, a.c.log_page);
-                d = __builtin_fmaf(k.x, q[e], d);
-                d = __builtin_fmaf(k.y, q[e + 1], d);
-                d = __builtin_fmaf(k.z, q[e + 2], d);
-                d = __builtin_fmaf(k.w, q[e + 3], d);
+    constexpr uint32_t kDim = 32 * NB, kLine = kDim + 2;
+    __shared__ uint32_t start[kAttnRows + 1], sums[4];
+    __shared__ __align__(16) float part[4][16][kLine];  // of a wave and column: values
+    __shared__ float wave_m[4][16], wave_l[4][16];
+    __shared__ uint32_t last_one;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, g = lane >> 4;
+    const uint32_t group = a.heads / a.c.kv_heads, tiles = (group + 15) / 16, per = a.c.kv_heads * tiles;
+    const uint32_t line = (group < 16 ? group : 16) * (kDim + 2);  // floats of a unit's part
+
+    // the rows' parts
+    auto span = [&](uint32_t row, int32_t& request, int32_t& first, int32_t& last) -> bool {
+        request = a.requests ? a.requests[row] : (int32_t)row;
+        last = a.positions[row];
+        first = a.window && (uint32_t)(last + 1) > a.window ? last + 1 - (int32_t)a.window : 0;
+        return request >= 0 && (uint32_t)request < a.table_rows && last >= -1 && last < (int64_t)a.width << a.c.log_page;
+    };
+    {
+        uint32_t n[kAttnRows / 256], mine = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kAttnRows / 256; ++k) {
+            const uint32_t row = tid * (kAttnRows / 256) + k;
+            n[k] = 0;
+            if (row < a.rows) {
+                int32_t request, first, last;
+                if (span(row, request, first, last)) {
+                    const uint32_t len = attn_part((uint32_t)(last + 1), a.most);
+                    n[k] = last < 0 ? 1 : (uint32_t)last / len - (uint32_t)first / len + 1;
+                } else if (request != -1) {
+                    report_error(a.err_word, bounds_key(a.row0 + row));
+                }
             }
-            s = d * a.scale;
+            mine += n[k];
         }
-        const float w = wave_max(s);
-        if (lane == 0) red[wave] = w;
+        uint32_t sum = mine;
+        for (int s = 1; s < 64; s <<= 1) {
+            const uint32_t o = (uint32_t)__shfl_up((int)sum, s, 64);
+            if ((int)lane >= s) sum += o;
+        }
+        if (lane == 63) sums[wave] = sum;
         __syncthreads();
-        const float top = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        const float e = tok <= last ? expf(s - top) : 0.0f, shrink = m == -INFINITY ? 0.0f : expf(m - top);
-        p[tid] = e;
-        const float part = wave_sum(e);
-        if (lane == 0) red[4 + wave] = part;
-        __syncthreads();
-        sum = sum * shrink + ((red[4] + red[5]) + (red[6] + red[7]));
-        acc = acc * shrink;
-        m = top;
-        if (tid < dim) {
-            const uint32_t n = last - base + 1 < 256 ? (uint32_t)(last - base + 1) : 256;
-            for (uint32_t j = 0; j < n; ++j) {
-                const uint8_t* vp = a.c.v + (uint64_t)ids[j] * a.c.v_stride + plane;
-                const float4 v = kv_load4<T>(vp, (uint32_t)(base + j) & mask, tid & ~3u, dim, a.c.log_page);
-                const float one = (tid & 2) ? (tid & 1 ? v.w : v.z) : (tid & 1 ? v.y : v.x);
-                acc = __builtin_fmaf(p[j], one, acc);
-            }
+        for (uint32_t w = 0; w < wave; ++w) sum += sums[w];
+        sum -= mine;
+#pragma unroll
+        for (uint32_t k = 0; k < kAttnRows / 256; ++k) {
+            const uint32_t row = tid * (kAttnRows / 256) + k;
+            if (row <= a.rows) start[row] = sum;
+            sum += n[k];
+            if (row + 1 == kAttnRows) start[kAttnRows] = sum;
         }
         __syncthreads();
     }
-    const float y = last < 0 ? 0.0f : acc / sum;
-    const bool off = tid < dim && !finite(y);
-    if (__syncthreads_or(lost)) {
-        if (tid == 0) report_error(a.err_word, bounds_key(row));
-        return;
+    const uint64_t units = (uint64_t)start[a.rows] * per;
+
+    for (uint64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const uint32_t u = (uint32_t)(unit / per), hc = (uint32_t)(unit - (uint64_t)u * per), kvh = hc / tiles, tile = hc - kvh * tiles;
+        const uint32_t row = segment_of(start, a.rows, u), split = u - start[row], parts = start[row + 1] - start[row];
+        const uint32_t cols = group - 16 * tile < 16 ? group - 16 * tile : 16, head0 = kvh * group + 16 * tile;
+        int32_t request, first, last;
+        span(row, request, first, last);
+        const uint32_t len = attn_part((uint32_t)(last + 1), a.most);
+        // tokens t0 .. t1 of this part
+        const int32_t from = (int32_t)(((uint32_t)first / len + split) * len);
+        const int32_t t0 = from > first ? from : first, t1 = (int64_t)from + len - 1 < last ? from + (int32_t)len - 1 : last;
+
+        AttnWave<T, NB> w;
+        w.start(a.q + row * a.q_stride + (uint64_t)(head0 + i) * kDim, i < cols, a.scale);
+        const int32_t* table = a.tables + (uint64_t)request * a.width;
+        const uint64_t plane = kvh * kv_plane<T>(kDim, a.c.log_page);
+        const uint32_t mask = (1u << a.c.log_page) - 1;
+        bool lost = false;
+        for (int64_t c0 = t0 & ~31; c0 <= t1; c0 += 1024) {
+            // lane k: the page of the sixteen tokens from c0 + 16 k on
+            int32_t id = 0;
+            const int64_t at = c0 + 16 * lane;
+            if (at <= t1 && at + 15 >= t0) {
+                id = table[at >> a.c.log_page];
+                if (id < 0 || (uint64_t)id >= a.c.pages) lost = true, id = 0;
+            }
+            auto page = [&](int64_t t) { return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(id, (int)((t - c0) >> 4)); };
+            const int64_t c1 = c0 + 1023 < t1 ? c0 + 1023 : t1;
+            auto load_k = [&](int64_t t) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    w.load_k(h, a.c.k + page(t + 16 * h) * a.c.k_stride + plane, (uint32_t)(t + 16 * h) & mask, a.c.log_page);
+            };
+            auto load_v = [&](int64_t t) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    w.load_v(h, a.c.v + page(t + 16 * h) * a.c.v_stride + plane, (uint32_t)(t + 16 * h) & mask, a.c.log_page);
+            };
+            int64_t t = c0 + 32 * wave;
+            if (t <= c1) load_k(t), load_v(t);
+            for (; t <= c1; t += 128) {
+                const bool all = t >= t0 && t + 31 <= t1, more = t + 128 <= c1;
+                uint32_t seen = 0;
+                if (!all) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int64_t tok = t + 16 * (k / 4) + 4 * g + k % 4;
+                        seen |= (uint32_t)(tok >= t0 && tok <= t1) << k;
+                    }
+                }
+                float s[8];
+                w.scores(s);
+                if (more) load_k(t + 128);
+                w.weights(s, all, seen);
+                if (!all) w.drop(seen);
+                w.products(s);
+                if (more) load_v(t + 128);
+            }
+        }
+        if (__ballot(lost)) {  // (every wave of a row's units finds its own; what is joined is then no number)
+            w.l = NAN;
+            if (lane == 0) report_error(a.err_word, bounds_key(a.row0 + row));
+        }
+
+        // the waves join
+        w.l = column_sum(w.l);
+        if (g == 0) wave_m[wave][i] = w.m, wave_l[wave][i] = w.l;
+        __syncthreads();
+        float top = fmaxf(fmaxf(wave_m[0][i], wave_m[1][i]), fmaxf(wave_m[2][i], wave_m[3][i]));
+        const float f = w.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w.m - top);
+        if (i < cols) {
+#pragma unroll
+            for (int e = 0; e < 2 * NB; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) part[wave][i][(4 * g + r) * (2 * NB) + e] = w.acc[e][r] * f;
+        }
+        __syncthreads();
+        // a wave takes every fourth column, a lane pairs of values
+        float* scratch = a.scratch + unit * line;
+        for (uint32_t c = wave; c < cols; c += 4) {
+            const float ct = fmaxf(fmaxf(wave_m[0][c], wave_m[1][c]), fmaxf(wave_m[2][c], wave_m[3][c]));
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float l = wave_l[k][c];
+                sum += l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f(wave_m[k][c] - ct);  // (0: without tokens)
+            }
+            float* out = a.out + row * a.out_stride + (uint64_t)(head0 + c) * kDim;
+            float y[(kDim + 127) / 128][2];
+            bool off = false;
+#pragma unroll
+            for (uint32_t k = 0; k < (kDim + 127) / 128; ++k) {
+                const uint32_t d = 2 * lane + 128 * k;
+                y[k][0] = y[k][1] = 0.0f;
+                if (d >= kDim) continue;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    y[k][j] = (part[0][c][d + j] + part[1][c][d + j]) + (part[2][c][d + j] + part[3][c][d + j]);
+                if (parts > 1) {
+                    attn_put(scratch + c * (kDim + 2) + d, y[k][0], y[k][1]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) y[k][j] = last < 0 ? 0.0f : y[k][j] / sum, off |= !finite(y[k][j]);
+                }
+            }
+            if (parts > 1) {
+                if (lane == 0) attn_put(scratch + c * (kDim + 2) + kDim, ct, sum);
+                continue;
+            }
+            if (__ballot(off)) {
+                if (lane == 0) report_error(a.err_word, model_key(a.row0 + row, kStAttnOut, 0));
+                continue;
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < (kDim + 127) / 128; ++k) {
+                const uint32_t d = 2 * lane + 128 * k;
+                if (d < kDim) out[d] = y[k][0], out[d + 1] = y[k][1];
+            }
+        }
+        __syncthreads();
+        if (parts == 1) continue;
+        uint32_t* count = a.count + (uint64_t)row * per + hc;
+        if (tid == 0) {
+            const uint32_t old = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last_one = old == parts - 1;
+            if (last_one) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!last_one) continue;
+        // the row's parts in order
+        const uint64_t unit0 = (uint64_t)start[row] * per + hc, step = (uint64_t)per * line;
+        const float* parts0 = a.scratch + unit0 * line;
+        for (uint32_t c = wave; c < cols; c += 4) {
+            const float* p = parts0 + c * (kDim + 2);
+            float ct = -INFINITY;
+            for (uint32_t k = lane; k < parts; k += 64) ct = fmaxf(ct, attn_get(p + k * step + kDim).x);
+            ct = wave_max_dpp(ct);
+            float sum = 0.0f, y[(kDim + 127) / 128][2] = {};
+            for (uint32_t k = 0; k < parts; ++k) {
+                const float2 ml = attn_get(p + k * step + kDim);
+                const float fk = __builtin_amdgcn_exp2f(ml.x - ct);  // (a part has tokens)
+                sum = __builtin_fmaf(ml.y, fk, sum);
+#pragma unroll
+                for (uint32_t v = 0; v < (kDim + 127) / 128; ++v) {
+                    const uint32_t d = 2 * lane + 128 * v;
+                    if (d >= kDim) continue;
+                    const float2 x = attn_get(p + k * step + d);
+                    y[v][0] = __builtin_fmaf(x.x, fk, y[v][0]);
+                    y[v][1] = __builtin_fmaf(x.y, fk, y[v][1]);
+                }
+            }
+            bool off = false;
+#pragma unroll
+            for (uint32_t v = 0; v < (kDim + 127) / 128; ++v)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) y[v][j] = y[v][j] / sum, off |= 2 * lane + 128 * v < kDim && !finite(y[v][j]);
+            if (__ballot(off)) {
+                if (lane == 0) report_error(a.err_word, model_key(a.row0 + row, kStAttnOut, 0));
+                continue;
+            }
+            float* out = a.out + row * a.out_stride + (uint64_t)(head0 + c) * kDim;
+#pragma unroll
+            for (uint32_t v = 0; v < (kDim + 127) / 128; ++v) {
+                const uint32_t d = 2 * lane + 128 * v;
+                if (d < kDim) out[d] = y[v][0], out[d + 1] = y[v][1];
+            }
+        }
+        __syncthreads();
     }
-    if (__syncthreads_or(off)) {
-        if (tid == 0) report_error(a.err_word, model_key(row, kStAttnOut, 0));
-        return;
-    }
-    if (tid < dim) a.out[row * a.out_stride + (uint64_t)head * dim + tid] = y;
 }
 
-hipError_t launch_kv_attention(const AttnArgs& a, hipStream_t s) {
-    if (a.rows == 0 || a.rows > 65535 || a.heads == 0 || a.heads > 65535 || a.c.dim % 32 || a.c.dim > 256)
-        return hipErrorInvalidValue;
-    const dim3 grid(a.rows, a.heads), block(256);
-    switch (a.c.type) {
-        case kF32: hipLaunchKernelGGL(kv_attention_kernel<kF32>, grid, block, 0, s, a); break;
-        case kF16: hipLaunchKernelGGL(kv_attention_kernel<kF16>, grid, block, 0, s, a); break;
-        case kBF16: hipLaunchKernelGGL(kv_attention_kernel<kBF16>, grid, block, 0, s, a); break;
-        case kQ8_0: hipLaunchKernelGGL(kv_attention_kernel<kQ8_0>, grid, block, 0, s, a); break;
+// The parts that a row may have: they fill the CUs two or three times over, and one workgroup
+// joins them.
+static uint32_t attn_most(const AttnArgs& a) {
+    const uint32_t tiles = (a.heads / a.c.kv_heads + 15) / 16, n = 512 / (a.c.kv_heads * tiles);
+    return n < 32 ? 32 : n > 128 ? 128 : n;
+}
+// Units of a row at most, and the rows of a launch: what their parts take stays within 256 MB.
+static uint64_t attn_units(const AttnArgs& a) {
+    const uint64_t tokens = (uint64_t)a.width << a.c.log_page, tiles = (a.heads / a.c.kv_heads + 15) / 16;
+    uint64_t parts = (tokens + kAttnPart - 1) / kAttnPart;
+    const uint64_t most = attn_most(a);
+    parts = parts < 1 ? 1 : parts < most ? parts : most;
+    return parts * a.c.kv_heads * tiles;
+}
+static uint64_t attn_row_bytes(const AttnArgs& a) {
+    const uint64_t group = a.heads / a.c.kv_heads;
+    return attn_units(a) * (group < 16 ? group : 16) * (a.c.dim + 2) * sizeof(float);
+}
+static uint32_t attn_rows(const AttnArgs& a) {
+    uint64_t n = (256ull << 20) / attn_row_bytes(a);
+    n = n < 1 ? 1 : n < kAttnRows ? n : kAttnRows;
+    return n < a.rows ? (uint32_t)n : a.rows;
+}
+size_t kv_attention_bytes(const AttnArgs& a) { return attn_rows(a) * attn_row_bytes(a); }
+uint64_t kv_attention_counters(const AttnArgs& a) {
+    const uint64_t tiles = (a.heads / a.c.kv_heads + 15) / 16;
+    return attn_rows(a) * a.c.kv_heads * tiles;
+}
+
+template <uint32_t T, int NB>
+static void attn_launch(const AttnArgs& a, uint32_t grid, hipStream_t s) {
+    hipLaunchKernelGGL((kv_attention_kernel<T, NB>), dim3(grid), dim3(256), 0, s, a);
+}
+template <uint32_t T>
+static hipError_t attn_dims(const AttnArgs& a, uint32_t grid, hipStream_t s) {
+    switch (a.c.dim / 32) {
+        case 1: attn_launch<T, 1>(a, grid, s); break;
+        case 2: attn_launch<T, 2>(a, grid, s); break;
+        case 3: attn_launch<T, 3>(a, grid, s); break;
+        case 4: attn_launch<T, 4>(a, grid, s); break;
+        case 5: attn_launch<T, 5>(a, grid, s); break;
+        case 6: attn_launch<T, 6>(a, grid, s); break;
+        case 7: attn_launch<T, 7>(a, grid, s); break;
+        case 8: attn_launch<T, 8>(a, grid, s); break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();
+}
+
+hipError_t launch_kv_attention(AttnArgs a, hipStream_t s) {
+    if (a.rows == 0 || a.rows > 65535 || a.heads == 0 || a.heads > 65535 || a.c.dim % 32 || a.c.dim > 256 ||
+        a.heads % a.c.kv_heads)
+        return hipErrorInvalidValue;
+    a.most = attn_most(a);
+    const uint32_t rows = a.rows, most_rows = attn_rows(a);
+    const float* q = a.q;
+    float* out = a.out;
+    const int32_t *positions = a.positions, *requests = a.requests, *tables = a.tables;
+    for (uint32_t r = 0; r < rows; r += most_rows) {  // (the parts and counters are the same memory)
+        a.row0 = r;
+        a.rows = rows - r < most_rows ? rows - r : most_rows;
+        a.q = q + r * a.q_stride, a.out = out + r * a.out_stride;
+        a.positions = positions + r;
+        a.requests = requests ? requests + r : nullptr;
+        const uint64_t units = attn_units(a) * a.rows, most = 8ull * device_cus();
+        const uint32_t grid = (uint32_t)(units < most ? units : most);
+        if (!requests) {  // row t is request t
+            a.tables = tables + (uint64_t)r * a.width;
+        }
+        hipError_t e;
+        switch (a.c.type) {
+            case kF32: e = attn_dims<kF32>(a, grid, s); break;
+            case kF16: e = attn_dims<kF16>(a, grid, s); break;
+            case kBF16: e = attn_dims<kBF16>(a, grid, s); break;
+            case kQ8_0: e = attn_dims<kQ8_0>(a, grid, s); break;
+            default: return hipErrorInvalidValue;
+        }
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // ---------------------------------------------------------------------------

@@ -291,6 +291,8 @@ struct StoreArgs {
     unsigned long long* err_word;
 };
 hipError_t launch_kv_store(const StoreArgs& a, hipStream_t s);
+// Attention: a row's tokens in parts, the rows of a launch at most.
+constexpr uint32_t kAttnPart = 256, kAttnRows = 1024;
 struct AttnArgs {
     KvLayer c;
     const float* q;
@@ -300,8 +302,13 @@ struct AttnArgs {
     float scale;
     float* out;
     unsigned long long* err_word;
+    float* scratch;   // kv_attention_bytes
+    uint32_t* count;  // kv_attention_counters words, 0 between launches
+    uint32_t most, row0;  // of a launch: parts of a row, the first row
 };
-hipError_t launch_kv_attention(const AttnArgs& a, hipStream_t s);
+size_t kv_attention_bytes(const AttnArgs& a);
+uint64_t kv_attention_counters(const AttnArgs& a);
+hipError_t launch_kv_attention(AttnArgs a, hipStream_t s);
 // The beams' tables and part-filled pages after a choice; tensors: k, v, k, v, ...
 constexpr uint32_t kReorderMaxBeams = 32, kReorderLayers = 64;
 struct ReorderArgs {
