@@ -39,16 +39,6 @@ __device__ __forceinline__ float4 route_load(const float* p, uint32_t e, uint32_
                        e + 3 < n ? p[e + 3] : 0.0f);
 }
 
-// The maximum over the wave, in every lane (call it with every lane active).
-__device__ __forceinline__ double wave_max_f64(double v) {
-    auto up = [](double a, double b) { return b > a ? b : a; };
-    v = up(v, dpp_d<kQuadXor1>(v));
-    v = up(v, dpp_d<kQuadXor2>(v));
-    v = up(v, dpp_d<kRowHalfMirror>(v));
-    v = up(v, dpp_d<kRowRor8>(v));
-    return up(up(readlane_d(v, 0), readlane_d(v, 16)), up(readlane_d(v, 32), readlane_d(v, 48)));
-}
-
 // The best experts of token t by one wave; lane l holds experts l, l + 64, ...
 // (NI of them).  Ranks are f64 (score + bias), or with no bias the f32 logits as
 // ordered u32 keys (1 and up; equal floats have equal keys): a round of the

@@ -181,6 +181,15 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     auto at = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
     return up(up(at(0), at(16)), up(at(32), at(48)));
 }
+// The maximum over the wave, in every lane (call it with every lane active).
+__device__ __forceinline__ double wave_max_f64(double v) {
+    auto up = [](double a, double b) { return b > a ? b : a; };
+    v = up(v, dpp_d<kQuadXor1>(v));
+    v = up(v, dpp_d<kQuadXor2>(v));
+    v = up(v, dpp_d<kRowHalfMirror>(v));
+    v = up(v, dpp_d<kRowRor8>(v));
+    return up(up(readlane_d(v, 0), readlane_d(v, 16)), up(readlane_d(v, 32), readlane_d(v, 48)));
+}
 __device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {
     for (int m = 1; m < 64; m <<= 1) {
         const uint32_t o = (uint32_t)__shfl_xor((int)v, m, 64);
@@ -207,6 +216,7 @@ __device__ __forceinline__ uint4 load_stream16(const void* p) {
 }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));  // four floats at any float's address
 
 // The same for four floats read once per launch: the cached keys of the
 // attention scores.  Llama-3-8B decode step at a context of 1024, ms per token

@@ -332,10 +332,12 @@ struct SelectArgs {
     float* out_scores;
     int32_t *parents, *tokens;
     unsigned long long* err_word;
-    double* rank;  // scratch
-    int32_t* token;
+    uint32_t* count;  // a word for each beam and group, 0 between launches
+    // of a launch: tokens of a workgroup, the first group; scratch (beam_select_bytes)
+    uint32_t chunk, group0;
+    unsigned long long *ranks, *lists;
 };
-size_t beam_select_bytes(uint64_t rows, uint64_t best);
+size_t beam_select_bytes(uint64_t rows, uint64_t vocabulary, uint64_t best);
 hipError_t launch_beam_select(SelectArgs a, void* scratch, hipStream_t s);
 
 // ---- llama.hip ----
