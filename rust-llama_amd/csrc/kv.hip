@@ -625,13 +625,17 @@ struct AttnWave {
     }
 };
 
-// The tokens of a part of a row: 256, for long rows a power of two more, so that the parts are at
-// most `most`.  It follows from the row's own length alone, and parts begin at multiples of it: a
-// row's result has the same bits in any company.
-__device__ __forceinline__ uint32_t attn_part(uint32_t tokens, uint32_t most) {
-    uint32_t n = kAttnPart;
-    while ((uint64_t)n * most < tokens) n *= 2;
-    return n;
+// Tokens of a part: the units of all rows (parts times `per`) are to fill the slots of the
+// CUs once.  rows rows of `tokens` in all, the longest of `most`, make no more than
+// tokens / p + rows parts of p tokens; of many rows, which fill the slots as they are, the long ones
+// are cut to pieces of no more than twice the mean.  A row has 128 parts at most: one
+// workgroup joins them.
+__device__ __forceinline__ uint32_t attn_part(uint64_t tokens, uint32_t rows, uint32_t most, uint32_t slots, uint32_t per) {
+    const uint32_t s = slots / per + 1, half = s / 2 + 1, budget = s > rows && s - rows > half ? s - rows : half;
+    uint64_t p = (tokens + budget - 1) / budget;
+    if (p * kAttnParts < most) p = (most + kAttnParts - 1) / kAttnParts;
+    p = (p + 127) / 128 * 128;
+    return p < kAttnPart ? kAttnPart : (uint32_t)p;
 }
 
 __device__ __forceinline__ void attn_put(float* to, float x, float y) {
@@ -651,9 +655,11 @@ __device__ __forceinline__ float2 attn_get(const float* from) {
 // order, by the last of them to arrive (published as the router's logits are: an exchange is
 // performed at the device's coherent level when it returns).
 template <uint32_t T, int NB>
-__global__ __launch_bounds__(256) void kv_attention_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, NB <= (T == kF32 ? 3 : 4) ? 2 : 1) void kv_attention_kernel(AttnArgs a) {
     constexpr uint32_t kDim = 32 * NB, kLine = kDim + 2;
-    __shared__ uint32_t start[kAttnRows + 1], sums[4];
+    __shared__ uint32_t start[kAttnRows + 1], sums[4], counts[4], longest[4];
+    __shared__ uint64_t totals[4];
+    __shared__ int32_t firsts[kAttnRows], lasts[kAttnRows], of[kAttnRows];
     __shared__ __align__(16) float part[4][16][kLine];  // of a wave and column: values
     __shared__ float wave_m[4][16], wave_l[4][16];
     __shared__ uint32_t last_one;
@@ -661,28 +667,45 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(AttnArgs a) {
     const uint32_t group = a.heads / a.c.kv_heads, tiles = (group + 15) / 16, per = a.c.kv_heads * tiles;
     const uint32_t line = (group < 16 ? group : 16) * (kDim + 2);  // floats of a unit's part
 
-    // the rows' parts
-    auto span = [&](uint32_t row, int32_t& request, int32_t& first, int32_t& last) -> bool {
-        request = a.requests ? a.requests[row] : (int32_t)row;
-        last = a.positions[row];
-        first = a.window && (uint32_t)(last + 1) > a.window ? last + 1 - (int32_t)a.window : 0;
-        return request >= 0 && (uint32_t)request < a.table_rows && last >= -1 && last < (int64_t)a.width << a.c.log_page;
-    };
+    // the rows' tokens, then their parts
+    uint32_t len;
     {
-        uint32_t n[kAttnRows / 256], mine = 0;
+        constexpr uint32_t kMine = kAttnRows / 256;
+        uint64_t total = 0;
+        uint32_t live = 0, most = 0;
 #pragma unroll
-        for (uint32_t k = 0; k < kAttnRows / 256; ++k) {
-            const uint32_t row = tid * (kAttnRows / 256) + k;
+        for (uint32_t k = 0; k < kMine; ++k) {
+            const uint32_t row = tid * kMine + k;
+            if (row >= a.rows) break;
+            const int32_t request = a.requests ? a.requests[row] : (int32_t)row, last = a.positions[row];
+            const int32_t first = a.window && (uint32_t)(last + 1) > a.window ? last + 1 - (int32_t)a.window : 0;
+            const bool sound = request >= 0 && (uint32_t)request < a.table_rows && last >= -1 && last < (int64_t)a.width << a.c.log_page;
+            if (!sound && request != -1) report_error(a.err_word, bounds_key(a.row0 + row));
+            firsts[row] = first, lasts[row] = last, of[row] = sound ? request : -1;
+            if (!sound) continue;
+            const uint32_t n = (uint32_t)(last + 1 - first);
+            total += n, live += 1, most = n > most ? n : most;
+        }
+        for (int s = 1; s < 64; s <<= 1) {
+            total += __shfl_xor(total, s, 64);
+            live += (uint32_t)__shfl_xor((int)live, s, 64);
+            const uint32_t o = (uint32_t)__shfl_xor((int)most, s, 64);
+            most = o > most ? o : most;
+        }
+        if (lane == 0) totals[wave] = total, counts[wave] = live, longest[wave] = most;
+        __syncthreads();
+        total = 0, live = 0, most = 0;
+        for (uint32_t w = 0; w < 4; ++w) {
+            total += totals[w], live += counts[w];
+            most = longest[w] > most ? longest[w] : most;
+        }
+        len = attn_part(total, live, most, a.slots, per);
+        uint32_t n[kMine], mine = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kMine; ++k) {
+            const uint32_t row = tid * kMine + k;
             n[k] = 0;
-            if (row < a.rows) {
-                int32_t request, first, last;
-                if (span(row, request, first, last)) {
-                    const uint32_t len = attn_part((uint32_t)(last + 1), a.most);
-                    n[k] = last < 0 ? 1 : (uint32_t)last / len - (uint32_t)first / len + 1;
-                } else if (request != -1) {
-                    report_error(a.err_word, bounds_key(a.row0 + row));
-                }
-            }
+            if (row < a.rows && of[row] >= 0) n[k] = lasts[row] < 0 ? 1 : (uint32_t)lasts[row] / len - (uint32_t)firsts[row] / len + 1;
             mine += n[k];
         }
         uint32_t sum = mine;
@@ -695,8 +718,8 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(AttnArgs a) {
         for (uint32_t w = 0; w < wave; ++w) sum += sums[w];
         sum -= mine;
 #pragma unroll
-        for (uint32_t k = 0; k < kAttnRows / 256; ++k) {
-            const uint32_t row = tid * (kAttnRows / 256) + k;
+        for (uint32_t k = 0; k < kMine; ++k) {
+            const uint32_t row = tid * kMine + k;
             if (row <= a.rows) start[row] = sum;
             sum += n[k];
             if (row + 1 == kAttnRows) start[kAttnRows] = sum;
@@ -709,12 +732,10 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(AttnArgs a) {
         const uint32_t u = (uint32_t)(unit / per), hc = (uint32_t)(unit - (uint64_t)u * per), kvh = hc / tiles, tile = hc - kvh * tiles;
         const uint32_t row = segment_of(start, a.rows, u), split = u - start[row], parts = start[row + 1] - start[row];
         const uint32_t cols = group - 16 * tile < 16 ? group - 16 * tile : 16, head0 = kvh * group + 16 * tile;
-        int32_t request, first, last;
-        span(row, request, first, last);
-        const uint32_t len = attn_part((uint32_t)(last + 1), a.most);
+        const int32_t request = of[row], first = firsts[row], last = lasts[row];
         // tokens t0 .. t1 of this part
         const int32_t from = (int32_t)(((uint32_t)first / len + split) * len);
-        const int32_t t0 = from > first ? from : first, t1 = (int64_t)from + len - 1 < last ? from + (int32_t)len - 1 : last;
+        const int32_t t0 = from > first ? from : first, t1 = (int64_t)from + len - 1 < last ? (int32_t)(from + len - 1) : last;
 
         AttnWave<T, NB> w;
         w.start(a.q + row * a.q_stride + (uint64_t)(head0 + i) * kDim, i < cols, a.scale);
@@ -875,33 +896,21 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(AttnArgs a) {
     }
 }
 
-// The parts that a row may have: they fill the CUs two or three times over, and one workgroup
-// joins them.
-static uint32_t attn_most(const AttnArgs& a) {
-    const uint32_t tiles = (a.heads / a.c.kv_heads + 15) / 16, n = 512 / (a.c.kv_heads * tiles);
-    return n < 32 ? 32 : n > 128 ? 128 : n;
+// Units of `rows` rows at most (attn_part: budget + rows parts, and one more of a row whose window
+// begins within a part).
+static uint64_t attn_units(const AttnArgs& a, uint64_t rows) {
+    const uint64_t tiles = (a.heads / a.c.kv_heads + 15) / 16, per = a.c.kv_heads * tiles;
+    return per * (a.slots / per + 2 + 2 * rows);
 }
-// Units of a row at most, and the rows of a launch: what their parts take stays within 256 MB.
-static uint64_t attn_units(const AttnArgs& a) {
-    const uint64_t tokens = (uint64_t)a.width << a.c.log_page, tiles = (a.heads / a.c.kv_heads + 15) / 16;
-    uint64_t parts = (tokens + kAttnPart - 1) / kAttnPart;
-    const uint64_t most = attn_most(a);
-    parts = parts < 1 ? 1 : parts < most ? parts : most;
-    return parts * a.c.kv_heads * tiles;
-}
-static uint64_t attn_row_bytes(const AttnArgs& a) {
+static uint32_t attn_slots() { return 2 * (uint32_t)device_cus(); }
+size_t kv_attention_bytes(AttnArgs a) {
+    a.slots = attn_slots();
     const uint64_t group = a.heads / a.c.kv_heads;
-    return attn_units(a) * (group < 16 ? group : 16) * (a.c.dim + 2) * sizeof(float);
+    return attn_units(a, a.rows < kAttnRows ? a.rows : kAttnRows) * (group < 16 ? group : 16) * (a.c.dim + 2) * sizeof(float);
 }
-static uint32_t attn_rows(const AttnArgs& a) {
-    uint64_t n = (256ull << 20) / attn_row_bytes(a);
-    n = n < 1 ? 1 : n < kAttnRows ? n : kAttnRows;
-    return n < a.rows ? (uint32_t)n : a.rows;
-}
-size_t kv_attention_bytes(const AttnArgs& a) { return attn_rows(a) * attn_row_bytes(a); }
 uint64_t kv_attention_counters(const AttnArgs& a) {
     const uint64_t tiles = (a.heads / a.c.kv_heads + 15) / 16;
-    return attn_rows(a) * a.c.kv_heads * tiles;
+    return (a.rows < kAttnRows ? a.rows : kAttnRows) * a.c.kv_heads * tiles;
 }
 
 template <uint32_t T, int NB>
@@ -928,18 +937,18 @@ hipError_t launch_kv_attention(AttnArgs a, hipStream_t s) {
     if (a.rows == 0 || a.rows > 65535 || a.heads == 0 || a.heads > 65535 || a.c.dim % 32 || a.c.dim > 256 ||
         a.heads % a.c.kv_heads)
         return hipErrorInvalidValue;
-    a.most = attn_most(a);
-    const uint32_t rows = a.rows, most_rows = attn_rows(a);
+    a.slots = attn_slots();
+    const uint32_t rows = a.rows;
     const float* q = a.q;
     float* out = a.out;
     const int32_t *positions = a.positions, *requests = a.requests, *tables = a.tables;
-    for (uint32_t r = 0; r < rows; r += most_rows) {  // (the parts and counters are the same memory)
+    for (uint32_t r = 0; r < rows; r += kAttnRows) {  // (the parts and counters are the same memory)
         a.row0 = r;
-        a.rows = rows - r < most_rows ? rows - r : most_rows;
+        a.rows = rows - r < kAttnRows ? rows - r : kAttnRows;
         a.q = q + r * a.q_stride, a.out = out + r * a.out_stride;
         a.positions = positions + r;
         a.requests = requests ? requests + r : nullptr;
-        const uint64_t units = attn_units(a) * a.rows, most = 8ull * device_cus();
+        const uint64_t units = attn_units(a, a.rows), most = 8ull * device_cus();
         const uint32_t grid = (uint32_t)(units < most ? units : most);
         if (!requests) {  // row t is request t
             a.tables = tables + (uint64_t)r * a.width;

@@ -292,7 +292,7 @@ struct StoreArgs {
 };
 hipError_t launch_kv_store(const StoreArgs& a, hipStream_t s);
 // Attention: a row's tokens in parts, the rows of a launch at most.
-constexpr uint32_t kAttnPart = 256, kAttnRows = 1024;
+constexpr uint32_t kAttnPart = 256, kAttnParts = 128, kAttnRows = 1024;
 struct AttnArgs {
     KvLayer c;
     const float* q;
@@ -304,9 +304,9 @@ struct AttnArgs {
     unsigned long long* err_word;
     float* scratch;   // kv_attention_bytes
     uint32_t* count;  // kv_attention_counters words, 0 between launches
-    uint32_t most, row0;  // of a launch: parts of a row, the first row
+    uint32_t slots, row0;  // of a launch: workgroups that run at once, the first row
 };
-size_t kv_attention_bytes(const AttnArgs& a);
+size_t kv_attention_bytes(AttnArgs a);
 uint64_t kv_attention_counters(const AttnArgs& a);
 hipError_t launch_kv_attention(AttnArgs a, hipStream_t s);
 // The beams' tables and part-filled pages after a choice; tensors: k, v, k, v, ...
