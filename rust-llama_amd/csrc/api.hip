@@ -1257,7 +1257,7 @@ int32_t rlq_beam_reorder(rlq_context* ctx, const int32_t* parents, const int32_t
     DeviceGuard g(ctx->device);
     ReorderArgs a{parents, lengths, tables, (uint32_t)groups, (uint32_t)beams, (uint32_t)width, c.log_page, c.kv_heads,
                   (uint32_t)kv_value_bytes(c.type, c.dim), (uint32_t)kv_scale_bytes(c.type, c.dim), c.pages, c.k_stride,
-                  c.v_stride, 0, 0, ctx->err_words, {}};
+                  c.v_stride, 0, 0, 0, ctx->err_words, {}};
     for (uint64_t i = 0; i < n_layers; i += kReorderLayers) {
         const uint64_t n = n_layers - i < kReorderLayers ? n_layers - i : kReorderLayers;
         for (uint64_t k = 0; k < n; ++k) {

@@ -976,84 +976,83 @@ hipError_t launch_kv_attention(AttnArgs a, hipStream_t s) {
 // A thread takes one column, or one piece at one place of all beams' pages: it has
 // loaded all before it stores any, so the beams may change places among themselves.
 //
-// grid: pieces (or columns), groups, tensors (the tables first).
+// grid: runs of pieces (or of columns), groups, tensors (the tables first).
+// (lane b holds beam b's page and that of its parent; lanes behind the last beam the first beam's.  A beam
+// that stays is loaded too: it is some other's parent in most cases, and no branch lies between the loads)
+template <int MB, class V>
+__device__ __forceinline__ void reorder_piece(uint8_t* at, uint64_t stride, int32_t page, int32_t source, uint32_t moved) {
+    V v[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) v[b] = *(const V*)(at + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(source, b) * stride);
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+        if ((moved >> b) & 1) *(V*)(at + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(page, b) * stride) = v[b];
+}
+
 template <int MB>
 __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
-    __shared__ int32_t from[MB], source[MB], mine[MB];
-    __shared__ uint32_t tail_s, rows_s;
-    const uint32_t tid = threadIdx.x, g = blockIdx.y, B = a.beams;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, g = blockIdx.y, B = a.beams;
     const uint64_t beam0 = (uint64_t)g * B;
-    uint64_t wrong = ~0ull;
-    if (tid < B) {
-        const int32_t p = a.parents[beam0 + tid], len = a.lengths[beam0 + tid];
-        from[tid] = p == -1 ? (int32_t)tid : p;
-        const uint64_t tail = (uint64_t)(len < 0 ? 0 : len) >> a.log_page;
-        const uint32_t rows = len & ((1 << a.log_page) - 1);
-        if (p < -1 || p >= (int32_t)B || len < 0 || len != a.lengths[beam0] || tail + (rows > 0) > a.width) wrong = beam0 + tid;
-        else if (rows) {
-            mine[tid] = a.tables[(beam0 + tid) * a.width + tail];
-            if (mine[tid] < 0 || (uint64_t)mine[tid] >= a.pages) wrong = beam0 + tid;
-        }
-        if (tid == 0) tail_s = (uint32_t)tail, rows_s = rows;
+    // lane b of every wave: beam b
+    const bool some = lane < B;
+    const int32_t len0 = a.lengths[beam0], len = some ? a.lengths[beam0 + lane] : len0;
+    const int32_t p = some ? a.parents[beam0 + lane] : -1;
+    const uint32_t tail = (uint32_t)(len0 < 0 ? 0 : len0) >> a.log_page, rows = (uint32_t)len0 & ((1u << a.log_page) - 1);
+    bool wrong = p < -1 || p >= (int32_t)B || len < 0 || len != len0 || (uint64_t)tail + (rows > 0) > a.width;
+    const bool off = __ballot(wrong) != 0;
+    int32_t page = 0;
+    if (!off && rows && some) {
+        page = a.tables[(beam0 + lane) * a.width + tail];
+        wrong = page < 0 || (uint64_t)page >= a.pages;
     }
-    if (__syncthreads_or(wrong != ~0ull)) {  // (every workgroup of the group finds the same)
-        if (wrong != ~0ull) report_error(a.err_word, bounds_key(wrong));
+    if (__ballot(wrong)) {  // (every wave of the group's workgroups finds the same)
+        if (wrong) report_error(a.err_word, bounds_key(beam0 + lane));
         return;
     }
-    if (tid < B) source[tid] = mine[from[tid]];
-    __syncthreads();
-    const uint32_t tail = tail_s, rows = rows_s;
+    const int32_t parent = p == -1 ? (int32_t)lane : p;
+    const uint32_t moved = (uint32_t)__ballot(some && parent != (int32_t)lane);
+    if (!moved) return;
     if (blockIdx.z == 0) {
         if (!a.last) return;  // (the tables are taken over by the last launch)
         for (uint32_t c = blockIdx.x * 256 + tid; c < tail; c += gridDim.x * 256) {
-            int32_t v[MB];
+            int32_t v[MB] = {};
 #pragma unroll
             for (int b = 0; b < MB; ++b)
-                if (b < (int)B) v[b] = a.tables[(beam0 + from[b]) * a.width + c];
+                if ((moved >> b) & 1) v[b] = a.tables[(beam0 + (uint32_t)__builtin_amdgcn_readlane(parent, b)) * a.width + c];
 #pragma unroll
             for (int b = 0; b < MB; ++b)
-                if (b < (int)B && from[b] != b) a.tables[(beam0 + b) * a.width + c] = v[b];
+                if ((moved >> b) & 1) a.tables[(beam0 + b) * a.width + c] = v[b];
         }
         return;
     }
     if (!rows) return;
     uint8_t* base = a.tensors[blockIdx.z - 1];
     const uint64_t stride = (blockIdx.z - 1) & 1 ? a.v_stride : a.k_stride;
+    const int32_t source = __shfl(page, some ? parent : 0, 64);
     // a plane's rows in use, as pieces of 16 bytes; Q8_0: and the scales' in pieces of 2
-    const uint32_t pieces = rows * a.row_bytes / 16, scales = rows * a.scale_bytes / 2, all = pieces + scales;
     const uint32_t plane = (a.row_bytes + a.scale_bytes) << a.log_page;
-    const uint64_t n = (uint64_t)a.kv_heads * all;
-    for (uint64_t i = blockIdx.x * 256ull + tid; i < n; i += gridDim.x * 256ull) {
-        const uint32_t h = (uint32_t)(i / all), r = (uint32_t)(i - (uint64_t)h * all);
-        const uint64_t at = (uint64_t)h * plane;
-        if (r < pieces) {
-            uint4 v[MB];
-#pragma unroll
-            for (int b = 0; b < MB; ++b)
-                if (b < (int)B && from[b] != b) v[b] = *(const uint4*)(base + (uint64_t)source[b] * stride + at + 16 * r);
-#pragma unroll
-            for (int b = 0; b < MB; ++b)
-                if (b < (int)B && from[b] != b) *(uint4*)(base + (uint64_t)mine[b] * stride + at + 16 * r) = v[b];
-        } else {
-            const uint64_t o = at + ((uint64_t)a.row_bytes << a.log_page) + 2 * (r - pieces);
-            uint16_t v[MB];
-#pragma unroll
-            for (int b = 0; b < MB; ++b)
-                if (b < (int)B && from[b] != b) v[b] = *(const uint16_t*)(base + (uint64_t)source[b] * stride + o);
-#pragma unroll
-            for (int b = 0; b < MB; ++b)
-                if (b < (int)B && from[b] != b) *(uint16_t*)(base + (uint64_t)mine[b] * stride + o) = v[b];
-        }
+    const uint32_t pieces = rows * a.row_bytes / 16, scales = rows * a.scale_bytes / 2;
+    for (uint32_t h = blockIdx.x; h < a.kv_heads * a.slices; h += gridDim.x) {
+        const uint32_t head = h / a.slices, slice = h - head * a.slices;
+        const uint64_t at = (uint64_t)head * plane;
+#pragma unroll 1
+        for (uint32_t i = slice * 256 + tid; i < pieces; i += a.slices * 256)
+            reorder_piece<MB, u32x4>(base + at + 16 * i, stride, page, source, moved);
+        const uint64_t after = at + ((uint64_t)a.row_bytes << a.log_page);
+#pragma unroll 1
+        for (uint32_t i = slice * 256 + tid; i < scales; i += a.slices * 256)
+            reorder_piece<MB, uint16_t>(base + after + 2 * i, stride, page, source, moved);
     }
 }
 
-hipError_t launch_beam_reorder(const ReorderArgs& a, hipStream_t s) {
+hipError_t launch_beam_reorder(ReorderArgs a, hipStream_t s) {
     if (a.groups == 0 || a.groups > 65535 || a.beams == 0 || a.beams > kReorderMaxBeams || a.n_tensors > 2 * kReorderLayers)
         return hipErrorInvalidValue;
-    const uint64_t pieces = (uint64_t)a.kv_heads * (a.row_bytes / 16 + a.scale_bytes / 2) << a.log_page;
-    uint64_t x = (pieces + 255) / 256;
-    x = x < 1 ? 1 : x > 1024 ? 1024 : x;
-    const dim3 grid((uint32_t)x, a.groups, 1 + a.n_tensors), block(256);
+    // a workgroup takes a head's plane, or a slice of it, so that there are some thousand of them
+    const uint64_t units = (uint64_t)a.groups * a.n_tensors * a.kv_heads, most = ((a.row_bytes << a.log_page) / 16 + 255) / 256;
+    a.slices = units >= 2048 ? 1 : (uint32_t)((2048 + units - 1) / units);
+    if (a.slices > most) a.slices = (uint32_t)most;
+    const dim3 grid(a.kv_heads * a.slices, a.groups, 1 + a.n_tensors), block(256);
     if (a.beams <= 4) hipLaunchKernelGGL(beam_reorder_kernel<4>, grid, block, 0, s, a);
     else if (a.beams <= 8) hipLaunchKernelGGL(beam_reorder_kernel<8>, grid, block, 0, s, a);
     else if (a.beams <= 16) hipLaunchKernelGGL(beam_reorder_kernel<16>, grid, block, 0, s, a);

@@ -317,10 +317,11 @@ struct ReorderArgs {
     uint32_t groups, beams, width, log_page, kv_heads, row_bytes, scale_bytes;
     uint64_t pages, k_stride, v_stride;
     uint32_t n_tensors, last;  // last: the launch that takes the tables over
+    uint32_t slices;  // of a head's plane
     unsigned long long* err_word;
     uint8_t* tensors[2 * kReorderLayers];
 };
-hipError_t launch_beam_reorder(const ReorderArgs& a, hipStream_t s);
+hipError_t launch_beam_reorder(ReorderArgs a, hipStream_t s);
 
 // ---- beam.hip ----
 constexpr uint32_t kSelectMaxBeams = 64, kSelectMaxBest = 64;
