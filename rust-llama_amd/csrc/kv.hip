@@ -14,29 +14,35 @@ namespace rlq {
 // Pages of the requests
 // ---------------------------------------------------------------------------
 
-constexpr uint32_t kPlanThreads = 1024, kPlanPer = kKvMaxRequests / kPlanThreads;
-
 // Why a request gets no pages (rlq.h, RLQ_INVALID_STATE of rlq_kv_pages).
 enum PagesRefusal : uint32_t { kBadCount = 0, kNoPage = 1, kNoColumn = 2, kNoRow = 3, kBadLength = 4 };
 
-// The sum over the threads before this one, and over all of them.
-__device__ __forceinline__ uint64_t plan_scan(uint64_t v, uint64_t* part, uint64_t& total) {
+// Three sums over the threads before this one, and over all.
+template <uint32_t N>
+__device__ __forceinline__ void plan_scan(uint64_t (&v)[3], uint64_t (&total)[3], uint64_t (*part)[3]) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t sum = v;
+    uint64_t sum[3] = {v[0], v[1], v[2]};
     for (int m = 1; m < 64; m <<= 1) {
-        const uint64_t o = __shfl_up(sum, m, 64);
-        if ((int)lane >= m) sum += o;
+        uint64_t o[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) o[k] = __shfl_up(sum[k], m, 64);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) sum[k] += (int)lane >= m ? o[k] : 0;
     }
-    __syncthreads();  // (part is free)
-    if (lane == 63) part[wave] = sum;
+    if (lane == 63)
+        for (int k = 0; k < 3; ++k) part[wave][k] = sum[k];
     __syncthreads();
-    uint64_t before = 0;
-    total = 0;
-    for (uint32_t w = 0; w < kPlanThreads / 64; ++w) {
-        if (w < wave) before += part[w];
-        total += part[w];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        uint64_t before = 0;
+        total[k] = 0;
+        for (uint32_t w = 0; w < N / 64; ++w) {
+            const uint64_t p = part[w][k];
+            before += w < wave ? p : 0;
+            total[k] += p;
+        }
+        v[k] = before + sum[k] - v[k];
     }
-    return before + sum - v;
 }
 
 // The last of the n + 1 ascending numbers that is not above v (at[0] = 0 <= v < at[n]).
@@ -51,7 +57,8 @@ __device__ __forceinline__ uint32_t segment_of(const P* at, uint32_t n, uint32_t
     return lo;
 }
 
-// Row t of the batch: its request, position and slot; -1 behind the last.
+// Row t of the batch: its request, position and slot; -1 behind the last.  after: the
+// requests' lengths with their new tokens.
 template <class P>
 __device__ __forceinline__ void pages_row(const PagesArgs& a, const P* starts, uint32_t total, uint32_t t, const int32_t* after) {
     int32_t request = -1, position = -1;
@@ -73,82 +80,96 @@ __device__ __forceinline__ void pages_row(const PagesArgs& a, const P* starts, u
 // list, pages off its top (request after request, the t-th from the top is the t-th
 // page taken), and, where `rows`, the batch's rows.  Everything is checked before
 // anything is written.
-__global__ __launch_bounds__(1024) void pages_plan_kernel(PagesArgs a, uint32_t rows) {
-    __shared__ uint64_t part[kPlanThreads / 64];
-    __shared__ uint32_t need[kKvMaxRequests + 1], start[kKvMaxRequests + 1], gone[kKvMaxRequests];
-    __shared__ uint16_t ended[kKvMaxRequests];
+//
+// N threads, PER requests each.
+template <uint32_t N, uint32_t PER>
+__global__ __launch_bounds__(N) void pages_plan_kernel(PagesArgs a, uint32_t rows) {
+    constexpr uint32_t kMost = N * PER, kWaves = N / 64;
+    __shared__ uint64_t part[kWaves][3];
+    __shared__ uint32_t need[kMost + 1], start[kMost + 1], gone[kMost];
+    __shared__ int32_t later[kMost];
+    __shared__ uint16_t ended[kMost];
     __shared__ uint32_t n_ended, first_bad;
     __shared__ unsigned long long bad_page;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.requests;
     const int64_t free0 = *a.count;
     if (tid == 0) n_ended = 0, first_bad = 0xffffffffu, bad_page = ~0ull;
+    // a request's columns of the table in use, the pages and the rows it gets
+    int32_t before[PER], more[PER];
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) {
+        const uint32_t r = tid * PER + i;
+        before[i] = r < n ? a.before[r] : 0;
+        more[i] = r < n ? a.more[r] : 0;
+    }
     __syncthreads();
 
-    // a request's columns of the table in use, the pages and the rows it gets
-    int32_t before[kPlanPer], more[kPlanPer];
-    uint64_t pages = 0, tokens = 0;
     uint32_t refused = 0xffffffffu;  // request * 8 + the reason
     auto refuse = [&](uint32_t r, uint32_t why) { refused = r * 8 + why < refused ? r * 8 + why : refused; };
     auto held = [&](int64_t len) { return (uint64_t)(len + (1 << a.log_page) - 1) >> a.log_page; };
+    uint64_t sums[3] = {}, totals[3];  // pages, rows, pages that come back
 #pragma unroll
-    for (uint32_t i = 0; i < kPlanPer; ++i) {
-        const uint32_t r = tid * kPlanPer + i;
-        before[i] = r < n ? a.before[r] : 0;
-        more[i] = r < n ? a.more[r] : 0;
+    for (uint32_t i = 0; i < PER; ++i) {
+        const uint32_t r = tid * PER + i;
         const int64_t after = (int64_t)before[i] + (more[i] > 0 ? more[i] : 0);
-        if (before[i] < 0 || after > 0x7fffffff) {
-            refuse(r, kBadLength);
-            before[i] = more[i] = 0;
-        } else if (held(after) > a.width) {
-            refuse(r, kNoColumn);
+        if (before[i] < 0 || after > 0x7fffffff || held(after) > a.width) {
+            refuse(r, before[i] < 0 || after > 0x7fffffff ? kBadLength : kNoColumn);
             before[i] = more[i] = 0;
         }
         if (r < n) {
             gone[r] = 0;
-            if (more[i] < 0) ended[atomicAdd(&n_ended, 1u)] = (uint16_t)r;
+            if (more[i] < 0 && before[i]) ended[atomicAdd(&n_ended, 1u)] = (uint16_t)r;
         }
-        if (more[i] > 0) pages += held(after) - held(before[i]), tokens += (uint32_t)more[i];
+        if (more[i] > 0) sums[0] += held(after) - held(before[i]), sums[1] += (uint32_t)more[i];
     }
     __syncthreads();
-    for (uint32_t i = wave; i < n_ended; i += kPlanThreads / 64) {  // (a wave per ended request)
-        const uint32_t r = ended[i];
-        const int32_t* row = a.owned + (uint64_t)r * a.width;
+    // a wave per ended request, 512 of its entries at a time
+    auto entries = [&](uint32_t r, auto&& take) {
+        const uint64_t row = (uint64_t)r * a.width;
         const uint32_t cols = (uint32_t)held(a.before[r]);
-        uint32_t some = 0;
-        for (uint32_t c = 0; c < cols; c += 64) {
-            const int32_t p = c + lane < cols ? row[c + lane] : -1;
-            if (p >= 0 && (uint32_t)p >= a.pages) atomicMin(&bad_page, (unsigned long long)r * a.width + c + lane);
-            some += (uint32_t)__builtin_popcountll(__ballot(p >= 0));
+        for (uint32_t c = lane; c < cols + lane; c += 512) {
+            int32_t p[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) p[k] = c + 64 * k < cols ? a.owned[row + c + 64 * k] : -1;
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) take(row + c + 64 * k, p[k]);
         }
-        if (lane == 0) gone[r] = some;
+    };
+    for (uint32_t i = wave; i < n_ended; i += kWaves) {
+        uint32_t some = 0;
+        entries(ended[i], [&](uint64_t at, int32_t p) {
+            if (p >= 0 && (uint32_t)p >= a.pages) atomicMin(&bad_page, (unsigned long long)at);
+            some += (uint32_t)__builtin_popcountll(__ballot(p >= 0));
+        });
+        if (lane == 0) gone[ended[i]] = some;
     }
-    __syncthreads();
-
-    uint64_t total_need, total_gone, total_rows, back = 0;
-    uint64_t at_need = plan_scan(pages, part, total_need), at_row = plan_scan(tokens, part, total_rows);
+    if (n_ended) __syncthreads();
 #pragma unroll
-    for (uint32_t i = 0; i < kPlanPer; ++i)
-        if (tid * kPlanPer + i < n) back += gone[tid * kPlanPer + i];
-    uint64_t at_gone = plan_scan(back, part, total_gone);
-    const bool sound = free0 >= 0 && free0 <= (int64_t)a.pages && (uint64_t)free0 + total_gone <= a.pages;
-    const uint64_t top = (sound ? (uint64_t)free0 : 0) + total_gone;
+    for (uint32_t i = 0; i < PER; ++i)
+        if (tid * PER + i < n) sums[2] += gone[tid * PER + i];
+    plan_scan<N>(sums, totals, part);
+    const bool sound = free0 >= 0 && free0 <= (int64_t)a.pages && (uint64_t)free0 + totals[2] <= a.pages;
+    const uint64_t top = (sound ? (uint64_t)free0 : 0) + totals[2];
     if (!sound) refuse(0, kBadCount);
+    auto cut = [](uint64_t v) { return (uint32_t)(v < 0xffffffffull ? v : 0xffffffffull); };
 #pragma unroll
-    for (uint32_t i = 0; i < kPlanPer; ++i) {
-        const uint32_t r = tid * kPlanPer + i;
+    for (uint32_t i = 0; i < PER; ++i) {
+        const uint32_t r = tid * PER + i;
         if (r >= n) break;
         const int64_t after = (int64_t)before[i] + (more[i] > 0 ? more[i] : 0);
-        need[r] = (uint32_t)(at_need < 0xffffffffull ? at_need : 0xffffffffull);
-        start[r] = (uint32_t)(at_row < 0xffffffffull ? at_row : 0xffffffffull);
+        need[r] = cut(sums[0]);
+        start[r] = cut(sums[1]);
+        later[r] = more[i] < 0 ? 0 : (int32_t)after;
         const uint32_t g = gone[r];
-        gone[r] = (uint32_t)(at_gone < 0xffffffffull ? at_gone : 0xffffffffull);
-        at_gone += g;
-        if (more[i] > 0) at_need += held(after) - held(before[i]), at_row += (uint32_t)more[i];
-        if (at_need > top) refuse(r, kNoPage);
-        if (at_row > a.tokens) refuse(r, kNoRow);
+        gone[r] = cut(sums[2]);
+        sums[2] += g;
+        if (more[i] > 0) sums[0] += held(after) - held(before[i]), sums[1] += (uint32_t)more[i];
+        if (sums[0] > top) refuse(r, kNoPage);
+        if (sums[1] > a.tokens) refuse(r, kNoRow);
     }
     if (refused != 0xffffffffu) atomicMin(&first_bad, refused);
-    if (tid == 0) need[n] = (uint32_t)total_need, start[n] = (uint32_t)total_rows;  // (not past 32 bits, or refused)
+    const uint32_t total_need = (uint32_t)totals[0], total_rows = (uint32_t)totals[1];  // (within 32 bits, or refused)
+    if (tid == 0) need[n] = total_need, start[n] = total_rows;
     __syncthreads();
     const bool bad = first_bad != 0xffffffffu || bad_page != ~0ull;
     if (tid == 0) {
@@ -158,52 +179,55 @@ __global__ __launch_bounds__(1024) void pages_plan_kernel(PagesArgs a, uint32_t 
     }
     if (bad) return;
 
-    for (uint32_t i = wave; i < n_ended; i += kPlanThreads / 64) {
-        const uint32_t r = ended[i], cols = (uint32_t)held(a.before[r]);
-        int32_t* row = a.owned + (uint64_t)r * a.width;
-        uint64_t to = (uint64_t)free0 + gone[r];
-        for (uint32_t c = 0; c < cols; c += 64) {
-            const int32_t p = c + lane < cols ? row[c + lane] : -1;
+    for (uint32_t i = wave; i < n_ended; i += kWaves) {
+        uint64_t to = (uint64_t)free0 + gone[ended[i]];
+        entries(ended[i], [&](uint64_t at, int32_t p) {
             const unsigned long long m = __ballot(p >= 0);
             if (p >= 0) {
                 a.free[to + __builtin_popcountll(m & ((1ull << lane) - 1))] = p;
-                row[c + lane] = -1;
+                a.owned[at] = -1;
             }
             to += __builtin_popcountll(m);
-        }
+        });
     }
-    __syncthreads();
-    for (uint32_t t = tid; t < (uint32_t)total_need; t += kPlanThreads) {
+    if (n_ended) __syncthreads();
+    for (uint32_t t = tid; t < total_need; t += N) {
         const uint32_t r = segment_of(need, n, t);
-        const uint64_t at = (uint64_t)r * a.width + held(a.before[r]) + (t - need[r]);
+        // (a request's last new page is that of its last token)
+        const uint64_t at = (uint64_t)r * a.width + held(later[r]) - (need[r + 1] - t);
         const int32_t p = a.free[top - 1 - t];
         a.tables[at] = p;
         if (a.owned != a.tables) a.owned[at] = p;
     }
-    __syncthreads();  // (the lengths may take the place of `before`)
+    if (n_ended || rows) __syncthreads();  // (the lengths may take the place of `before`; the rows read the tables)
 #pragma unroll
-    for (uint32_t i = 0; i < kPlanPer; ++i) {
-        const uint32_t r = tid * kPlanPer + i;
+    for (uint32_t i = 0; i < PER; ++i) {
+        const uint32_t r = tid * PER + i;
         if (r >= n) break;
-        a.after[r] = more[i] < 0 ? 0 : before[i] + more[i];
+        a.after[r] = later[r];
         a.starts[r] = (int32_t)start[r];
     }
     if (tid == 0) a.starts[n] = (int32_t)total_rows, *a.count_after = (int32_t)(top - total_need);
     if (!rows) return;
-    __syncthreads();
-    for (uint32_t t = tid; t < a.tokens; t += kPlanThreads) pages_row(a, start, (uint32_t)total_rows, t, a.after);
+    for (uint32_t t = tid; t < a.tokens; t += N) pages_row(a, start, total_rows, t, later);
 }
 
 __global__ __launch_bounds__(256) void pages_rows_kernel(PagesArgs a) {
+    __shared__ int32_t starts[kKvMaxRequests + 1];
+    for (uint32_t r = threadIdx.x; r <= a.requests; r += 256) starts[r] = a.starts[r];
+    const uint32_t refused = *a.refused;
+    __syncthreads();
     const uint32_t t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= a.tokens || *a.refused) return;
-    pages_row(a, a.starts, (uint32_t)a.starts[a.requests], t, a.after);
+    if (t < a.tokens && !refused) pages_row(a, starts, (uint32_t)starts[a.requests], t, a.after);
 }
 
 hipError_t launch_kv_pages(const PagesArgs& a, hipStream_t s) {
     if (a.requests == 0 || a.requests > kKvMaxRequests || a.tokens > 0x7fffffffu) return hipErrorInvalidValue;
     const bool one = a.tokens <= 4096;
-    hipLaunchKernelGGL(pages_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, one ? 1u : 0u);
+    if (a.requests <= 256 && a.tokens <= 1024)
+        hipLaunchKernelGGL((pages_plan_kernel<256, 1>), dim3(1), dim3(256), 0, s, a, 1u);
+    else
+        hipLaunchKernelGGL((pages_plan_kernel<1024, kKvMaxRequests / 1024>), dim3(1), dim3(1024), 0, s, a, one ? 1u : 0u);
     if (!one) hipLaunchKernelGGL(pages_rows_kernel, dim3((a.tokens + 255) / 256), dim3(256), 0, s, a);
     return hipGetLastError();
 }
