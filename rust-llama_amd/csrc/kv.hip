@@ -250,14 +250,170 @@ __device__ __forceinline__ uint32_t bf16_bits(float v) {  // ties to even; v is 
     return (b + 0x7fffu + ((b >> 16) & 1)) >> 16;
 }
 
-// A token's query, key and value heads, dim / 4 lanes a head and four values a lane.
-// The first 2 * half values of a query or key head are rotated:
+// N words at an address that is a multiple of A bytes.
+template <class W, int N, int A>
+struct __attribute__((packed, aligned(A))) Words {
+    W w[N];
+};
+template <class W, int N, int A>
+__device__ __forceinline__ void words(const void* p, W (&out)[N]) {
+    const Words<W, N, A> t = *(const Words<W, N, A>*)p;
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = t.w[i];
+}
+// sine and cosine of a by quarter turns: a - n pi/2 with pi/2 in two f64 (n below 2^38, so that what is
+// left out, n 2^-108, is far below a last bit), then the Taylor polynomials, whose
+// first terms left out are below 2^-60 for |r| <= pi/4.
+__device__ __forceinline__ double2 sine_cosine(double a) {
+    if (!(fabs(a) < 2.7e11)) {
+        double s, c;
+        sincos(a, &s, &c);
+        return make_double2(s, c);
+    }
+    const double n = __builtin_rint(a * 0.63661977236758134308);
+    double r = __builtin_fma(-n, 1.5707963267948965580, a);
+    r = __builtin_fma(-n, 6.1232339957367660359e-17, r);
+    const double z = r * r;
+    double s = 1.0 / 355687428096000.0, c = 1.0 / 20922789888000.0;  // 1 / 17!, 1 / 16!
+    s = __builtin_fma(s, z, -1.0 / 1307674368000.0);
+    c = __builtin_fma(c, z, -1.0 / 87178291200.0);
+    s = __builtin_fma(s, z, 1.0 / 6227020800.0);
+    c = __builtin_fma(c, z, 1.0 / 479001600.0);
+    s = __builtin_fma(s, z, -1.0 / 39916800.0);
+    c = __builtin_fma(c, z, -1.0 / 3628800.0);
+    s = __builtin_fma(s, z, 1.0 / 362880.0);
+    c = __builtin_fma(c, z, 1.0 / 40320.0);
+    s = __builtin_fma(s, z, -1.0 / 5040.0);
+    c = __builtin_fma(c, z, -1.0 / 720.0);
+    s = __builtin_fma(s, z, 1.0 / 120.0);
+    c = __builtin_fma(c, z, 1.0 / 24.0);
+    s = __builtin_fma(s, z, -1.0 / 6.0);
+    c = __builtin_fma(c, z, -0.5);
+    s = __builtin_fma(s * z, r, r);
+    c = __builtin_fma(c, z, 1.0);
+    const int64_t q = (int64_t)n;
+    const double u = q & 1 ? c : s, v = q & 1 ? s : c;
+    return make_double2(q & 2 ? -u : u, (q + 1) & 2 ? -v : v);
+}
+
+// Whether a stored value would be no finite number of the cache's type.
+template <uint32_t T>
+__device__ __forceinline__ bool store_off(float y) {
+    if constexpr (T == kF16) return !finite((float)(_Float16)y);
+    if constexpr (T == kBF16) return !finite(y) || !finite(__uint_as_float(bf16_bits(y) << 16));
+    return !finite(y);
+}
+// Four values from element e on of a token's place in a plane; Q8_0: by eight lanes, a block.
+template <uint32_t T>
+__device__ __forceinline__ void store_put(uint8_t* plane, uint64_t row, uint32_t e, uint32_t dim, uint32_t log_page,
+                                          const float (&y)[4]) {
+    uint8_t* to = plane + row * kv_row<T>(dim);
+    if constexpr (T == kF32) {
+        *(float4*)(to + 4 * e) = make_float4(y[0], y[1], y[2], y[3]);
+    } else if constexpr (T == kQ8_0) {
+        const NormQ q = norm_q8_0(y);
+        *(uint32_t*)(to + e) = q.q;
+        if (e % 32 == 0)
+            *(uint16_t*)(plane + ((uint64_t)dim << log_page) + 2 * (row * (dim / 32) + e / 32)) = (uint16_t)float_to_half_bits(q.d);
+    } else {
+        uint32_t b[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+            b[j] = T == kF16 ? (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)y[j]) : bf16_bits(y[j]);
+        *(uint2*)(to + 2 * e) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+    }
+}
+
+// A token's query, key and value heads.  The first 2 * half values of a query or key head are
+// rotated:
 //   (x, y) -> (x cos a - y sin a, x sin a + y cos a),  a = position * freq[i]
 // of neighbours (pairs) or of values half apart; angle, sine, cosine, products and sum in
 // f64, rounded once to f32, so that the stored 16 bits and levels are defined to the last
-// one.  A wave loads whole heads before it stores them: q_out may be q.
+// one.
+//
+// A workgroup of N threads per token, a thread U times four values.  All are loaded, with their partners,
+// before the angles are made and stored after every one has been checked: a token with an
+// error keeps its place, and q_out may be q.  Needs whole fours of rotated values (half a
+// multiple of 4, of pairs 2).
+template <uint32_t T, int N, int U>
+__global__ __launch_bounds__(N) void kv_store_kernel(StoreArgs a) {
+    __shared__ double2 turn[128];  // cosine, sine
+    const uint32_t tid = threadIdx.x, dim = a.c.dim, L = dim / 4, kv = a.c.kv_heads, units = (a.heads + 2 * kv) * L;
+    const uint64_t t = blockIdx.x;
+    const int64_t slot = a.slots[t];
+    const uint32_t magic = 0xffffffffu / L + 1;  // x / L = x magic >> 32 for x below 2^26
+    float x[U][4], o[U][4];
+    uint32_t head[U], e[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t i = tid + N * u < units ? tid + N * u : units - 1;
+        head[u] = __umulhi(i, magic);
+        e[u] = 4 * (i - head[u] * L);
+        const bool q = head[u] < a.heads, k = head[u] < a.heads + kv;
+        const float* p = q ? a.q + t * a.q_stride + (uint64_t)head[u] * dim
+                           : k ? a.k + t * a.k_stride + (uint64_t)(head[u] - a.heads) * dim
+                               : a.v + t * a.v_stride + (uint64_t)(head[u] - a.heads - kv) * dim;
+        words<float, 4, 4>(p + e[u], x[u]);
+        const bool turns = k && e[u] < 2 * a.half;
+        if (!a.pairs && turns) words<float, 4, 4>(p + (e[u] < a.half ? e[u] + a.half : e[u] - a.half), o[u]);
+        else o[u][0] = x[u][1], o[u][1] = x[u][0], o[u][2] = x[u][3], o[u][3] = x[u][2];
+    }
+    if (slot == -1) return;  // a row behind the batch's last
+    if (slot < 0 || (uint64_t)slot >= a.c.pages << a.c.log_page) {
+        if (tid == 0) report_error(a.err_word, bounds_key(t));
+        return;
+    }
+    if (tid < a.half) {
+        const double2 sc = sine_cosine((double)a.positions[t] * (double)a.freqs[tid]);
+        turn[tid] = make_double2(sc.y, sc.x);
+    }
+    __syncthreads();
+    int bad = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const bool q = head[u] < a.heads, k = head[u] < a.heads + kv, have = tid + N * u < units;
+        if (k && e[u] < 2 * a.half) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t i = e[u] + j;
+                const bool second = a.pairs ? j & 1 : i >= a.half;
+                const double2 cs = turn[a.pairs ? i / 2 : second ? i - a.half : i];
+                const double m = (double)x[u][j] * cs.x, r = (double)o[u][j] * cs.y;
+                x[u][j] = (float)(second ? r + m : m - r);
+            }
+        }
+        bool off = false;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) off |= q ? !finite(x[u][j]) : store_off<T>(x[u][j]);
+        bool scale = false;
+        if constexpr (T == kQ8_0) scale = !q && norm_q8_0(x[u]).bad;
+        if (have && (off || scale)) {
+            bad = 1;
+            const uint64_t at = (uint64_t)head[u] * dim + e[u];
+            report_error(a.err_word, off ? error_key(t, kKindNonFinite, at)
+                                         : error_key(t, kKindScale, (at - (uint64_t)a.heads * dim) / 32));
+        }
+    }
+    if (__syncthreads_or(bad)) return;
+    const uint64_t page = (uint64_t)slot >> a.c.log_page, row = (uint64_t)slot & ((1u << a.c.log_page) - 1);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (tid + N * u >= units) continue;
+        if (head[u] < a.heads) {
+            Words<float, 4, 4> y{{x[u][0], x[u][1], x[u][2], x[u][3]}};
+            *(Words<float, 4, 4>*)(a.q_out + t * a.out_stride + (uint64_t)head[u] * dim + e[u]) = y;
+        } else {
+            const uint32_t g = head[u] - a.heads;
+            uint8_t* base = g < kv ? a.c.k + page * a.c.k_stride : a.c.v + page * a.c.v_stride;
+            store_put<T>(base + (g < kv ? g : g - kv) * kv_plane<T>(dim, a.c.log_page), row, e[u], dim, a.c.log_page, x[u]);
+        }
+    }
+}
+
+// The same for any half and number of heads: dim / 4 lanes a head, a wave whole heads at a time, which it loads
+// before it stores them; the values are made twice, to be checked and to be stored.
 template <uint32_t T>
-__global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a) {
+__global__ __launch_bounds__(256) void kv_store_any_kernel(StoreArgs a) {
     __shared__ double2 turn[128];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, dim = a.c.dim;
     const uint64_t t = blockIdx.x;
@@ -268,9 +424,8 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a) {
         return;
     }
     if (threadIdx.x < a.half) {
-        double s, c;
-        sincos((double)a.positions[t] * (double)a.freqs[threadIdx.x], &s, &c);
-        turn[threadIdx.x] = make_double2(c, s);
+        const double2 sc = sine_cosine((double)a.positions[t] * (double)a.freqs[threadIdx.x]);
+        turn[threadIdx.x] = make_double2(sc.y, sc.x);
     }
     __syncthreads();
     const uint32_t L = dim / 4, per = 64 / L, group = lane / L, e = 4 * (lane % L);
@@ -295,9 +450,7 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a) {
                 const double m = (double)y[j] * cs.x, o = (double)x[other] * cs.y;
                 y[j] = (float)(second ? o + m : m - o);
             }
-            off |= !finite(y[j]);
-            if (T == kF16 && !q) off |= !finite((float)(_Float16)y[j]);
-            if (T == kBF16 && !q) off |= !finite(__uint_as_float(bf16_bits(y[j]) << 16));
+            off |= q ? !finite(y[j]) : store_off<T>(y[j]);
         }
         return off;
     };
@@ -326,37 +479,36 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs a) {
         const uint32_t g = h - a.heads < kv ? h - a.heads : h - a.heads - kv;
         uint8_t* plane = (h - a.heads < kv ? a.c.k + page * a.c.k_stride : a.c.v + page * a.c.v_stride) +
                          g * kv_plane<T>(dim, a.c.log_page);
-        uint8_t* to = plane + row * kv_row<T>(dim);
-        if constexpr (T == kF32) {
-            *(float4*)(to + 4 * e) = make_float4(y[0], y[1], y[2], y[3]);
-        } else if constexpr (T == kQ8_0) {
-            const NormQ q = norm_q8_0(y);
-            *(uint32_t*)(to + e) = q.q;
-            if (e % 32 == 0)
-                *(uint16_t*)(plane + ((uint64_t)dim << a.c.log_page) + 2 * (row * (dim / 32) + e / 32)) =
-                    (uint16_t)float_to_half_bits(q.d);
-        } else {
-            uint32_t b[4];
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j)
-                b[j] = T == kF16 ? (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)y[j]) : bf16_bits(y[j]);
-            *(uint2*)(to + 2 * e) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
-        }
+        store_put<T>(plane, row, e, dim, a.c.log_page, y);
     }
+}
+
+template <uint32_t T>
+static hipError_t store_launch(const StoreArgs& a, hipStream_t s) {
+    const uint64_t units = (uint64_t)(a.heads + 2 * a.c.kv_heads) * (a.c.dim / 4);
+    const dim3 grid((uint32_t)a.tokens);
+    // few tokens: large workgroups, one or two fours a thread
+    const bool few = a.tokens <= (uint64_t)device_cus(), whole = a.half % (a.pairs ? 2 : 4) == 0;
+    if (!whole || units > (few ? 4096 : 2048)) hipLaunchKernelGGL(kv_store_any_kernel<T>, grid, dim3(256), 0, s, a);
+    else if (few && units <= 1024) hipLaunchKernelGGL((kv_store_kernel<T, 1024, 1>), grid, dim3(1024), 0, s, a);
+    else if (few && units <= 2048) hipLaunchKernelGGL((kv_store_kernel<T, 1024, 2>), grid, dim3(1024), 0, s, a);
+    else if (few) hipLaunchKernelGGL((kv_store_kernel<T, 1024, 4>), grid, dim3(1024), 0, s, a);
+    else if (units <= 512) hipLaunchKernelGGL((kv_store_kernel<T, 256, 2>), grid, dim3(256), 0, s, a);
+    else if (units <= 1024) hipLaunchKernelGGL((kv_store_kernel<T, 256, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((kv_store_kernel<T, 256, 8>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
 }
 
 hipError_t launch_kv_store(const StoreArgs& a, hipStream_t s) {
     if (a.tokens == 0 || a.tokens > 0x7fffffffu || a.c.dim % 32 || a.c.dim > 256 || 2 * a.half > a.c.dim)
         return hipErrorInvalidValue;
-    const dim3 grid((uint32_t)a.tokens), block(256);
     switch (a.c.type) {
-        case kF32: hipLaunchKernelGGL(kv_store_kernel<kF32>, grid, block, 0, s, a); break;
-        case kF16: hipLaunchKernelGGL(kv_store_kernel<kF16>, grid, block, 0, s, a); break;
-        case kBF16: hipLaunchKernelGGL(kv_store_kernel<kBF16>, grid, block, 0, s, a); break;
-        case kQ8_0: hipLaunchKernelGGL(kv_store_kernel<kQ8_0>, grid, block, 0, s, a); break;
+        case kF32: return store_launch<kF32>(a, s);
+        case kF16: return store_launch<kF16>(a, s);
+        case kBF16: return store_launch<kBF16>(a, s);
+        case kQ8_0: return store_launch<kQ8_0>(a, s);
         default: return hipErrorInvalidValue;
     }
-    return hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------
@@ -367,17 +519,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-// N words at an address that is a multiple of A bytes.
-template <class W, int N, int A>
-struct __attribute__((packed, aligned(A))) Words {
-    W w[N];
-};
-template <class W, int N, int A>
-__device__ __forceinline__ void words(const void* p, W (&out)[N]) {
-    const Words<W, N, A> t = *(const Words<W, N, A>*)p;
-#pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = t.w[i];
-}
 constexpr int pow2_of(int n) { return n & -n; }
 
 __device__ __forceinline__ f32x4 mma_f16(const uint32_t (&a)[4], const uint32_t (&b)[4], f32x4 c) {
