@@ -581,6 +581,10 @@ __device__ __forceinline__ float column_sum(float v) {
 // 16-bit keys and values need 2 (f16) or 3 (bf16) times 256 cycles per 32 tokens of 128 values, of
 // about 1900 that HBM takes for them (one SIMD's share).  Q8_0: scores with f16 levels, block by block, times
 // the block's scale; values as f32 (level times scale, exact) on 16x16x4.
+// Blocks of 32 values to which two workgroups' registers fit a CU (a wave's tile, queries and
+// accumulators, 256 of them).
+constexpr uint32_t attn_wide(uint32_t type) { return type == kF32 ? 3 : 4; }
+
 template <uint32_t T, int NB>  // NB: blocks of 32 values
 struct AttnWave {
     static constexpr int kDim = 32 * NB, kOwn = 2 * NB;  // values of a token that a lane holds for O
@@ -598,30 +602,33 @@ struct AttnWave {
     uint32_t vw[8][T == kF32 ? kOwn : NB];  // (Q8_0: kOwn levels, two to a word)
     uint32_t ks[2][T == kQ8_0 ? 2 * NB : 1], vs[8];
 
-    __device__ __forceinline__ void start(const float* q, bool some, float scale) {
+    // The column's query: loaded, then (with the first keys on their way) made operands.
+    float raw[T == kF32 ? kOwn : NB][T == kF32 ? 4 : 8];
+    __device__ __forceinline__ void load_q(const float* q, bool some) {
         const uint32_t g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int c = 0; c < (T == kF32 ? kOwn : NB); ++c) {
+#pragma unroll
+            for (int j = 0; j < (T == kF32 ? 4 : 8); ++j) raw[c][j] = 0.0f;
+            if (some) words<float, (T == kF32 ? 4 : 8), 4>(q + (T == kF32 ? 16 * c + 4 * g : 32 * c + 8 * g), raw[c]);
+        }
+    }
+    __device__ __forceinline__ void start(float scale) {
         const float f = scale * 1.44269504088896340736f;  // exp(x) = 2^(x log2 e)
         m = -INFINITY, l = 0.0f, qe = 0;
 #pragma unroll
         for (int e = 0; e < kOwn; ++e) acc[e] = f32x4{0, 0, 0, 0};
         if constexpr (T == kF32) {
 #pragma unroll
-            for (int c = 0; c < kOwn; ++c) {
-                float x[4] = {};
-                if (some) words<float, 4, 4>(q + 16 * c + 4 * g, x);
+            for (int c = 0; c < kOwn; ++c)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) qf[c][j] = x[j] * f;
-            }
+                for (int j = 0; j < 4; ++j) qf[c][j] = raw[c][j] * f;
         } else {
-            float x[NB][8], top = 0.0f;
+            float top = 0.0f;
 #pragma unroll
-            for (int c = 0; c < NB; ++c) {
+            for (int c = 0; c < NB; ++c)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[c][j] = 0.0f;
-                if (some) words<float, 8, 4>(q + 32 * c + 8 * g, x[c]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[c][j] *= f, top = fmaxf(top, fabsf(x[c][j]));
-            }
+                for (int j = 0; j < 8; ++j) raw[c][j] *= f, top = fmaxf(top, fabsf(raw[c][j]));
             if constexpr (T != kBF16) {  // the largest to 2^13 .. 2^14
                 top = column_max(top);
                 const int e = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
@@ -629,12 +636,12 @@ struct AttnWave {
 #pragma unroll
                 for (int c = 0; c < NB; ++c)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[c][j] = __builtin_amdgcn_ldexpf(x[c][j], -qe);
+                    for (int j = 0; j < 8; ++j) raw[c][j] = __builtin_amdgcn_ldexpf(raw[c][j], -qe);
             }
 #pragma unroll
             for (int c = 0; c < NB; ++c) {
-                if constexpr (T == kBF16) split_bf16(x[c], q0[c], q1[c], q2[c]);
-                else split_f16(x[c], q0[c], q1[c]);
+                if constexpr (T == kBF16) split_bf16(raw[c], q0[c], q1[c], q2[c]);
+                else split_f16(raw[c], q0[c], q1[c]);
             }
         }
     }
@@ -790,19 +797,6 @@ struct AttnWave {
     }
 };
 
-// Tokens of a part: the units of all rows (parts times `per`) are to fill the slots of the
-// CUs once.  rows rows of `tokens` in all, the longest of `most`, make no more than
-// tokens / p + rows parts of p tokens; of many rows, which fill the slots as they are, the long ones
-// are cut to pieces of no more than twice the mean.  A row has 128 parts at most: one
-// workgroup joins them.
-__device__ __forceinline__ uint32_t attn_part(uint64_t tokens, uint32_t rows, uint32_t most, uint32_t slots, uint32_t per) {
-    const uint32_t s = slots / per + 1, half = s / 2 + 1, budget = s > rows && s - rows > half ? s - rows : half;
-    uint64_t p = (tokens + budget - 1) / budget;
-    if (p * kAttnParts < most) p = (most + kAttnParts - 1) / kAttnParts;
-    p = (p + 127) / 128 * 128;
-    return p < kAttnPart ? kAttnPart : (uint32_t)p;
-}
-
 __device__ __forceinline__ void attn_put(float* to, float x, float y) {
     const unsigned long long v = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
     const unsigned long long old =
@@ -815,73 +809,65 @@ __device__ __forceinline__ float2 attn_get(const float* from) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-// A workgroup takes units: a part of a row for up to 16 query heads of one KV head; its four
-// waves take every fourth 32 tokens of it and join in LDS.  The parts of a row are joined, in
-// order, by the last of them to arrive (published as the router's logits are: an exchange is
-// performed at the device's coherent level when it returns).
+// The tokens of all rows, in tiles of 128 row after row, are dealt evenly: slot j of a KV head (and of
+// 16 of its query heads) takes `share` tiles from j * share on, whatever rows they are of.  The slots of
+// all heads fill the CUs once.  A slot goes through the segments that it has of rows; four waves take 32 tokens
+// of every tile, and join in LDS.  A row that lies in one slot is written by it; of others each slot puts its part where
+// every workgroup can read it, and the last to arrive joins the parts in order (published as the
+// router's logits are: an exchange is performed at the device's coherent level when it returns).
+// So the order in which a row is added up follows from the call's rows alone, and a row of one tile (or
+// in one slot) is added up as if it were alone.
+//
+// The rows' tiles are counted by every workgroup: to 64 rows a lane each, else in LDS.
 template <uint32_t T, int NB>
-__global__ __launch_bounds__(256, NB <= (T == kF32 ? 3 : 4) ? 2 : 1) void kv_attention_kernel(AttnArgs a) {
-    constexpr uint32_t kDim = 32 * NB, kLine = kDim + 2;
-    __shared__ uint32_t start[kAttnRows + 1], sums[4], counts[4], longest[4];
-    __shared__ uint64_t totals[4];
+__global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_kernel(AttnArgs a) {
+    constexpr uint32_t kDim = 32 * NB, kLine = kDim + 2, kV = (kDim + 127) / 128;
+    __shared__ uint32_t start[kAttnRows + 1], sums[4];
     __shared__ int32_t firsts[kAttnRows], lasts[kAttnRows], of[kAttnRows];
     __shared__ __align__(16) float part[4][16][kLine];  // of a wave and column: values
     __shared__ float wave_m[4][16], wave_l[4][16];
     __shared__ uint32_t last_one;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, g = lane >> 4;
     const uint32_t group = a.heads / a.c.kv_heads, tiles = (group + 15) / 16, per = a.c.kv_heads * tiles;
-    const uint32_t line = (group < 16 ? group : 16) * (kDim + 2);  // floats of a unit's part
+    const uint32_t line = (group < 16 ? group : 16) * (kDim + 2);  // floats of a part
 
-    // the rows' tokens, then their parts
-    uint32_t len;
-    {
+    // a row's request (-1: left alone), first and last token
+    auto span = [&](uint32_t row, int32_t& request, int32_t& first, int32_t& last) {
+        request = a.requests ? a.requests[row] : (int32_t)row, last = a.positions[row];
+        first = a.window && (uint32_t)(last + 1) > a.window ? last + 1 - (int32_t)a.window : 0;
+        if (request >= 0 && (uint32_t)request < a.table_rows && last >= -1 && last < (int64_t)a.width << a.c.log_page) return;
+        if (request != -1) report_error(a.err_word, bounds_key(a.row0 + row));
+        request = -1;
+    };
+    auto tiles_of = [](int32_t first, int32_t last) { return last < 0 ? 1u : ((uint32_t)last >> 7) - ((uint32_t)first >> 7) + 1; };
+    const bool few = a.rows <= 64;
+    int32_t my_request = -1, my_first = 0, my_last = -1;  // few: of row `lane`
+    uint32_t my_start = 0, my_tiles = 0, total;
+    if (few) {
+        if (lane < a.rows) span(lane, my_request, my_first, my_last);
+        my_tiles = my_request >= 0 ? tiles_of(my_first, my_last) : 0;
+        const uint32_t sum = wave_scan_u32(my_tiles);
+        my_start = sum - my_tiles;
+        total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+    } else {
         constexpr uint32_t kMine = kAttnRows / 256;
-        uint64_t total = 0;
-        uint32_t live = 0, most = 0;
-#pragma unroll
-        for (uint32_t k = 0; k < kMine; ++k) {
-            const uint32_t row = tid * kMine + k;
-            if (row >= a.rows) break;
-            const int32_t request = a.requests ? a.requests[row] : (int32_t)row, last = a.positions[row];
-            const int32_t first = a.window && (uint32_t)(last + 1) > a.window ? last + 1 - (int32_t)a.window : 0;
-            const bool sound = request >= 0 && (uint32_t)request < a.table_rows && last >= -1 && last < (int64_t)a.width << a.c.log_page;
-            if (!sound && request != -1) report_error(a.err_word, bounds_key(a.row0 + row));
-            firsts[row] = first, lasts[row] = last, of[row] = sound ? request : -1;
-            if (!sound) continue;
-            const uint32_t n = (uint32_t)(last + 1 - first);
-            total += n, live += 1, most = n > most ? n : most;
-        }
-        for (int s = 1; s < 64; s <<= 1) {
-            total += __shfl_xor(total, s, 64);
-            live += (uint32_t)__shfl_xor((int)live, s, 64);
-            const uint32_t o = (uint32_t)__shfl_xor((int)most, s, 64);
-            most = o > most ? o : most;
-        }
-        if (lane == 0) totals[wave] = total, counts[wave] = live, longest[wave] = most;
-        __syncthreads();
-        total = 0, live = 0, most = 0;
-        for (uint32_t w = 0; w < 4; ++w) {
-            total += totals[w], live += counts[w];
-            most = longest[w] > most ? longest[w] : most;
-        }
-        len = attn_part(total, live, most, a.slots, per);
         uint32_t n[kMine], mine = 0;
 #pragma unroll
         for (uint32_t k = 0; k < kMine; ++k) {
             const uint32_t row = tid * kMine + k;
             n[k] = 0;
-            if (row < a.rows && of[row] >= 0) n[k] = lasts[row] < 0 ? 1 : (uint32_t)lasts[row] / len - (uint32_t)firsts[row] / len + 1;
+            if (row >= a.rows) continue;
+            int32_t request, first, last;
+            span(row, request, first, last);
+            firsts[row] = first, lasts[row] = last, of[row] = request;
+            n[k] = request >= 0 ? tiles_of(first, last) : 0;
             mine += n[k];
         }
-        uint32_t sum = mine;
-        for (int s = 1; s < 64; s <<= 1) {
-            const uint32_t o = (uint32_t)__shfl_up((int)sum, s, 64);
-            if ((int)lane >= s) sum += o;
-        }
+        uint32_t sum = wave_scan_u32(mine);
         if (lane == 63) sums[wave] = sum;
         __syncthreads();
-        for (uint32_t w = 0; w < wave; ++w) sum += sums[w];
         sum -= mine;
+        for (uint32_t w = 0; w < wave; ++w) sum += sums[w];
 #pragma unroll
         for (uint32_t k = 0; k < kMine; ++k) {
             const uint32_t row = tid * kMine + k;
@@ -890,47 +876,74 @@ __global__ __launch_bounds__(256, NB <= (T == kF32 ? 3 : 4) ? 2 : 1) void kv_att
             if (row + 1 == kAttnRows) start[kAttnRows] = sum;
         }
         __syncthreads();
+        total = start[a.rows];
     }
-    const uint64_t units = (uint64_t)start[a.rows] * per;
+    const uint32_t least = (total + a.slots - 1) / a.slots, share = least < kAttnShare ? kAttnShare : least;
+    const uint32_t slot = blockIdx.x / per, hc = blockIdx.x - slot * per, kvh = hc / tiles;
+    const uint32_t cols = group - 16 * (hc - kvh * tiles) < 16 ? group - 16 * (hc - kvh * tiles) : 16;
+    const uint32_t head0 = kvh * group + 16 * (hc - kvh * tiles);
+    const uint64_t plane = kvh * kv_plane<T>(kDim, a.c.log_page);
+    const uint32_t mask = (1u << a.c.log_page) - 1;
+    const uint64_t end64 = (uint64_t)(slot + 1) * share;
+    const uint32_t end = end64 < total ? (uint32_t)end64 : total;
 
-    for (uint64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-        const uint32_t u = (uint32_t)(unit / per), hc = (uint32_t)(unit - (uint64_t)u * per), kvh = hc / tiles, tile = hc - kvh * tiles;
-        const uint32_t row = segment_of(start, a.rows, u), split = u - start[row], parts = start[row + 1] - start[row];
-        const uint32_t cols = group - 16 * tile < 16 ? group - 16 * tile : 16, head0 = kvh * group + 16 * tile;
-        const int32_t request = of[row], first = firsts[row], last = lasts[row];
-        // tokens t0 .. t1 of this part
-        const int32_t from = (int32_t)(((uint32_t)first / len + split) * len);
-        const int32_t t0 = from > first ? from : first, t1 = (int64_t)from + len - 1 < last ? (int32_t)(from + len - 1) : last;
+    uint32_t next;
+    for (uint64_t tile = (uint64_t)slot * share; tile < end; tile = next) {
+        uint32_t row, row0, row1;
+        int32_t request, first, last;
+        if (few) {
+            row = 63 - (uint32_t)__builtin_clzll(__ballot(my_tiles > 0 && my_start <= tile));
+            row0 = (uint32_t)__builtin_amdgcn_readlane((int)my_start, (int)row);
+            row1 = row0 + (uint32_t)__builtin_amdgcn_readlane((int)my_tiles, (int)row);
+            request = __builtin_amdgcn_readlane(my_request, (int)row);
+            first = __builtin_amdgcn_readlane(my_first, (int)row), last = __builtin_amdgcn_readlane(my_last, (int)row);
+        } else {
+            row = (uint32_t)__builtin_amdgcn_readfirstlane((int)segment_of(start, a.rows, (uint32_t)tile));
+            row0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)start[row]);
+            row1 = (uint32_t)__builtin_amdgcn_readfirstlane((int)start[row + 1]);
+            request = __builtin_amdgcn_readfirstlane(of[row]);
+            first = __builtin_amdgcn_readfirstlane(firsts[row]), last = __builtin_amdgcn_readfirstlane(lasts[row]);
+        }
+        next = row1 < end ? row1 : end;
+        const uint32_t slot0 = row0 / share, parts = (row1 - 1) / share - slot0 + 1;
+        // tokens t0 .. t1 of this segment, from a tile's beginning on
+        const int64_t from = ((int64_t)((uint32_t)first >> 7) + (int64_t)(tile - row0)) << 7;
+        const int64_t to = from + ((int64_t)(next - tile) << 7) - 1;
+        const int64_t t0 = from > first ? from : first, t1 = to < last ? to : last;
 
         AttnWave<T, NB> w;
-        w.start(a.q + row * a.q_stride + (uint64_t)(head0 + i) * kDim, i < cols, a.scale);
         const int32_t* table = a.tables + (uint64_t)request * a.width;
-        const uint64_t plane = kvh * kv_plane<T>(kDim, a.c.log_page);
-        const uint32_t mask = (1u << a.c.log_page) - 1;
         bool lost = false;
-        for (int64_t c0 = t0 & ~31; c0 <= t1; c0 += 1024) {
-            // lane k: the page of the sixteen tokens from c0 + 16 k on
-            int32_t id = 0;
+        int32_t id = 0;
+        // lane k: the page of the sixteen tokens from c0 + 16 k on
+        auto pages = [&](int64_t c0) {
             const int64_t at = c0 + 16 * lane;
-            if (at <= t1 && at + 15 >= t0) {
-                id = table[at >> a.c.log_page];
-                if (id < 0 || (uint64_t)id >= a.c.pages) lost = true, id = 0;
-            }
-            auto page = [&](int64_t t) { return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(id, (int)((t - c0) >> 4)); };
+            id = 0;
+            if (at <= t1 && at + 15 >= t0) id = table[at >> a.c.log_page];
+        };
+        auto check = [&] {
+            if (id < 0 || (uint64_t)id >= a.c.pages) lost = true, id = 0;
+        };
+        int64_t c0 = from;
+        auto page = [&](int64_t t) { return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(id, (int)((t - c0) >> 4)); };
+        auto load_k = [&](int64_t t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                w.load_k(h, a.c.k + page(t + 16 * h) * a.c.k_stride + plane, (uint32_t)(t + 16 * h) & mask, a.c.log_page);
+        };
+        auto load_v = [&](int64_t t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                w.load_v(h, a.c.v + page(t + 16 * h) * a.c.v_stride + plane, (uint32_t)(t + 16 * h) & mask, a.c.log_page);
+        };
+        pages(c0);
+        w.load_q(a.q + row * a.q_stride + (uint64_t)(head0 + i) * kDim, i < cols);
+        check();
+        if (c0 + 32 * wave <= t1) load_k(c0 + 32 * wave), load_v(c0 + 32 * wave);
+        w.start(a.scale);
+        for (;;) {
             const int64_t c1 = c0 + 1023 < t1 ? c0 + 1023 : t1;
-            auto load_k = [&](int64_t t) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    w.load_k(h, a.c.k + page(t + 16 * h) * a.c.k_stride + plane, (uint32_t)(t + 16 * h) & mask, a.c.log_page);
-            };
-            auto load_v = [&](int64_t t) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    w.load_v(h, a.c.v + page(t + 16 * h) * a.c.v_stride + plane, (uint32_t)(t + 16 * h) & mask, a.c.log_page);
-            };
-            int64_t t = c0 + 32 * wave;
-            if (t <= c1) load_k(t), load_v(t);
-            for (; t <= c1; t += 128) {
+            for (int64_t t = c0 + 32 * wave; t <= c1; t += 128) {
                 const bool all = t >= t0 && t + 31 <= t1, more = t + 128 <= c1;
                 uint32_t seen = 0;
                 if (!all) {
@@ -948,8 +961,13 @@ __global__ __launch_bounds__(256, NB <= (T == kF32 ? 3 : 4) ? 2 : 1) void kv_att
                 w.products(s);
                 if (more) load_v(t + 128);
             }
+            if (c0 + 1024 > t1) break;
+            c0 += 1024;
+            pages(c0);
+            check();
+            if (c0 + 32 * wave <= t1) load_k(c0 + 32 * wave), load_v(c0 + 32 * wave);
         }
-        if (__ballot(lost)) {  // (every wave of a row's units finds its own; what is joined is then no number)
+        if (__ballot(lost)) {  // (every segment finds its own; what is joined is then no number)
             w.l = NAN;
             if (lane == 0) report_error(a.err_word, bounds_key(a.row0 + row));
         }
@@ -958,7 +976,7 @@ __global__ __launch_bounds__(256, NB <= (T == kF32 ? 3 : 4) ? 2 : 1) void kv_att
         w.l = column_sum(w.l);
         if (g == 0) wave_m[wave][i] = w.m, wave_l[wave][i] = w.l;
         __syncthreads();
-        float top = fmaxf(fmaxf(wave_m[0][i], wave_m[1][i]), fmaxf(wave_m[2][i], wave_m[3][i]));
+        const float top = fmaxf(fmaxf(wave_m[0][i], wave_m[1][i]), fmaxf(wave_m[2][i], wave_m[3][i]));
         const float f = w.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w.m - top);
         if (i < cols) {
 #pragma unroll
@@ -967,115 +985,120 @@ __global__ __launch_bounds__(256, NB <= (T == kF32 ? 3 : 4) ? 2 : 1) void kv_att
                 for (int r = 0; r < 4; ++r) part[wave][i][(4 * g + r) * (2 * NB) + e] = w.acc[e][r] * f;
         }
         __syncthreads();
-        // a wave takes every fourth column, a lane pairs of values
-        float* scratch = a.scratch + unit * line;
+        auto write = [&](uint32_t c, float (&y)[kV][2], float sum) {  // column c's values 2 lane + 128 k and the next
+            bool off = false;
+#pragma unroll
+            for (uint32_t k = 0; k < kV; ++k)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    y[k][j] = last < 0 ? 0.0f : y[k][j] / sum;
+                    off |= 2 * lane + 128 * k < kDim && !finite(y[k][j]);
+                }
+            if (__ballot(off)) {
+                if (lane == 0) report_error(a.err_word, model_key(a.row0 + row, kStAttnOut, 0));
+                return;
+            }
+            float* out = a.out + row * a.out_stride + (uint64_t)(head0 + c) * kDim;
+#pragma unroll
+            for (uint32_t k = 0; k < kV; ++k) {
+                const uint32_t d = 2 * lane + 128 * k;
+                if (d < kDim) out[d] = y[k][0], out[d + 1] = y[k][1];
+            }
+        };
+        // a wave takes every fourth column
+        auto scratch = [&](uint32_t k) {  // part k of the row; a slot ends one row that goes on and begins one
+            return a.scratch + (((uint64_t)hc * a.slots + slot0 + k) * 2 + (k == 0)) * line;
+        };
+        float* mine = scratch(slot - slot0);
         for (uint32_t c = wave; c < cols; c += 4) {
             const float ct = fmaxf(fmaxf(wave_m[0][c], wave_m[1][c]), fmaxf(wave_m[2][c], wave_m[3][c]));
-            float sum = 0.0f;
+            float sum = 0.0f, y[kV][2];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float l = wave_l[k][c];
                 sum += l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f(wave_m[k][c] - ct);  // (0: without tokens)
             }
-            float* out = a.out + row * a.out_stride + (uint64_t)(head0 + c) * kDim;
-            float y[(kDim + 127) / 128][2];
-            bool off = false;
 #pragma unroll
-            for (uint32_t k = 0; k < (kDim + 127) / 128; ++k) {
+            for (uint32_t k = 0; k < kV; ++k) {
                 const uint32_t d = 2 * lane + 128 * k;
-                y[k][0] = y[k][1] = 0.0f;
-                if (d >= kDim) continue;
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
-                    y[k][j] = (part[0][c][d + j] + part[1][c][d + j]) + (part[2][c][d + j] + part[3][c][d + j]);
-                if (parts > 1) {
-                    attn_put(scratch + c * (kDim + 2) + d, y[k][0], y[k][1]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) y[k][j] = last < 0 ? 0.0f : y[k][j] / sum, off |= !finite(y[k][j]);
-                }
+                    y[k][j] = d < kDim ? (part[0][c][d + j] + part[1][c][d + j]) + (part[2][c][d + j] + part[3][c][d + j]) : 0.0f;
             }
-            if (parts > 1) {
-                if (lane == 0) attn_put(scratch + c * (kDim + 2) + kDim, ct, sum);
-                continue;
-            }
-            if (__ballot(off)) {
-                if (lane == 0) report_error(a.err_word, model_key(a.row0 + row, kStAttnOut, 0));
+            if (parts == 1) {
+                write(c, y, sum);
                 continue;
             }
 #pragma unroll
-            for (uint32_t k = 0; k < (kDim + 127) / 128; ++k) {
-                const uint32_t d = 2 * lane + 128 * k;
-                if (d < kDim) out[d] = y[k][0], out[d + 1] = y[k][1];
-            }
+            for (uint32_t k = 0; k < kV; ++k)
+                if (2 * lane + 128 * k < kDim) attn_put(mine + c * (kDim + 2) + 2 * lane + 128 * k, y[k][0], y[k][1]);
+            if (lane == 0) attn_put(mine + c * (kDim + 2) + kDim, ct, sum);
         }
         __syncthreads();
         if (parts == 1) continue;
-        uint32_t* count = a.count + (uint64_t)row * per + hc;
         if (tid == 0) {
+            uint32_t* count = a.count + (uint64_t)hc * a.slots + slot0;
             const uint32_t old = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             last_one = old == parts - 1;
             if (last_one) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         __syncthreads();
         if (!last_one) continue;
-        // the row's parts in order
-        const uint64_t unit0 = (uint64_t)start[row] * per + hc, step = (uint64_t)per * line;
-        const float* parts0 = a.scratch + unit0 * line;
         for (uint32_t c = wave; c < cols; c += 4) {
-            const float* p = parts0 + c * (kDim + 2);
-            float ct = -INFINITY;
-            for (uint32_t k = lane; k < parts; k += 64) ct = fmaxf(ct, attn_get(p + k * step + kDim).x);
-            ct = wave_max_dpp(ct);
-            float sum = 0.0f, y[(kDim + 127) / 128][2] = {};
-            for (uint32_t k = 0; k < parts; ++k) {
-                const float2 ml = attn_get(p + k * step + kDim);
-                const float fk = __builtin_amdgcn_exp2f(ml.x - ct);  // (a part has tokens)
-                sum = __builtin_fmaf(ml.y, fk, sum);
+            const uint32_t at = c * (kDim + 2);
+            float2 ml[2];  // of parts `lane` and lane + 64
 #pragma unroll
-                for (uint32_t v = 0; v < (kDim + 127) / 128; ++v) {
-                    const uint32_t d = 2 * lane + 128 * v;
-                    if (d >= kDim) continue;
-                    const float2 x = attn_get(p + k * step + d);
-                    y[v][0] = __builtin_fmaf(x.x, fk, y[v][0]);
-                    y[v][1] = __builtin_fmaf(x.y, fk, y[v][1]);
+            for (uint32_t k = 0; k < 2; ++k)
+                ml[k] = lane + 64 * k < parts ? attn_get(scratch(lane + 64 * k) + at + kDim) : make_float2(-INFINITY, 0.0f);
+            float fs[2], sum, y[kV][2] = {};
+            for (uint32_t k0 = 0; k0 < parts; k0 += 4) {
+                float2 x[4][kV];
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k)
+#pragma unroll
+                    for (uint32_t v = 0; v < kV; ++v)
+                        x[k][v] = k0 + k < parts && 2 * lane + 128 * v < kDim ? attn_get(scratch(k0 + k) + at + 2 * lane + 128 * v)
+                                                                              : make_float2(0.0f, 0.0f);
+                if (k0 == 0) {
+                    const float ct = wave_max_dpp(fmaxf(ml[0].x, ml[1].x));
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) fs[k] = __builtin_amdgcn_exp2f(ml[k].x - ct);
+                    sum = wave_sum(ml[0].y * fs[0] + ml[1].y * fs[1]);
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    if (k0 + k >= parts) continue;
+                    const float fk = readlane_f(k0 + k < 64 ? fs[0] : fs[1], (int)((k0 + k) & 63));
+#pragma unroll
+                    for (uint32_t v = 0; v < kV; ++v) {
+                        y[v][0] = __builtin_fmaf(x[k][v].x, fk, y[v][0]);
+                        y[v][1] = __builtin_fmaf(x[k][v].y, fk, y[v][1]);
+                    }
                 }
             }
-            bool off = false;
-#pragma unroll
-            for (uint32_t v = 0; v < (kDim + 127) / 128; ++v)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) y[v][j] = y[v][j] / sum, off |= 2 * lane + 128 * v < kDim && !finite(y[v][j]);
-            if (__ballot(off)) {
-                if (lane == 0) report_error(a.err_word, model_key(a.row0 + row, kStAttnOut, 0));
-                continue;
-            }
-            float* out = a.out + row * a.out_stride + (uint64_t)(head0 + c) * kDim;
-#pragma unroll
-            for (uint32_t v = 0; v < (kDim + 127) / 128; ++v) {
-                const uint32_t d = 2 * lane + 128 * v;
-                if (d < kDim) out[d] = y[v][0], out[d + 1] = y[v][1];
-            }
+            write(c, y, sum);
         }
         __syncthreads();
     }
 }
 
-// Units of `rows` rows at most (attn_part: budget + rows parts, and one more of a row whose window
-// begins within a part).
-static uint64_t attn_units(const AttnArgs& a, uint64_t rows) {
-    const uint64_t tiles = (a.heads / a.c.kv_heads + 15) / 16, per = a.c.kv_heads * tiles;
-    return per * (a.slots / per + 2 + 2 * rows);
+// Slots of a KV head (and 16 of its query heads); the rows of a launch, whose tiles are counted in 32 bits.
+static uint32_t attn_slots(const AttnArgs& a) {
+    const uint32_t per = a.c.kv_heads * ((a.heads / a.c.kv_heads + 15) / 16);
+    const uint32_t wide = attn_wide(a.c.type), n = (a.c.dim / 32 <= wide ? 2u : 1u) * (uint32_t)device_cus() / per;
+    return n < 1 ? 1 : n < kAttnParts ? n : kAttnParts;
 }
-static uint32_t attn_slots() { return 2 * (uint32_t)device_cus(); }
-size_t kv_attention_bytes(AttnArgs a) {
-    a.slots = attn_slots();
-    const uint64_t group = a.heads / a.c.kv_heads;
-    return attn_units(a, a.rows < kAttnRows ? a.rows : kAttnRows) * (group < 16 ? group : 16) * (a.c.dim + 2) * sizeof(float);
+static uint32_t attn_rows(const AttnArgs& a) {
+    const uint64_t tokens = (uint64_t)a.width << a.c.log_page, tiles = (tokens < 1ull << 31 ? tokens : 1ull << 31) / 128 + 2;
+    const uint64_t n = 0xffffffffull / tiles;
+    return (uint32_t)(n < kAttnRows ? n : kAttnRows);
+}
+size_t kv_attention_bytes(const AttnArgs& a) {
+    const uint64_t group = a.heads / a.c.kv_heads, per = a.c.kv_heads * ((group + 15) / 16);
+    return per * attn_slots(a) * 2 * (group < 16 ? group : 16) * (a.c.dim + 2) * sizeof(float);
 }
 uint64_t kv_attention_counters(const AttnArgs& a) {
-    const uint64_t tiles = (a.heads / a.c.kv_heads + 15) / 16;
-    return (a.rows < kAttnRows ? a.rows : kAttnRows) * a.c.kv_heads * tiles;
+    return (uint64_t)a.c.kv_heads * ((a.heads / a.c.kv_heads + 15) / 16) * attn_slots(a);
 }
 
 template <uint32_t T, int NB>
@@ -1102,22 +1125,15 @@ hipError_t launch_kv_attention(AttnArgs a, hipStream_t s) {
     if (a.rows == 0 || a.rows > 65535 || a.heads == 0 || a.heads > 65535 || a.c.dim % 32 || a.c.dim > 256 ||
         a.heads % a.c.kv_heads)
         return hipErrorInvalidValue;
-    a.slots = attn_slots();
-    const uint32_t rows = a.rows;
-    const float* q = a.q;
-    float* out = a.out;
-    const int32_t *positions = a.positions, *requests = a.requests, *tables = a.tables;
-    for (uint32_t r = 0; r < rows; r += kAttnRows) {  // (the parts and counters are the same memory)
+    a.slots = attn_slots(a);
+    const uint32_t rows = a.rows, most = attn_rows(a), grid = (uint32_t)kv_attention_counters(a);
+    const AttnArgs all = a;
+    for (uint32_t r = 0; r < rows; r += most) {  // (the parts and counters are the same memory)
         a.row0 = r;
-        a.rows = rows - r < kAttnRows ? rows - r : kAttnRows;
-        a.q = q + r * a.q_stride, a.out = out + r * a.out_stride;
-        a.positions = positions + r;
-        a.requests = requests ? requests + r : nullptr;
-        const uint64_t units = attn_units(a, a.rows), most = 8ull * device_cus();
-        const uint32_t grid = (uint32_t)(units < most ? units : most);
-        if (!requests) {  // row t is request t
-            a.tables = tables + (uint64_t)r * a.width;
-        }
+        a.rows = rows - r < most ? rows - r : most;
+        a.q = all.q + r * a.q_stride, a.out = all.out + r * a.out_stride, a.positions = all.positions + r;
+        if (all.requests) a.requests = all.requests + r;
+        else a.tables = all.tables + (uint64_t)r * a.width, a.table_rows = all.table_rows - r;  // (row t is request t)
         hipError_t e;
         switch (a.c.type) {
             case kF32: e = attn_dims<kF32>(a, grid, s); break;

@@ -190,6 +190,18 @@ __device__ __forceinline__ double wave_max_f64(double v) {
     v = up(v, dpp_d<kRowRor8>(v));
     return up(up(readlane_d(v, 0), readlane_d(v, 16)), up(readlane_d(v, 32), readlane_d(v, 48)));
 }
+// The sum over the lanes up to this one (call it with every lane active).
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
+    constexpr int kRowShr = 0x110, kRowBcast15 = 0x142, kRowBcast31 = 0x143;
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kRowShr + 1, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kRowShr + 2, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kRowShr + 4, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kRowShr + 8, 0xf, 0xf, false);
+    // the rows' last lanes into the rows behind them (1 and 3, then 2 and 3)
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kRowBcast15, 0xa, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kRowBcast31, 0xc, 0xf, false);
+    return v;
+}
 __device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {
     for (int m = 1; m < 64; m <<= 1) {
         const uint32_t o = (uint32_t)__shfl_xor((int)v, m, 64);

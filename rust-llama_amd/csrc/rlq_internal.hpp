@@ -291,8 +291,9 @@ struct StoreArgs {
     unsigned long long* err_word;
 };
 hipError_t launch_kv_store(const StoreArgs& a, hipStream_t s);
-// Attention: a row's tokens in parts, the rows of a launch at most.
-constexpr uint32_t kAttnPart = 256, kAttnParts = 128, kAttnRows = 1024;
+// Attention: tiles of 128 tokens a slot takes at least, slots of a head at most (one workgroup
+// joins a row's parts), rows of a launch at most.
+constexpr uint32_t kAttnShare = 1, kAttnParts = 128, kAttnRows = 1024;
 struct AttnArgs {
     KvLayer c;
     const float* q;
@@ -304,9 +305,9 @@ struct AttnArgs {
     unsigned long long* err_word;
     float* scratch;   // kv_attention_bytes
     uint32_t* count;  // kv_attention_counters words, 0 between launches
-    uint32_t slots, row0;  // of a launch: workgroups that run at once, the first row
+    uint32_t slots, row0;  // of a launch: slots of a head, the first row
 };
-size_t kv_attention_bytes(AttnArgs a);
+size_t kv_attention_bytes(const AttnArgs& a);
 uint64_t kv_attention_counters(const AttnArgs& a);
 hipError_t launch_kv_attention(AttnArgs a, hipStream_t s);
 // The beams' tables and part-filled pages after a choice; tensors: k, v, k, v, ...
