@@ -580,7 +580,9 @@ __device__ __forceinline__ float column_sum(float v) {
 // so the products are those of f32 with the stored values; the matrix cores have room for that:
 // 16-bit keys and values need 2 (f16) or 3 (bf16) times 256 cycles per 32 tokens of 128 values, of
 // about 1900 that HBM takes for them (one SIMD's share).  Q8_0: scores with f16 levels, block by block, times
-// the block's scale; values as f32 (level times scale, exact) on 16x16x4.
+// the block's scale; a value, level times scale, as the sum of two f16, which holds it exactly: a product of 18
+// bits that is a multiple of 2^-24, 127 times a scale of 515 at most (with a larger scale among
+// them the 32 tokens take f32 values on 16x16x4, 2048 cycles of the matrix cores instead of 384).
 // Blocks of 32 values to which two workgroups' registers fit a CU (a wave's tile, queries and
 // accumulators, 256 of them).
 constexpr uint32_t attn_wide(uint32_t type) { return type == kF32 ? 3 : 4; }
@@ -589,7 +591,7 @@ template <uint32_t T, int NB>  // NB: blocks of 32 values
 struct AttnWave {
     static constexpr int kDim = 32 * NB, kOwn = 2 * NB;  // values of a token that a lane holds for O
     static constexpr bool k16 = T == kF16 || T == kBF16;
-    static constexpr float kTop = T == kF16 ? 14.0f : 0.0f;  // weights are 2^kTop times exp(s - max)
+    static constexpr float kTop = T == kF16 || T == kQ8_0 ? 14.0f : 0.0f;  // weights are 2^kTop times exp(s - max)
 
     // q (columns past the last head 0): f32, or in terms
     uint32_t q0[T == kF32 ? 1 : NB][4], q1[T == kF32 ? 1 : NB][4], q2[T == kBF16 ? NB : 1][4];
@@ -599,7 +601,8 @@ struct AttnWave {
     f32x4 acc[kOwn]; // of column i: values (4g + r) * kOwn + e in [e][r]
     // a tile on its way
     uint32_t kw[2][T == kF32 ? kOwn : NB][T == kQ8_0 ? 2 : 4];
-    uint32_t vw[8][T == kF32 ? kOwn : NB];  // (Q8_0: kOwn levels, two to a word)
+    static constexpr int kWords = T == kF32 ? kOwn : T == kQ8_0 ? (NB + 1) / 2 : NB;
+    uint32_t vw[8][kWords];
     uint32_t ks[2][T == kQ8_0 ? 2 * NB : 1], vs[8];
 
     // The column's query: loaded, then (with the first keys on their way) made operands.
@@ -667,18 +670,21 @@ struct AttnWave {
             const uint32_t at = row + 4 * g + j;
             const uint8_t* p = plane + at * (uint32_t)kv_row<T>(kDim);
             if constexpr (T == kQ8_0) {
-                uint16_t t[NB];
-                words<uint16_t, NB, pow2_of(2 * NB)>(p + i * kOwn, t);
+                if constexpr (NB % 2 == 0) {
+                    words<uint32_t, kWords, pow2_of(2 * NB)>(p + i * kOwn, vw[4 * h + j]);
+                } else {
+                    uint16_t t[NB];
+                    words<uint16_t, NB, 2>(p + i * kOwn, t);
 #pragma unroll
-                for (int k = 0; k < NB; ++k) vw[4 * h + j][k] = t[k];
+                    for (int k = 0; k < kWords; ++k) vw[4 * h + j][k] = t[2 * k] | (2 * k + 1 < NB ? (uint32_t)t[(2 * k + 1) % NB] << 16 : 0);
+                }
                 // the scale of the lane's first value, and that of its last
                 const uint8_t* s = plane + ((uint32_t)kDim << log_page) + at * (2 * NB);
                 const uint32_t b = i * kOwn / 32, c = (i * kOwn + kOwn - 1) / 32;
                 vs[4 * h + j] = *(const uint16_t*)(s + 2 * b);
                 if constexpr (32 % kOwn != 0) vs[4 * h + j] |= (uint32_t)*(const uint16_t*)(s + 2 * c) << 16;
             } else {
-                constexpr int n = T == kF32 ? kOwn : NB;
-                words<uint32_t, n, pow2_of(4 * n) < 16 ? pow2_of(4 * n) : 16>(p + i * (4 * n), vw[4 * h + j]);
+                words<uint32_t, kWords, pow2_of(4 * kWords) < 16 ? pow2_of(4 * kWords) : 16>(p + i * (4 * kWords), vw[4 * h + j]);
             }
         }
     }
@@ -757,7 +763,7 @@ struct AttnWave {
         for (int t = 0; t < 8; ++t) {
             if ((seen >> t) & 1) continue;
 #pragma unroll
-            for (int k = 0; k < (T == kF32 ? kOwn : NB); ++k) vw[t][k] = 0;
+            for (int k = 0; k < kWords; ++k) vw[t][k] = 0;
             vs[t] = 0;
         }
     }
@@ -776,8 +782,45 @@ struct AttnWave {
                 if constexpr (T == kF16) acc[e] = mma_f16(a, p1, mma_f16(a, p0, acc[e]));
                 else acc[e] = mma_bf16(a, p2, mma_bf16(a, p1, mma_bf16(a, p0, acc[e])));
             }
-        } else {
-            const uint32_t i = threadIdx.x & 15;
+            return;
+        }
+        const uint32_t i = threadIdx.x & 15;
+        // whether value e has the scale of the lane's first value
+        auto same = [&](int e) { return 32 % kOwn == 0 || (i * kOwn + e) / 32 == i * kOwn / 32; };
+        if constexpr (T == kQ8_0) {
+            uint32_t top = 0;  // exponents and signs as they are: a scale is not negative
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const uint32_t x = vs[t] & 0xffffu, y = vs[t] >> 16;
+                top = x > top ? x : top;
+                if (32 % kOwn != 0) top = y > top ? y : top;
+            }
+            if (!__ballot(top > 0x6007u)) {  // f16 515.5
+                uint32_t p0[4], p1[4], d0[4], d1[4];
+                split_f16(p, p0, p1);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    d0[k] = __builtin_amdgcn_perm(vs[2 * k + 1], vs[2 * k], 0x05040100u);
+                    d1[k] = 32 % kOwn != 0 ? __builtin_amdgcn_perm(vs[2 * k + 1], vs[2 * k], 0x07060302u) : 0;
+                }
+#pragma unroll
+                for (int e = 0; e < kOwn; ++e) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t b = __builtin_amdgcn_perm(vw[2 * k + 1][e / 4], vw[2 * k][e / 4], 0x0c040c00u + (e % 4) * 0x10001u);
+                        const f16x2 q = __builtin_bit_cast(f16x2, b ^ 0x64806480u) - (_Float16)1152.0f;
+                        const f16x2 d = __builtin_bit_cast(f16x2, same(e) ? d0[k] : d1[k]);
+                        const f16x2 v = q * d;
+                        hi[k] = __builtin_bit_cast(uint32_t, v);
+                        lo[k] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(q, d, -v));
+                    }
+                    acc[e] = mma_f16(lo, p0, mma_f16(hi, p1, mma_f16(hi, p0, acc[e])));
+                }
+                return;
+            }
+        }
+        {
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 const float s0 = half_to_float(vs[t]), s1 = half_to_float(vs[t] >> 16);
@@ -787,8 +830,7 @@ struct AttnWave {
                     if constexpr (T == kF32) {
                         v = __uint_as_float(vw[t][e]);
                     } else {
-                        const float q = (float)(int8_t)(vw[t][e / 2] >> (8 * (e % 2)));
-                        v = q * (32 % kOwn == 0 || (i * kOwn + e) / 32 == i * kOwn / 32 ? s0 : s1);
+                        v = (float)(int8_t)(vw[t][e / 4] >> (8 * (e % 4))) * (same(e) ? s0 : s1);
                     }
                     acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[t], acc[e], 0, 0, 0);
                 }
@@ -822,7 +864,7 @@ __device__ __forceinline__ float2 attn_get(const float* from) {
 template <uint32_t T, int NB>
 __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_kernel(AttnArgs a) {
     constexpr uint32_t kDim = 32 * NB, kLine = kDim + 2, kV = (kDim + 127) / 128;
-    __shared__ uint32_t start[kAttnRows + 1], sums[4];
+    __shared__ uint32_t start[kAttnRows + 1], sums[4], mosts[4];
     __shared__ int32_t firsts[kAttnRows], lasts[kAttnRows], of[kAttnRows];
     __shared__ __align__(16) float part[4][16][kLine];  // of a wave and column: values
     __shared__ float wave_m[4][16], wave_l[4][16];
@@ -842,16 +884,16 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
     auto tiles_of = [](int32_t first, int32_t last) { return last < 0 ? 1u : ((uint32_t)last >> 7) - ((uint32_t)first >> 7) + 1; };
     const bool few = a.rows <= 64;
     int32_t my_request = -1, my_first = 0, my_last = -1;  // few: of row `lane`
-    uint32_t my_start = 0, my_tiles = 0, total;
+    uint32_t my_start = 0, my_tiles = 0, total, longest;
     if (few) {
         if (lane < a.rows) span(lane, my_request, my_first, my_last);
         my_tiles = my_request >= 0 ? tiles_of(my_first, my_last) : 0;
         const uint32_t sum = wave_scan_u32(my_tiles);
         my_start = sum - my_tiles;
-        total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63), longest = wave_max_u32(my_tiles);
     } else {
         constexpr uint32_t kMine = kAttnRows / 256;
-        uint32_t n[kMine], mine = 0;
+        uint32_t n[kMine], mine = 0, most = 0;
 #pragma unroll
         for (uint32_t k = 0; k < kMine; ++k) {
             const uint32_t row = tid * kMine + k;
@@ -861,12 +903,15 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
             span(row, request, first, last);
             firsts[row] = first, lasts[row] = last, of[row] = request;
             n[k] = request >= 0 ? tiles_of(first, last) : 0;
-            mine += n[k];
+            mine += n[k], most = n[k] > most ? n[k] : most;
         }
         uint32_t sum = wave_scan_u32(mine);
-        if (lane == 63) sums[wave] = sum;
+        most = wave_max_u32(most);
+        if (lane == 63) sums[wave] = sum, mosts[wave] = most;
         __syncthreads();
         sum -= mine;
+        longest = 0;
+        for (uint32_t w = 0; w < 4; ++w) longest = mosts[w] > longest ? mosts[w] : longest;
         for (uint32_t w = 0; w < wave; ++w) sum += sums[w];
 #pragma unroll
         for (uint32_t k = 0; k < kMine; ++k) {
@@ -878,7 +923,12 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
         __syncthreads();
         total = start[a.rows];
     }
-    const uint32_t least = (total + a.slots - 1) / a.slots, share = least < kAttnShare ? kAttnShare : least;
+    // (a row of more than kAttnParts parts would keep the one that joins them; and 32 parts of one tile are joined
+    // in the time that 16 of two take more: 4000 tokens of two KV heads of 64 13.4 us and 11.9, 16 rows of
+    // 4096 with one of 128 18.7 and 15.6)
+    const uint32_t least = (total + a.slots - 1) / a.slots;
+    const uint32_t row_least = longest > 16 && longest < 2 * kAttnParts ? 2 : (longest + kAttnParts - 1) / kAttnParts;
+    const uint32_t share = least < row_least ? row_least : least < 1 ? 1 : least;
     const uint32_t slot = blockIdx.x / per, hc = blockIdx.x - slot * per, kvh = hc / tiles;
     const uint32_t cols = group - 16 * (hc - kvh * tiles) < 16 ? group - 16 * (hc - kvh * tiles) : 16;
     const uint32_t head0 = kvh * group + 16 * (hc - kvh * tiles);
@@ -1044,6 +1094,7 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
         }
         __syncthreads();
         if (!last_one) continue;
+        constexpr uint32_t kBatch = 8 / kV;  // parts on their way
         for (uint32_t c = wave; c < cols; c += 4) {
             const uint32_t at = c * (kDim + 2);
             float2 ml[2];  // of parts `lane` and lane + 64
@@ -1051,10 +1102,10 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
             for (uint32_t k = 0; k < 2; ++k)
                 ml[k] = lane + 64 * k < parts ? attn_get(scratch(lane + 64 * k) + at + kDim) : make_float2(-INFINITY, 0.0f);
             float fs[2], sum, y[kV][2] = {};
-            for (uint32_t k0 = 0; k0 < parts; k0 += 4) {
-                float2 x[4][kV];
+            for (uint32_t k0 = 0; k0 < parts; k0 += kBatch) {
+                float2 x[kBatch][kV];
 #pragma unroll
-                for (uint32_t k = 0; k < 4; ++k)
+                for (uint32_t k = 0; k < kBatch; ++k)
 #pragma unroll
                     for (uint32_t v = 0; v < kV; ++v)
                         x[k][v] = k0 + k < parts && 2 * lane + 128 * v < kDim ? attn_get(scratch(k0 + k) + at + 2 * lane + 128 * v)
@@ -1066,7 +1117,7 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
                     sum = wave_sum(ml[0].y * fs[0] + ml[1].y * fs[1]);
                 }
 #pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) {
+                for (uint32_t k = 0; k < kBatch; ++k) {
                     if (k0 + k >= parts) continue;
                     const float fk = readlane_f(k0 + k < 64 ? fs[0] : fs[1], (int)((k0 + k) & 63));
 #pragma unroll
@@ -1086,7 +1137,7 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
 static uint32_t attn_slots(const AttnArgs& a) {
     const uint32_t per = a.c.kv_heads * ((a.heads / a.c.kv_heads + 15) / 16);
     const uint32_t wide = attn_wide(a.c.type), n = (a.c.dim / 32 <= wide ? 2u : 1u) * (uint32_t)device_cus() / per;
-    return n < 1 ? 1 : n < kAttnParts ? n : kAttnParts;
+    return n < 1 ? 1 : n;
 }
 static uint32_t attn_rows(const AttnArgs& a) {
     const uint64_t tokens = (uint64_t)a.width << a.c.log_page, tiles = (tokens < 1ull << 31 ? tokens : 1ull << 31) / 128 + 2;

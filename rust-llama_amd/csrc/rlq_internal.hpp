@@ -291,9 +291,8 @@ struct StoreArgs {
     unsigned long long* err_word;
 };
 hipError_t launch_kv_store(const StoreArgs& a, hipStream_t s);
-// Attention: tiles of 128 tokens a slot takes at least, slots of a head at most (one workgroup
-// joins a row's parts), rows of a launch at most.
-constexpr uint32_t kAttnShare = 1, kAttnParts = 128, kAttnRows = 1024;
+// Attention: parts of a row at most (one workgroup joins them), rows of a launch at most.
+constexpr uint32_t kAttnParts = 128, kAttnRows = 1024;
 struct AttnArgs {
     KvLayer c;
     const float* q;

@@ -73,7 +73,7 @@ def tolerance(dim, spread, most):
 
 
 def attend(ctx, rng, dtype, rows, heads, kv, dim, page, longest, window=0, scale=None, positions=None, requests=None,
-           table_rows=None, even=False, spread_pages=1):
+           table_rows=None, even=False, spread_pages=1, size=1.0):
     table_rows = table_rows or rows
     width = max(1, -(-max(longest, 1) // page))
     pool = table_rows * width
@@ -82,7 +82,7 @@ def attend(ctx, rng, dtype, rows, heads, kv, dim, page, longest, window=0, scale
         cache = rlq.KvCache(base[0][:, 1], base[1][:, 0], dtype, page, dim)
     else:
         cache = rlq.KvCache.make(dtype, pool, kv, page, dim)
-    k, v = fill(rng, cache)
+    k, v = fill(rng, cache, size)
     tables = rng.permutation(pool).astype(np.int32).reshape(table_rows, width)
     if positions is None:
         positions = np.full(rows, longest - 1) if even else rng.integers(-1, longest, rows)
@@ -167,6 +167,24 @@ def test_attention_far_scores_and_scales(ctx):
         for scale in (3.0, 0.001, -0.5):
             say("attention scale", dtype, scale)
             attend(ctx, rng, dtype, 3, 4, 2, 64, 16, 200, scale=scale)
+
+
+@pytest.mark.parametrize("dtype,size", [(DT.F16, 1e-6), (DT.F16, 1e4), (DT.BF16, 1e-30), (DT.BF16, 1e20), (DT.F32, 1e-30),
+                                        (DT.F32, 1e15), (DT.Q8_0, 1e-3), (DT.Q8_0, 1e4), (DT.Q8_0, 1e6)])
+def test_attention_of_small_and_large_values(ctx, dtype, size):
+    """Keys and values of f16's subnormal range, near the types' ends, and 8-bit blocks whose scales are
+    f16 subnormals, beyond 515 (where level times scale leaves f16), or near f16's largest."""
+    say("attention value size", dtype, size)
+    rng = np.random.default_rng(14)
+    for dim in (64, 96):
+        attend(ctx, rng, dtype, 3, 6, 2, dim, 16, 150, scale=0.1 / size, size=size)
+
+
+def test_attention_of_scales_beyond_f16(ctx):
+    """Blocks with a value beyond 127 times f16's largest have an infinite scale: no finite result, and said so."""
+    say("attention infinite scales")
+    with raises("NonFinite", 6), np.errstate(all="ignore"):
+        attend(ctx, np.random.default_rng(14), DT.Q8_0, 3, 6, 2, 64, 16, 150, scale=0.1 / 2e6, size=2e6)
 
 
 @pytest.mark.parametrize("dtype", [DT.F16, DT.BF16, DT.F32])
