@@ -14,8 +14,8 @@ namespace rlq {
 // Floats as whole numbers of the same order (-0 as 0).
 constexpr uint32_t kLeast = 0x00800000u;  // of the floats above -infinity
 __device__ __forceinline__ uint32_t beam_key(float z) {
-    const uint32_t b = __float_as_uint(z == 0.0f ? 0.0f : z);
-    return (b >> 31) ? ~b : b | 0x80000000u;
+    const uint32_t b = __float_as_uint(z + 0.0f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float beam_value(uint32_t key) {
     return __uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
@@ -57,23 +57,103 @@ __device__ __forceinline__ float beam_exp(float x) {
     return __builtin_fmaf(p, r * 0.693147181f, p);
 }
 
+constexpr uint32_t kOnceBeams = 8;     // of a group whose chunks one workgroup merges
 constexpr uint32_t kWaveMost = 256;  // candidates that a wave puts down at once
-constexpr uint32_t kListMost = kSelectMaxBest + 4 * kWaveMost;
+constexpr uint32_t kListMost = kSelectMaxBest + kWaveMost;  // of a wave's list
 
-// A workgroup per chunk of a beam's row, 4 U logits a thread at a time in registers.
-//   Sum: every wave about its own maximum.
-//   Best: of the maxima of a lane's quarters (256 in a wave) the best'th largest is no larger than
-//   the best'th largest logit of the wave; it is found bit by bit with ballots, and only the logits from it on,
-//   a few more than `best`, are put into a list in LDS, where each counts those before it.
-//   (Where very many are equal, they are taken one by one instead.)
-// The last chunk of a row merges the chunks' sorted lists, a lane for each; the last row of a group
-// the beams'.  One launch.
+// LDS that a wave writes and reads by itself: its operations are performed in order.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The first k of n different numbers in LDS, in descending order at its beginning; by the
+// lanes `lane` of `lanes` (a wave, or all waves of the workgroup with `join` between), up to M numbers a lane.  Each
+// number counts those before it.
+template <int M, class Join>
+__device__ __forceinline__ void keep_best(unsigned long long* list, uint32_t n, uint32_t k, uint32_t lane, uint32_t lanes,
+                                          Join&& join) {
+    uint64_t mine[M];
+    uint32_t place[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        mine[i] = lane + lanes * i < n ? list[lane + lanes * i] : 0;
+        place[i] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        if (lanes * i >= n) continue;  // (uniform)
+        uint32_t j = 0;
+        for (; j + 8 <= n; j += 8) {
+            uint64_t o[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) o[u] = list[j + u];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) place[i] += o[u] > mine[i];
+        }
+        for (; j < n; ++j) place[i] += list[j] > mine[i];
+    }
+    join();
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+        if (mine[i] && place[i] < k) list[place[i]] = mine[i];
+    join();
+}
+
+// f64 ranks as whole numbers of the same order; 0: none (-infinity).  kNoRank: a rank that is no number.
+constexpr uint64_t kNoRank = ~0ull;
+__device__ __forceinline__ uint64_t rank_key(double r) {
+    if (!(r > -INFINITY)) return r != r ? kNoRank : 0;
+    const uint64_t b = (uint64_t)__double_as_longlong(r + 0.0);
+    return b ^ ((uint64_t)((int64_t)b >> 63) | 1ull << 63);
+}
+__device__ __forceinline__ double rank_value(uint64_t key) {
+    return __longlong_as_double((long long)((key >> 63) ? key ^ 1ull << 63 : ~key));
+}
+
+// Lists of k numbers in descending order, one of each lane with `some` (0: no more), merged by a wave: lane i gets the
+// i'th largest (0: none), the lane that it is of, the lowest of equal ones, and its place there.  A round
+// looks for the largest upper half; only where several lanes have it the lower halves decide.
+__device__ __forceinline__ void merge_lists(const unsigned long long* list, bool some, uint32_t k, uint64_t& key, uint32_t& from,
+                                            uint32_t& place) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint64_t head = some ? list[0] : 0, after = some && k > 1 ? list[1] : 0;
+    uint32_t at = 0;
+    key = 0, from = place = 0;
+    for (uint32_t i = 0; i < k; ++i) {
+        const uint32_t hi = (uint32_t)(head >> 32), best = wave_max_u32(hi);
+        if (best == 0) break;
+        unsigned long long mask = __ballot(hi == best);
+        if (mask & (mask - 1)) {
+            const uint32_t lo = hi == best ? (uint32_t)head : 0, low = wave_max_u32(lo);
+            mask = __ballot(hi == best && lo == low);
+        }
+        const int b = __builtin_ctzll(mask);
+        const uint64_t k0 = (uint64_t)best << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)head, b);
+        const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)at, b);
+        if (lane == i) key = k0, from = (uint32_t)b, place = p;
+        if ((int)lane == b) {
+            head = after, ++at;
+            after = at + 1 < k ? list[at + 1] : 0;
+        }
+    }
+}
+
+// A workgroup per chunk of a beam's row; its waves go through it 256 U logits at a time, the next on their
+// way, each by itself:
+//   Sum: about the wave's own maximum.
+//   Best: of the maxima of a lane's quarters (256 in a wave) the k'th largest is no larger than the
+//   k'th largest logit; it is searched bit by bit with ballots, until k to k + 3 of them reach it.  Only logits from
+//   it on, and from the k'th best so far, go to the wave's list in LDS (a few more than k at first, then fewer and
+//   fewer).  Where very many are equal, they are taken one by one instead.
+// The waves' lists are joined, then the last chunk of a row merges the chunks' sorted lists, a lane for each, and the
+// last row of a group the beams'.  One launch.
 template <int U>
 __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
     extern __shared__ __align__(16) unsigned long long buf[];
     __shared__ float wave_m[4];
     __shared__ double wave_sum[4];
-    __shared__ uint32_t listed, flag;
+    __shared__ uint32_t wave_have[4], flag;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocabulary, k = a.best;
     const uint32_t row = blockIdx.y, chunk = blockIdx.x, chunks = gridDim.x, group = row / a.beams;
     const float* z = a.logits + (uint64_t)row * a.stride;
@@ -82,22 +162,31 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
     float m = -INFINITY;
     double sum = 0.0;
     bool bad = !(score < INFINITY);
-    uint32_t have = 0;
+    uint32_t have = 0, least = kLeast;
     if (score > -INFINITY && !bad) {
+        unsigned long long* list = buf + wave * kListMost;
+        const uint32_t mine = 4 * tid;  // of every 1024: a wave's are together
+        f32x4 next[U];
+        auto load = [&](uint32_t s) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t t = s + 1024 * u + mine;
+                if (t + 3 < t1) {
+                    next[u] = __builtin_nontemporal_load((const f32x4a4*)(z + t));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) next[u][j] = t + j < t1 ? z[t + j] : -INFINITY;
+                }
+            }
+        };
+        load(t0);
         for (uint32_t s = t0; s < t1; s += 1024 * U) {
             float v[U][4];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t t = s + 4 * (tid + 256 * u);
-                if (t + 3 < t1) {
-                    const f32x4 f = *(const f32x4a4*)(z + t);
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[u][j] = f[j];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[u][j] = t + j < t1 ? z[t + j] : -INFINITY;
-                }
-            }
+                for (int j = 0; j < 4; ++j) v[u][j] = next[u][j];
+            if (t1 - s > 1024 * U) load(s + 1024 * U);
             uint32_t key[U][4], quarter[4] = {0, 0, 0, 0};
             float top = -INFINITY;
 #pragma unroll
@@ -110,40 +199,40 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
                     top = fmaxf(top, v[u][j]);
                 }
             top = wave_max_dpp(top);
-            if (top > -INFINITY) {  // (uniform)
-                if (top > m) {
-                    sum *= (double)beam_exp(m - top);
-                    m = top;
-                }
+            if (!(top > -INFINITY)) continue;  // (uniform in the wave)
+            if (top > m) {
+                sum *= (double)beam_exp(m - top);
+                m = top;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                sum += (double)((beam_exp(v[u][0] - m) + beam_exp(v[u][1] - m)) + (beam_exp(v[u][2] - m) + beam_exp(v[u][3] - m)));
+            // a sorted list of k bounds what can follow; without one, or where it lets much through, the quarters do
+            uint32_t n = 0;
+            auto count = [&] {
+                n = 0;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    sum += (double)((beam_exp(v[u][0] - m) + beam_exp(v[u][1] - m)) + (beam_exp(v[u][2] - m) + beam_exp(v[u][3] - m)));
-            }
-            // the list so far is in buf[0 .. have), sorted; a full one bounds what can follow
-            uint32_t least = have == k ? (uint32_t)(buf[k - 1] >> 32) : kLeast;
-            if (tid == 0) listed = have;
-            __syncthreads();
-            {
-                // the largest t with `best` quarters or more of t at least
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) n += (uint32_t)__builtin_popcountll(__ballot(key[u][j] >= least));
+            };
+            count();
+            if (n == 0) continue;
+            if (n > 64) {
                 uint32_t t = 0;
                 for (int bit = 31; bit >= 0; --bit) {
                     const uint32_t c = t | 1u << bit;
-                    uint32_t n = 0;
+                    n = 0;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) n += (uint32_t)__builtin_popcountll(__ballot(quarter[j] >= c));
                     if (n >= k) t = c;
+                    if (n >= k && n < k + 4) break;
                 }
                 least = t > least ? t : least;
+                count();
             }
-            uint32_t n = 0;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) n += (uint32_t)__builtin_popcountll(__ballot(key[u][j] >= least));
+            uint32_t at = have;
             if (n <= kWaveMost) {
-                uint32_t at = 0;
-                if (lane == 0 && n) at = atomicAdd(&listed, n);
-                at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -151,7 +240,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
                         const bool take = key[u][j] >= least;
                         const unsigned long long mask = __ballot(take);
                         if (!mask) continue;
-                        if (take) buf[at + __builtin_popcountll(mask & ((1ull << lane) - 1))] = beam_pair(key[u][j], s + 4 * (tid + 256 * u) + j);
+                        if (take) list[at + __builtin_popcountll(mask & ((1ull << lane) - 1))] = beam_pair(key[u][j], s + 1024 * u + mine + j);
                         at += (uint32_t)__builtin_popcountll(mask);
                     }
             } else {
@@ -162,143 +251,143 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
                     for (int u = 0; u < U; ++u)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const uint64_t p = beam_pair(key[u][j], s + 4 * (tid + 256 * u) + j);
+                            const uint64_t p = beam_pair(key[u][j], s + 1024 * u + mine + j);
                             if (key[u][j] >= least && p < before && p > best) best = p;
                         }
                     best = wave_max_u64(best);
                     if (!best) break;
-                    if (lane == 0) buf[atomicAdd(&listed, 1u)] = best;
-                    before = best;
+                    if (lane == 0) list[at] = best;
+                    ++at, before = best;
                 }
             }
-            __syncthreads();
-            // each of the list counts those before it (all are different)
-            const uint32_t all = listed;
-            constexpr int kMine = (kListMost + 255) / 256;
-            uint64_t mine[kMine];
-            uint32_t place[kMine];
-#pragma unroll
-            for (int i = 0; i < kMine; ++i) {
-                const uint32_t c = tid + 256 * i;
-                mine[i] = c < all ? buf[c] : 0;
-                place[i] = 0;
-                if (256u * i >= all) continue;  // (uniform)
-                for (uint32_t j = 0; j < all; ++j) place[i] += buf[j] > mine[i];
+            wave_order();
+            // sorted when there are k for the first time, and before another wave's worth would not fit
+            if ((have < k && at >= k) || at > kSelectMaxBest) {
+                keep_best<(int)(kListMost + 63) / 64>(list, at, k, lane, 64, [] { wave_order(); });
+                at = at < k ? at : k;
+                if (at == k) least = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(list[k - 1] >> 32));
             }
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kMine; ++i)
-                if (mine[i] && place[i] < k) buf[place[i]] = mine[i];
-            have = all < k ? all : k;
-            __syncthreads();
+            have = at;
+        }
+        if (have > k) {
+            keep_best<1>(list, have, k, lane, 64, [] { wave_order(); });
+            have = k;
         }
     }
-    bad = __syncthreads_or(bad);
     sum = wave_sum_f64(sum);
-    if (lane == 0) wave_m[wave] = m, wave_sum[wave] = sum;
-    __syncthreads();
+    if (lane == 0) wave_m[wave] = m, wave_sum[wave] = sum, wave_have[wave] = have;
+    bad = __syncthreads_or(bad);
     m = fmaxf(fmaxf(wave_m[0], wave_m[1]), fmaxf(wave_m[2], wave_m[3]));
     sum = 0.0;
     for (int w = 0; w < 4; ++w)
         if (wave_m[w] > -INFINITY) sum += wave_sum[w] * (double)beam_exp(wave_m[w] - m);
     if (bad) sum = NAN;
+    {  // the waves' lists, one behind the other
+        uint32_t at = 0;
+        for (uint32_t w = 0; w < wave; ++w) at += wave_have[w];
+        const unsigned long long pair = lane < have ? buf[wave * kListMost + lane] : 0;
+        const uint32_t all = wave_have[0] + wave_have[1] + wave_have[2] + wave_have[3];
+        __syncthreads();
+        if (lane < have) buf[at + lane] = pair;
+        __syncthreads();
+        keep_best<1>(buf, all, k, tid, 256, [] { __syncthreads(); });
+        have = all < k ? all : k;
+    }
 
-    // the row: every chunk's list
-    if (chunks > 1) {
-        unsigned long long* put = a.lists + ((uint64_t)row * chunks + chunk) * (k + 2);
+    // the row: every chunk's list.  Few beams: of all of the group at once
+    const bool once = a.once;
+    if (chunks > 1 || once) {
+        const uint32_t words = chunks * (k + 2), mine = (row - group * a.beams) * words + chunk * (k + 2);
+        unsigned long long* put = a.lists + (uint64_t)group * a.beams * words + mine;
         if (tid < k) beam_put(put + tid, tid < have ? buf[tid] : 0);
         if (tid == k) beam_put(put + k, __float_as_uint(m));
         if (tid == k + 1) beam_put(put + k + 1, (unsigned long long)__double_as_longlong(sum));
-        if (!beam_last(a.count + row, chunks, &flag)) return;
-        const unsigned long long* lists = a.lists + (uint64_t)row * chunks * (k + 2);
-        for (uint32_t i = tid; i < chunks * (k + 2); i += 256) {
-            const uint32_t c = i / (k + 2), j = i - c * (k + 2);
-            const unsigned long long x = beam_get(lists + i);
-            if (j < k) buf[c * k + j] = x;
-            else buf[chunks * k + 2 * c + (j - k)] = x;
-        }
+        if (!beam_last(once ? a.count + group : a.count + row, once ? chunks * a.beams : chunks, &flag)) return;
+        const unsigned long long* lists = put - (once ? mine : chunk * (k + 2));
+        for (uint32_t i = tid; i < (once ? a.beams : 1) * words; i += 256) buf[i] = beam_get(lists + i);
         __syncthreads();
     }
-    double rank = -INFINITY;  // of place `lane` in the row
+    // row r's ranks and tokens of place `lane`, from its chunks' lists at `lists`
+    auto row_merge = [&](const unsigned long long* lists, float of, uint64_t& rank, int32_t& token) {
+        const bool some = lane < chunks;
+        const unsigned long long* list = lists + lane * (k + 2);
+        const float cm = some ? __uint_as_float((uint32_t)list[k]) : -INFINITY;
+        const double cs = some ? __longlong_as_double((long long)list[k + 1]) : 0.0;
+        const float top = wave_max_dpp(cm);
+        // (a sum that is no number stays one)
+        const double all = wave_sum_f64(cs != cs ? cs : cm > -INFINITY ? cs * (double)beam_exp(cm - top) : 0.0);
+        uint64_t pair;
+        uint32_t from, place;
+        merge_lists(list, some, k, pair, from, place);
+        rank = all != all ? kNoRank : pair ? rank_key((double)of - ((double)top + log(all)) + (double)beam_value((uint32_t)(pair >> 32))) : 0;
+        token = all == all && pair ? (int32_t)~(uint32_t)pair : -1;
+    };
+    uint64_t rank = 0;
     int32_t token = -1;
-    if (wave == 0) {
-        uint64_t pair = lane < have ? buf[lane] : 0;
-        if (chunks > 1) {
-            const bool some = lane < chunks;
-            const float cm = some ? __uint_as_float((uint32_t)buf[chunks * k + 2 * lane]) : -INFINITY;
-            const double cs = some ? __longlong_as_double((long long)buf[chunks * k + 2 * lane + 1]) : 0.0;
-            m = wave_max_dpp(cm);
-            // (a sum that is no number stays one)
-            sum = wave_sum_f64(cs != cs ? cs : cm > -INFINITY ? cs * (double)beam_exp(cm - m) : 0.0);
-            uint32_t next = 1;
-            uint64_t head = some ? buf[lane * k] : 0;
-            pair = 0;
-            for (uint32_t i = 0; i < k; ++i) {
-                const uint64_t best = wave_max_u64(head);
-                if (!best) break;
-                if (lane == i) pair = best;
-                if (head == best) head = next < k ? buf[lane * k + next] : 0, ++next;
+    unsigned long long* ranks = buf;  // [beams][k], then the tokens
+    uint32_t* tokens = (uint32_t*)(buf + a.beams * k);
+    if (once) {
+        const uint32_t words = chunks * (k + 2);
+        uint64_t got[kOnceBeams / 4];
+        int32_t tok[kOnceBeams / 4];
+#pragma unroll
+        for (uint32_t i = 0; i < kOnceBeams / 4; ++i) {
+            const uint32_t b = wave + 4 * i;
+            if (b < a.beams) row_merge(buf + b * words, a.scores[(uint64_t)group * a.beams + b], got[i], tok[i]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kOnceBeams / 4; ++i) {
+            const uint32_t b = wave + 4 * i;
+            if (b < a.beams && lane < k) ranks[b * k + lane] = got[i], tokens[b * k + lane] = (uint32_t)tok[i];
+        }
+        __syncthreads();
+    } else {
+        if (wave == 0) {
+            if (chunks > 1) {
+                row_merge(buf, score, rank, token);
+            } else {
+                const uint64_t pair = lane < have ? buf[lane] : 0;
+                rank = sum != sum ? kNoRank : pair ? rank_key((double)score - ((double)m + log(sum)) + (double)beam_value((uint32_t)(pair >> 32))) : 0;
+                token = sum == sum && pair ? (int32_t)~(uint32_t)pair : -1;
             }
         }
-        if (sum != sum) rank = NAN;
-        else if (pair) rank = (double)score - ((double)m + log(sum)) + (double)beam_value((uint32_t)(pair >> 32)), token = (int32_t)~(uint32_t)pair;
-    }
-
-    // the group: every beam's
-    int32_t parent = token < 0 ? -1 : 0;
-    if (a.beams > 1) {
+        // the group: every beam's
         unsigned long long* put = a.ranks + (uint64_t)row * 2 * k;
         if (wave == 0 && lane < k) {
-            beam_put(put + lane, (unsigned long long)__double_as_longlong(rank));
+            beam_put(put + lane, rank);
             beam_put(put + k + lane, (uint32_t)token);
         }
         if (!beam_last(a.count + (uint64_t)a.groups * a.beams + group, a.beams, &flag)) return;
-        const unsigned long long* ranks = a.ranks + (uint64_t)group * a.beams * 2 * k;
-        uint32_t* tokens = (uint32_t*)(buf + a.beams * k);
+        const unsigned long long* all = a.ranks + (uint64_t)group * a.beams * 2 * k;
         for (uint32_t i = tid; i < a.beams * 2 * k; i += 256) {
             const uint32_t b = i / (2 * k), j = i - b * 2 * k;
-            const unsigned long long x = beam_get(ranks + i);
-            if (j < k) buf[b * k + j] = x;
+            const unsigned long long x = beam_get(all + i);
+            if (j < k) ranks[b * k + j] = x;
             else tokens[b * k + j - k] = (uint32_t)x;
         }
         __syncthreads();
-        if (wave != 0) return;
-        const unsigned long long* list = buf + lane * k;
-        const bool some = lane < a.beams;
-        double head = some ? __longlong_as_double((long long)list[0]) : -INFINITY;
-        const bool off = __ballot(head != head) != 0;
-        uint32_t next = 1;
-        rank = off ? NAN : -INFINITY, token = parent = -1;
-        for (uint32_t i = 0; i < k && !off; ++i) {
-            const double best = wave_max_f64(head);
-            if (!(best > -INFINITY)) break;
-            const int b = __builtin_ctzll(__ballot(head == best));  // the lowest beam of equal ones
-            if (lane == i) rank = best, parent = b, token = (int32_t)tokens[b * k + __builtin_amdgcn_readlane((int)next, b) - 1];
-            if ((int)lane == b) head = next < k ? __longlong_as_double((long long)list[next]) : -INFINITY, ++next;
-        }
-    } else if (wave != 0) {
-        return;
     }
-    if (__ballot(rank != rank)) {
-        rank = -INFINITY, token = parent = -1;
-        if (lane == 0) report_error(a.err_word, model_key(a.group0 + group, kStOOut, 0));
-    }
+    if (wave != 0) return;
+    uint32_t beam, place;
+    const bool off = __ballot(lane < a.beams && ranks[lane * k] == kNoRank) != 0;
+    merge_lists(ranks + lane * k, lane < a.beams && !off, k, rank, beam, place);
+    if (off && lane == 0) report_error(a.err_word, model_key(a.group0 + group, kStOOut, 0));
     if (lane < k) {
         const uint64_t o = (uint64_t)group * k + lane;
-        a.out_scores[o] = (float)rank, a.parents[o] = parent, a.tokens[o] = token;
+        a.out_scores[o] = rank ? (float)rank_value(rank) : -INFINITY;
+        a.parents[o] = rank ? (int32_t)beam : -1;
+        a.tokens[o] = rank ? (int32_t)tokens[beam * k + place] : -1;
     }
 }
 
 // Logits of a thread at a time, and of a workgroup: few rows are cut finer, to fill the CUs (4 rows of 128256
-// tokens: 252 workgroups); at most 64 chunks, which a wave's lanes merge.
-static uint32_t select_unroll(uint64_t rows, uint64_t vocabulary) {
-    const uint64_t chunks = (vocabulary + 2047) / 2048;
-    return rows * chunks <= 1024 && chunks <= 64 ? 2 : rows * chunks <= 2048 && chunks <= 128 ? 4 : 8;
-}
+// tokens: 252 workgroups), many into about 1024 workgroups; at most 64 chunks, which a wave's lanes merge.
+static uint32_t select_unroll(uint64_t rows, uint64_t vocabulary) { return rows * vocabulary <= (1u << 21) ? 2 : 4; }
 static uint32_t select_chunk(uint64_t rows, uint64_t vocabulary) {
-    const uint64_t unit = 1024 * select_unroll(rows, vocabulary);
+    const uint64_t unit = 1024 * select_unroll(rows, vocabulary), most = 1024 / rows < 1 ? 1 : 1024 / rows < 64 ? 1024 / rows : 64;
     uint64_t n = (vocabulary + unit - 1) / unit;
-    n = n < 64 ? n : 64;
+    n = n < most ? n : most;
     return (uint32_t)(((vocabulary + n - 1) / n + 3) / 4 * 4);
 }
 static uint64_t select_chunks(uint64_t rows, uint64_t vocabulary) {
@@ -318,9 +407,13 @@ hipError_t launch_beam_select(SelectArgs a, void* scratch, hipStream_t s) {
     a.ranks = (unsigned long long*)scratch;
     a.lists = a.ranks + rows * 2 * a.best;
     uint64_t words = chunks > 1 ? chunks * (a.best + 2) : 0;
-    if (words < kListMost) words = kListMost;
+    if (words < 4 * kListMost) words = 4 * kListMost;
     const uint64_t of_beams = ((uint64_t)a.beams * a.best * 3 + 1) / 2;  // (at most 48 KB)
     if (words < of_beams) words = of_beams;
+    // all chunks of a group in one workgroup's LDS (32 KB at most): one exchange less
+    const uint64_t of_group = a.beams * chunks * (a.best + 2);
+    a.once = a.beams <= kOnceBeams && of_group <= 4096;
+    if (a.once && words < of_group) words = of_group;
     for (uint64_t g = 0; g < a.groups;) {  // (a grid's second dimension has 65535 workgroups)
         const uint64_t n = a.groups - g < 65535 / a.beams ? a.groups - g : 65535 / a.beams;
         SelectArgs p = a;
@@ -329,11 +422,8 @@ hipError_t launch_beam_select(SelectArgs a, void* scratch, hipStream_t s) {
         p.group0 = (uint32_t)g, p.groups = (uint32_t)n;
         const dim3 grid((uint32_t)chunks, (uint32_t)(n * a.beams)), block(256);
         const size_t lds = words * sizeof(unsigned long long);
-        switch (select_unroll(rows, a.vocabulary)) {
-            case 2: hipLaunchKernelGGL(beam_select_kernel<2>, grid, block, lds, s, p); break;
-            case 4: hipLaunchKernelGGL(beam_select_kernel<4>, grid, block, lds, s, p); break;
-            default: hipLaunchKernelGGL(beam_select_kernel<8>, grid, block, lds, s, p); break;
-        }
+        if (select_unroll(rows, a.vocabulary) == 2) hipLaunchKernelGGL(beam_select_kernel<2>, grid, block, lds, s, p);
+        else hipLaunchKernelGGL(beam_select_kernel<4>, grid, block, lds, s, p);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         g += n;

@@ -335,7 +335,7 @@ struct SelectArgs {
     unsigned long long* err_word;
     uint32_t* count;  // a word for each beam and group, 0 between launches
     // of a launch: tokens of a workgroup, the first group; scratch (beam_select_bytes)
-    uint32_t chunk, group0;
+    uint32_t chunk, group0, once;
     unsigned long long *ranks, *lists;
 };
 size_t beam_select_bytes(uint64_t rows, uint64_t vocabulary, uint64_t best);
