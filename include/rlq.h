@@ -486,7 +486,8 @@ int32_t rlq_kv_attention(rlq_context *ctx, const rlq_kv_cache *cache, const floa
  * beams' scores [groups, beams] (-infinity: a beam without a place, its logits are not looked
  * at).  Candidates are ranked by score + logit - log(sum of exp(logits of the beam)), in f64 (the
  * exponentials f32); out_scores, parents (beam) and tokens [groups, best] are the best in
- * order, the lowest (beam, token) of equal ones, scores rounded once.  Logits of -infinity are
+ * order, the lowest beam of equal ones, within a beam by the logits and the lowest token of equal ones; scores
+ * are rounded once.  Logits of -infinity are
  * never chosen; places with no candidate left get -infinity, -1 and -1.  beams and best at most 64.
  * RLQ_NON_FINITE at rlq_sync (a = RLQ_CHECK_MATRIX_OUTPUT, b = the group): a score or a logit of a
  * live beam is NaN or +infinity; the group's places are as without candidates.  At

@@ -663,6 +663,11 @@ class Context:
     def _rows(self, t, tail):
         """(pointer, floats from row to row) of an f32 tensor [rows, *tail] whose rows are
         contiguous but may lie apart, such as a part of a product's rows."""
+        if len(tail) == 2 and isinstance(t, torch.Tensor) and t.ndim == 3:  # (the usual case, half of the time)
+            (_, a, b), (step, s1, s2) = t.shape, t.stride()
+            if a == tail[0] and b == tail[1] and s2 == 1 and s1 == b and step >= a * b and t.dtype is torch.float32 \
+                    and t.get_device() == self._device:
+                return t.data_ptr(), step
         if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or not t.is_cuda:
             raise TypeError("expected a torch.float32 tensor on the GPU")
         if t.get_device() != self._device:

@@ -3,8 +3,8 @@
 // A candidate of a group is a beam b and a token t with
 //   rank = score_b + z_bt - log sum_u exp z_bu
 // in f64 from the f32 logits (the exponentials f32, their sum f64); the best
-// candidates in order, the lowest (b, t) of equal ones.  Within a beam the order is
-// that of the logits, so a beam's logits are read once: for its sum and for its best tokens,
+// candidates in order.  Within a beam the order is that of the logits (the lower token of equal ones), of equal ranks
+// the lower beam's is first.  So a beam's logits are read once: for its sum and for its best tokens,
 // which meet those of the other beams as f64 ranks.
 #include "rlq_device.hpp"
 #include "rlq_internal.hpp"
@@ -57,7 +57,7 @@ __device__ __forceinline__ float beam_exp(float x) {
     return __builtin_fmaf(p, r * 0.693147181f, p);
 }
 
-constexpr uint32_t kOnceBeams = 8;     // of a group whose chunks one workgroup merges
+constexpr uint32_t kFound = 512;       // candidates of a group that are ranked by counting
 constexpr uint32_t kWaveMost = 256;  // candidates that a wave puts down at once
 constexpr uint32_t kListMost = kSelectMaxBest + kWaveMost;  // of a wave's list
 
@@ -98,6 +98,22 @@ __device__ __forceinline__ void keep_best(unsigned long long* list, uint32_t n, 
     for (int i = 0; i < M; ++i)
         if (mine[i] && place[i] < k) list[place[i]] = mine[i];
     join();
+}
+
+// A number that k of the wave's 64 N keys reach, and no more than k + 3 where their bits allow it; 0 if there are no k
+// above 0.  Bit by bit with ballots.
+template <int N>
+__device__ __forceinline__ uint32_t bound_of(const uint32_t (&key)[N], uint32_t k) {
+    uint32_t t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = t | 1u << bit;
+        uint32_t n = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) n += (uint32_t)__builtin_popcountll(__ballot(key[j] >= c));
+        if (n >= k) t = c;
+        if (n >= k && n < k + 4) break;
+    }
+    return t;
 }
 
 // f64 ranks as whole numbers of the same order; 0: none (-infinity).  kNoRank: a rank that is no number.
@@ -161,78 +177,58 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
     const uint32_t t0 = chunk * a.chunk, t1 = V - t0 < a.chunk ? V : t0 + a.chunk;
     float m = -INFINITY;
     double sum = 0.0;
-    bool bad = !(score < INFINITY);
+    int bad = !(score < INFINITY);
     uint32_t have = 0, least = kLeast;
     if (score > -INFINITY && !bad) {
         unsigned long long* list = buf + wave * kListMost;
         const uint32_t mine = 4 * tid;  // of every 1024: a wave's are together
-        f32x4 next[U];
+        f32x4 v[U];
         auto load = [&](uint32_t s) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t t = s + 1024 * u + mine;
                 if (t + 3 < t1) {
-                    next[u] = __builtin_nontemporal_load((const f32x4a4*)(z + t));
+                    v[u] = __builtin_nontemporal_load((const f32x4a4*)(z + t));
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) next[u][j] = t + j < t1 ? z[t + j] : -INFINITY;
+                    for (int j = 0; j < 4; ++j) v[u][j] = t + j < t1 ? z[t + j] : -INFINITY;
                 }
             }
         };
         load(t0);
         for (uint32_t s = t0; s < t1; s += 1024 * U) {
-            float v[U][4];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[u][j] = next[u][j];
-            if (t1 - s > 1024 * U) load(s + 1024 * U);
             uint32_t key[U][4], quarter[4] = {0, 0, 0, 0};
-            float top = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                bad |= __builtin_isunordered(v[u][0], v[u][1]) || __builtin_isunordered(v[u][2], v[u][3]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    bad |= !(v[u][j] < INFINITY);
                     key[u][j] = beam_key(v[u][j]);
                     quarter[j] = key[u][j] > quarter[j] ? key[u][j] : quarter[j];
-                    top = fmaxf(top, v[u][j]);
                 }
-            top = wave_max_dpp(top);
-            if (!(top > -INFINITY)) continue;  // (uniform in the wave)
-            if (top > m) {
-                sum *= (double)beam_exp(m - top);
-                m = top;
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                sum += (double)((beam_exp(v[u][0] - m) + beam_exp(v[u][1] - m)) + (beam_exp(v[u][2] - m) + beam_exp(v[u][3] - m)));
-            // a sorted list of k bounds what can follow; without one, or where it lets much through, the quarters do
-            uint32_t n = 0;
-            auto count = [&] {
-                n = 0;
+            const uint32_t a01 = quarter[0] > quarter[1] ? quarter[0] : quarter[1];
+            const uint32_t a23 = quarter[2] > quarter[3] ? quarter[2] : quarter[3];
+            const uint32_t highest = wave_max_u32(a01 > a23 ? a01 : a23);
+            const bool some = highest >= kLeast;  // (uniform in the wave)
+            if (some) {
+                const float top = beam_value(highest);
+                bad |= !(top < INFINITY);
+                if (top > m) {
+                    sum *= (double)beam_exp(m - top);
+                    m = top;
+                }
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) n += (uint32_t)__builtin_popcountll(__ballot(key[u][j] >= least));
-            };
-            count();
-            if (n == 0) continue;
-            if (n > 64) {
-                uint32_t t = 0;
-                for (int bit = 31; bit >= 0; --bit) {
-                    const uint32_t c = t | 1u << bit;
-                    n = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) n += (uint32_t)__builtin_popcountll(__ballot(quarter[j] >= c));
-                    if (n >= k) t = c;
-                    if (n >= k && n < k + 4) break;
-                }
-                least = t > least ? t : least;
-                count();
+                    sum += (double)((beam_exp(v[u][0] - m) + beam_exp(v[u][1] - m)) + (beam_exp(v[u][2] - m) + beam_exp(v[u][3] - m)));
             }
+            if (t1 - s > 1024 * U) load(s + 1024 * U);
+            if (highest < least || !some) continue;
+            // the k'th best so far bounds what can follow; before there is one, or where it lets too much through, the
+            // k'th largest quarter does
             uint32_t at = have;
-            if (n <= kWaveMost) {
+            auto put = [&] {
+                at = have;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -240,10 +236,19 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
                         const bool take = key[u][j] >= least;
                         const unsigned long long mask = __ballot(take);
                         if (!mask) continue;
-                        if (take) list[at + __builtin_popcountll(mask & ((1ull << lane) - 1))] = beam_pair(key[u][j], s + 1024 * u + mine + j);
+                        const uint32_t to = at + (uint32_t)__builtin_popcountll(mask & ((1ull << lane) - 1));
+                        if (take && to < kListMost) list[to] = beam_pair(key[u][j], s + 1024 * u + mine + j);
                         at += (uint32_t)__builtin_popcountll(mask);
                     }
-            } else {
+            };
+            if (least > kLeast) put();
+            if (least == kLeast || at > kListMost) {
+                const uint32_t t = bound_of<4>(quarter, k);
+                least = t > least ? t : least;
+                put();
+            }
+            if (at > kListMost) {  // very many equal ones
+                at = have;
                 uint64_t before = ~0ull;
                 for (uint32_t i = 0; i < k; ++i) {
                     uint64_t best = 0;
@@ -304,70 +309,172 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
         if (tid == k + 1) beam_put(put + k + 1, (unsigned long long)__double_as_longlong(sum));
         if (!beam_last(once ? a.count + group : a.count + row, once ? chunks * a.beams : chunks, &flag)) return;
         const unsigned long long* lists = put - (once ? mine : chunk * (k + 2));
-        for (uint32_t i = tid; i < (once ? a.beams : 1) * words; i += 256) buf[i] = beam_get(lists + i);
+        const uint32_t n = (once ? a.beams : 1) * words;
+        for (uint32_t i = tid; i < n; i += 8 * 256) {
+            unsigned long long x[8];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) x[u] = i + 256 * u < n ? beam_get(lists + i + 256 * u) : 0;
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u)
+                if (i + 256 * u < n) buf[i + 256 * u] = x[u];
+        }
         __syncthreads();
     }
-    // row r's ranks and tokens of place `lane`, from its chunks' lists at `lists`
-    auto row_merge = [&](const unsigned long long* lists, float of, uint64_t& rank, int32_t& token) {
+    // score less the log of the sum, of a row whose chunks' lists are at `lists` (no number: an error)
+    auto row_offset = [&](const unsigned long long* lists, float of) {
         const bool some = lane < chunks;
         const unsigned long long* list = lists + lane * (k + 2);
         const float cm = some ? __uint_as_float((uint32_t)list[k]) : -INFINITY;
         const double cs = some ? __longlong_as_double((long long)list[k + 1]) : 0.0;
         const float top = wave_max_dpp(cm);
-        // (a sum that is no number stays one)
+        // (a sum that is no number stays one; no logits at all: their ranks are not made)
         const double all = wave_sum_f64(cs != cs ? cs : cm > -INFINITY ? cs * (double)beam_exp(cm - top) : 0.0);
-        uint64_t pair;
-        uint32_t from, place;
-        merge_lists(list, some, k, pair, from, place);
-        rank = all != all ? kNoRank : pair ? rank_key((double)of - ((double)top + log(all)) + (double)beam_value((uint32_t)(pair >> 32))) : 0;
-        token = all == all && pair ? (int32_t)~(uint32_t)pair : -1;
+        return all != all ? (double)NAN : top > -INFINITY ? (double)of - ((double)top + log(all)) : 0.0;
     };
+    auto rank_of = [](double offset, uint64_t pair) { return pair ? rank_key(offset + (double)beam_value((uint32_t)(pair >> 32))) : 0; };
+    if (once) {
+        // all lists of the group at once, a thread for each
+        const uint32_t words = chunks * (k + 2), lists = a.beams * chunks;
+        double* offset = (double*)(buf + a.beams * words);
+        unsigned long long* heads = (unsigned long long*)(offset + kSelectMaxBeams);
+        unsigned long long* found = heads + 256;
+        uint32_t* found_at = (uint32_t*)(found + kFound);
+        auto out = [&](uint32_t p, uint64_t r, uint32_t at) {
+            const uint64_t to = (uint64_t)group * k + p;
+            const uint32_t l = at / 64;
+            a.out_scores[to] = r ? (float)rank_value(r) : -INFINITY;
+            a.parents[to] = r ? (int32_t)(l / chunks) : -1;
+            a.tokens[to] = r ? (int32_t)~(uint32_t)buf[l * (k + 2) + at % 64] : -1;
+        };
+        for (uint32_t b = wave; b < a.beams; b += 4) {
+            const double o = row_offset(buf + b * words, a.scores[(uint64_t)group * a.beams + b]);
+            if (lane == 0) offset[b] = o;
+        }
+        if (tid == 0) wave_have[0] = 0;
+        __syncthreads();
+        const double o = tid < lists ? offset[tid / chunks] : 0.0;
+        heads[tid] = tid < lists ? rank_of(o, buf[tid * (k + 2)]) : 0;
+        const bool off = __syncthreads_or(o != o);
+        if (off) {
+            if (tid == 0) report_error(a.err_word, model_key(a.group0 + group, kStOOut, 0));
+            for (uint32_t p = tid; p < k; p += 256) out(p, 0, 0);
+            return;
+        }
+        // of the heads, k to k + 3 reach `bound` (all waves find it)
+        uint32_t top[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) top[u] = (uint32_t)(heads[lane + 64 * u] >> 32);
+        const uint64_t bound = (uint64_t)bound_of<4>(top, k) << 32;
+        const uint64_t least_rank = bound > 1 ? bound : 1;
+        // their lists, the lanes a list's places: every fourth list a wave
+        uint32_t turn = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            unsigned long long reach = __ballot(top[u] >= (uint32_t)(bound >> 32) && top[u] > 0);
+            for (; reach; reach &= reach - 1, ++turn) {
+                if (turn % 4 != wave) continue;
+                const uint32_t l = 64 * u + (uint32_t)__builtin_ctzll(reach);
+                const uint64_t r = lane < k ? rank_of(offset[l / chunks], buf[l * (k + 2) + lane]) : 0;
+                const unsigned long long mask = __ballot(r >= least_rank);
+                uint32_t at = 0;
+                if (lane == 0) at = atomicAdd(&wave_have[0], (uint32_t)__builtin_popcountll(mask));
+                at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + lane;  // (a list's first places reach it)
+                if (r >= least_rank && at < kFound) found[at] = r, found_at[at] = l * 64 + lane;
+            }
+        }
+        __syncthreads();
+        const uint32_t n = wave_have[0];
+        if (n <= kFound) {
+            if (wave != 0) return;
+            uint32_t left = n;
+            if (n > 64) {  // those that reach the k'th of them
+                constexpr int kMine = kFound / 64;
+                uint64_t r[kMine];
+                uint32_t hi[kMine], at[kMine];
+#pragma unroll
+                for (int u = 0; u < kMine; ++u) {
+                    const uint32_t c = lane + 64 * u;
+                    r[u] = c < n ? found[c] : 0, at[u] = c < n ? found_at[c] : 0;
+                    hi[u] = (uint32_t)(r[u] >> 32);
+                }
+                const uint32_t t = bound_of<kMine>(hi, k);
+                wave_order();
+                left = 0;
+#pragma unroll
+                for (int u = 0; u < kMine; ++u) {
+                    const bool take = hi[u] >= t && r[u];
+                    const unsigned long long mask = __ballot(take);
+                    const uint32_t to = left + (uint32_t)__builtin_popcountll(mask & ((1ull << lane) - 1));
+                    if (take) found[to] = r[u], found_at[to] = at[u];
+                    left += (uint32_t)__builtin_popcountll(mask);
+                }
+                wave_order();
+            }
+            for (uint32_t c = lane; c < left; c += 64) {
+                const uint64_t mine = found[c];
+                const uint32_t where = found_at[c];
+                uint32_t p = 0;
+#pragma unroll 8
+                for (uint32_t j = 0; j < left; ++j) p += found[j] > mine || (found[j] == mine && found_at[j] < where);
+                if (p < k) out(p, mine, where);
+            }
+            for (uint32_t p = left + lane; p < k; p += 64) out(p, 0, 0);
+            return;
+        }
+        // very many ranks between the best heads: a place at a time
+        const unsigned long long* list = buf + tid * (k + 2);
+        uint64_t head = heads[tid];
+        uint32_t at = 0;
+        __syncthreads();
+        for (uint32_t i = 0; i < k; ++i) {
+            const uint64_t best = wave_max_u64(head);
+            if (lane == 0) heads[wave] = best;
+            __syncthreads();
+            uint64_t most = 0;
+            for (int w = 0; w < 4; ++w) most = heads[w] > most ? heads[w] : most;
+            const unsigned long long mask = __ballot(head == most);
+            if (lane == 0) heads[4 + wave] = mask ? wave * 64 + (uint32_t)__builtin_ctzll(mask) : 256;
+            __syncthreads();
+            uint32_t owner = 256;
+            for (int w = 3; w >= 0; --w) owner = heads[4 + w] < 256 ? (uint32_t)heads[4 + w] : owner;
+            if (tid == owner) {
+                out(i, most, tid * 64 + at);
+                if (most) ++at, head = at < k ? rank_of(o, list[at]) : 0;
+            }
+            __syncthreads();
+        }
+        return;
+    }
     uint64_t rank = 0;
     int32_t token = -1;
     unsigned long long* ranks = buf;  // [beams][k], then the tokens
     uint32_t* tokens = (uint32_t*)(buf + a.beams * k);
-    if (once) {
-        const uint32_t words = chunks * (k + 2);
-        uint64_t got[kOnceBeams / 4];
-        int32_t tok[kOnceBeams / 4];
-#pragma unroll
-        for (uint32_t i = 0; i < kOnceBeams / 4; ++i) {
-            const uint32_t b = wave + 4 * i;
-            if (b < a.beams) row_merge(buf + b * words, a.scores[(uint64_t)group * a.beams + b], got[i], tok[i]);
+    if (wave == 0) {
+        uint64_t pair = lane < have ? buf[lane] : 0;
+        double o = sum != sum ? (double)NAN : m > -INFINITY ? (double)score - ((double)m + log(sum)) : 0.0;
+        if (chunks > 1) {
+            uint32_t from, place;
+            o = row_offset(buf, score);
+            merge_lists(buf + lane * (k + 2), lane < chunks, k, pair, from, place);
         }
-        __syncthreads();
-#pragma unroll
-        for (uint32_t i = 0; i < kOnceBeams / 4; ++i) {
-            const uint32_t b = wave + 4 * i;
-            if (b < a.beams && lane < k) ranks[b * k + lane] = got[i], tokens[b * k + lane] = (uint32_t)tok[i];
-        }
-        __syncthreads();
-    } else {
-        if (wave == 0) {
-            if (chunks > 1) {
-                row_merge(buf, score, rank, token);
-            } else {
-                const uint64_t pair = lane < have ? buf[lane] : 0;
-                rank = sum != sum ? kNoRank : pair ? rank_key((double)score - ((double)m + log(sum)) + (double)beam_value((uint32_t)(pair >> 32))) : 0;
-                token = sum == sum && pair ? (int32_t)~(uint32_t)pair : -1;
-            }
-        }
-        // the group: every beam's
-        unsigned long long* put = a.ranks + (uint64_t)row * 2 * k;
-        if (wave == 0 && lane < k) {
-            beam_put(put + lane, rank);
-            beam_put(put + k + lane, (uint32_t)token);
-        }
-        if (!beam_last(a.count + (uint64_t)a.groups * a.beams + group, a.beams, &flag)) return;
-        const unsigned long long* all = a.ranks + (uint64_t)group * a.beams * 2 * k;
-        for (uint32_t i = tid; i < a.beams * 2 * k; i += 256) {
-            const uint32_t b = i / (2 * k), j = i - b * 2 * k;
-            const unsigned long long x = beam_get(all + i);
-            if (j < k) ranks[b * k + j] = x;
-            else tokens[b * k + j - k] = (uint32_t)x;
-        }
-        __syncthreads();
+        rank = o != o ? kNoRank : rank_of(o, pair);
+        token = rank && rank != kNoRank ? (int32_t)~(uint32_t)pair : -1;
     }
+    // the group: every beam's
+    unsigned long long* put = a.ranks + (uint64_t)row * 2 * k;
+    if (wave == 0 && lane < k) {
+        beam_put(put + lane, rank);
+        beam_put(put + k + lane, (uint32_t)token);
+    }
+    if (!beam_last(a.count + (uint64_t)a.groups * a.beams + group, a.beams, &flag)) return;
+    const unsigned long long* all = a.ranks + (uint64_t)group * a.beams * 2 * k;
+    for (uint32_t i = tid; i < a.beams * 2 * k; i += 256) {
+        const uint32_t b = i / (2 * k), j = i - b * 2 * k;
+        const unsigned long long x = beam_get(all + i);
+        if (j < k) ranks[b * k + j] = x;
+        else tokens[b * k + j - k] = (uint32_t)x;
+    }
+    __syncthreads();
     if (wave != 0) return;
     uint32_t beam, place;
     const bool off = __ballot(lane < a.beams && ranks[lane * k] == kNoRank) != 0;
@@ -411,9 +518,9 @@ hipError_t launch_beam_select(SelectArgs a, void* scratch, hipStream_t s) {
     const uint64_t of_beams = ((uint64_t)a.beams * a.best * 3 + 1) / 2;  // (at most 48 KB)
     if (words < of_beams) words = of_beams;
     // all chunks of a group in one workgroup's LDS (32 KB at most): one exchange less
-    const uint64_t of_group = a.beams * chunks * (a.best + 2);
-    a.once = a.beams <= kOnceBeams && of_group <= 4096;
-    if (a.once && words < of_group) words = of_group;
+    const uint64_t of_group = a.beams * chunks * (a.best + 2), beside = kSelectMaxBeams + 256 + kFound + kFound / 2;
+    a.once = a.beams * chunks <= 256 && of_group <= 4096;
+    if (a.once && words < of_group + beside) words = of_group + beside;
     for (uint64_t g = 0; g < a.groups;) {  // (a grid's second dimension has 65535 workgroups)
         const uint64_t n = a.groups - g < 65535 / a.beams ? a.groups - g : 65535 / a.beams;
         SelectArgs p = a;
