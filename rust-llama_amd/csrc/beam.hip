@@ -489,10 +489,11 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
 }
 
 // Logits of a thread at a time, and of a workgroup: few rows are cut finer, to fill the CUs (4 rows of 128256
-// tokens: 252 workgroups), many into about 1024 workgroups; at most 64 chunks, which a wave's lanes merge.
+// tokens: 252 workgroups), many into about 512 workgroups (128 rows of 151936: 40.2 us; 768 the same, 1024 42, 1536 45.5,
+// 384 45.5); at most 64 chunks, which a wave's lanes merge.
 static uint32_t select_unroll(uint64_t rows, uint64_t vocabulary) { return rows * vocabulary <= (1u << 21) ? 2 : 4; }
 static uint32_t select_chunk(uint64_t rows, uint64_t vocabulary) {
-    const uint64_t unit = 1024 * select_unroll(rows, vocabulary), most = 1024 / rows < 1 ? 1 : 1024 / rows < 64 ? 1024 / rows : 64;
+    const uint64_t unit = 1024 * select_unroll(rows, vocabulary), most = 512 / rows < 1 ? 1 : 512 / rows < 64 ? 512 / rows : 64;
     uint64_t n = (vocabulary + unit - 1) / unit;
     n = n < most ? n : most;
     return (uint32_t)(((vocabulary + n - 1) / n + 3) / 4 * 4);

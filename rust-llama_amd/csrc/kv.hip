@@ -226,6 +226,8 @@ hipError_t launch_kv_pages(const PagesArgs& a, hipStream_t s) {
     const bool one = a.tokens <= 4096;
     if (a.requests <= 256 && a.tokens <= 1024)
         hipLaunchKernelGGL((pages_plan_kernel<256, 1>), dim3(1), dim3(256), 0, s, a, 1u);
+    else if (a.requests <= 1024)
+        hipLaunchKernelGGL((pages_plan_kernel<1024, 1>), dim3(1), dim3(1024), 0, s, a, one ? 1u : 0u);
     else
         hipLaunchKernelGGL((pages_plan_kernel<1024, kKvMaxRequests / 1024>), dim3(1), dim3(1024), 0, s, a, one ? 1u : 0u);
     if (!one) hipLaunchKernelGGL(pages_rows_kernel, dim3((a.tokens + 255) / 256), dim3(256), 0, s, a);
