@@ -427,7 +427,8 @@ typedef struct rlq_kv_cache {
  *   after[r] = before + more (0: ended), *count_after = what is left on the list,
  *   starts[r] = the request's first row, starts[requests] = rows in use;
  *   row t of request r: slots[t] = tables[r][p / page] * page + p % page with
- *   positions[t] = p = before + t - starts[r], out_requests[t] = r; rows behind the last: -1.
+ *   positions[t] = p = before + t - starts[r], out_requests[t] = r; rows behind the last: -1.  (-2 as the slot
+ *   of a token whose column of the table holds no page: rlq_kv_store reports it.)
  * tables and owned are [requests, width] i32; owned null: tables.  (A table whose rows
  * share pages, as after rlq_beam_reorder, has its own pages in `owned`.)  `pages` is the size
  * of the free list's memory, and page numbers on it are below that.  after may be before,

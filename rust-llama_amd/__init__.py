@@ -773,7 +773,7 @@ class Context:
         (rlq_kv_attention): row t sees the tokens up to positions[t] (int32; -1: none, the
         result is 0) of request requests[t] (int32, none given: row t is request t; -1: a row
         behind the last, left as it was), whose pages are tables[request] (int32 [requests, width]);
-        the last `window` of them if that is not 0.  scale: 1 / sqrt(dim) if none.  -> out
+        the last `window` of them if that is not 0.  scale: 1 / sqrt(dim) if none (or 0).  -> out
         [rows, heads, dim].  Rows of q and out may lie apart."""
         if stream is not None and isinstance(q, torch.Tensor) and out is None:
             with _on(stream, q):

@@ -162,8 +162,15 @@ __device__ __forceinline__ void merge_lists(const unsigned long long* list, bool
 //   k'th largest logit; it is searched bit by bit with ballots, until k to k + 3 of them reach it.  Only logits from
 //   it on, and from the k'th best so far, go to the wave's list in LDS (a few more than k at first, then fewer and
 //   fewer).  Where very many are equal, they are taken one by one instead.
-// The waves' lists are joined, then the last chunk of a row merges the chunks' sorted lists, a lane for each, and the
-// last row of a group the beams'.  One launch.
+// The waves' lists are joined and put where every workgroup can read them.  Where a group's lists are few (256, 32 KB)
+// its last workgroup takes all of them into LDS: of their first ranks the best'th bounds what can be chosen, and
+// what reaches it, some tens of candidates, is ranked by counting.  Else the last chunk of a row merges the row's
+// sorted lists, a lane for each, and the last row of the group the beams'.  One launch.
+//
+// Bound: four beams of 128256 tokens, the best 8: 15.4 us, of which the loads are 2.3, sums and lists 2.2, the waves'
+// lists 1.6, putting and counting 3.4 (252 workgroups count at one place), the choice 5.  16 groups of
+// eight beams of 151936 tokens, the best 16: 41 us; the loads alone 13.4 (5.8 TB/s), sums and lists 11 beside them
+// (30 VALU instructions a logit, eight of them the exponential), then 17 of joining.
 template <int U>
 __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
     extern __shared__ __align__(16) unsigned long long buf[];

@@ -69,7 +69,8 @@ __device__ __forceinline__ void pages_row(const PagesArgs& a, const P* starts, u
         request = (int32_t)r;
         position = after[r] - (int32_t)ahead;
         const int32_t page = a.tables[(uint64_t)r * a.width + ((uint32_t)position >> a.log_page)];
-        slot = ((int64_t)page << a.log_page) + (position & ((1 << a.log_page) - 1));
+        // (no page: no slot that a store would take or leave alone)
+        slot = page < 0 ? -2 : ((int64_t)page << a.log_page) + (position & ((1 << a.log_page) - 1));
     }
     a.out_requests[t] = request;
     a.positions[t] = position;
@@ -82,6 +83,11 @@ __device__ __forceinline__ void pages_row(const PagesArgs& a, const P* starts, u
 // anything is written.
 //
 // N threads, PER requests each.
+//
+// Bound: latencies one after another (the lengths, the ended requests' entries, the list, the tables) and the
+// barriers between: 32 requests of up to 8192 tokens, one new token each, a tenth of them ended, 6.2 us (11.6 with
+// the entries loaded 64 at a time); 256 requests that take 2000 pages 9.9, and their 65536 rows 3.7 in a launch of
+// their own.
 template <uint32_t N, uint32_t PER>
 __global__ __launch_bounds__(N) void pages_plan_kernel(PagesArgs a, uint32_t rows) {
     constexpr uint32_t kMost = N * PER, kWaves = N / 64;
@@ -223,6 +229,8 @@ __global__ __launch_bounds__(256) void pages_rows_kernel(PagesArgs a) {
 
 hipError_t launch_kv_pages(const PagesArgs& a, hipStream_t s) {
     if (a.requests == 0 || a.requests > kKvMaxRequests || a.tokens > 0x7fffffffu) return hipErrorInvalidValue;
+    // one workgroup writes 4096 rows in the time of another launch (four rounds of 1024 threads); few requests and
+    // rows: a small workgroup, whose barriers and sums are cheaper (32 requests 6.2 us, 7.0 with 1024 threads)
     const bool one = a.tokens <= 4096;
     if (a.requests <= 256 && a.tokens <= 1024)
         hipLaunchKernelGGL((pages_plan_kernel<256, 1>), dim3(1), dim3(256), 0, s, a, 1u);
@@ -337,6 +345,10 @@ __device__ __forceinline__ void store_put(uint8_t* plane, uint64_t row, uint32_t
 // before the angles are made and stored after every one has been checked: a token with an
 // error keeps its place, and q_out may be q.  Needs whole fours of rotated values (half a
 // multiple of 4, of pairs 2).
+//
+// Bound: one token: a launch, one round of loads, two barriers, 4.7 us (10.6 with loads for the check and again
+// for the store, angles before them and a library's sine); 1777 tokens of 14 query and 2 KV heads of 64 into Q8_0
+// 9.0 us for 15 MB: f64 rotation and the quantizer beside one round of latencies.
 template <uint32_t T, int N, int U>
 __global__ __launch_bounds__(N) void kv_store_kernel(StoreArgs a) {
     __shared__ double2 turn[128];  // cosine, sine
@@ -862,6 +874,15 @@ __device__ __forceinline__ float2 attn_get(const float* from) {
 // So the order in which a row is added up follows from the call's rows alone, and a row of one tile (or
 // in one slot) is added up as if it were alone.
 //
+// Two workgroups a CU (registers): one loads while the other is in its prologue or joins (32 rows of 4096 tokens, 8
+// KV heads of 128 in f16: one a CU 194 us, two 97).  Rows cut at multiples of 256 tokens instead of dealt: ragged
+// rows (32 up to 8192) 53 us, dealt 42.
+//
+// Bound: HBM where there is enough to read: one row of 131072 tokens (bf16) 102 us, 5.3 TB/s; 32 rows of 4096 f16
+// 96 us, 5.6; f32 183, 5.9; Q8_0 62, 4.6 (VALU issues during half of its cycles).  Small calls: six latencies
+// one after another (positions, pages, keys, then parts put, counted and read): 100 tokens 6.2 us, 1000 8.4,
+// 16000 21.
+//
 // The rows' tiles are counted by every workgroup: to 64 rows a lane each, else in LDS.
 template <uint32_t T, int NB>
 __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_kernel(AttnArgs a) {
@@ -878,7 +899,7 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
     // a row's request (-1: left alone), first and last token
     auto span = [&](uint32_t row, int32_t& request, int32_t& first, int32_t& last) {
         request = a.requests ? a.requests[row] : (int32_t)row, last = a.positions[row];
-        first = a.window && (uint32_t)(last + 1) > a.window ? last + 1 - (int32_t)a.window : 0;
+        first = a.window && (uint32_t)last + 1 > a.window ? (int32_t)((uint32_t)last + 1 - a.window) : 0;
         if (request >= 0 && (uint32_t)request < a.table_rows && last >= -1 && last < (int64_t)a.width << a.c.log_page) return;
         if (request != -1) report_error(a.err_word, bounds_key(a.row0 + row));
         request = -1;
@@ -1148,6 +1169,7 @@ static uint32_t attn_rows(const AttnArgs& a) {
 }
 size_t kv_attention_bytes(const AttnArgs& a) {
     const uint64_t group = a.heads / a.c.kv_heads, per = a.c.kv_heads * ((group + 15) / 16);
+    if (attn_slots(a) == 1) return 0;  // (every row in one slot)
     return per * attn_slots(a) * 2 * (group < 16 ? group : 16) * (a.c.dim + 2) * sizeof(float);
 }
 uint64_t kv_attention_counters(const AttnArgs& a) {
@@ -1209,6 +1231,10 @@ hipError_t launch_kv_attention(AttnArgs a, hipStream_t s) {
 // is being filled is each beam's own: its first tokens are copied, in every tensor.
 // A thread takes one column, or one piece at one place of all beams' pages: it has
 // loaded all before it stores any, so the beams may change places among themselves.
+//
+// Bound: the stores: eight groups of eight beams, 16 tensors of 8 heads of 57 rows of 256 bytes, 32 us (with branches
+// between the loads the pieces went through scratch memory: 61); one group of four in two layers 3.8 us, two
+// latencies and a launch.
 //
 // grid: runs of pieces (or of columns), groups, tensors (the tables first).
 // (lane b holds beam b's page and that of its parent; lanes behind the last beam the first beam's.  A beam
@@ -1286,7 +1312,9 @@ hipError_t launch_beam_reorder(ReorderArgs a, hipStream_t s) {
     const uint64_t units = (uint64_t)a.groups * a.n_tensors * a.kv_heads, most = ((a.row_bytes << a.log_page) / 16 + 255) / 256;
     a.slices = units >= 2048 ? 1 : (uint32_t)((2048 + units - 1) / units);
     if (a.slices > most) a.slices = (uint32_t)most;
-    const dim3 grid(a.kv_heads * a.slices, a.groups, 1 + a.n_tensors), block(256);
+    // (a launch of 2^32 threads would not run whole)
+    const uint64_t x = (uint64_t)a.kv_heads * a.slices, fits = (1ull << 31) / ((uint64_t)a.groups * (1 + a.n_tensors) * 256);
+    const dim3 grid((uint32_t)(x < fits ? x : fits < 1 ? 1 : fits), a.groups, 1 + a.n_tensors), block(256);
     if (a.beams <= 4) hipLaunchKernelGGL(beam_reorder_kernel<4>, grid, block, 0, s, a);
     else if (a.beams <= 8) hipLaunchKernelGGL(beam_reorder_kernel<8>, grid, block, 0, s, a);
     else if (a.beams <= 16) hipLaunchKernelGGL(beam_reorder_kernel<16>, grid, block, 0, s, a);

@@ -67,7 +67,8 @@ def pages(before, more, tables, owned, free, count, page, tokens):
             tables[r, c] = own[r, c] = p
         for i in range(m):
             t, pos = starts[-1] + i, b + i
-            slots[t], positions[t], requests[t] = int(tables[r, pos // page]) * page + pos % page, pos, r
+            p = int(tables[r, pos // page])
+            slots[t], positions[t], requests[t] = -2 if p < 0 else p * page + pos % page, pos, r
         after.append(end)
         starts.append(starts[-1] + m)
     return (np.array(after, np.int32), np.array([len(stack)], np.int32), np.array(starts, np.int32), slots, positions,

@@ -160,6 +160,39 @@ def test_attention_rows_of_few_and_many_requests(ctx):
     assert (got == 0).all()
 
 
+@pytest.mark.parametrize("rows", [63, 64, 65, 255, 1023, 1024, 1025, 2100])
+def test_attention_row_counts(ctx, rows):
+    """Rows counted by lanes, in LDS, and over several launches; with and without requests, empty rows among them."""
+    say("attention rows", rows)
+    rng = np.random.default_rng(rows)
+    attend(ctx, rng, DT.F16, rows, 2, 1, 32, 16, 20)
+    positions = np.where(np.arange(rows) % 7 == 0, -1, rng.integers(0, 300, rows))
+    requests = np.where(np.arange(rows) % 11 == 0, -1, np.arange(rows) % 3)
+    attend(ctx, rng, DT.F16, rows, 2, 1, 32, 16, 300, positions=positions, requests=requests, table_rows=3)
+
+
+def test_attention_at_the_last_position(ctx):
+    """A position at the end of 32 bits: a window over the last pages of a table that names few."""
+    say("attention last position")
+    cache = rlq.KvCache.make(DT.F16, 3, 1, 256, 32)
+    k, v = fill(np.random.default_rng(1), cache)
+    width = 2 ** 31 // 256
+    tables = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    tables[0, -2:] = torch.tensor([2, 1], dtype=torch.int32, device="cuda")
+    q = np.random.default_rng(2).standard_normal((1, 2, 32)).astype(np.float32)
+    last = 2 ** 31 - 1
+    got = ctx.kv_attention(cache, cuda(q), tables, cuda(np.array([last], np.int32)), window=300)
+    ctx.sync()
+    flat = [x[[2, 1], 0].reshape(512, 32)[-300:] for x in (k, v)]
+    s = flat[0] @ q[0].T.astype(np.float64) * 32 ** -0.5
+    p = np.exp(s - s.max(0))
+    want = (p / p.sum(0)).T @ flat[1]
+    assert np.abs(got[0].cpu().numpy() - want).max() <= 1e-5  # (32 products and 300 weights in f32: 2^-24 (40 + 64) |v|)
+    ctx.kv_attention(cache, cuda(q), tables, cuda(np.array([last], np.int32)), window=600)
+    with raises("Bounds", 0):
+        ctx.sync()
+
+
 def test_attention_far_scores_and_scales(ctx):
     """Scores that spread over hundreds (one token has all the weight), a scale of its own, negative too."""
     rng = np.random.default_rng(4)
@@ -359,6 +392,19 @@ def test_store_many_tokens(ctx, tokens):
     store(ctx, rng, DT.Q8_0, tokens, 8, 2, 64, 128, 32, True, 2 ** 31 - 1 - tokens)
 
 
+def test_store_of_large_angles(ctx):
+    """Angles beyond the polynomial's reduction, and just before it."""
+    say("store large angles")
+    rng = np.random.default_rng(3)
+    cache = rlq.KvCache.make(DT.F32, 1, 1, 16, 64)
+    k, v = (rng.standard_normal((8, 1, 64)).astype(np.float32) for _ in range(2))
+    positions = np.array([2 ** 31 - 1, 2 ** 31 - 8, 10 ** 9 + 7, 3, 0, -5, -2 ** 31, 123456789], np.int32)
+    freqs = np.geomspace(1e-7, 1e6, 32).astype(np.float32)
+    ctx.kv_store(cache, cuda(k), cuda(v), cuda(np.arange(8)), positions=cuda(positions), freqs=cuda(freqs), pairs=False)
+    ctx.sync()
+    assert np.array_equal(cache.k[0, 0, :8].cpu().numpy(), K.rotate(k, positions, freqs, False)[:, 0])
+
+
 def test_store_rounds_once(ctx):
     """Halfway values, subnormals and the largest value of each type; zero blocks of Q8_0."""
     say("store rounding")
@@ -487,6 +533,25 @@ def test_pages_with_holes(ctx):
     assert p.count[0] == 24 - 9 + 5 - 1
 
 
+def test_pages_of_tokens_without_a_page(ctx):
+    """A table whose part-filled page is missing: the slots say so, and the store reports them."""
+    say("pages: a missing page")
+    for tokens in (4, 5000):
+        p = Pages(2, 4, 8, 16, 3)
+        p.step(ctx, [20, 30], 50)
+        p.on["tables"][0, 1] = -1
+        _, _, _, slots, _, requests = ctx.kv_pages(p.on["lengths"], cuda(np.array([2, 1], np.int32)), p.on["tables"], p.on["free"],
+                                                   p.on["count"], 16, tokens)
+        ctx.sync()
+        assert slots[:2].tolist() == [-2, -2] and slots[2] >= 0 and (slots[3:] == -1).all() and (requests[:3] >= 0).all()
+        cache = rlq.KvCache.make(DT.F16, 8, 1, 16, 32)
+        x = torch.ones((3, 1, 32), device="cuda")
+        ctx.kv_store(cache, x, x, slots[:3].contiguous())
+        with raises("Bounds", 0):
+            ctx.sync()
+        assert cache.k.sum() == 32
+
+
 def test_pages_refusals(ctx):
     say("pages refusals")
 
@@ -605,6 +670,60 @@ def test_given_stream(ctx):
         torch.cuda.synchronize()
         assert np.array_equal(out.cpu().numpy(), got)
     ctx.sync()
+
+
+@pytest.mark.parametrize("handle", [False, True], ids=["stream", "handle"])
+@pytest.mark.parametrize("name", ["kv_pages", "kv_store", "kv_attention", "beam_select", "beam_reorder"])
+def test_calls_on_a_given_stream_beside_a_busy_one(name, handle):
+    """What a call makes is the given stream's, and it does not wait for torch's current one."""
+    say("given stream, busy", name, handle)
+    rng = np.random.default_rng(15)
+    own = rlq.Context(0)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cache = rlq.KvCache.make(DT.F16, 40, 2, 16, 64)
+    fill(rng, cache)
+    x = cuda(rng.standard_normal((4, 8, 64)).astype(np.float32))
+    slots, positions = cuda(np.array([3, 40, 77, 200])), cuda(np.array([90, 33, 5, 64], np.int32))
+    tables, freqs = cuda(rng.permutation(40).astype(np.int32).reshape(4, 10)), cuda(np.full(32, 0.1, np.float32))
+    logits, scores = cuda(rng.standard_normal((2, 2, 9000)).astype(np.float32)), torch.zeros((2, 2), device="cuda")
+    lengths, new, free = cuda(np.array([5, 20, 0, 7], np.int32)), cuda(np.array([3, 1, 4, 0], np.int32)), torch.arange(40, **i32)
+    count, same = torch.full((1,), 9, **i32), torch.full((2, 2), 20, **i32)
+    parents = cuda(np.array([[0, 0], [1, 1]], np.int32))  # (the same again changes nothing more)
+    calls = {
+        "kv_pages": lambda s: own.kv_pages(lengths, new, tables.clone() if s is None else tables, free, count, 16, 12, stream=s),
+        "kv_store": lambda s: (own.kv_store(cache, x[:, 4:6], x[:, 6:], slots, x[:, :4], positions, freqs, stream=s),),
+        "kv_attention": lambda s: (own.kv_attention(cache, x[:, :4], tables, positions, stream=s),),
+        "beam_select": lambda s: own.beam_select(logits, scores, 4, stream=s),
+        "beam_reorder": lambda s: own.beam_reorder(parents, same, tables, [cache], stream=s) or (),
+    }
+    call = calls[name]
+    want = call(None)
+    own.sync()
+    s = torch.cuda.Stream()
+    at = s.cuda_stream if handle else s
+    torch.cuda.synchronize()
+    call(at)
+    big = torch.ones((8192, 8192), device="cuda")
+    out = torch.mm(big, big)
+    torch.cuda.synchronize()
+    sizes = [k * 512 for k in (1, 2, 4, 8, 16, 24)] + [t.numel() * t.element_size() for t in want]
+    taken = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(64)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        torch.mm(big, big, out=out)
+    for t in taken:
+        t.fill_(7)
+    del t
+    taken = taken[::2]
+    got = call(at)
+    s.synchronize()
+    busy = not torch.cuda.current_stream().query()
+    torch.cuda.synchronize()
+    assert busy
+    own.sync()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    own.close()
 
 
 def test_python_checks(ctx):
