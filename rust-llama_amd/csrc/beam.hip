@@ -353,6 +353,12 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
             a.parents[to] = r ? (int32_t)(l / chunks) : -1;
             a.tokens[to] = r ? (int32_t)~(uint32_t)buf[l * (k + 2) + at % 64] : -1;
         };
+        // of two places of equal rank, whether the first is (a score far from the logits rounds them away): the lower
+        // beam's, then the larger logit's, then the lower token's
+        auto first_of = [&](uint32_t x, uint32_t y) {
+            const uint32_t bx = x / 64 / chunks, by = y / 64 / chunks;
+            return bx != by ? bx < by : buf[x / 64 * (k + 2) + x % 64] > buf[y / 64 * (k + 2) + y % 64];
+        };
         for (uint32_t b = wave; b < a.beams; b += 4) {
             const double o = row_offset(buf + b * words, a.scores[(uint64_t)group * a.beams + b]);
             if (lane == 0) offset[b] = o;
@@ -420,9 +426,11 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
             for (uint32_t c = lane; c < left; c += 64) {
                 const uint64_t mine = found[c];
                 const uint32_t where = found_at[c];
-                uint32_t p = 0;
+                uint32_t p = 0, same = 0;
 #pragma unroll 8
-                for (uint32_t j = 0; j < left; ++j) p += found[j] > mine || (found[j] == mine && found_at[j] < where);
+                for (uint32_t j = 0; j < left; ++j) p += found[j] > mine, same += found[j] == mine;
+                if (same > 1)
+                    for (uint32_t j = 0; j < left; ++j) p += found[j] == mine && first_of(found_at[j], where);
                 if (p < k) out(p, mine, where);
             }
             for (uint32_t p = left + lane; p < k; p += 64) out(p, 0, 0);
@@ -439,14 +447,23 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
             __syncthreads();
             uint64_t most = 0;
             for (int w = 0; w < 4; ++w) most = heads[w] > most ? heads[w] : most;
-            const unsigned long long mask = __ballot(head == most);
-            if (lane == 0) heads[4 + wave] = mask ? wave * 64 + (uint32_t)__builtin_ctzll(mask) : 256;
+            // of equal ones the lowest beam's, and its largest logit (two tokens are never the same pair)
+            const bool equal = head == most && most > 0;
+            const unsigned long long mask = __ballot(equal);
+            if (lane == 0) heads[4 + wave] = mask ? (wave * 64 + (uint32_t)__builtin_ctzll(mask)) / chunks : kSelectMaxBeams;
             __syncthreads();
-            uint32_t owner = 256;
-            for (int w = 3; w >= 0; --w) owner = heads[4 + w] < 256 ? (uint32_t)heads[4 + w] : owner;
-            if (tid == owner) {
+            uint32_t beam = kSelectMaxBeams;
+            for (int w = 3; w >= 0; --w) beam = heads[4 + w] < kSelectMaxBeams ? (uint32_t)heads[4 + w] : beam;
+            const uint64_t pair = equal && tid / chunks == beam ? list[at] : 0, largest = wave_max_u64(pair);
+            if (lane == 0) heads[8 + wave] = largest;
+            __syncthreads();
+            uint64_t first = 0;
+            for (int w = 0; w < 4; ++w) first = heads[8 + w] > first ? heads[8 + w] : first;
+            if (most == 0) {
+                if (tid == 0) out(i, 0, 0);
+            } else if (pair == first) {
                 out(i, most, tid * 64 + at);
-                if (most) ++at, head = at < k ? rank_of(o, list[at]) : 0;
+                ++at, head = at < k ? rank_of(o, list[at]) : 0;
             }
             __syncthreads();
         }

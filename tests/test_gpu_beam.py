@@ -92,6 +92,25 @@ def test_select_far_logits(ctx):
     choose(ctx, z, np.full((3, 2), -np.inf, np.float32), 3)
 
 
+@pytest.mark.parametrize("beams,vocabulary,best", [(1, 20000, 4), (3, 20000, 4), (3, 20000, 40), (32, 20000, 8), (32, 20000, 16), (2, 300, 8)])
+def test_select_scores_that_hide_the_logits(ctx, beams, vocabulary, best):
+    """Beside the type's lowest score every logit is rounded away: ranks are equal, a beam's order is that of its logits."""
+    say("select hidden", beams, vocabulary, best)
+    rng = np.random.default_rng(best)
+    z = rng.standard_normal((2, beams, vocabulary)).astype(np.float32)
+    scores = np.full((2, beams), np.finfo(np.float32).min, np.float32)
+    z[1, 0, np.arange(vocabulary) != 7] = -np.inf  # a live beam of one token before them
+    scores[1, 0] = 0
+    got = ctx.beam_select(cuda(z), cuda(scores), best)
+    ctx.sync()
+    for g in range(2):
+        want = [(0, 7)] if g else []
+        for b in range(g, beams):
+            want += [(b, t) for t in np.argsort(-z[g, b], kind="stable")[:best]]
+        want += [(-1, -1)] * best
+        assert [(int(p), int(t)) for p, t in zip(got[1][g].tolist(), got[2][g].tolist())] == [(b, int(t)) for b, t in want[:best]]
+
+
 def test_select_errors_are_the_groups_own(ctx):
     say("select errors")
     rng = np.random.default_rng(2)
