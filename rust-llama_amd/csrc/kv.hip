@@ -946,12 +946,13 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
         __syncthreads();
         total = start[a.rows];
     }
-    // (a row of more than kAttnParts parts would keep the one that joins them; and 32 parts of one tile are joined
-    // in the time that 16 of two take more: 4000 tokens of two KV heads of 64 13.4 us and 11.9, 16 rows of
-    // 4096 with one of 128 18.7 and 15.6)
-    const uint32_t least = (total + a.slots - 1) / a.slots;
-    const uint32_t row_least = longest > 16 && longest < 2 * kAttnParts ? 2 : (longest + kAttnParts - 1) / kAttnParts;
-    const uint32_t share = least < row_least ? row_least : least < 1 ? 1 : least;
+    // A row has kAttnParts parts at most, which one wave's lanes join: of n tiles, in twos or more, wherever it begins in its
+    // first slot, at most (n - 2) / share + 2.  And 32 parts of one tile are joined in the time that 16 of two take
+    // more: 4000 tokens of two KV heads of 64 13.4 us and 11.9, 16 rows of 4096 with one of 128 18.7 and 15.6.
+    const uint32_t least = total / a.slots + (total % a.slots != 0);
+    const uint32_t joined = longest > 16 ? (longest - 2) / (kAttnParts - 1) + 1 : 1;
+    const uint32_t row_least = longest > 16 && joined < 2 ? 2 : joined;
+    const uint32_t share = least < row_least ? row_least : least;
     const uint32_t slot = blockIdx.x / per, hc = blockIdx.x - slot * per, kvh = hc / tiles;
     const uint32_t cols = group - 16 * (hc - kvh * tiles) < 16 ? group - 16 * (hc - kvh * tiles) : 16;
     const uint32_t head0 = kvh * group + 16 * (hc - kvh * tiles);

@@ -145,6 +145,16 @@ def test_attention_long_rows_are_split(ctx, dtype):
     attend(ctx, rng, dtype, 2, 8, 8, 32, 128, 7000, window=6001)
 
 
+@pytest.mark.parametrize("lengths", [(100, 256 * 128), (100, 256 * 128 - 127), (129, 384 * 128), (100, 255 * 128 + 1, 384 * 128, 300),
+                                     (1, 128 * 128), (1, 17 * 128, 16 * 128)])
+def test_attention_rows_that_begin_inside_a_slot(ctx, lengths):
+    """A row of as many tiles as its parts may have, behind others: its first and last part are not whole."""
+    say("attention inside", lengths)
+    rng = np.random.default_rng(len(lengths))
+    for kv in (1, 2):
+        attend(ctx, rng, DT.F16, len(lengths), 2 * kv, kv, 32, 256, max(lengths), positions=np.asarray(lengths) - 1)
+
+
 def test_attention_rows_of_few_and_many_requests(ctx):
     rng = np.random.default_rng(8)
     say("attention: tokens of a prompt")
