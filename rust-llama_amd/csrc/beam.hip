@@ -169,8 +169,9 @@ __device__ __forceinline__ void merge_lists(const unsigned long long* list, bool
 //
 // Bound: four beams of 128256 tokens, the best 8: 15.4 us, of which the loads are 2.3, sums and lists 2.2, the waves'
 // lists 1.6, putting and counting 3.4 (252 workgroups count at one place), the choice 5.  16 groups of
-// eight beams of 151936 tokens, the best 16: 41 us; the loads alone 13.4 (5.8 TB/s), sums and lists 11 beside them
-// (30 VALU instructions a logit, eight of them the exponential), then 17 of joining.
+// eight beams of 151936 tokens, the best 16: 38 us; the loads alone 13.4 (5.8 TB/s), sums and lists 11 beside them
+// (30 VALU instructions a logit, eight of them the exponential; 23 of them, or twice the waves, take as long), then
+// 14 of joining.
 template <int U>
 __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
     extern __shared__ __align__(16) unsigned long long buf[];
@@ -513,8 +514,8 @@ __global__ __launch_bounds__(256) void beam_select_kernel(SelectArgs a) {
 }
 
 // Logits of a thread at a time, and of a workgroup: few rows are cut finer, to fill the CUs (4 rows of 128256
-// tokens: 252 workgroups), many into about 512 workgroups (128 rows of 151936: 40.2 us; 768 the same, 1024 42, 1536 45.5,
-// 384 45.5); at most 64 chunks, which a wave's lanes merge.
+// tokens: 252 workgroups), many into about 512 workgroups (128 rows of 151936: 38.2 us; 768 the same, 1024 39.9,
+// 384 42.7); at most 64 chunks, which a wave's lanes merge.
 static uint32_t select_unroll(uint64_t rows, uint64_t vocabulary) { return rows * vocabulary <= (1u << 21) ? 2 : 4; }
 static uint32_t select_chunk(uint64_t rows, uint64_t vocabulary) {
     const uint64_t unit = 1024 * select_unroll(rows, vocabulary), most = 512 / rows < 1 ? 1 : 512 / rows < 64 ? 512 / rows : 64;
