@@ -1199,7 +1199,7 @@ int32_t rlq_kv_attention(rlq_context* ctx, const rlq_kv_cache* cache, const floa
     const hipStream_t s = pick(ctx, stream);
     AttnArgs a{c, q, q_stride, out_stride, (uint32_t)rows, (uint32_t)heads, (uint32_t)table_rows, (uint32_t)width,
                (uint32_t)window, tables, positions, requests, scale == 0.0f ? 1.0f / sqrtf((float)c.dim) : scale, out,
-               ctx->err_words, nullptr, nullptr, 0, 0};
+               ctx->err_words, nullptr, nullptr, 0, 0, 0};
     HIP_TRY(ensure(ctx, ctx->kv, kv_attention_bytes(a), s));
     HIP_TRY(ensure_arrivals(ctx, kv_attention_counters(a), s));
     a.scratch = (float*)ctx->kv.p;

@@ -761,13 +761,9 @@ struct AttnWave {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[e][r] *= f;
         }
-        const float base = m - kTop;
+        const float base = fmaxf(m, -3.402823466e38f) - kTop;  // (a column that has no token yet: -inf is less)
 #pragma unroll
         for (int t = 0; t < 8; ++t) s[t] = __builtin_amdgcn_exp2f(s[t] - base);
-        if (!all) {  // (a column that has no token yet: -inf less -inf)
-#pragma unroll
-            for (int t = 0; t < 8; ++t) s[t] = (seen >> t) & 1 ? s[t] : 0.0f;
-        }
         l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     }
 
@@ -780,6 +776,27 @@ struct AttnWave {
             for (int k = 0; k < kWords; ++k) vw[t][k] = 0;
             vs[t] = 0;
         }
+    }
+
+    // The tokens (bits) of which this lane holds a value that is not finite.
+    __device__ __forceinline__ uint32_t not_finite() const {
+        uint32_t off = 0;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            constexpr uint32_t e = T == kF32 ? 0x7f800000u : T == kBF16 ? 0x7f80u : 0x7c00u;
+            bool some = false;
+            if constexpr (T == kQ8_0) {
+                some = (vs[t] & e) == e || (vs[t] & e << 16) == e << 16;
+            } else {
+#pragma unroll
+                for (int k = 0; k < kWords; ++k) {
+                    some |= (vw[t][k] & e) == e;
+                    if constexpr (T != kF32) some |= (vw[t][k] & e << 16) == e << 16;
+                }
+            }
+            off |= (uint32_t)some << t;
+        }
+        return off;
     }
 
     __device__ __forceinline__ void products(const float (&p)[8]) {
@@ -874,6 +891,14 @@ __device__ __forceinline__ float2 attn_get(const float* from) {
 // So the order in which a row is added up follows from the call's rows alone, and a row of one tile (or
 // in one slot) is added up as if it were alone.
 //
+// Rows one behind the other of one request at one position after the other (a prompt's tokens, drafted ones) go
+// together where their heads of a KV head fit a tile's 16 columns: `pack` rows at most read their tokens once.
+// They differ in the first and last tokens only, which each column masks for itself; a value there that is no finite number
+// is taken out and makes the columns that see it none.  With 4 query heads of 128 a KV head, f16: a prompt of 4000
+// tokens 2500 us apart, 765 together; five drafted rows of each of 32 requests up to 8192 158 and 79.  Not where the
+// rows apart have no more tiles than there are slots: five rows of 1000 tokens 10 us apart, on CUs of their own, 16
+// together.
+//
 // Two workgroups a CU (registers): one loads while the other is in its prologue or joins (32 rows of 4096 tokens, 8
 // KV heads of 128 in f16: one a CU 194 us, two 97).  Rows cut at multiples of 256 tokens instead of dealt: ragged
 // rows (32 up to 8192) 53 us, dealt 42.
@@ -887,14 +912,15 @@ __device__ __forceinline__ float2 attn_get(const float* from) {
 template <uint32_t T, int NB>
 __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_kernel(AttnArgs a) {
     constexpr uint32_t kDim = 32 * NB, kLine = kDim + 2, kV = (kDim + 127) / 128;
-    __shared__ uint32_t start[kAttnRows + 1], sums[4], mosts[4];
+    __shared__ uint32_t start[kAttnRows + 1], sums[4], mosts[4], begins[4];
     __shared__ int32_t firsts[kAttnRows], lasts[kAttnRows], of[kAttnRows];
+    __shared__ uint8_t size[kAttnRows];
     __shared__ __align__(16) float part[4][16][kLine];  // of a wave and column: values
     __shared__ float wave_m[4][16], wave_l[4][16];
     __shared__ uint32_t last_one;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, g = lane >> 4;
     const uint32_t group = a.heads / a.c.kv_heads, tiles = (group + 15) / 16, per = a.c.kv_heads * tiles;
-    const uint32_t line = (group < 16 ? group : 16) * (kDim + 2);  // floats of a part
+    const uint32_t pack = a.pack, line = (group < 16 ? pack * group : 16) * (kDim + 2);  // floats of a part
 
     // a row's request (-1: left alone), first and last token
     auto span = [&](uint32_t row, int32_t& request, int32_t& first, int32_t& last) {
@@ -904,41 +930,104 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
         if (request != -1) report_error(a.err_word, bounds_key(a.row0 + row));
         request = -1;
     };
+    auto follows = [](int32_t request, int32_t last, int32_t request0, int32_t last0) {  // the row before
+        return request >= 0 && request == request0 && last0 >= 0 && last - 1 == last0;
+    };
     auto tiles_of = [](int32_t first, int32_t last) { return last < 0 ? 1u : ((uint32_t)last >> 7) - ((uint32_t)first >> 7) + 1; };
     const bool few = a.rows <= 64;
-    int32_t my_request = -1, my_first = 0, my_last = -1;  // few: of row `lane`
-    uint32_t my_start = 0, my_tiles = 0, total, longest;
+    // few: of row `lane`; the first of those that go together has their number and their tiles, the others none
+    int32_t my_request = -1, my_first = 0, my_last = -1;
+    uint32_t my_rows = 1, my_start = 0, my_tiles = 0, total, longest;
     if (few) {
         if (lane < a.rows) span(lane, my_request, my_first, my_last);
         my_tiles = my_request >= 0 ? tiles_of(my_first, my_last) : 0;
-        const uint32_t sum = wave_scan_u32(my_tiles);
+        uint32_t sum = wave_scan_u32(my_tiles);
+        total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        const bool on = follows(my_request, my_last, __shfl_up(my_request, 1, 64), __shfl_up(my_last, 1, 64)) && lane > 0;
+        const unsigned long long breaks = __ballot(!on);
+        if (pack > 1 && total > a.slots && ~breaks) {
+            const uint32_t run = 63 - (uint32_t)__builtin_clzll(breaks & ((2ull << lane) - 1));
+            const unsigned long long heads = __ballot((lane - run) % pack == 0), after = lane < 63 ? heads >> (lane + 1) : 0;
+            my_rows = (heads >> lane) & 1 ? (after ? (uint32_t)__builtin_ctzll(after) + 1 : 64 - lane) : 0;
+            my_tiles = my_request >= 0 && my_rows ? tiles_of(my_first, my_last + (int32_t)(my_rows - 1)) : 0;
+            sum = wave_scan_u32(my_tiles);
+            total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        }
         my_start = sum - my_tiles;
-        total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63), longest = wave_max_u32(my_tiles);
+        longest = wave_max_u32(my_tiles);
     } else {
         constexpr uint32_t kMine = kAttnRows / 256;
-        uint32_t n[kMine], mine = 0, most = 0;
+        uint32_t n[kMine], begin = 0, sum, mine;  // begin: the last of the thread's rows that does not follow the one before
+        bool on[kMine], any = false;
+        int32_t request0 = -1, last0 = -1;
+        const uint32_t row0 = tid * kMine;
+        if (row0 > 0 && row0 < a.rows) request0 = a.requests ? a.requests[row0 - 1] : -1, last0 = a.positions[row0 - 1];
 #pragma unroll
         for (uint32_t k = 0; k < kMine; ++k) {
-            const uint32_t row = tid * kMine + k;
-            n[k] = 0;
+            const uint32_t row = row0 + k;
+            n[k] = 0, on[k] = false;
             if (row >= a.rows) continue;
             int32_t request, first, last;
             span(row, request, first, last);
-            firsts[row] = first, lasts[row] = last, of[row] = request;
+            on[k] = follows(request, last, request0, last0);
+            request0 = request, last0 = last;
+            firsts[row] = first, lasts[row] = last, of[row] = request, size[row] = 1;
             n[k] = request >= 0 ? tiles_of(first, last) : 0;
-            mine += n[k], most = n[k] > most ? n[k] : most;
+            begin = on[k] ? begin : row;
+            any |= on[k];
         }
-        uint32_t sum = wave_scan_u32(mine);
-        most = wave_max_u32(most);
-        if (lane == 63) sums[wave] = sum, mosts[wave] = most;
-        __syncthreads();
+        auto scan = [&] {  // of the rows' tiles
+            mine = 0;
+            uint32_t most = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < kMine; ++k) mine += n[k], most = n[k] > most ? n[k] : most;
+            sum = wave_scan_u32(mine);
+            most = wave_max_u32(most);
+            if (lane == 63) sums[wave] = sum, mosts[wave] = most;
+        };
+        scan();
+        any = __syncthreads_or(any);
+        total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        if (pack > 1 && total > a.slots && any) {
+            // the beginning of the row's run, of all threads before this one
+            uint32_t upto = begin;
+            for (int m = 1; m < 64; m <<= 1) {
+                const uint32_t o = __shfl_up(upto, m, 64);
+                upto = (int)lane >= m && o > upto ? o : upto;
+            }
+            if (lane == 63) begins[wave] = upto;
+            upto = __shfl_up(upto, 1, 64);
+            upto = lane ? upto : 0;
+            __syncthreads();
+            for (uint32_t w = 0; w < wave; ++w) upto = begins[w] > upto ? begins[w] : upto;
+#pragma unroll
+            for (uint32_t k = 0; k < kMine; ++k) {
+                const uint32_t row = row0 + k;
+                if (row >= a.rows) continue;
+                upto = on[k] ? upto : row;
+                const uint32_t at = (row - upto) % pack;
+                if (at) size[row] = 0;
+                // (the last of those that go together tells the first)
+                const bool end = row + 1 == a.rows || at + 1 == pack || !follows(of[row + 1], lasts[row + 1], of[row], lasts[row]);
+                if (at && end) size[row - at] = (uint8_t)(at + 1);
+            }
+            __syncthreads();
+#pragma unroll
+            for (uint32_t k = 0; k < kMine; ++k) {
+                const uint32_t row = row0 + k;
+                if (row >= a.rows) continue;
+                n[k] = of[row] >= 0 && size[row] ? tiles_of(firsts[row], lasts[row] + (size[row] - 1)) : 0;
+            }
+            scan();
+            __syncthreads();
+        }
         sum -= mine;
         longest = 0;
         for (uint32_t w = 0; w < 4; ++w) longest = mosts[w] > longest ? mosts[w] : longest;
         for (uint32_t w = 0; w < wave; ++w) sum += sums[w];
 #pragma unroll
         for (uint32_t k = 0; k < kMine; ++k) {
-            const uint32_t row = tid * kMine + k;
+            const uint32_t row = row0 + k;
             if (row <= a.rows) start[row] = sum;
             sum += n[k];
             if (row + 1 == kAttnRows) start[kAttnRows] = sum;
@@ -954,7 +1043,8 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
     const uint32_t row_least = longest > 16 && joined < 2 ? 2 : joined;
     const uint32_t share = least < row_least ? row_least : least;
     const uint32_t slot = blockIdx.x / per, hc = blockIdx.x - slot * per, kvh = hc / tiles;
-    const uint32_t cols = group - 16 * (hc - kvh * tiles) < 16 ? group - 16 * (hc - kvh * tiles) : 16;
+    const uint32_t wide = group - 16 * (hc - kvh * tiles) < 16 ? group - 16 * (hc - kvh * tiles) : 16;  // heads of a row
+    const uint32_t my_row = i / wide;  // column i's among those that go together
     const uint32_t head0 = kvh * group + 16 * (hc - kvh * tiles);
     const uint64_t plane = kvh * kv_plane<T>(kDim, a.c.log_page);
     const uint32_t mask = (1u << a.c.log_page) - 1;
@@ -963,87 +1053,116 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
 
     uint32_t next;
     for (uint64_t tile = (uint64_t)slot * share; tile < end; tile = next) {
-        uint32_t row, row0, row1;
-        int32_t request, first, last;
+        uint32_t row, row0, row1, rows;
+        int32_t request, first, last;  // last: the first row's
         if (few) {
             row = 63 - (uint32_t)__builtin_clzll(__ballot(my_tiles > 0 && my_start <= tile));
             row0 = (uint32_t)__builtin_amdgcn_readlane((int)my_start, (int)row);
             row1 = row0 + (uint32_t)__builtin_amdgcn_readlane((int)my_tiles, (int)row);
             request = __builtin_amdgcn_readlane(my_request, (int)row);
             first = __builtin_amdgcn_readlane(my_first, (int)row), last = __builtin_amdgcn_readlane(my_last, (int)row);
+            rows = (uint32_t)__builtin_amdgcn_readlane((int)my_rows, (int)row);
         } else {
             row = (uint32_t)__builtin_amdgcn_readfirstlane((int)segment_of(start, a.rows, (uint32_t)tile));
             row0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)start[row]);
             row1 = (uint32_t)__builtin_amdgcn_readfirstlane((int)start[row + 1]);
             request = __builtin_amdgcn_readfirstlane(of[row]);
             first = __builtin_amdgcn_readfirstlane(firsts[row]), last = __builtin_amdgcn_readfirstlane(lasts[row]);
+            rows = (uint32_t)__builtin_amdgcn_readfirstlane((int)size[row]);
         }
         next = row1 < end ? row1 : end;
         const uint32_t slot0 = row0 / share, parts = (row1 - 1) / share - slot0 + 1;
-        // tokens t0 .. t1 of this segment, from a tile's beginning on
-        const int64_t from = ((int64_t)((uint32_t)first >> 7) + (int64_t)(tile - row0)) << 7;
-        const int64_t to = from + ((int64_t)(next - tile) << 7) - 1;
-        const int64_t t0 = from > first ? from : first, t1 = to < last ? to : last;
+        const uint32_t cols = rows * wide;
+        // of the segment's tokens, t0 to before t1 (from a tile's beginning on), column i sees s0 to before s1, all
+        // columns see a0 to before a1 (positions are below 2^31)
+        const uint32_t from = (((uint32_t)first >> 7) + (uint32_t)(tile - row0)) << 7, to = from + ((uint32_t)(next - tile) << 7);
+        const uint32_t seen0 = (uint32_t)last + 1;  // that the first row sees
+        auto first_of = [&](uint32_t k) { return a.window && seen0 + k > a.window ? seen0 + k - a.window : 0; };  // row k
+        const uint32_t t0 = from > (uint32_t)first ? from : (uint32_t)first, t1 = to < last + rows ? to : last + rows;
+        const uint32_t mine_of = my_row < rows ? my_row : rows - 1;  // (columns behind the last: as the last row's)
+        const uint32_t fm = first_of(mine_of), s0 = t0 > fm ? t0 : fm, s1 = t1 < seen0 + mine_of ? t1 : seen0 + mine_of;
+        const uint32_t fa = first_of(rows - 1), a0 = t0 > fa ? t0 : fa, a1 = t1 < seen0 ? t1 : seen0;
 
         AttnWave<T, NB> w;
         const int32_t* table = a.tables + (uint64_t)request * a.width;
         bool lost = false;
         int32_t id = 0;
+        uint32_t c0 = from;
         // lane k: the page of the sixteen tokens from c0 + 16 k on
-        auto pages = [&](int64_t c0) {
-            const int64_t at = c0 + 16 * lane;
+        auto pages = [&](uint32_t c0) {
+            const uint32_t at = c0 + 16 * lane;
             id = 0;
-            if (at <= t1 && at + 15 >= t0) id = table[at >> a.c.log_page];
+            if (at < t1 && at + 16 > t0) id = table[at >> a.c.log_page];
         };
         auto check = [&] {
-            if (id < 0 || (uint64_t)id >= a.c.pages) lost = true, id = 0;
+            const bool off = id < 0 || (uint64_t)id >= a.c.pages;
+            for (unsigned long long m = __ballot(off); m; m &= m - 1) {  // (a column that sees none of its tokens keeps on)
+                const uint32_t at = c0 + 16 * (uint32_t)__builtin_ctzll(m);
+                lost |= at < s1 && at + 16 > s0;
+            }
+            if (off) id = 0;
         };
-        int64_t c0 = from;
-        auto page = [&](int64_t t) { return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(id, (int)((t - c0) >> 4)); };
-        auto load_k = [&](int64_t t) {
+        auto page = [&](uint32_t t) { return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(id, (int)((t - c0) >> 4)); };
+        auto load_k = [&](uint32_t t) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                w.load_k(h, a.c.k + page(t + 16 * h) * a.c.k_stride + plane, (uint32_t)(t + 16 * h) & mask, a.c.log_page);
+                w.load_k(h, a.c.k + page(t + 16 * h) * a.c.k_stride + plane, (t + 16 * h) & mask, a.c.log_page);
         };
-        auto load_v = [&](int64_t t) {
+        auto load_v = [&](uint32_t t) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                w.load_v(h, a.c.v + page(t + 16 * h) * a.c.v_stride + plane, (uint32_t)(t + 16 * h) & mask, a.c.log_page);
+                w.load_v(h, a.c.v + page(t + 16 * h) * a.c.v_stride + plane, (t + 16 * h) & mask, a.c.log_page);
         };
         pages(c0);
-        w.load_q(a.q + row * a.q_stride + (uint64_t)(head0 + i) * kDim, i < cols);
+        w.load_q(a.q + (row + my_row) * a.q_stride + (uint64_t)(head0 + i - my_row * wide) * kDim, i < cols);
         check();
-        if (c0 + 32 * wave <= t1) load_k(c0 + 32 * wave), load_v(c0 + 32 * wave);
+        if (c0 + 32 * wave < t1) load_k(c0 + 32 * wave), load_v(c0 + 32 * wave);
         w.start(a.scale);
         for (;;) {
-            const int64_t c1 = c0 + 1023 < t1 ? c0 + 1023 : t1;
-            for (int64_t t = c0 + 32 * wave; t <= c1; t += 128) {
-                const bool all = t >= t0 && t + 31 <= t1, more = t + 128 <= c1;
+            const uint32_t c1 = c0 + 1024 < t1 ? c0 + 1024 : t1;
+            for (uint32_t t = c0 + 32 * wave; t < c1; t += 128) {
+                const bool all = t >= a0 && t + 32 <= a1, more = t + 128 < c1;
                 uint32_t seen = 0;
                 if (!all) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const int64_t tok = t + 16 * (k / 4) + 4 * g + k % 4;
-                        seen |= (uint32_t)(tok >= t0 && tok <= t1) << k;
+                        const uint32_t tok = t + 16 * (k / 4) + 4 * g + k % 4;
+                        seen |= (uint32_t)(tok >= s0 && tok < s1) << k;
                     }
                 }
                 float s[8];
                 w.scores(s);
                 if (more) load_k(t + 128);
                 w.weights(s, all, seen);
-                if (!all) w.drop(seen);
+                if (!all) {
+                    uint32_t some = seen;
+                    if (rows > 1) {  // the tokens that some column sees and whose values all are finite
+                        uint32_t off = w.not_finite();
+                        some = 0;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const uint32_t tok = t + 16 * (k / 4) + 4 * g + k % 4;
+                            some |= (uint32_t)(tok >= t0 && tok < t1) << k;
+                        }
+                        off |= __shfl_xor(off, 1, 64), off |= __shfl_xor(off, 2, 64);
+                        off |= __shfl_xor(off, 4, 64), off |= __shfl_xor(off, 8, 64);
+                        if (off & seen) w.l = NAN;
+                        some &= ~off;
+                    }
+                    w.drop(some);
+                }
                 w.products(s);
                 if (more) load_v(t + 128);
             }
-            if (c0 + 1024 > t1) break;
+            if (c0 + 1024 >= t1) break;
             c0 += 1024;
             pages(c0);
             check();
-            if (c0 + 32 * wave <= t1) load_k(c0 + 32 * wave), load_v(c0 + 32 * wave);
+            if (c0 + 32 * wave < t1) load_k(c0 + 32 * wave), load_v(c0 + 32 * wave);
         }
-        if (__ballot(lost)) {  // (every segment finds its own; what is joined is then no number)
+        if (lost && i < cols) {  // (every segment finds its own; what is joined is then no number)
             w.l = NAN;
-            if (lane == 0) report_error(a.err_word, bounds_key(a.row0 + row));
+            report_error(a.err_word, bounds_key(a.row0 + row + my_row));
         }
 
         // the waves join
@@ -1069,10 +1188,10 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
                     off |= 2 * lane + 128 * k < kDim && !finite(y[k][j]);
                 }
             if (__ballot(off)) {
-                if (lane == 0) report_error(a.err_word, model_key(a.row0 + row, kStAttnOut, 0));
+                if (lane == 0) report_error(a.err_word, model_key(a.row0 + row + c / wide, kStAttnOut, 0));
                 return;
             }
-            float* out = a.out + row * a.out_stride + (uint64_t)(head0 + c) * kDim;
+            float* out = a.out + (row + c / wide) * a.out_stride + (uint64_t)(head0 + c % wide) * kDim;
 #pragma unroll
             for (uint32_t k = 0; k < kV; ++k) {
                 const uint32_t d = 2 * lane + 128 * k;
@@ -1168,10 +1287,15 @@ static uint32_t attn_rows(const AttnArgs& a) {
     const uint64_t n = 0xffffffffull / tiles;
     return (uint32_t)(n < kAttnRows ? n : kAttnRows);
 }
+// Rows that go together at most: of those that fill a tile's columns.
+static uint32_t attn_pack(const AttnArgs& a) {
+    const uint32_t group = a.heads / a.c.kv_heads;
+    return group > 8 || a.rows == 1 || !a.requests ? 1 : 16 / group;
+}
 size_t kv_attention_bytes(const AttnArgs& a) {
     const uint64_t group = a.heads / a.c.kv_heads, per = a.c.kv_heads * ((group + 15) / 16);
     if (attn_slots(a) == 1) return 0;  // (every row in one slot)
-    return per * attn_slots(a) * 2 * (group < 16 ? group : 16) * (a.c.dim + 2) * sizeof(float);
+    return per * attn_slots(a) * 2 * (group < 16 ? attn_pack(a) * group : 16) * (a.c.dim + 2) * sizeof(float);
 }
 uint64_t kv_attention_counters(const AttnArgs& a) {
     return (uint64_t)a.c.kv_heads * ((a.heads / a.c.kv_heads + 15) / 16) * attn_slots(a);
@@ -1202,6 +1326,7 @@ hipError_t launch_kv_attention(AttnArgs a, hipStream_t s) {
         a.heads % a.c.kv_heads)
         return hipErrorInvalidValue;
     a.slots = attn_slots(a);
+    a.pack = attn_pack(a);
     const uint32_t rows = a.rows, most = attn_rows(a), grid = (uint32_t)kv_attention_counters(a);
     const AttnArgs all = a;
     for (uint32_t r = 0; r < rows; r += most) {  // (the parts and counters are the same memory)

@@ -304,7 +304,7 @@ struct AttnArgs {
     unsigned long long* err_word;
     float* scratch;   // kv_attention_bytes
     uint32_t* count;  // kv_attention_counters words, 0 between launches
-    uint32_t slots, row0;  // of a launch: slots of a head, the first row
+    uint32_t slots, row0, pack;  // of a launch: slots of a head, the first row, rows that go together at most
 };
 size_t kv_attention_bytes(const AttnArgs& a);
 uint64_t kv_attention_counters(const AttnArgs& a);

@@ -292,6 +292,87 @@ def test_attention_does_not_look_at_masked_places(ctx, dtype):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("heads,kv", [(1, 1), (4, 2), (3, 1), (8, 2), (5, 1), (14, 2), (16, 2), (9, 1), (34, 2)])
+@pytest.mark.parametrize("dtype", [DT.F32, DT.F16, DT.BF16, DT.Q8_0])
+def test_attention_of_runs_of_rows(ctx, dtype, heads, kv):
+    """Rows of a request at one position after the other, in runs of all lengths, that end and begin anywhere; with rows
+    without a token, gaps, steps back and other requests between them."""
+    say("attention runs", dtype, heads, kv)
+    rng = np.random.default_rng(heads)
+    positions, requests = [], []
+    for n in (1, 2, 3, 4, 5, 7, 16, 17, 3):
+        start, r = int(rng.integers(0, 270)), int(rng.integers(0, 3))
+        positions += range(start, start + n)
+        requests += [r] * n
+    positions += [-1, 0, 1, 2, 2, 1, 4, 126, 127, 128, 129, 299]
+    requests += [1, 1, 1, 1, 1, 1, 1, 2, 2, 2, 2, -1]
+    for window in (0, 1, 40):  # (many heads or rows: they go together where there is more to do than the CUs hold)
+        attend(ctx, rng, dtype, len(positions), 8 * heads, 8 * kv, 64, 16, 300, window=window, positions=positions,
+               requests=requests, table_rows=3)
+        n = 7 * len(positions)
+        attend(ctx, rng, dtype, n, heads, kv, 32, 32, 300, window=window, positions=positions * 7, requests=requests * 7,
+               table_rows=3)
+
+
+@pytest.mark.parametrize("dtype", [DT.F16, DT.BF16, DT.Q8_0])
+def test_attention_of_long_runs(ctx, dtype):
+    """Runs over several slots; rows of a prompt that is longer than a launch's rows."""
+    say("attention long runs", dtype)
+    rng = np.random.default_rng(20)
+    positions = np.concatenate([n - 5 + np.arange(5) for n in (20000, 9000, 130, 257)])
+    attend(ctx, rng, dtype, 20, 8, 2, 128, 64, 20000, positions=positions, requests=np.repeat(np.arange(4), 5), table_rows=4)
+    attend(ctx, rng, dtype, 1500, 2, 1, 32, 16, 1600, positions=100 + np.arange(1500), requests=np.zeros(1500), table_rows=1)
+
+
+@pytest.mark.parametrize("dtype", [DT.F32, DT.F16, DT.BF16, DT.Q8_0])
+@pytest.mark.parametrize("start", [20, 125])
+def test_attention_of_runs_keeps_rows_apart(ctx, dtype, start):
+    """A value or key that is no number, or a page that is none, is the error of the rows that see it."""
+    rng = np.random.default_rng(start)
+    dim, page, n, heads = 64, 16, 6, 256  # (so many that rows go together); KV head 1 is that of heads 2 and 3
+    for window in (0, 10):
+        cache, q, tables, positions, got = attend(ctx, rng, dtype, n, heads, heads // 2, dim, page, 160, window=window,
+                                                  positions=start + np.arange(n), requests=np.zeros(n), table_rows=1)
+        req = cuda(np.zeros(n, np.int32))
+
+        def call(t, held, name, a, free=lambda r, h: False):
+            out = torch.full((n, heads, dim), 5.0, device="cuda")
+            ctx.kv_attention(cache, cuda(q), cuda(t), cuda(positions), req, window=window, out=out)
+            with raises(name, *a):
+                ctx.sync()
+            out = out.cpu().numpy()
+            for r in range(n):
+                for h in range(heads):
+                    if free(r, h):
+                        assert np.isfinite(out[r, h]).all() and (out[r, h] != 5).all()
+                        continue
+                    assert (out[r, h] == 5).all() if held(r, h) else np.array_equal(out[r, h], got[r, h]), (r, h)
+
+        for plane in (cache.k, cache.v):
+            for token, rows in ((start + 3, range(3, n)), (start - 9, [0] if window else range(n)), (start + n - 1, [n - 1])):
+                say("attention runs apart", dtype, window, token)
+                where = plane[int(tables[0, token // page]), 1]
+                kept = where.clone()
+                low = np.zeros((n, heads), bool)
+                if dtype == DT.Q8_0:  # an infinite scale
+                    where[page * dim:].view(torch.float16)[(token % page) * (dim // 32)] = float("inf")
+                    if plane is cache.k:  # a score of -infinity where the block's product is negative: a weight of 0
+                        levels = where[token % page * dim:][:32].view(torch.int8).double().cpu().numpy()
+                        low = q[..., :32] @ levels < 0
+                else:
+                    where[token % page, 5] = float("nan")
+                sees = [(r, h) for r in rows for h in (2, 3)]
+                off = [r for r, h in sees if not low[r, h]]
+                if off:
+                    call(tables, lambda r, h: (r, h) in sees, "NonFinite", (6, off[0]), lambda r, h: (r, h) in sees and low[r, h])
+                where.copy_(kept)
+        if start % page + n > page:  # the last rows' page is none
+            t = tables.copy()
+            t[0, start // page + 1] = -1
+            first = page * (start // page + 1) - start
+            call(t, lambda r, h: r >= first, "Bounds", (first,))
+
+
 def test_attention_errors_are_the_rows_own(ctx):
     say("attention errors")
     rng = np.random.default_rng(9)
