@@ -912,7 +912,7 @@ __device__ __forceinline__ float2 attn_get(const float* from) {
 template <uint32_t T, int NB>
 __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_kernel(AttnArgs a) {
     constexpr uint32_t kDim = 32 * NB, kLine = kDim + 2, kV = (kDim + 127) / 128;
-    __shared__ uint32_t start[kAttnRows + 1], sums[4], mosts[4], begins[4];
+    __shared__ uint32_t start[kAttnRows + 1], sums[4], mosts[4], begins[4], runs[4];
     __shared__ int32_t firsts[kAttnRows], lasts[kAttnRows], of[kAttnRows];
     __shared__ uint8_t size[kAttnRows];
     __shared__ __align__(16) float part[4][16][kLine];  // of a wave and column: values
@@ -986,7 +986,10 @@ __global__ __launch_bounds__(256, NB <= attn_wide(T) ? 2 : 1) void kv_attention_
             if (lane == 63) sums[wave] = sum, mosts[wave] = most;
         };
         scan();
-        any = __syncthreads_or(any);
+        const bool some_on = __ballot(any) != 0;
+        if (lane == 63) runs[wave] = some_on;
+        __syncthreads();
+        any = (runs[0] | runs[1] | runs[2] | runs[3]) != 0;
         total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
         if (pack > 1 && total > a.slots && any) {
             // the beginning of the row's run, of all threads before this one
