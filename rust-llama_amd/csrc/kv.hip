@@ -595,8 +595,8 @@ __device__ __forceinline__ float column_sum(float v) {
 // 16-bit keys and values need 2 (f16) or 3 (bf16) times 256 cycles per 32 tokens of 128 values, of
 // about 1900 that HBM takes for them (one SIMD's share).  Q8_0: scores with f16 levels, block by block, times
 // the block's scale; a value, level times scale, as the sum of two f16, which holds it exactly: a product of 18
-// bits that is a multiple of 2^-24, 127 times a scale of 515 at most (with a larger scale among
-// them the 32 tokens take f32 values on 16x16x4, 2048 cycles of the matrix cores instead of 384).
+// bits that is a multiple of 2^-24, -128 times a scale of 511.75 at most, which is f16's largest (with a larger scale
+// among them the 32 tokens take f32 values on 16x16x4, 2048 cycles of the matrix cores instead of 384).
 // Blocks of 32 values to which two workgroups' registers fit a CU (a wave's tile, queries and
 // accumulators, 256 of them).
 constexpr uint32_t attn_wide(uint32_t type) { return type == kF32 ? 3 : 4; }
@@ -826,7 +826,7 @@ struct AttnWave {
                 top = x > top ? x : top;
                 if (32 % kOwn != 0) top = y > top ? y : top;
             }
-            if (!__ballot(top > 0x6007u)) {  // f16 515.5
+            if (!__ballot(top > 0x5fffu)) {  // f16 511.75
                 uint32_t p0[4], p1[4], d0[4], d1[4];
                 split_f16(p, p0, p1);
 #pragma unroll
