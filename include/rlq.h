@@ -455,7 +455,7 @@ int32_t rlq_kv_pages(rlq_context *ctx, const int32_t *before, const int32_t *mor
  * nearest (Q8_0: as rlq_quantize_device).  Slots are distinct; of a slot named twice each
  * value is one of the tokens'.  Slot -1: a row behind the batch's last one, left alone.
  * At rlq_sync, with nothing of the token written: RLQ_TENSOR_BOUNDS (a = the token:
- * a slot outside the cache), RLQ_NON_FINITE_INPUT (a value that is not finite, or beyond
+ * a slot outside the cache), RLQ_NON_FINITE_INPUT (a value that, rotated, is not finite, or beyond
  * F16's or BF16's range; a = its index in [q | k | v], b = the token), RLQ_UNREPRESENTABLE_SCALE (Q8_0; a =
  * its block in [k | v], b = the token).  At most 8388606 tokens. */
 #define RLQ_ROPE_PAIRS 1u
