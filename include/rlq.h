@@ -473,7 +473,8 @@ int32_t rlq_kv_store(rlq_context *ctx, const rlq_kv_cache *cache, const float *q
  * was.  Several rows may be of one request (a prompt's tokens; drafted ones).
  * q, out [rows, heads, dim] f32, rows q_stride (out_stride) floats apart; tables [table_rows, width] i32.
  * scale 0: 1 / sqrt(dim).  heads a multiple of kv_heads.  Scores, weights and sums are f32 (16-bit and
- * 8-bit values taken as they are); what lies behind positions[t] or before the window is not
+ * 8-bit values taken as they are; beside F16 and Q8_0 caches queries and weights enter the products rounded to 23 bits,
+ * what is below 2^-16 of the largest to 2^-38 of that); what lies behind positions[t] or before the window is not
  * looked at.  At most 65535 rows.  At rlq_sync: RLQ_TENSOR_BOUNDS (a = the row: a request or
  * position outside the table, or a page outside the cache; its out is left as it was),
  * RLQ_NON_FINITE (a = RLQ_CHECK_ATTENTION_OUTPUT, b = the row; a query head with such a

@@ -46,3 +46,50 @@ def test_attention_of_the_lowest_level(ctx, dim, scale):
     ctx.sync()
     err = np.abs(got.double().cpu().numpy() - want)
     assert (err <= tolerance(dim, spread, most) + U * np.abs(want)).all(), err.max()
+
+
+@pytest.mark.parametrize("dtype", [DT.F32, DT.F16, DT.BF16, DT.Q8_0])
+def test_attention_of_many_small_weights(ctx, dtype):
+    """Every 32nd token takes nearly all of the weight and has no value, the others have value 1 and weights of 2^-32 to 2^-28
+    of that: the result is the sum of those.
+
+    Worst case of f32, relative to the result: a score (33 at most, to base 2) is off by nine roundings (its query times
+    scale, the query's terms, four partial sums, the difference to the maximum), 9 * 33 * U * ln 2 = 1.2e-5; a weight by half of
+    f16's least step, 2^-39 of the largest one's, up or down, so that 10000 of them are by five standard deviations
+    4.1e-5 of the sum; the sum itself by some 100 roundings, 6e-6.  1e-4 is beyond all of them, and weights cut towards zero
+    would be off by 1.4e-3."""
+    say("attention small weights", dtype)
+    rng = np.random.default_rng(77)
+    n, heads, dim, page = 20001, 4, 64, 64
+    width = -(-n // page)
+    cache = rlq.KvCache.make(dtype, width, 1, page, dim)
+    far = -rng.uniform(28, 32, width * page) * np.log(2)
+    far[::32] = 0
+    if dtype == DT.Q8_0:
+        d = rng.uniform(0.2, 0.25, width * page).astype(np.float16)
+        kl, vl = (np.zeros((width * page, dim), np.int8) for _ in range(2))
+        kl[:, 0], kl[:, 1], vl[:] = np.round(far / d), rng.integers(-128, 128, width * page), 64
+        kl[::32, 1], vl[::32] = 0, 0
+        ks, vs = np.repeat(d[:, None], dim // 32, 1), np.full((width * page, dim // 32), 2.0 ** -6, np.float16)
+        planes = []
+        for t, levels, scales in ((cache.k, kl, ks), (cache.v, vl, vs)):
+            b = np.concatenate([levels.reshape(width, 1, -1).view(np.uint8), scales.reshape(width, 1, -1).view(np.uint8)], -1)
+            t.copy_(cuda(b))
+            planes.append(K.values(b, True, page, dim))
+    else:
+        k, v = (np.zeros((width * page, dim), np.float32) for _ in range(2))
+        k[:, 0], k[:, 1], v[:] = far, rng.uniform(-1, 1, width * page), 1
+        k[::32, 1], v[::32] = 0, 0
+        for t, x in ((cache.k, k), (cache.v, v)):
+            t.copy_(cuda(x.reshape(width, 1, page, dim), t.dtype))
+        planes = [t.double().cpu().numpy() for t in (cache.k, cache.v)]
+    q = np.zeros((2, heads, dim), np.float32)
+    q[..., 0], q[..., 1] = 1 - np.arange(heads) / 64, 2.0 ** -7
+    tables, positions = np.arange(width, dtype=np.int32).reshape(1, -1), np.array([n - 1, n // 2], np.int32)
+    requests = np.zeros(2, np.int32)
+    want, _, _ = K.attention(*planes, q, tables, positions, requests, 1.0, 0, np.zeros_like(q))
+    got = ctx.kv_attention(cache, cuda(q), cuda(tables), cuda(positions), cuda(requests), 1.0)
+    ctx.sync()
+    err = np.abs(got.double().cpu().numpy() / want - 1)
+    print("relative error", err.max(), flush=True)
+    assert err.max() <= 1e-4
