@@ -1224,10 +1224,11 @@ int32_t rlq_beam_select(rlq_context* ctx, const float* logits, uint64_t stride, 
     if (!aligned({logits, scores, out_scores, parents, tokens}, 4)) return fail(err, RLQ_INVALID_ARGUMENT);
     DeviceGuard g(ctx->device);
     const hipStream_t s = pick(ctx, stream);
-    HIP_TRY(ensure(ctx, ctx->kv, beam_select_bytes(groups * beams, vocabulary, best), s));
-    HIP_TRY(ensure_arrivals(ctx, groups * beams + groups, s));
-    const SelectArgs a{logits, stride, scores, (uint32_t)groups, (uint32_t)beams, (uint32_t)vocabulary, (uint32_t)best,
-                       out_scores, parents, tokens, ctx->err_words, (uint32_t*)ctx->arrivals.p, 0, 0, 0, nullptr, nullptr};
+    SelectArgs a{logits, stride, scores, (uint32_t)groups, (uint32_t)beams, (uint32_t)vocabulary, (uint32_t)best,
+                 out_scores, parents, tokens, ctx->err_words, nullptr, 0, 0, 0, nullptr, nullptr};
+    HIP_TRY(ensure(ctx, ctx->kv, beam_select_bytes(a), s));
+    HIP_TRY(ensure_arrivals(ctx, beam_select_counters(a), s));
+    a.count = (uint32_t*)ctx->arrivals.p;
     HIP_TRY(launch_beam_select(a, ctx->kv.p, s));
     return ok(err);
 }

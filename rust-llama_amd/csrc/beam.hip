@@ -527,28 +527,37 @@ static uint64_t select_chunks(uint64_t rows, uint64_t vocabulary) {
     const uint64_t c = select_chunk(rows, vocabulary);
     return (vocabulary + c - 1) / c;
 }
-size_t beam_select_bytes(uint64_t rows, uint64_t vocabulary, uint64_t best) {
-    return rows * (select_chunks(rows, vocabulary) * (best + 2) + 2 * best) * sizeof(unsigned long long);
+// Groups of a launch (a grid's second dimension has 65535 workgroups), which use the same scratch and counters.
+static uint64_t select_groups(const SelectArgs& a) { return a.groups < 65535 / a.beams ? a.groups : 65535 / a.beams; }
+// Whether all chunks of a group go through one workgroup's LDS (32 KB at most): one exchange less.
+static bool select_once(const SelectArgs& a, uint64_t chunks) {
+    return a.beams * chunks <= 256 && a.beams * chunks * (a.best + 2) <= 4096;
 }
+size_t beam_select_bytes(const SelectArgs& a) {
+    const uint64_t chunks = select_chunks((uint64_t)a.groups * a.beams, a.vocabulary);
+    const bool once = select_once(a, chunks);
+    const uint64_t lists = chunks > 1 || once ? chunks * (a.best + 2) : 0, ranks = once ? 0 : 2 * a.best;
+    return select_groups(a) * a.beams * (lists + ranks) * sizeof(unsigned long long);
+}
+uint64_t beam_select_counters(const SelectArgs& a) { return select_groups(a) * (a.beams + 1); }
 
 hipError_t launch_beam_select(SelectArgs a, void* scratch, hipStream_t s) {
     if (a.groups == 0 || a.groups > 65535 || a.beams == 0 || a.beams > kSelectMaxBeams || a.best == 0 ||
         a.best > kSelectMaxBest || a.vocabulary == 0)
         return hipErrorInvalidValue;
-    const uint64_t rows = (uint64_t)a.groups * a.beams, chunks = select_chunks(rows, a.vocabulary);
+    const uint64_t rows = (uint64_t)a.groups * a.beams, chunks = select_chunks(rows, a.vocabulary), most = select_groups(a);
     a.chunk = select_chunk(rows, a.vocabulary);
+    a.once = select_once(a, chunks);
     a.ranks = (unsigned long long*)scratch;
-    a.lists = a.ranks + rows * 2 * a.best;
+    a.lists = a.ranks + (a.once ? 0 : most * a.beams * 2 * a.best);
     uint64_t words = chunks > 1 ? chunks * (a.best + 2) : 0;
     if (words < 4 * kListMost) words = 4 * kListMost;
     const uint64_t of_beams = ((uint64_t)a.beams * a.best * 3 + 1) / 2;  // (at most 48 KB)
     if (words < of_beams) words = of_beams;
-    // all chunks of a group in one workgroup's LDS (32 KB at most): one exchange less
     const uint64_t of_group = a.beams * chunks * (a.best + 2), beside = kSelectMaxBeams + 256 + kFound + kFound / 2;
-    a.once = a.beams * chunks <= 256 && of_group <= 4096;
     if (a.once && words < of_group + beside) words = of_group + beside;
-    for (uint64_t g = 0; g < a.groups;) {  // (a grid's second dimension has 65535 workgroups)
-        const uint64_t n = a.groups - g < 65535 / a.beams ? a.groups - g : 65535 / a.beams;
+    for (uint64_t g = 0; g < a.groups;) {
+        const uint64_t n = a.groups - g < most ? a.groups - g : most;
         SelectArgs p = a;
         p.logits += g * a.beams * a.stride, p.scores += g * a.beams;
         p.out_scores += g * a.best, p.parents += g * a.best, p.tokens += g * a.best;

@@ -333,12 +333,13 @@ struct SelectArgs {
     float* out_scores;
     int32_t *parents, *tokens;
     unsigned long long* err_word;
-    uint32_t* count;  // a word for each beam and group, 0 between launches
+    uint32_t* count;  // beam_select_counters words, 0 between launches
     // of a launch: tokens of a workgroup, the first group; scratch (beam_select_bytes)
     uint32_t chunk, group0, once;
     unsigned long long *ranks, *lists;
 };
-size_t beam_select_bytes(uint64_t rows, uint64_t vocabulary, uint64_t best);
+size_t beam_select_bytes(const SelectArgs& a);
+uint64_t beam_select_counters(const SelectArgs& a);
 hipError_t launch_beam_select(SelectArgs a, void* scratch, hipStream_t s);
 
 // ---- llama.hip ----
