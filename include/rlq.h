@@ -453,7 +453,8 @@ int32_t rlq_kv_pages(rlq_context *ctx, const int32_t *before, const int32_t *mor
  * angles are the reference's, multiplied up in f32.)  half 0: no rotation (positions and freqs are
  * not looked at).  q and q_out may be null (heads 0), and q_out may be q.  The cache's values are those f32, rounded to
  * nearest (Q8_0: as rlq_quantize_device).  Slots are distinct; of a slot named twice each
- * value is one of the tokens'.  Slot -1: a row behind the batch's last one, left alone.
+ * value is one of the tokens' (Q8_0: each level and each scale, so a value may be one's level with
+ * another's scale).  Slot -1: a row behind the batch's last one, left alone.
  * At rlq_sync, with nothing of the token written: RLQ_TENSOR_BOUNDS (a = the token:
  * a slot outside the cache), RLQ_NON_FINITE_INPUT (a value that, rotated, is not finite, or beyond
  * F16's or BF16's range; a = its index in [q | k | v], b = the token), RLQ_UNREPRESENTABLE_SCALE (Q8_0; a =

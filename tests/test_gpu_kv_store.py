@@ -1,4 +1,4 @@
-"""rlq_kv_store: the place that an error names, within the four values of a thread too."""
+"""rlq_kv_store: the place that an error names, within the four values of a thread too, and slots named twice."""
 import numpy as np
 import pytest
 
@@ -59,3 +59,36 @@ def test_store_error_of_rotated_values(ctx, half, pairs):
                 planted(ctx, DT.F16, half, pairs, head * 128 + e)
                 with raises("NonFiniteInput", head * 128 + first, 1):
                     ctx.sync()
+
+
+@pytest.mark.parametrize("dtype", [DT.F32, DT.F16, DT.BF16, DT.Q8_0])
+def test_store_of_a_slot_named_twice(ctx, dtype):
+    """What lies in a slot that several tokens name is each of them's in part: every value (of Q8_0 every level and every
+    scale) is one of the tokens', and every other slot is as without them."""
+    say("store slot twice", dtype)
+    tokens, kv, dim = 600, 2, 128
+    x = torch.arange(1, tokens + 1, device="cuda", dtype=torch.float32).view(-1, 1, 1).expand(tokens, kv, dim).contiguous() / 1024
+    slots = torch.arange(tokens, device="cuda") % 7 + 16
+    slots[50] = 3
+    cache = rlq.KvCache.make(dtype, 3, kv, 16, dim)
+    ctx.kv_store(cache, x, -x, slots)
+    ctx.sync()
+    alone = rlq.KvCache.make(dtype, 40, kv, 16, dim)
+    ctx.kv_store(alone, x, -x, torch.arange(tokens, device="cuda"))
+    ctx.sync()
+
+    def parts(t):  # levels and scales, or values: [kv, tokens, ..]
+        if dtype != DT.Q8_0:
+            return [t.transpose(0, 1).reshape(kv, -1, dim)]
+        levels, scales = t[..., :16 * dim], t[..., 16 * dim:].contiguous().view(torch.float16)
+        return [levels.unflatten(-1, (16, dim)).transpose(0, 1).reshape(kv, -1, dim),
+                scales.unflatten(-1, (16, dim // 32)).transpose(0, 1).reshape(kv, -1, dim // 32)]
+
+    for t, own in ((cache.k, alone.k), (cache.v, alone.v)):
+        for got, each in zip(parts(t), parts(own)):
+            for s in range(48):
+                named = [i for i in range(tokens) if int(slots[i]) == s] if s != 3 else [50]
+                if not named:
+                    assert (got[:, s] == 0).all()
+                    continue
+                assert (got[:, s].unsqueeze(1) == each[:, named]).any(1).all(), s
