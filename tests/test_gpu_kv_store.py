@@ -1,9 +1,10 @@
-"""rlq_kv_store: the place that an error names, within the four values of a thread too, and slots named twice."""
+"""rlq_kv_store: the place that an error names, within the four values of a thread too, slots named twice, and token sizes on
+both sides of every border between its kernels."""
 import numpy as np
 import pytest
 
 from rlq_loader import load
-from test_gpu_kv import cuda, raises, say
+from test_gpu_kv import cuda, raises, say, store
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +93,56 @@ def test_store_of_a_slot_named_twice(ctx, dtype):
                     assert (got[:, s] == 0).all()
                     continue
                 assert (got[:, s].unsqueeze(1) == each[:, named]).any(1).all(), s
+
+
+# Fours of values a token: to 512, 1024, 2048 and more of many tokens (more than CUs), to 1024, 2048, 4096 and more of few.
+SIZES = [(12, 2, 128), (13, 2, 128), (7, 3, 160), (28, 2, 128), (29, 2, 128), (23, 1, 192), (48, 8, 128), (49, 8, 128), (64, 8, 128),
+         (112, 8, 128), (113, 8, 128), (40, 4, 224), (0, 40, 128)]
+
+
+@pytest.mark.parametrize("dtype", [DT.F32, DT.F16, DT.BF16, DT.Q8_0])
+@pytest.mark.parametrize("heads,kv,dim", SIZES)
+def test_store_sizes(ctx, dtype, heads, kv, dim):
+    """Bit for bit, of few and of many tokens, into new queries and in place, rows behind the last among them."""
+    rng = np.random.default_rng(heads + dim)
+    for tokens, pairs in ((3, False), (257, True)):
+        for in_place in (False, True) if heads else (False,):
+            say("store size", dtype, heads, kv, dim, tokens, in_place)
+            store(ctx, rng, dtype, tokens, heads, kv, dim, 64, 8, pairs ^ in_place, 1000, in_place, behind=2)
+
+
+@pytest.mark.parametrize("dtype", [DT.F32, DT.F16, DT.BF16, DT.Q8_0])
+@pytest.mark.parametrize("pairs", [False, True])
+def test_store_of_a_prompt(ctx, dtype, pairs):
+    """300 tokens of 32 query and 8 key heads of 128, all of them rotated."""
+    say("store prompt", dtype, pairs)
+    store(ctx, np.random.default_rng(9), dtype, 300, 32, 8, 128, 16, 64, pairs, 5000, behind=1)
+
+
+@pytest.mark.parametrize("heads,kv", [(12, 2), (28, 2), (32, 8), (64, 8), (113, 8)])
+@pytest.mark.parametrize("dtype", [DT.F16, DT.Q8_0])
+def test_store_errors_of_many_tokens(ctx, dtype, heads, kv):
+    """Tokens with an error among sound ones, in every kernel: they keep their places, and the first is named."""
+    dim, tokens = 128, 257
+    rng = np.random.default_rng(heads)
+    x = rng.standard_normal((tokens, heads + 2 * kv, dim)).astype(np.float32)
+    bad = {40: (heads + 2 * kv - 1, 127), 41: (0, 0), 200: (heads, 50), 256: (heads + kv, 33)}
+    for t, (h, e) in bad.items():
+        x[t, h, e] = np.nan
+    positions, freqs = cuda(np.arange(tokens, dtype=np.int32)), cuda(np.full(8, 0.01, np.float32))
+    for n in (60, tokens):  # (as many tokens as CUs at most, and more)
+        say("store errors", dtype, heads, kv, n)
+        y = cuda(x[:n])
+        cache, clean = (rlq.KvCache.make(dtype, 17, kv, 16, dim) for _ in range(2))
+        out, want = (torch.full((n, heads, dim), 8.0, device="cuda") for _ in range(2))
+        slots = np.arange(n) + 3
+        args = y[:, heads:heads + kv], y[:, heads + kv:]
+        ctx.kv_store(cache, *args, cuda(slots), y[:, :heads], positions[:n], freqs, out=out)
+        h, e = bad[40]
+        with raises("NonFiniteInput", h * dim + e, 40):
+            ctx.sync()
+        slots[[t for t in bad if t < n]] = -1
+        ctx.kv_store(clean, *args, cuda(slots), y[:, :heads], positions[:n], freqs, out=want)
+        ctx.sync()
+        assert torch.equal(cache.k, clean.k) and torch.equal(cache.v, clean.v) and torch.equal(out, want)
+        assert (out[40:42] == 8).all() and not (out[42] == 8).all()
