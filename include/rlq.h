@@ -476,7 +476,9 @@ int32_t rlq_kv_store(rlq_context *ctx, const rlq_kv_cache *cache, const float *q
  * scale 0: 1 / sqrt(dim).  heads a multiple of kv_heads.  Scores, weights and sums are f32 (16-bit and
  * 8-bit values taken as they are; beside F16 and Q8_0 caches queries and weights enter the products rounded to 23 bits,
  * what is below 2^-16 of the largest to 2^-38 of that); what lies behind positions[t] or before the window is not
- * looked at.  At most 65535 rows.  At rlq_sync: RLQ_TENSOR_BOUNDS (a = the row: a request or
+ * looked at.  The same call gives the same bits; what shares the call may change the order in which a row's sums are
+ * added, but not of a row whose tokens lie within one aligned 128 of the positions.
+ * At most 65535 rows.  At rlq_sync: RLQ_TENSOR_BOUNDS (a = the row: a request or
  * position outside the table, or a page outside the cache; its out is left as it was),
  * RLQ_NON_FINITE (a = RLQ_CHECK_ATTENTION_OUTPUT, b = the row; a query head with such a
  * value is left as it was).  Capturing: make the same call once before. */

@@ -273,7 +273,7 @@ __device__ __forceinline__ void words(const void* p, W (&out)[N]) {
 }
 // sine and cosine of a by quarter turns: a - n pi/2 with pi/2 in two f64 (n below 2^38, so that what is
 // left out, n 2^-108, is far below a last bit), then the Taylor polynomials, whose
-// first terms left out are below 2^-60 for |r| <= pi/4.
+// first terms left out are below 2^-63 (sine) and 2^-58 (cosine) for |r| <= pi/4.
 __device__ __forceinline__ double2 sine_cosine(double a) {
     if (!(fabs(a) < 2.7e11)) {
         double s, c;
@@ -900,8 +900,8 @@ __device__ __forceinline__ float2 attn_get(const float* from) {
 // of every tile, and join in LDS.  A row that lies in one slot is written by it; of others each slot puts its part where
 // every workgroup can read it, and the last to arrive joins the parts in order (published as the
 // router's logits are: an exchange is performed at the device's coherent level when it returns).
-// So the order in which a row is added up follows from the call's rows alone, and a row of one tile (or
-// in one slot) is added up as if it were alone.
+// So the order in which a row is added up follows from the call's rows alone, and a row whose tokens lie in one tile (an
+// aligned 128 of the positions) is added up as if it were alone.
 //
 // Rows one behind the other of one request at one position after the other (a prompt's tokens, drafted ones) go
 // together where their heads of a KV head fit a tile's 16 columns: `pack` rows at most read their tokens once.

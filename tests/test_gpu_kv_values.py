@@ -1,10 +1,11 @@
-"""Attention over a paged cache whose stored values lie at the ends of what the cache's types hold."""
+"""Attention over a paged cache: stored values at the ends of what the cache's types hold, many small weights, and rows beside
+others."""
 import numpy as np
 import pytest
 
 import kv_oracle as K
 from rlq_loader import load
-from test_gpu_kv import cuda, say, tolerance
+from test_gpu_kv import cuda, fill, say, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +94,29 @@ def test_attention_of_many_small_weights(ctx, dtype):
     err = np.abs(got.double().cpu().numpy() / want - 1)
     print("relative error", err.max(), flush=True)
     assert err.max() <= 1e-4
+
+
+@pytest.mark.parametrize("dtype", [DT.F32, DT.F16, DT.BF16, DT.Q8_0])
+def test_attention_of_rows_in_one_tile_does_not_depend_on_company(ctx, dtype):
+    """Rows whose tokens lie within one aligned 128 of the positions, alone and beside long rows, runs of rows that go together
+    and rows of other requests: the same bits."""
+    say("attention company", dtype)
+    rng = np.random.default_rng(31)
+    heads, kv, dim, page, width = 8, 2, 64, 16, 640
+    cache = rlq.KvCache.make(dtype, 2 * width, kv, page, dim)
+    fill(rng, cache)
+    tables = cuda(rng.permutation(2 * width).astype(np.int32).reshape(2, width))
+    for window, positions in ((0, [0, 1, 30, 31, 32, 33, 100, 125, 126, 127]), (20, [19, 127, 147, 148, 149, 150, 151, 255, 9000, 9001])):
+        first = [max(0, p + 1 - window) if window else 0 for p in positions]
+        assert all(f >> 7 == p >> 7 for f, p in zip(first, positions))
+        long = [5000, 10000, 128, 129, 130, 131, 132, 8000, 8001, 8002] * 20
+        n = len(positions)
+        q = cuda(rng.standard_normal((n + len(long), heads, dim)).astype(np.float32))
+        at = cuda(np.array(positions + long, np.int32))
+        who = cuda(np.concatenate([np.zeros(n), np.arange(len(long)) // 10 % 2]).astype(np.int32))
+        for rows in (n, n + 10, n + len(long)):  # (few: counted by lanes; many: in LDS)
+            together = ctx.kv_attention(cache, q[:rows], tables, at[:rows], who[:rows], window=window)
+            for r in range(n):
+                alone = ctx.kv_attention(cache, q[r:r + 1], tables, at[r:r + 1], who[r:r + 1], window=window)
+                assert (alone[0] == together[r]).all(), (window, rows, r)
+        ctx.sync()
