@@ -313,6 +313,15 @@ __device__ __forceinline__ bool store_off(float y) {
     if constexpr (T == kBF16) return !finite(y) || !finite(__uint_as_float(bf16_bits(y) << 16));
     return !finite(y);
 }
+// The first such of four values, of which one is; q: of a query's, which are not stored.
+template <uint32_t T>
+__device__ __forceinline__ uint32_t first_off(const float (&y)[4], bool q) {
+    uint32_t first = 3;
+#pragma unroll
+    for (int j = 2; j >= 0; --j)
+        if (q ? !finite(y[j]) : store_off<T>(y[j])) first = (uint32_t)j;
+    return first;
+}
 // Four values from element e on of a token's place in a plane; Q8_0: by eight lanes, a block.
 template <uint32_t T>
 __device__ __forceinline__ void store_put(uint8_t* plane, uint64_t row, uint32_t e, uint32_t dim, uint32_t log_page,
@@ -403,12 +412,8 @@ __global__ __launch_bounds__(N) void kv_store_kernel(StoreArgs a) {
         if constexpr (T == kQ8_0) scale = !q && norm_q8_0(x[u]).bad;
         if (have && (off || scale)) {
             bad = 1;
-            uint32_t first = 3;  // of the four
-#pragma unroll
-            for (int j = 2; j >= 0; --j)
-                if (q ? !finite(x[u][j]) : store_off<T>(x[u][j])) first = (uint32_t)j;
             const uint64_t at = (uint64_t)head[u] * dim + e[u];
-            report_error(a.err_word, off ? error_key(t, kKindNonFinite, at + first)
+            report_error(a.err_word, off ? error_key(t, kKindNonFinite, at + first_off<T>(x[u], q))
                                          : error_key(t, kKindScale, (at - (uint64_t)a.heads * dim) / 32));
         }
     }
@@ -450,13 +455,13 @@ __global__ __launch_bounds__(256) void kv_store_any_kernel(StoreArgs a) {
     const uint32_t kv = a.c.kv_heads, heads = a.heads + 2 * kv;
     const uint64_t page = (uint64_t)slot >> a.c.log_page, row = (uint64_t)slot & ((1u << a.c.log_page) - 1);
 
-    // four values of head h, and the first that is not finite (4: none)
+    // four values of head h, and whether one is not finite
     auto values = [&](uint32_t h, float (&y)[4]) {
         const bool q = h < a.heads, k = !q && h < a.heads + kv;
         const float* x = q ? a.q + t * a.q_stride + (uint64_t)h * dim
                            : k ? a.k + t * a.k_stride + (uint64_t)(h - a.heads) * dim
                                : a.v + t * a.v_stride + (uint64_t)(h - a.heads - kv) * dim;
-        uint32_t off = 4;
+        bool off = false;
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
             const uint32_t i = e + j;
@@ -468,7 +473,7 @@ __global__ __launch_bounds__(256) void kv_store_any_kernel(StoreArgs a) {
                 const double m = (double)y[j] * cs.x, o = (double)x[other] * cs.y;
                 y[j] = (float)(second ? o + m : m - o);
             }
-            if (off == 4 && (q ? !finite(y[j]) : store_off<T>(y[j]))) off = j;
+            off |= q ? !finite(y[j]) : store_off<T>(y[j]);
         }
         return off;
     };
@@ -476,10 +481,9 @@ __global__ __launch_bounds__(256) void kv_store_any_kernel(StoreArgs a) {
     int bad = 0;
     for (uint32_t h = wave * per + group; h < heads && group < per; h += 4 * per) {
         float y[4];
-        const uint32_t off = values(h, y);
-        if (off < 4) {
+        if (values(h, y)) {
             bad = 1;
-            report_error(a.err_word, error_key(t, kKindNonFinite, (uint64_t)h * dim + e + off));
+            report_error(a.err_word, error_key(t, kKindNonFinite, (uint64_t)h * dim + e + first_off<T>(y, h < a.heads)));
         } else if (T == kQ8_0 && h >= a.heads && norm_q8_0(y).bad) {
             bad = 1;
             report_error(a.err_word, error_key(t, kKindScale, ((uint64_t)(h - a.heads) * dim + e) / 32));
