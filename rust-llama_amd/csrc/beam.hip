@@ -167,7 +167,7 @@ __device__ __forceinline__ void merge_lists(const unsigned long long* list, bool
 // what reaches it, some tens of candidates, is ranked by counting.  Else the last chunk of a row merges the row's
 // sorted lists, a lane for each, and the last row of the group the beams'.  One launch.
 //
-// Bound: four beams of 128256 tokens, the best 8: 15.4 us, of which the loads are 2.3, sums and lists 2.2, the waves'
+// Bound: four beams of 128256 tokens, the best 8: 14.9 us, of which the loads are 2.3, sums and lists 2.2, the waves'
 // lists 1.6, putting and counting 3.4 (252 workgroups count at one place), the choice 5.  16 groups of
 // eight beams of 151936 tokens, the best 16: 38 us; the loads alone 13.4 (5.8 TB/s), sums and lists 11 beside them
 // (30 VALU instructions a logit, eight of them the exponential; 23 of them, or twice the waves, take as long), then

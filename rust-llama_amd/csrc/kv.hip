@@ -86,7 +86,7 @@ __device__ __forceinline__ void pages_row(const PagesArgs& a, const P* starts, u
 //
 // Bound: latencies one after another (the lengths, the ended requests' entries, the list, the tables) and the
 // barriers between: 32 requests of up to 8192 tokens, one new token each, a tenth of them ended, 6.2 us (11.6 with
-// the entries loaded 64 at a time); 256 requests that take 2000 pages 9.9, and their 65536 rows 3.7 in a launch of
+// the entries loaded 64 at a time); 256 requests that take 2000 pages 10.4, and their 65536 rows 4.0 in a launch of
 // their own.
 template <uint32_t N, uint32_t PER>
 __global__ __launch_bounds__(N) void pages_plan_kernel(PagesArgs a, uint32_t rows) {
@@ -911,7 +911,7 @@ __device__ __forceinline__ float2 attn_get(const float* from) {
 // together where their heads of a KV head fit a tile's 16 columns: `pack` rows at most read their tokens once.
 // They differ in the first and last tokens only, which each column masks for itself; a value there that is no finite number
 // is taken out and makes the columns that see it none.  With 4 query heads of 128 a KV head, f16: a prompt of 4000
-// tokens 2500 us apart, 765 together; five drafted rows of each of 32 requests up to 8192 158 and 79.  Not where the
+// tokens 2500 us apart, 765 together; five drafted rows of each of 32 requests up to 8192 158 and 80.  Not where the
 // rows apart have no more tiles than there are slots: five rows of 1000 tokens 10 us apart, on CUs of their own, 16
 // together.
 //
@@ -920,8 +920,8 @@ __device__ __forceinline__ float2 attn_get(const float* from) {
 // rows (32 up to 8192) 53 us, dealt 42.
 //
 // Bound: HBM where there is enough to read: one row of 131072 tokens (bf16) 102 us, 5.3 TB/s; 32 rows of 4096 f16
-// 96 us, 5.6; f32 183, 5.9; Q8_0 62, 4.6 (VALU issues during half of its cycles).  Small calls: six latencies
-// one after another (positions, pages, keys, then parts put, counted and read): 100 tokens 6.2 us, 1000 8.4,
+// 96 us, 5.6; f32 184, 5.8; Q8_0 61, 4.6 (VALU issues during half of its cycles).  Small calls: six latencies
+// one after another (positions, pages, keys, then parts put, counted and read): 100 tokens 6.4 us, 1000 8.6,
 // 16000 21.
 //
 // The rows' tiles are counted by every workgroup: to 64 rows a lane each, else in LDS.
