@@ -621,7 +621,9 @@ template <uint32_t T, int NB>  // NB: blocks of 32 values
 struct AttnWave {
     static constexpr int kDim = 32 * NB, kOwn = 2 * NB;  // values of a token that a lane holds for O
     static constexpr bool k16 = T == kF16 || T == kBF16;
-    static constexpr float kTop = T == kF16 || T == kQ8_0 ? 14.0f : 0.0f;  // weights are 2^kTop times exp(s - max)
+    // Weights are exp(s - max) times kTop.  (In the exponent it would be rounded with the maximum: weights of scores up to 16 off
+    // by 3e-7 among the waves, rows of four tokens by 1.6e-7 instead of 1.0e-7, and one token's weight not 1.)
+    static constexpr float kTop = T == kF16 || T == kQ8_0 ? 16384.0f : 1.0f;
 
     // q (columns past the last head 0): f32, or in terms
     uint32_t q0[T == kF32 ? 1 : NB][4], q1[T == kF32 ? 1 : NB][4], q2[T == kBF16 ? NB : 1][4];
@@ -777,9 +779,9 @@ struct AttnWave {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[e][r] *= f;
         }
-        const float base = fmaxf(m, -3.402823466e38f) - kTop;  // (a column that has no token yet: -inf is less)
+        const float base = fmaxf(m, -3.402823466e38f);  // (a column that has no token yet: -inf is less)
 #pragma unroll
-        for (int t = 0; t < 8; ++t) s[t] = __builtin_amdgcn_exp2f(s[t] - base);
+        for (int t = 0; t < 8; ++t) s[t] = __builtin_amdgcn_exp2f(s[t] - base) * kTop;
         l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     }
 

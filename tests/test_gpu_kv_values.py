@@ -120,3 +120,22 @@ def test_attention_of_rows_in_one_tile_does_not_depend_on_company(ctx, dtype):
                 alone = ctx.kv_attention(cache, q[r:r + 1], tables, at[r:r + 1], who[r:r + 1], window=window)
                 assert (alone[0] == together[r]).all(), (window, rows, r)
         ctx.sync()
+
+
+@pytest.mark.parametrize("dtype", [DT.F32, DT.F16, DT.BF16, DT.Q8_0])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_attention_of_one_token_is_its_value(ctx, dtype, dim):
+    """The weight of a token alone is 1 whatever its score, so its value comes out bit for bit: rows of one token, and rows that
+    a window leaves one."""
+    say("attention one token", dtype, dim)
+    rng = np.random.default_rng(dim)
+    rows, heads, kv, page, width = 200, 8, 2, 16, 12
+    cache = rlq.KvCache.make(dtype, rows * width, kv, page, dim)
+    _, v = fill(rng, cache)
+    tables = rng.permutation(rows * width).astype(np.int32).reshape(rows, width)
+    q = (rng.standard_normal((rows, heads, dim)) * rng.uniform(0.1, 8, (rows, 1, 1))).astype(np.float32)
+    for window, positions in ((0, np.zeros(rows, np.int32)), (1, rng.integers(0, width * page, rows).astype(np.int32))):
+        got = ctx.kv_attention(cache, cuda(q), cuda(tables), cuda(positions), window=window)
+        ctx.sync()
+        want = v[tables[np.arange(rows), positions // page], :, positions % page].astype(np.float32)  # [rows, kv heads, dim]
+        assert np.array_equal(got.cpu().numpy(), np.repeat(want, heads // kv, 1))
