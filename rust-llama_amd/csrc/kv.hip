@@ -86,7 +86,7 @@ __device__ __forceinline__ void pages_row(const PagesArgs& a, const P* starts, u
 //
 // Bound: latencies one after another (the lengths, the ended requests' entries, the list, the tables) and the
 // barriers between: 32 requests of up to 8192 tokens, one new token each, a tenth of them ended, 6.2 us (11.6 with
-// the entries loaded 64 at a time); 256 requests that take 2000 pages 10.4, and their 65536 rows 4.0 in a launch of
+// the entries loaded 64 at a time); 256 requests that take 2000 pages 9.8, and their 65536 rows 3.8 in a launch of
 // their own.
 template <uint32_t N, uint32_t PER>
 __global__ __launch_bounds__(N) void pages_plan_kernel(PagesArgs a, uint32_t rows) {
